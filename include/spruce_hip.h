@@ -680,6 +680,70 @@ int spruce_pack_selected_mask(const uint8_t* mask, int64_t R, int64_t qb, int64_
 int spruce_kernel_metadata(int variant, int64_t Hq, int64_t Hkv, int64_t D,
                            char* json, size_t n);
 
+/* ------------------------------------------------------------------------
+ * The paged serving step: a prompt that comes in chunks, or goes on token by
+ * token, over a paged K/V cache.  No counterpart in the reference, whose
+ * kernels are prefill-only (kernels/sparse_prefill.py:63-66 hands every other
+ * call to Transformers).
+ *
+ * A ragged batch: S sequences, sequence s owning rows q_starts[s] ..
+ * q_starts[s + 1) of the packed [N, H, D] tensors (q_starts int32 [S + 1],
+ * ascending) and kv_lens[s] positions in the cache (int32 [S]), its new tokens
+ * included: new token i of n has position kv_lens[s] - n + i.  Position p is
+ * slot p % page_size of page page_table[s][p / page_size] (int32
+ * [S, table_width], rows table_stride apart); pages are
+ * [pages, Hkv, page_size, D] with any strides, contiguous along D.  All of
+ * these are read on the device: a captured launch takes the values they hold
+ * at replay.  Ids outside [0, pages) and positions past the table name no
+ * slot.
+ * ---------------------------------------------------------------------- */
+
+/* Pairs (x_i, x_{i + R/2}) or (x_{2i}, x_{2i+1}) of the R rotated dims. */
+#define SPRUCE_ROTARY_HALF 0
+#define SPRUCE_ROTARY_INTERLEAVED 1
+
+/*
+ * RMS norm of every head row (with a weight: q_weight / k_weight [D], either
+ * may be NULL for none) and rotary positions, for queries and keys in one
+ * launch:
+ *   y = x * (mean(x^2) + eps)^(-1/2) * weight
+ *   (a, b) <- factor * (a cos t - b sin t, b cos t + a sin t),
+ *   t = position * inv_freq[pair]
+ * over the first rotary_dim values of a row (a multiple of 16 up to D; 0: no
+ * rotation), the rest as they are.  Angles in 64 bits, the rest in 32,
+ * rounded once.
+ *   q [B, Hq, T, D], k [B, Hkv, T, D], outputs of the same shapes (they may be
+ *   the inputs), strides qs, ks, qos, kos, rows 16-byte aligned; bf16 / f16 /
+ *   f32; D in {64, 128}.
+ *   positions int32 (or int64 with pos64) [B, T], rows pos_stride apart
+ *   (0: one row for the batch), tokens contiguous.
+ *   inv_freq float64 [rotary_dim / 2].  weight_dtype: SPRUCE_DTYPE_F32 or
+ *   dtype.
+ */
+int spruce_rotate_heads(const void* q, const int64_t qs[4], const void* k, const int64_t ks[4], int64_t B,
+                        int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int dtype, const void* positions,
+                        int64_t pos_stride, int pos64, const double* inv_freq, int64_t rotary_dim, int layout,
+                        float factor, const void* q_weight, const void* k_weight, int weight_dtype, float eps,
+                        void* qo, const int64_t qos[4], void* ko, const int64_t kos[4], void* stream);
+
+/*
+ * Writes the new tokens' keys and values (k, v [N, Hkv, D], strides ks, vs)
+ * into their pages, the keys with the norm and rotation of
+ * spruce_rotate_heads on the way; with Hq > 0 the queries q [N, Hq, D] get
+ * theirs into qo in the same launch.  positions (NULL: the cache positions)
+ * gives the rotation angles' positions [N].  Rows before q_starts[0] or at and
+ * behind q_starts[S] are left alone, in qo too, and a token without a slot
+ * writes no key and value.  Two tokens with one slot leave either's values.
+ */
+int spruce_paged_append(const void* q, const int64_t qs[3], void* qo, const int64_t qos[3], const void* k,
+                        const int64_t ks[3], const void* v, const int64_t vs[3], int64_t N, int64_t Hq, int64_t Hkv,
+                        int64_t D, int dtype, void* k_pages, const int64_t kps[4], void* v_pages,
+                        const int64_t vps[4], int64_t pages, int64_t page_size, const int32_t* page_table,
+                        int64_t table_stride, int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens,
+                        int64_t S, const void* positions, int pos64, const double* inv_freq, int64_t rotary_dim,
+                        int layout, float factor, const void* q_weight, const void* k_weight, int weight_dtype,
+                        float eps, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

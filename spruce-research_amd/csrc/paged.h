@@ -1,0 +1,89 @@
+// The ragged batch over a paged K/V cache that the append and the chunk
+// attention share, and the lookups in it.
+#pragma once
+
+#include "common.h"
+
+namespace spruce {
+
+// Sequences s = 0..S-1 with their new tokens at rows q_starts[s] ..
+// q_starts[s + 1) of the packed tensors and kv_lens[s] cached keys, those of
+// the new tokens included: new token i stands at position kv_lens[s] - n + i
+// of n.  Position p lies in slot p % page of page page_table[s][p / page].
+// Everything is read on the device; what a caller may have wrong there (a
+// page outside [0, pages), lengths past the table, starts past the packed
+// rows) is bounded where it is read and never addresses memory.
+struct PagedBatch {
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* q_starts;
+  const int32_t* kv_lens;
+  int S, N, page, pages;
+  int cap;         // positions the table holds: width * page, below 2^31
+  uint32_t magic;  // p / page == (p * magic) >> shift for p < 2^31
+  int shift;
+};
+
+// With l = ceil(log2(page)), magic = floor(2^(31 + l) / page) + 1 exceeds
+// 2^(31 + l) / page by at most 1, so p * magic / 2^(31 + l) exceeds p / page
+// by less than 2^-l <= 1 / page for p < 2^31: the floor is the same.
+inline int prepare_batch(PagedBatch& b, const int32_t* table, int64_t table_stride, int64_t width,
+                         const int32_t* q_starts, const int32_t* kv_lens, int64_t S, int64_t N, int64_t page,
+                         int64_t pages) {
+  SPRUCE_REQUIRE((table || width == 0) && q_starts && kv_lens, "page_table, q_starts and kv_lens must be non-null device pointers");
+  SPRUCE_REQUIRE(S >= 1 && S < (int64_t)1 << 20, "sequences must be in [1, 2^20), got %lld", (long long)S);
+  SPRUCE_REQUIRE(N >= 0 && N < (int64_t)1 << 30, "invalid token count %lld", (long long)N);
+  SPRUCE_REQUIRE(page >= 1 && page < (int64_t)1 << 30, "invalid page size %lld", (long long)page);
+  SPRUCE_REQUIRE(pages >= 0 && pages < (int64_t)1 << 31, "invalid page count %lld", (long long)pages);
+  SPRUCE_REQUIRE(width >= 0 && table_stride >= width, "page_table rows (%lld) overlap (stride %lld)",
+                 (long long)width, (long long)table_stride);
+  SPRUCE_REQUIRE(width < ((int64_t)1 << 31) / page, "page_table covers 2^31 positions or more");
+  b.table = table;
+  b.table_stride = table_stride;
+  b.q_starts = q_starts;
+  b.kv_lens = kv_lens;
+  b.S = (int)S;
+  b.N = (int)N;
+  b.page = (int)page;
+  b.pages = (int)pages;
+  b.cap = (int)(width * page);
+  int l = 0;
+  while (((int64_t)1 << l) < page) ++l;
+  b.magic = (uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)page) + 1);
+  b.shift = 31 + l;
+  return SPRUCE_OK;
+}
+
+__device__ __forceinline__ int page_of(const PagedBatch& b, int pos) {
+  return (int)(((uint64_t)(uint32_t)pos * b.magic) >> b.shift);
+}
+
+// q_starts[s] and kv_lens[s] brought into range.
+__device__ __forceinline__ int start_at(const PagedBatch& b, int s) {
+  const int v = b.q_starts[s];
+  return v < 0 ? 0 : (v > b.N ? b.N : v);
+}
+__device__ __forceinline__ int keys_of(const PagedBatch& b, int s) {
+  const int v = b.kv_lens[s];
+  return v < 0 ? 0 : (v > b.cap ? b.cap : v);
+}
+
+// The page that holds position pos (0 <= pos < cap) of sequence s, -1 where
+// the table names none.
+__device__ __forceinline__ int page_id(const PagedBatch& b, int s, int pos) {
+  const int v = b.table[(int64_t)s * b.table_stride + page_of(b, pos)];
+  return v >= 0 && v < b.pages ? v : -1;
+}
+
+// The sequence of packed row n, wave-uniform: the starts at or below n are
+// counted 64 at a time.  -1 for rows before the first or behind the last.
+__device__ __forceinline__ int sequence_of(const PagedBatch& b, int n, int lane) {
+  int below = 0;
+  for (int s0 = 0; s0 <= b.S; s0 += 64) {
+    const int s = s0 + lane;
+    below += __builtin_popcountll(__ballot(s <= b.S && b.q_starts[s] <= n));
+  }
+  return below == 0 || below > b.S ? -1 : below - 1;
+}
+
+}  // namespace spruce

@@ -108,6 +108,13 @@ _SIGNATURES = {
     "spruce_tree_traverse": [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _i64,
                              ctypes.c_int, _p],
     "spruce_gate_candidate_scores": [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p],
+    "spruce_rotate_heads": [
+        _p, _STRIDES, _p, _STRIDES, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, _p, _i64, ctypes.c_int, _p, _i64,
+        ctypes.c_int, ctypes.c_float, _p, _p, ctypes.c_int, ctypes.c_float, _p, _STRIDES, _p, _STRIDES, _p],
+    "spruce_paged_append": [
+        _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _i64, _i64, _i64, _i64, ctypes.c_int,
+        _p, _STRIDES, _p, _STRIDES, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, ctypes.c_int, _p, _i64,
+        ctypes.c_int, ctypes.c_float, _p, _p, ctypes.c_int, ctypes.c_float, _p],
     "spruce_sparse_prefill_mask": [
         _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _i64,
         _i64, _i64, _i64, _i64, _i64, ctypes.c_float, ctypes.c_int, ctypes.c_int,

@@ -1,0 +1,174 @@
+"""Rotary frequencies and the refusals of the rotary and append calls: the
+checks come before the GPU is touched, so these run without one."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import spruce_hip
+from kernels.paged import append_paged_kv
+from kernels.rotary import rotary_frequencies, rotate_heads
+
+
+def test_plain_linear_and_ntk_frequencies():
+    R, base = 64, 1e6
+    plain, factor = rotary_frequencies(R, base)
+    assert plain.dtype == torch.float64 and factor == 1.0
+    for i in (0, 1, 17, 31):
+        assert plain[i].item() == pytest.approx(base ** (-2 * i / R), rel=1e-14)
+    linear, factor = rotary_frequencies(R, base, scaling="linear", factor=4.0)
+    assert factor == 1.0 and torch.equal(linear, plain / 4.0)
+    ntk, factor = rotary_frequencies(R, base, scaling="ntk", factor=4.0)
+    # The fastest pair turns as before, the slowest four times slower.
+    assert factor == 1.0 and ntk[0].item() == 1.0
+    assert ntk[-1].item() == pytest.approx(plain[-1].item() / 4.0, rel=1e-12)
+
+
+@pytest.mark.parametrize("dim,base,factor,length", [(128, 1e6, 4.0, 32768), (64, 1e4, 16.0, 2048)])
+def test_yarn_frequencies(dim, base, factor, length):
+    plain, _ = rotary_frequencies(dim, base)
+    yarn, attention = rotary_frequencies(dim, base, scaling="yarn", factor=factor, original_length=length)
+    assert attention == pytest.approx(0.1 * math.log(factor) + 1.0)
+    turns = plain * length / (2 * math.pi)
+    ratio = plain / yarn
+    # Away from the two borders (an index either way, for the rounding of their places).
+    fast, slow = (turns > 32 * base ** (2 / dim)), (turns < base ** (-4 / dim))
+    assert fast.any() and slow.any()
+    assert torch.allclose(ratio[fast], torch.ones_like(ratio[fast]), rtol=1e-12)
+    assert torch.allclose(ratio[slow], torch.full_like(ratio[slow], factor), rtol=1e-12)
+    assert (ratio[1:] >= ratio[:-1] - 1e-12).all()
+
+
+def test_yarn_agrees_with_transformers():
+    rope = pytest.importorskip("transformers.modeling_rope_utils")
+    from transformers import Qwen2Config
+    config = Qwen2Config(hidden_size=512, num_attention_heads=4, max_position_embeddings=131072, rope_theta=1e6,
+                         rope_scaling={"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768})
+    want, attention = rope.ROPE_INIT_FUNCTIONS["yarn"](config, torch.device("cpu"))
+    got, factor = rotary_frequencies(128, 1e6, scaling="yarn", factor=4.0, original_length=32768)
+    assert factor == pytest.approx(attention, rel=1e-6)
+    assert torch.allclose(got.float(), want, rtol=1e-5, atol=0)
+
+
+def test_frequency_refusals():
+    for kwargs, message in ((dict(rotary_dim=0), "rotary_dim"), (dict(rotary_dim=7), "rotary_dim"),
+                            (dict(rotary_dim=64, scaling="other"), "scaling must be"),
+                            (dict(rotary_dim=64, factor=0.5), "factor"), (dict(rotary_dim=64, base=1.0), "base"),
+                            (dict(rotary_dim=64, scaling="yarn", factor=2.0), "original_length"),
+                            (dict(rotary_dim=2, scaling="ntk", factor=2.0), "rotary_dim above 2")):
+        with pytest.raises(ValueError, match=message):
+            rotary_frequencies(**kwargs)
+
+
+def _rotate(B=1, T=3, Hq=4, Hkv=2, D=64, dtype=torch.bfloat16, k=None, q=None, positions=None, R=64, **kwargs):
+    q = torch.zeros(B, Hq, T, D, dtype=dtype) if q is None else q
+    k = torch.zeros(B, Hkv, T, D, dtype=dtype) if k is None else k
+    positions = torch.arange(T) if positions is None else positions
+    return rotate_heads(q, k, positions, rotary_frequencies(R)[0] if R else None, **kwargs)
+
+
+def test_rotate_refusals():
+    bf = torch.bfloat16
+    for kwargs, message in ((dict(D=96), "head_dim 64 or 128"), (dict(R=72), "rotary_dim"), (dict(R=128), "rotary_dim"),
+                            (dict(layout="other"), "layout must be"),
+                            (dict(k=torch.zeros(1, 2, 4, 64, dtype=bf)), "match in batch"),
+                            (dict(k=torch.zeros(1, 2, 3, 64)), "share one dtype"),
+                            (dict(q=torch.zeros(1, 4, 64, 3, dtype=bf).transpose(2, 3)), "contiguous final"),
+                            (dict(positions=torch.zeros(3)), "int32 or int64"),
+                            (dict(positions=torch.zeros(4, dtype=torch.int32)), "positions must be"),
+                            (dict(positions=torch.zeros(6, dtype=torch.int32)[::2]), "contiguous tokens"),
+                            (dict(q_weight=torch.ones(63)), "norm weights"),
+                            (dict(q_weight=torch.ones(64, dtype=torch.float16)), "share one dtype"),
+                            (dict(q_weight=torch.ones(64), k_weight=torch.ones(64, dtype=bf)), "share one dtype")):
+        with pytest.raises(ValueError, match=message):
+            _rotate(**kwargs)
+    with pytest.raises(ValueError, match="float64"):
+        rotate_heads(torch.zeros(1, 4, 3, 64), torch.zeros(1, 2, 3, 64), torch.arange(3), torch.ones(32))
+    with pytest.raises(RuntimeError, match="requires GPU tensors"):
+        _rotate()
+    grad = torch.zeros(1, 4, 3, 64, dtype=bf, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        _rotate(q=grad)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="requires GPU tensors"):
+        _rotate(q=grad)
+
+
+def _append(N=3, Hkv=2, D=64, dtype=torch.bfloat16, S=2, W=4, page=16, **change):
+    args = dict(k=torch.zeros(N, Hkv, D, dtype=dtype), v=torch.zeros(N, Hkv, D, dtype=dtype),
+                k_pages=torch.zeros(5, Hkv, page, D, dtype=dtype), v_pages=torch.zeros(5, Hkv, page, D, dtype=dtype),
+                page_table=torch.zeros(S, W, dtype=torch.int32), q_starts=torch.zeros(S + 1, dtype=torch.int32),
+                kv_lens=torch.zeros(S, dtype=torch.int32))
+    args.update(change)
+    return append_paged_kv(**args)
+
+
+def test_append_refusals():
+    bf, i32 = torch.bfloat16, torch.int32
+    for kwargs, message in ((dict(D=96), "head_dim 64 or 128"),
+                            (dict(v=torch.zeros(4, 2, 64, dtype=bf)), "k and v must match"),
+                            (dict(v_pages=torch.zeros(5, 2, 8, 64, dtype=bf)), "k_pages and v_pages must match"),
+                            (dict(k_pages=torch.zeros(5, 2, 16, 64), v_pages=torch.zeros(5, 2, 16, 64)), "dtype"),
+                            (dict(k_pages=torch.zeros(5, 3, 16, 64, dtype=bf),
+                                  v_pages=torch.zeros(5, 3, 16, 64, dtype=bf)), "match in KV heads"),
+                            (dict(page_table=torch.zeros(2, 4)), "page_table must be int32"),
+                            (dict(page_table=torch.zeros(4, 2, dtype=i32).T), "contiguous final"),
+                            (dict(q_starts=torch.zeros(2, dtype=i32)), "q_starts"),
+                            (dict(kv_lens=torch.zeros(2)), "kv_lens"),
+                            (dict(query=torch.zeros(2, 4, 64, dtype=bf)), "query must be"),
+                            (dict(query=torch.zeros(3, 0, 64, dtype=bf)), "must have a head"),
+                            (dict(positions=torch.zeros(1, 3, dtype=i32)), "positions must be")):
+        with pytest.raises(ValueError, match=message):
+            _append(**kwargs)
+    with pytest.raises(RuntimeError, match="requires GPU tensors"):
+        _append()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        _append(k=torch.zeros(3, 2, 64, dtype=bf, requires_grad=True))
+
+
+def _st(*s):
+    return (ctypes.c_int64 * len(s))(*s)
+
+
+def test_entry_points_refuse_before_the_launch():
+    lib, fake = spruce_hip.lib(), ctypes.c_void_p(1 << 20)
+
+    def rotate(D=128, dtype=0, R=128, layout=0, wd=2, qs=(0, 128, 512, 1), B=1, q=fake, freq=fake, w=None):
+        return lib.spruce_rotate_heads(q, _st(*qs), fake, _st(0, 128, 256, 1), B, 4, 2, 8, D, dtype, fake, 0, 0, freq,
+                                       R, layout, 1.0, w, None, wd, 1e-6, fake, _st(0, 128, 512, 1), fake,
+                                       _st(0, 128, 256, 1), None)
+    for kwargs, message in ((dict(D=96), "head_dim 64 or 128"), (dict(dtype=3), "dtype"), (dict(R=24), "rotary_dim"),
+                            (dict(R=144), "rotary_dim"), (dict(layout=2), "layout"), (dict(wd=1), "norm weights"),
+                            (dict(w=ctypes.c_void_p((1 << 20) + 4)), "norm weights must be 16-byte"),
+                            (dict(qs=(0, 128, 512, 2)), "contiguous final"), (dict(qs=(0, 100, 512, 1)), "16-byte"),
+                            (dict(q=ctypes.c_void_p((1 << 20) + 2)), "16-byte"), (dict(q=None), "non-null"),
+                            (dict(freq=None), "inv_freq"), (dict(B=-1), "invalid shape")):
+        assert rotate(**kwargs) == -1, kwargs
+        assert message in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
+    assert rotate(B=0) == 0
+
+    def append(N=8, Hq=4, page=16, pages=9, width=4, stride=4, S=2, table=fake, q=fake, kps=(4096, 2048, 128, 1)):
+        return lib.spruce_paged_append(q, _st(512, 128, 1), fake, _st(512, 128, 1), fake, _st(256, 128, 1), fake,
+                                       _st(256, 128, 1), N, Hq, 2, 128, 0, fake, _st(*kps), fake,
+                                       _st(4096, 2048, 128, 1), pages, page, table, stride, width, fake, fake, S, None,
+                                       0, None, 0, 0, 1.0, None, None, 2, 1e-6, None)
+    for kwargs, message in ((dict(page=0), "page size"), (dict(S=0), "sequences"), (dict(stride=3), "overlap"),
+                            (dict(width=1 << 28, stride=1 << 28), "2^31"), (dict(pages=-1), "page count"),
+                            (dict(N=-1), "token count"), (dict(table=None), "non-null"), (dict(q=None), "non-null"),
+                            (dict(kps=(4096, 2048, 100, 1)), "16-byte")):
+        assert append(**kwargs) == -1, kwargs
+        assert message in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
+    assert append(N=0) == 0
+
+
+def test_page_division_by_multiplication():
+    # prepare_batch's constants: l = ceil(log2(page)), magic = floor(2^(31 + l) / page) + 1.
+    top = (1 << 31) - 1
+    for page in [1, 2, 3, 5, 7, 16, 48, 100, 641, 4095, 4096, 4097, (1 << 29) + 1, (1 << 30) - 1]:
+        shift = (page - 1).bit_length()
+        magic = (1 << (31 + shift)) // page + 1
+        assert magic < 1 << 32
+        for k in [0, 1, 2, 3, 1000, top // page - 1, top // page]:
+            for p in (k * page - 1, k * page, k * page + 1, k * page + page - 1, top):
+                if 0 <= p <= top:
+                    assert (p * magic) >> (31 + shift) == p // page, (page, p)
