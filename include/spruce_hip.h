@@ -744,6 +744,33 @@ int spruce_paged_append(const void* q, const int64_t qs[3], void* qo, const int6
                         int layout, float factor, const void* q_weight, const void* k_weight, int weight_dtype,
                         float eps, void* stream);
 
+/*
+ * Attention of the new tokens over the cache: token n at position p attends
+ * the cached positions j <= p,
+ *   out_n = sum_j softmax_j(scale * q_n . k_j) v_j,
+ * query head h with KV head h / (Hq / Hkv).  With K > 0 only the 64-key
+ * blocks (positions 64 id .. 64 id + 63) that idx lists: idx [S, Hkv, Qc, K]
+ * int32, strides is, row b of a sequence for its new tokens in the b-th
+ * 64-position block that they touch; entries < 0 and blocks behind the
+ * token's own are skipped, duplicates attended as often as listed, tokens
+ * past row Qc attend nothing.  A token that attends no key writes zeros; keys
+ * without a slot get no weight; what masked keys and values hold, NaN
+ * included, reaches no row.  Rows of no sequence are left alone.
+ *   q, out [N, Hq, D] (strides qs, os), bf16 / f16, D in {64, 128}, at most 64
+ *   query heads per KV head, scale > 0; rows 16-byte aligned.
+ *   workspace: spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D, K)
+ *   bytes, 16-byte aligned, one call's own until it is done (long rows are
+ *   split over workgroups and joined from there).
+ */
+int64_t spruce_paged_attention_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t K);
+int spruce_paged_attention(const void* q, const int64_t qs[3], const void* k_pages, const int64_t kps[4],
+                           const void* v_pages, const int64_t vps[4], int64_t pages, int64_t page_size,
+                           const int32_t* page_table, int64_t table_stride, int64_t table_width,
+                           const int32_t* q_starts, const int32_t* kv_lens, int64_t S, int64_t N, int64_t Hq,
+                           int64_t Hkv, int64_t D, float scale, int dtype, const int32_t* idx, const int64_t is[4],
+                           int64_t Qc, int64_t K, void* out, const int64_t os[3], void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

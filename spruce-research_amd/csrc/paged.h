@@ -19,7 +19,7 @@ struct PagedBatch {
   const int32_t* q_starts;
   const int32_t* kv_lens;
   int S, N, page, pages;
-  int cap;         // positions the table holds: width * page, below 2^31
+  int cap;         // positions the table holds: width * page
   uint32_t magic;  // p / page == (p * magic) >> shift for p < 2^31
   int shift;
 };
@@ -37,7 +37,8 @@ inline int prepare_batch(PagedBatch& b, const int32_t* table, int64_t table_stri
   SPRUCE_REQUIRE(pages >= 0 && pages < (int64_t)1 << 31, "invalid page count %lld", (long long)pages);
   SPRUCE_REQUIRE(width >= 0 && table_stride >= width, "page_table rows (%lld) overlap (stride %lld)",
                  (long long)width, (long long)table_stride);
-  SPRUCE_REQUIRE(width < ((int64_t)1 << 31) / page, "page_table covers 2^31 positions or more");
+  // The kernels reach up to a tile past the last position in 32 bits.
+  SPRUCE_REQUIRE(width <= (((int64_t)1 << 31) - 1024) / page, "page_table covers 2^31 - 1024 positions or more");
   b.table = table;
   b.table_stride = table_stride;
   b.q_starts = q_starts;

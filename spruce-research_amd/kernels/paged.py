@@ -27,7 +27,7 @@ import torch
 import spruce_hip
 from kernels.rotary import _positions, _refuse_grad, _rotation, _weights
 
-__all__ = ["append_paged_kv"]
+__all__ = ["append_paged_kv", "paged_chunk_attention"]
 
 _I64X3 = ctypes.c_int64 * 3
 
@@ -110,4 +110,72 @@ def append_paged_kv(k, v, k_pages, v_pages, page_table, q_starts, kv_lens, *, qu
             spruce_hip.ptr(inv_freq), rotary_dim, code, factor, spruce_hip.ptr(q_weight), spruce_hip.ptr(k_weight),
             weight_code, eps, spruce_hip.stream_of(k))
     spruce_hip.check(rc, "spruce_paged_append")
+    return out
+
+
+def paged_chunk_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, scale, *, indices=None, out=None):
+    """Attention of the new tokens over their sequences' cached keys, their own
+    (already appended) included: a token at position p attends the positions up to p.
+
+    q ``[N,Hq,D]`` (bf16 or f16; any strides with a contiguous last dim and 16-byte
+    aligned rows); Hq a multiple of the pages' Hkv.  indices: optional int32
+    ``[S,Hkv,Qc,K]`` block lists; row b of a sequence lists the 64-key blocks
+    (of positions ``64 id .. 64 id + 63``) for its new tokens in the b-th
+    64-position block that these touch: the slice of a ``selected_blocks``
+    layer that belongs to the chunk.  Negative entries are padding, blocks
+    behind a token's own are ignored, duplicates attended as often as listed;
+    tokens past row Qc attend nothing.
+
+    Returns ``[N,Hq,D]`` (``out`` when given; rows of no sequence are left as they
+    were).  A token that attends no key gets zeros, a key without a page no
+    weight, and what masked keys and values hold reaches no row.
+    """
+    if q.dim() != 3 or k_pages.dim() != 4:
+        raise ValueError("q must be [N, Hq, D] and the pages [pages, Hkv, page_size, D]")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"the paged attention takes bfloat16 or float16, got {q.dtype}")
+    N, Hq, D = q.shape
+    S = _check_cache(k_pages, v_pages, page_table, q_starts, kv_lens, q)
+    pages, Hkv, page_size, _ = k_pages.shape
+    if D not in (64, 128):
+        raise ValueError(f"kernel supports head_dim 64 or 128, got {D}")
+    if k_pages.shape[3] != D:
+        raise ValueError("q and the pages must match in head_dim")
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError("query heads must be divisible by KV heads")
+    if q.stride(-1) != 1:
+        raise ValueError("q must have a contiguous final dimension")
+    if not 0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    Qc = K = 0
+    if indices is not None:
+        if indices.dim() != 4 or tuple(indices.shape[:2]) != (S, Hkv) or indices.dtype != torch.int32:
+            raise ValueError("indices must be int32 [S,Hkv,Qc,K]")
+        Qc, K = indices.shape[2:]
+        if Qc < 1 or K < 1:
+            raise ValueError("indices must hold a row and a column")
+        if indices.stride(-1) != 1 and K > 1:
+            raise ValueError("indices must have a contiguous final dimension")
+        if indices.device != q.device:
+            raise ValueError("indices must be on the same device as q")
+    if out is not None:
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1:
+            raise ValueError("out must match q in shape, dtype and device, with a contiguous final dimension")
+    _refuse_grad(q, k_pages, v_pages, out)
+    if not q.is_cuda:
+        raise RuntimeError("the paged HIP backend requires GPU tensors")
+    if out is None:
+        out = torch.empty((N, Hq, D), device=q.device, dtype=q.dtype)
+    lib = spruce_hip.lib()
+    need = lib.spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D, K)
+    work = torch.empty(need, device=q.device, dtype=torch.uint8)
+    with spruce_hip.on_device(q.device):
+        rc = lib.spruce_paged_attention(
+            spruce_hip.ptr(q), _I64X3(*q.stride()), spruce_hip.ptr(k_pages), spruce_hip.strides(k_pages),
+            spruce_hip.ptr(v_pages), spruce_hip.strides(v_pages), pages, page_size,
+            spruce_hip.ptr(page_table), page_table.stride(0), page_table.shape[1], spruce_hip.ptr(q_starts),
+            spruce_hip.ptr(kv_lens), S, N, Hq, Hkv, D, scale, spruce_hip.DTYPE_CODES[q.dtype],
+            spruce_hip.ptr(indices), None if indices is None else spruce_hip.strides(indices), Qc, K,
+            spruce_hip.ptr(out), _I64X3(*out.stride()), spruce_hip.ptr(work), need, spruce_hip.stream_of(q))
+    spruce_hip.check(rc, "spruce_paged_attention")
     return out

@@ -115,6 +115,9 @@ _SIGNATURES = {
         _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _i64, _i64, _i64, _i64, ctypes.c_int,
         _p, _STRIDES, _p, _STRIDES, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, ctypes.c_int, _p, _i64,
         ctypes.c_int, ctypes.c_float, _p, _p, ctypes.c_int, ctypes.c_float, _p],
+    "spruce_paged_attention": [
+        _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64,
+        ctypes.c_float, ctypes.c_int, _p, _STRIDES, _i64, _i64, _p, _STRIDES, _p, _i64, _p],
     "spruce_sparse_prefill_mask": [
         _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _i64,
         _i64, _i64, _i64, _i64, _i64, ctypes.c_float, ctypes.c_int, ctypes.c_int,
@@ -154,6 +157,8 @@ def lib():
         handle.spruce_kv_summary_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64]
         handle.spruce_select_flat_workspace_bytes.restype = _i64
         handle.spruce_select_flat_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64]
+        handle.spruce_paged_attention_workspace_bytes.restype = _i64
+        handle.spruce_paged_attention_workspace_bytes.argtypes = [_i64] * 6
         _lib = handle
     return _lib
 

@@ -1,0 +1,333 @@
+"""Attention of new tokens over a paged cache on the GPU against a plain form in
+64 bits, and the serving step (append, then attention) against the dense one.
+
+The bar of an output o = sum_j p_j v_j / sum_j p_j, with A = sum_j p_j |v_j| / sum_j p_j:
+  eps(type) / 2 * |o|      the output's rounding;
+  eps(type) / 2 * A        each weight's rounding to the matrix cores' type;
+  4 e A                    the 32-bit scores: e = 2^-24 (D + 4) max_j scale sum_d |q_d k_jd| (D products and
+                           sums, the scaling and the exponent's argument) + 2^-21 (the exponential and the sums
+                           of 32-bit weights), in numerator and denominator;
+and for float16 2^-25 (|o|'s smallest step) and 2^-25 sum_j |v_j| / sum_j p_j (weights below its
+smallest normal number, relative to the row's largest one).
+"""
+import pytest
+import torch
+
+from kernels.direct_index import direct_index_sparse_prefill
+from kernels.paged import append_paged_kv, paged_chunk_attention
+from kernels.rotary import rotary_frequencies, rotate_heads
+from test_rotary_gpu import make_batch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def make_cache(gen, total, Hkv, page, D, dtype, slot_major=True):
+    shape = (total, page, Hkv, D) if slot_major else (total, Hkv, page, D)
+    k, v = (torch.randn(shape, generator=gen, device=DEV).to(dtype) for _ in range(2))
+    return (k.transpose(1, 2), v.transpose(1, 2)) if slot_major else (k, v)
+
+
+def attend64(q, kp, vp, table, new, kv, scale, lists=None, starts=None):
+    """(o, bar) of every row of the sequences' tokens, in 64 bits; lists [S, Hkv, Qc, K] or None."""
+    page, Hkv, D = kp.shape[2], kp.shape[1], kp.shape[3]
+    Hq = q.shape[1]
+    G = Hq // Hkv
+    half = torch.finfo(q.dtype).eps / 2
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    bar = torch.zeros_like(out)
+    row = 0 if starts is None else None
+    for s, (n, m) in enumerate(zip(new, kv)):
+        at = row if starts is None else starts[s]
+        if starts is None:
+            row += n
+        if n == 0:
+            continue
+        keys = torch.arange(min(max(m, 0), table.shape[1] * page), device=q.device)
+        ids = table[s].long()[keys // page]
+        have = (ids >= 0) & (ids < kp.shape[0])
+        ids = torch.where(have, ids, 0)
+        pos = torch.arange(m - n, m, device=q.device)
+        for g in range(Hkv):
+            k = kp[ids, g, keys % page].double()
+            v = vp[ids, g, keys % page].double()
+            seen = have & (keys <= pos[:, None])
+            weight = seen.double()
+            if lists is not None:
+                base = (m - n) // 64
+                for i, p in enumerate(pos.tolist()):
+                    b = p // 64 - base
+                    listed = lists[s, g, b].tolist() if b < lists.shape[2] else []
+                    count = torch.zeros(len(keys) // 64 + 2, dtype=torch.float64)
+                    for j in listed:
+                        if 0 <= j <= p // 64:
+                            count[j] += 1
+                    weight[i] *= count.to(q.device)[keys // 64]
+            for h in range(g * G, (g + 1) * G):
+                x = q[at:at + n, h].double()
+                score = scale * x @ k.T
+                score = score.masked_fill(weight == 0, -torch.inf)
+                top = score.amax(-1, keepdim=True) if len(keys) else torch.zeros(n, 1, device=q.device).double()
+                top = torch.where(torch.isinf(top), 0.0, top)
+                p = (score - top).exp() * weight
+                total = p.sum(-1, keepdim=True)
+                safe = torch.where(weight[..., None] == 0, 0.0, v) if not bool(torch.isfinite(v).all()) else v
+                num = (p[..., None] * safe).sum(1) if safe.dim() == 3 else p @ safe
+                away = (p[..., None] * safe.abs()).sum(1) if safe.dim() == 3 else p @ safe.abs()
+                size = total.clamp(min=1e-300)
+                o = torch.where(total == 0, 0.0, num / size)
+                A = torch.where(total == 0, 0.0, away / size)
+                worst = scale * (x.abs() @ k.abs().T).masked_fill(weight == 0, 0.0)
+                worst = worst.amax(-1, keepdim=True) if len(keys) else torch.zeros_like(total)
+                e = 2.0 ** -24 * (D + 4) * worst + 2.0 ** -21
+                b = half * o.abs() * (1 + half) + A * (half + 4 * e)
+                if q.dtype == torch.float16:
+                    all_v = (weight[..., None] * safe.abs()).sum(1) if safe.dim() == 3 else weight @ safe.abs()
+                    b = b + 2.0 ** -25 * (1 + torch.where(total == 0, 0.0, all_v / size))
+                out[at:at + n, h], bar[at:at + n, h] = o, b
+    return out, bar
+
+
+def check(got, want, bar, what=""):
+    off = (got.double() - want).abs()
+    fine = (off <= bar) | (torch.isnan(got) & torch.isnan(want)) | (got.double() == want)
+    assert bool(fine.all()), (what, float((off - bar).nan_to_num(nan=9e9).max()), (~fine).nonzero()[:4].tolist())
+
+
+CASES = [
+    # new, kv, page, Hq, Hkv, D, slot_major
+    ([1], [1], 16, 8, 2, 128, True),
+    ([1], [517], 16, 8, 2, 128, True),
+    ([1, 1, 1, 1], [64, 65, 1, 2000], 32, 28, 4, 128, False),
+    ([1] * 70, [3 + 37 * s for s in range(70)], 16, 12, 2, 64, True),
+    ([4, 4, 1, 0, 3], [900, 4, 77, 50, 1500], 32, 16, 8, 64, True),
+    ([9, 2], [300, 4096], 48, 28, 4, 128, True),
+    ([5], [200], 1, 4, 4, 128, False),
+    ([3], [130], 7, 64, 1, 64, True),
+    ([64], [64], 64, 8, 2, 128, True),
+    ([97, 130], [97, 1000], 64, 28, 4, 128, True),
+    ([333], [5000], 128, 12, 2, 128, False),
+    ([65, 1, 700], [1000, 33, 700], 16, 16, 8, 64, True),
+    ([200], [64 * 20 + 13], 256, 5, 1, 128, True),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,kv,page,Hq,Hkv,D,slot_major", CASES)
+def test_attention(new, kv, page, Hq, Hkv, D, slot_major, dtype):
+    print(f"case new={new[:6]} kv={kv[:6]} page={page} {Hq}/{Hkv} D={D} {dtype}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(sum(new) + page)
+    table, starts, lens, total = make_batch(page, new, kv, page)
+    kp, vp = make_cache(gen, total, Hkv, page, D, dtype, slot_major)
+    N = sum(new) + 2
+    q = torch.randn(N, Hq + 1, D, generator=gen, device=DEV).to(dtype)[:, 1:]
+    out = torch.full((N, Hq, D), 5.0, device=DEV, dtype=dtype)
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5, out=out)
+    assert got is out and bool((out[-2:] == 5.0).all())
+    want, bar = attend64(q, kp, vp, table, new, kv, D ** -0.5)
+    check(out[:-2], want[:-2], bar[:-2])
+    again = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5)
+    assert torch.equal(again[:-2], out[:-2])
+
+
+def _lists(seed, new, kv, Hkv, K, empty=True):
+    """Random rows over all blocks: duplicates, padding anywhere, blocks behind the token's, empty rows."""
+    gen = torch.Generator().manual_seed(seed)
+    Qc = max((m - 1) // 64 - (m - n) // 64 + 1 for n, m in zip(new, kv) if n)
+    nb = max((m + 63) // 64 for m in kv)
+    idx = torch.randint(-2, nb + 2, (len(new), Hkv, Qc, K), generator=gen, dtype=torch.int32)
+    if empty:
+        idx[0, 0, 0] = -1
+    return idx
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,kv,page,Hq,Hkv,D,K", [
+    ([1], [700], 16, 8, 2, 128, 4),
+    ([1, 1, 5], [64, 2000, 66], 32, 28, 4, 128, 9),
+    ([64], [640], 64, 8, 2, 64, 3),
+    ([130], [1000], 64, 28, 4, 128, 6),
+    ([300, 77], [900, 77], 48, 12, 2, 128, 40),
+    ([200], [3000], 128, 16, 8, 64, 1),
+])
+def test_listed_blocks(new, kv, page, Hq, Hkv, D, K, dtype):
+    print(f"case new={new} kv={kv} page={page} {Hq}/{Hkv} D={D} K={K} {dtype}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(sum(new) + page)
+    table, starts, lens, total = make_batch(page, new, kv, page)
+    kp, vp = make_cache(gen, total, Hkv, page, D, dtype)
+    q = torch.randn(sum(new), Hq, D, generator=gen, device=DEV).to(dtype)
+    idx = _lists(K, new, kv, Hkv, K)
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5, indices=idx.to(DEV))
+    want, bar = attend64(q, kp, vp, table, new, kv, D ** -0.5, idx)
+    check(got, want, bar)
+    # Rows that the lists do not reach attend nothing.
+    short = idx[:, :, :1].to(DEV)
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5, indices=short)
+    want, bar = attend64(q, kp, vp, table, new, kv, D ** -0.5, short.cpu())
+    check(got, want, bar)
+
+
+@pytest.mark.parametrize("new", [1, 5, 70])
+def test_nothing_of_masked_keys_gets_through(new):
+    # Stale slots behind a sequence's end, other pages and later tokens of the chunk hold NaN and infinities.
+    page, Hkv, D = 16, 2, 128
+    for dtype in (torch.bfloat16, torch.float16):
+        for kv in (new, 200, 1000 + new):
+            if kv < new:
+                continue
+            gen = torch.Generator(device=DEV).manual_seed(kv)
+            table, starts, lens, total = make_batch(kv, [new], [kv], page)
+            kp, vp = make_cache(gen, total, Hkv, page, D, dtype)
+            q = torch.randn(new, 8, D, generator=gen, device=DEV).to(dtype)
+            pos = torch.arange(total * page, device=DEV).view(total, page)
+            own = torch.full((total, page), -1, device=DEV)
+            for i, t in enumerate(table[0].tolist()):
+                own[t] = i * page + pos[0]
+            stale = (own < 0) | (own >= kv)
+            kp.transpose(1, 2)[stale] = float("nan")
+            vp.transpose(1, 2)[stale] = float("inf")
+            last = own == kv - 1           # the last token sees itself alone
+            if new > 1:
+                kp.transpose(1, 2)[last] = float("nan")
+                vp.transpose(1, 2)[last] = float("-inf")
+            got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5)
+            assert bool(torch.isfinite(got[:-1] if new > 1 else got).all()), (new, kv, dtype)
+            if new > 1:
+                assert bool(torch.isnan(got[-1]).all())
+            clean_k, clean_v = kp.nan_to_num(0.0), vp.nan_to_num(0.0, 0.0, 0.0)
+            want, bar = attend64(q, clean_k, clean_v, table, [new], [kv], D ** -0.5)
+            keep = slice(0, new - 1) if new > 1 else slice(0, 1)
+            check(got[keep], want[keep], bar[keep], (new, kv, dtype))
+
+
+def test_lengths_that_do_not_fit_and_missing_pages():
+    page, Hkv, D, dtype = 16, 2, 64, torch.bfloat16
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    table, _, _, total = make_batch(9, [1, 1, 1, 1], [96, 96, 96, 96], page)
+    kp, vp = make_cache(gen, total, Hkv, page, D, dtype)
+    table[1, 2] = -1
+    table[1, 5] = total
+    table[2] = -5                       # no page at all: zeros
+    # Rows 0-2 and 63.. belong to no sequence; sequence 0 has 20 new tokens and 5 positions, sequence 3 more
+    # positions than its table row.
+    new, kv, starts = [20, 20, 10, 10], [5, 90, 50, 120], [3, 23, 43, 53]
+    q = torch.randn(66, 4, D, generator=gen, device=DEV).to(dtype)
+    out = torch.full_like(q, 5.0)
+    paged_chunk_attention(q, kp, vp, table, torch.tensor([*starts, 63], dtype=torch.int32, device=DEV),
+                          torch.tensor(kv, dtype=torch.int32, device=DEV), 0.125, out=out)
+    want, bar = attend64(q, kp, vp, table, new, kv, 0.125, starts=starts)
+    check(out[3:63], want[3:63], bar[3:63])
+    assert bool((out[:3] == 5.0).all()) and bool((out[63:] == 5.0).all())
+    assert bool((out[3:18] == 0).all()) and bool((out[43:53] == 0).all())
+    # No position, no page and no column at all.
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    two = torch.tensor([0, 2], dtype=torch.int32, device=DEV)
+    for t in (table[:1], table[:1, :0]):
+        assert bool((paged_chunk_attention(q[:2], kp, vp, t, two, none, 0.125) == 0).all())
+    empty = torch.empty(0, Hkv, page, D, device=DEV, dtype=dtype)
+    assert bool((paged_chunk_attention(q[:2], empty, empty, table[:1], two, none + 9, 0.125) == 0).all())
+    assert paged_chunk_attention(q[:0], kp, vp, table[:1], none.repeat(2), none, 0.125).shape == (0, 4, D)
+
+
+def test_hostile_starts_stay_in_bounds():
+    # Starts that overlap, go backwards or leave the packed rows: rows are unspecified, memory behind them is not.
+    page, dtype = 16, torch.bfloat16
+    table, _, _, total = make_batch(1, [1] * 4, [80] * 4, page)
+    kp, vp = make_cache(torch.Generator(device=DEV).manual_seed(0), total, 2, page, 64, dtype)
+    q = torch.randn(40, 4, 64, device=DEV, dtype=dtype)
+    lens = torch.tensor([80, 80, -3, 2 ** 31 - 1], dtype=torch.int32, device=DEV)
+    for starts in ([0, 40, 0, 40, 0], [-7, 100, 3, 2 ** 31 - 1, 5], [40, 30, 20, 10, 0], [-(2 ** 31), 0, 10, 20, 900]):
+        big = torch.full((60, 4, 64), 5.0, device=DEV, dtype=dtype)
+        at = torch.tensor(starts, dtype=torch.int32, device=DEV)
+        paged_chunk_attention(q, kp, vp, table, at, lens, 0.125, out=big[10:50])
+        assert bool((big[:10] == 5.0).all()) and bool((big[50:] == 5.0).all())
+        kq, vq = (torch.full((total + 2, 2, page, 64), 5.0, device=DEV, dtype=dtype) for _ in range(2))
+        append_paged_kv(q[:, :2], q[:, 2:], kq[1:-1], vq[1:-1], table, at, lens)
+        for x in (kq, vq):
+            assert bool((x[0] == 5.0).all()) and bool((x[-1] == 5.0).all())
+
+
+def test_extreme_scores():
+    # Scores far apart (one key takes all), all equal, and all far below zero.
+    page, D = 32, 64
+    table, starts, lens, total = make_batch(3, [2, 1], [400, 300], page)
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    kp, vp = make_cache(gen, total, 1, page, D, torch.bfloat16)
+    q = torch.randn(3, 4, D, generator=gen, device=DEV).to(torch.bfloat16)
+    for f in (200.0, 0.0, -200.0):
+        got = paged_chunk_attention((q.abs() * f).to(torch.bfloat16), kp.abs(), vp, table, starts, lens, 1.0)
+        want, bar = attend64((q.abs() * f).to(torch.bfloat16), kp.abs(), vp, table, [2, 1], [400, 300], 1.0)
+        check(got, want, bar, f)
+
+
+def test_streams_graphs_and_two_calls_at_once():
+    page, Hkv, D, dtype = 16, 4, 128, torch.bfloat16
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    new, kv = [1] * 6, [33, 1200, 77, 5000, 16, 2048]
+    table, starts, lens, total = make_batch(6, new, [5000] * 6, page)
+    lens = torch.tensor(kv, dtype=torch.int32, device=DEV)
+    kp, vp = make_cache(gen, total, Hkv, page, D, dtype)
+    q = [torch.randn(6, 28, D, generator=gen, device=DEV).to(dtype) for _ in range(2)]
+    want = [paged_chunk_attention(x, kp, vp, table, starts, lens, 0.08) for x in q]
+    streams = [torch.cuda.Stream() for _ in q]
+    got = []
+    for stream, x in zip(streams, q):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            got.append(paged_chunk_attention(x, kp, vp, table, starts, lens, 0.08))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # Two graphs over the same tensors; replays follow the lengths that the tensors then hold.
+    k, v = (torch.randn(6, Hkv, D, generator=gen, device=DEV).to(dtype) for _ in range(2))
+    inv_freq = rotary_frequencies(D, device=DEV)[0]
+    graphs, outs = [], []
+    for x in q:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            turned = append_paged_kv(k, v, kp, vp, table, starts, lens, query=x, inv_freq=inv_freq)
+            outs.append(paged_chunk_attention(turned, kp, vp, table, starts, lens, 0.08))
+        graphs.append(graph)
+    for step in range(3):
+        lens.copy_(torch.tensor([m + 700 * step for m in kv[:1]] + [m + step for m in kv[1:3]] + [5000 - step] + kv[4:],
+                                dtype=torch.int32))
+        for i in (0, 1):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            turned = append_paged_kv(k, v, kp, vp, table, starts, lens, query=q[i], inv_freq=inv_freq)
+            eager = paged_chunk_attention(turned, kp, vp, table, starts, lens, 0.08)
+            assert torch.equal(outs[i], eager), (step, i)
+            k.mul_(1.01)
+
+
+def test_chunks_and_tokens_agree_with_the_whole_prompt():
+    # A prompt taken in ragged chunks and then token by token, appended and attended, against the dense
+    # operators over the whole of it: norms, rotation and block lists included.
+    T, Hq, Hkv, D, page, dtype = 333, 8, 2, 128, 16, torch.bfloat16
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    q, k, v = (torch.randn(T, H, D, generator=gen, device=DEV).to(dtype) for H in (Hq, Hkv, Hkv))
+    qw, kw = (1 + 0.1 * torch.randn(D, generator=gen, device=DEV) for _ in range(2))
+    inv_freq, factor = rotary_frequencies(D, 1e6, scaling="yarn", factor=4.0, original_length=128, device=DEV)
+    turn = dict(inv_freq=inv_freq, factor=factor, q_weight=qw, k_weight=kw)
+    nb = (T + 63) // 64
+    idx = torch.full((1, Hkv, nb, 3), -1, dtype=torch.int32)
+    for b in range(nb):
+        idx[0, :, b, :2] = torch.tensor([0, b]) if b else torch.tensor([0, -1])
+        idx[0, 1, b, 2] = b // 2 if b > 3 else -1
+    idx = idx.to(DEV)
+    qr, kr = rotate_heads(q[None].transpose(1, 2), k[None].transpose(1, 2), torch.arange(T, device=DEV), **turn)
+    whole = direct_index_sparse_prefill(qr, kr, v[None].transpose(1, 2), idx, D ** -0.5)[0]
+    table, _, _, total = make_batch(1, [T], [T], page)
+    kp, vp = (torch.zeros(total, page, Hkv, D, device=DEV, dtype=dtype).transpose(1, 2) for _ in range(2))
+    parts, at = [], 0
+    for n in (130, 100, 60, 40, 1, 1, 1):
+        starts = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+        lens = torch.tensor([at + n], dtype=torch.int32, device=DEV)
+        turned = append_paged_kv(k[at:at + n], v[at:at + n], kp, vp, table, starts, lens, query=q[at:at + n], **turn)
+        assert torch.equal(turned, qr[0].transpose(0, 1)[at:at + n])
+        rows = idx[:, :, at // 64:(at + n - 1) // 64 + 1]
+        parts.append(paged_chunk_attention(turned, kp, vp, table, starts, lens, D ** -0.5, indices=rows))
+        at += n
+    assert at == T
+    want, bar = attend64(qr[0].transpose(0, 1), kp, vp, table, [T], [T], D ** -0.5, idx.cpu())
+    check(torch.cat(parts), want, bar)
+    check(whole, want, bar)       # the dense operator's own sums obey the same bar

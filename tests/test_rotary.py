@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import spruce_hip
-from kernels.paged import append_paged_kv
+from kernels.paged import append_paged_kv, paged_chunk_attention
 from kernels.rotary import rotary_frequencies, rotate_heads
 
 
@@ -172,3 +172,58 @@ def test_page_division_by_multiplication():
             for p in (k * page - 1, k * page, k * page + 1, k * page + page - 1, top):
                 if 0 <= p <= top:
                     assert (p * magic) >> (31 + shift) == p // page, (page, p)
+
+
+def _attend(N=3, Hq=4, Hkv=2, D=64, dtype=torch.bfloat16, S=2, W=4, page=16, scale=0.1, indices=None, out=None,
+            **change):
+    args = dict(q=torch.zeros(N, Hq, D, dtype=dtype), k_pages=torch.zeros(5, Hkv, page, D, dtype=dtype),
+                v_pages=torch.zeros(5, Hkv, page, D, dtype=dtype), page_table=torch.zeros(S, W, dtype=torch.int32),
+                q_starts=torch.zeros(S + 1, dtype=torch.int32), kv_lens=torch.zeros(S, dtype=torch.int32))
+    args.update(change)
+    return paged_chunk_attention(scale=scale, indices=indices, out=out, **args)
+
+
+def test_attention_refusals():
+    bf, i32 = torch.bfloat16, torch.int32
+    for kwargs, message in ((dict(D=96), "head_dim 64 or 128"), (dict(dtype=torch.float32), "bfloat16 or float16"),
+                            (dict(Hq=3), "divisible"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
+                            (dict(scale=float("nan")), "scale"),
+                            (dict(q=torch.zeros(3, 64, dtype=bf)), "q must be"),
+                            (dict(q=torch.zeros(3, 64, 4, dtype=bf).transpose(1, 2)), "contiguous final"),
+                            (dict(k_pages=torch.zeros(5, 2, 16, 128, dtype=bf),
+                                  v_pages=torch.zeros(5, 2, 16, 128, dtype=bf)), "match in head_dim"),
+                            (dict(kv_lens=torch.zeros(3, dtype=i32)), "kv_lens"),
+                            (dict(indices=torch.zeros(2, 2, 1, 3)), "indices must be int32"),
+                            (dict(indices=torch.zeros(2, 1, 1, 3, dtype=i32)), "indices must be int32"),
+                            (dict(indices=torch.zeros(2, 2, 1, 0, dtype=i32)), "a row and a column"),
+                            (dict(indices=torch.zeros(2, 2, 3, 4, dtype=i32).transpose(2, 3)), "contiguous final"),
+                            (dict(out=torch.zeros(3, 4, 64)), "out must match")):
+        with pytest.raises(ValueError, match=message):
+            _attend(**kwargs)
+    with pytest.raises(RuntimeError, match="requires GPU tensors"):
+        _attend()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        _attend(q=torch.zeros(3, 4, 64, dtype=bf, requires_grad=True))
+
+
+def test_attention_entry_point_refuses_before_the_launch():
+    lib, fake = spruce_hip.lib(), ctypes.c_void_p(1 << 20)
+    need = lib.spruce_paged_attention_workspace_bytes(8, 2, 4, 2, 128, 0)
+    assert need > 0 and need % 16 == 0
+
+    def call(D=128, dtype=0, Hq=4, scale=0.1, qs=(512, 128, 1), K=0, idx=None, is_=(1, 1, 1, 1), Qc=1, ws=fake,
+             ws_bytes=need, width=4, N=8, q=fake):
+        return lib.spruce_paged_attention(q, _st(*qs), fake, _st(4096, 2048, 128, 1), fake, _st(4096, 2048, 128, 1), 9,
+                                          16, fake, 4, width, fake, fake, 2, N, Hq, 2, D, scale, dtype, idx, _st(*is_),
+                                          Qc, K, fake, _st(512, 128, 1), ws, ws_bytes, None)
+    for kwargs, message in ((dict(D=96), "head_dim 64 or 128"), (dict(dtype=2), "bf16 or f16"),
+                            (dict(Hq=5), "divisible"), (dict(Hq=130), "at most 64"), (dict(scale=0.0), "scale"),
+                            (dict(scale=float("inf")), "scale"), (dict(qs=(512, 128, 2)), "contiguous final"),
+                            (dict(qs=(500, 128, 1)), "16-byte"), (dict(K=4), "indices"),
+                            (dict(K=4, idx=fake, is_=(1, 1, 1, 2)), "contiguous final"), (dict(K=-1), "list width"),
+                            (dict(ws=None), "workspace"), (dict(ws_bytes=need - 4), "workspace too small"),
+                            (dict(ws=ctypes.c_void_p((1 << 20) + 4)), "workspace must be 16-byte"),
+                            (dict(width=5), "overlap"), (dict(N=-1), "token count"), (dict(q=None), "non-null")):
+        assert call(**kwargs) == -1, kwargs
+        assert message in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
+    assert call(N=0) == 0
