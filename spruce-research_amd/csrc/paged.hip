@@ -5,7 +5,16 @@
 //
 // Rows of one (sequence, KV head) are packed token by token, head by head
 // (row r: token r / G, query head g G + r % G), so few tokens of a wide group
-// fill a matrix tile as many tokens of a narrow one do.
+// fill a matrix tile as many tokens of a narrow one do.  What bounds a row tile
+// turns with its height: up to 64 packed rows (a decoding step, a few drafted
+// tokens) each key is read for few products and memory is the bound; above,
+// the matrix cores are.  A workgroup of eight waves works on one unit (rows of
+// a sequence and KV head against a range of its keys) in one of two ways:
+//   few rows    32 rows; every wave takes 32 keys at a time of its own,
+//               without a barrier until the waves' sums are joined;
+//   many rows   256 rows, 32 a wave; all waves share each 64-key block in LDS.
+// One launch holds the units of both kinds, since the lengths that tell them
+// apart are on the device: a batch may mix them.
 #include "attention_impl.h"
 #include "paged.h"
 
@@ -26,22 +35,36 @@ struct PagedAttn {
   const int32_t* idx;  // block lists [S, Hkv, Qc, K], or null
   int64_t is[3];
   int Qc, K;
-  float* part_o;   // [units][kRows][D]
-  float* part_ml;  // [units][2][kRows]
-  int grid;        // units that have a workgroup and a partial slot
+  float* part_o;   // [groups][32 * D], a 32 x 32 accumulator's order
+  float* part_ml;  // [groups][2][32]
+  int many_units, few_units;  // units of either kind that have partial slots
 };
 
-constexpr int kRows = 32;      // rows of a unit
-constexpr int kKeys = 32;      // keys a wave takes at a time
-constexpr int kWaves = 4;      // waves of a workgroup, each with keys of its own
-constexpr int kStep = kKeys * kWaves;
-constexpr int kSlots = 512;    // units that the splits aim at: two workgroups a CU
-constexpr int kMinSteps = 2;   // steps below which a row's keys are not split further
+constexpr int kWaves = 8;
+constexpr int kFewRows = 64;     // packed rows of a sequence up to which it takes the few-row way
+constexpr int kCus = 256;
+constexpr int kFewSlots = 512;   // few-row units that the splits aim at
+constexpr int kManySlots = 768;  // and the most many-row units that splitting may make
+
+// Unit shapes: rows of a unit, and keys of a step, its unit of work.
+struct Few {
+  static constexpr bool many = false;
+  static constexpr int rows = 32, step = 32 * kWaves;
+};
+struct Many {
+  static constexpr bool many = true;
+  static constexpr int rows = 32 * kWaves, step = kBlock;
+};
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
+// 16 bytes of a row.  A native vector: copies of the struct uint4 between
+// memory spaces have kept arrays of it out of registers.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ u32x4 load16(const uint16_t* p) { return *reinterpret_cast<const u32x4*>(p); }
 
 template <bool F16>
-__device__ __forceinline__ f32x4v mfma16x16x32(uint4 a, uint4 b, f32x4v c) {
+__device__ __forceinline__ f32x4v mfma16x16x32(u32x4 a, u32x4 b, f32x4v c) {
   if constexpr (F16)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
                                                   0, 0);
@@ -53,9 +76,6 @@ __device__ __forceinline__ f32x4v mfma16x16x32(uint4 a, uint4 b, f32x4v c) {
 // The same value in every lane, for the compiler too: it must branch on the
 // scalar unit around matrix instructions, which run whatever EXEC holds.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  return (int64_t)(((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x));
-}
 
 // Sum of v over the lanes up to this one (row shifts within 16 lanes, then
 // the rows' last lanes broadcast onward).
@@ -69,12 +89,40 @@ __device__ __forceinline__ int wave_prefix(int v) {
   return v;
 }
 
-// The work of one sequence: row tiles per KV head, and 128-key steps of each.
+// A key of a tile, or the last key below `end` where it lies past that.
+__device__ __forceinline__ int nearest(int key, int end) { return key < end ? key : end - 1; }
+
+// A position as an int: -1 for any below zero, the largest int for any past it.
+__device__ __forceinline__ int clip(int64_t pos) {
+  return pos < 0 ? -1 : (pos < 0x7fffffff ? (int)pos : 0x7fffffff);
+}
+
+// The work of one sequence: its kind, row tiles per KV head, and key steps of each.
 struct SeqWork {
-  int n;        // new tokens
+  int n;         // new tokens
   int64_t pos0;  // position of the first
-  int tiles, steps, sub;
+  bool many;
+  int tiles, steps;
+  int sub, rows;  // with lists: tiles of one 64-position block, and rows of one
 };
+
+template <typename SHAPE>
+__device__ __forceinline__ void tile_sequence(const PagedAttn& p, int s, SeqWork& w) {
+  if (p.idx != nullptr) {
+    const int64_t b0 = w.pos0 >> 6, b1 = (w.pos0 + w.n - 1) >> 6;
+    const int rows = (w.n < kBlock ? w.n : kBlock) * p.G;
+    w.sub = (rows + SHAPE::rows - 1) / SHAPE::rows;
+    w.rows = ((rows + 31) / 32 + w.sub - 1) / w.sub * 32;  // shared out evenly
+    w.tiles = (int)(b1 - b0 + 1) * w.sub;
+    w.steps = (int)(((int64_t)p.K * kBlock + SHAPE::step - 1) / SHAPE::step);
+  } else {
+    w.sub = 1;
+    w.rows = SHAPE::rows;
+    w.tiles = (int)(((int64_t)w.n * p.G + SHAPE::rows - 1) / SHAPE::rows);
+    w.steps = (keys_of(p.batch, s) + SHAPE::step - 1) / SHAPE::step;
+  }
+  if (w.steps < 1) w.steps = 1;
+}
 
 __device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
   SeqWork w{};
@@ -83,107 +131,191 @@ __device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
   w.n = e > a ? e - a : 0;
   // Positions go by the lengths as given; only what they address is bounded.
   w.pos0 = (int64_t)p.batch.kv_lens[s] - ((int64_t)p.batch.q_starts[s + 1] - p.batch.q_starts[s]) +
-           (a - p.batch.q_starts[s]);
+           ((int64_t)a - p.batch.q_starts[s]);
   if (w.n == 0) return w;
-  if (p.idx != nullptr) {
-    const int64_t b0 = w.pos0 >> 6, b1 = (w.pos0 + w.n - 1) >> 6;
-    const int tok = w.n < kBlock ? w.n : kBlock;
-    w.sub = (tok * p.G + kRows - 1) / kRows;
-    w.tiles = (int)(b1 - b0 + 1) * w.sub;
-    w.steps = (int)(((int64_t)p.K * kBlock + kStep - 1) / kStep);
-  } else {
-    w.sub = 1;
-    w.tiles = (int)(((int64_t)w.n * p.G + kRows - 1) / kRows);
-    w.steps = (keys_of(p.batch, s) + kStep - 1) / kStep;
-  }
-  if (w.steps < 1) w.steps = 1;
+  w.many = (int64_t)w.n * p.G > kFewRows;
+  if (w.many)
+    tile_sequence<Many>(p, s, w);
+  else
+    tile_sequence<Few>(p, s, w);
   return w;
 }
 
-// Keys are split so that about kSlots units of equal size come out: a unit
-// takes `per` steps of its row tile at most.  Every workgroup works this out
-// from the lengths, 64 sequences at a time.
-__device__ __forceinline__ int steps_per_unit(const PagedAttn& p, int lane) {
-  int64_t all = 0;
+// How many steps a unit takes of its row tile at most, for either kind; every
+// workgroup works this out from the lengths, 64 sequences at a time.
+struct Pace {
+  int many, few;
+};
+
+__device__ __forceinline__ Pace choose_pace(const PagedAttn& p, int lane) {
+  int64_t few = 0, many = 0, tiles = 0;
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
     const SeqWork w = sequence_work(p, s0 + lane);
-    all += (int64_t)w.tiles * w.steps;
+    const int64_t work = (int64_t)w.tiles * w.steps;
+    few += w.many ? 0 : work;
+    many += w.many ? work : 0;
+    tiles += w.many ? w.tiles : 0;
   }
 #pragma unroll
-  for (int m = 1; m < 64; m *= 2) all += __shfl_xor(all, m);
-  const int64_t per = (all * p.Hkv + kSlots - 1) / kSlots;
-  return per < kMinSteps ? kMinSteps : uniform((int)(per < (1 << 30) ? per : (1 << 30)));
+  for (int m = 1; m < 64; m *= 2) {
+    few += __shfl_xor(few, m);
+    many += __shfl_xor(many, m);
+    tiles += __shfl_xor(tiles, m);
+  }
+  Pace pace;
+  // Few rows: about kFewSlots units of equal size.
+  const int64_t per = (few * p.Hkv + kFewSlots - 1) / kFewSlots;
+  pace.few = uniform((int)(per < 1 ? 1 : (per < (1 << 30) ? per : 1 << 30)));
+  // Many rows: lane l weighs l + 1 splits of the average tile.  A split costs
+  // its blocks and a fixed part worth about eight more (first loads, last
+  // reduction, store) and four for its part in the join; CUs take one unit
+  // at a time.
+  const int64_t units = tiles * p.Hkv;
+  pace.many = 1 << 30;
+  if (units > 0 && units * 2 <= kManySlots) {
+    const int avg = (int)(many / tiles);
+    const int ns = lane + 1, part = (avg + ns - 1) / ns;
+    const int rounds = (int)((units * ns + kCus - 1) / kCus);
+    uint32_t cost = (uint32_t)rounds * (uint32_t)(part + 8 + (ns > 1 ? 4 : 0));
+    if (units * ns > kManySlots || ns > avg || cost >= 1u << 25) cost = (1u << 25) - 1;
+    uint32_t best = cost << 6 | (uint32_t)lane;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const uint32_t o = (uint32_t)__shfl_xor((int)best, m);
+      best = o < best ? o : best;
+    }
+    const int n = (int)(best & 63) + 1;
+    pace.many = uniform(n == 1 ? 1 << 30 : (avg + n - 1) / n);
+  }
+  return pace;
 }
 
 struct Unit {
-  int s, tile, g, split, splits, first;  // first: unit of split 0 of this tile and head
-  SeqWork w;
+  int s, tile, g, split, splits;
+  int first, stride;  // unit of split 0 of this tile and head, and from split to split
+  int n, steps, sub, rows;
+  int64_t pos0;
 };
 
-// The unit `want` counted over units (BY_TILE false), or the (tile, head)
-// `want` counted without the splits.  false behind the last.
-template <bool BY_TILE>
-__device__ __forceinline__ bool find_unit(const PagedAttn& p, int want, int per, int lane, Unit& u) {
+// The unit `want` of one kind, counted with its splits (BY_TILE false), or
+// the (tile, head) `want` counted without.  Past the last: false, and `want`
+// less by how many there are.
+template <bool MANY, bool BY_TILE>
+__device__ __forceinline__ bool find_unit(const PagedAttn& p, int& want, int per, int lane, Unit& u) {
   int units = 0, tiles = 0;
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
     const SeqWork w = sequence_work(p, s0 + lane);
+    const bool kind = w.many == MANY;
     const int splits = (w.steps + per - 1) / per;
-    const int mt = w.tiles * p.Hkv, mu = mt * splits;
+    const int mt = kind ? w.tiles * p.Hkv : 0, mu = mt * splits;
     const int pt = wave_prefix(mt), pu = wave_prefix(mu);
-    const int mine = (BY_TILE ? tiles + pt : units + pu);
+    const int mine = BY_TILE ? tiles + pt : units + pu;
     const uint64_t past = __ballot(mine > want);
     if (past) {
       const int l = __builtin_ctzll(past);
       const int th = __builtin_amdgcn_readlane(mt, l);
       u.s = s0 + l;
       u.splits = __builtin_amdgcn_readlane(splits, l);
-      u.w.n = __builtin_amdgcn_readlane(w.n, l);
-      u.w.pos0 = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w.pos0 >> 32), l) << 32) |
-                           (uint32_t)__builtin_amdgcn_readlane((int)w.pos0, l));
-      u.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
-      u.w.steps = __builtin_amdgcn_readlane(w.steps, l);
-      u.w.sub = __builtin_amdgcn_readlane(w.sub, l);
+      u.n = __builtin_amdgcn_readlane(w.n, l);
+      u.pos0 = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w.pos0 >> 32), l) << 32) |
+                         (uint32_t)__builtin_amdgcn_readlane((int)w.pos0, l));
+      u.steps = __builtin_amdgcn_readlane(w.steps, l);
+      u.sub = __builtin_amdgcn_readlane(w.sub, l);
+      u.rows = __builtin_amdgcn_readlane(w.rows, l);
       const int before = units + __builtin_amdgcn_readlane(pu, l) - th * u.splits;
       const int in = want - (BY_TILE ? tiles + __builtin_amdgcn_readlane(pt, l) - th : before);
-      if (in < 0 || in >= th * (BY_TILE ? 1 : u.splits)) return false;  // starts that overlap
-      // Within a sequence: split slowest, then tile, head fastest.
+      if (th <= 0 || in < 0 || in >= th * (BY_TILE ? 1 : u.splits)) return false;  // starts that overlap
+      // Within a sequence: split slowest, then tile, head fastest: the eight
+      // XCDs take units in turn, so each L2 serves one head where Hkv divides 8.
       u.split = BY_TILE ? 0 : in / th;
       const int r = in - u.split * th;
       u.tile = r / p.Hkv;
       u.g = r - u.tile * p.Hkv;
       u.first = before + r;
+      u.stride = th;
       return true;
     }
     tiles += __builtin_amdgcn_readlane(pt, 63);
     units += __builtin_amdgcn_readlane(pu, 63);
   }
+  want -= BY_TILE ? tiles : units;
   return false;
 }
 
-// Rows [row0, row0 + rows) of the tile in the sequence's packed rows, and the
-// block list that they share.
+// Rows [row0, row0 + rows) of a unit in the sequence's packed rows, the block
+// list that they share, and the keys below `end` that the last of them sees.
 struct TileRows {
-  int row0, rows;
+  int row0, rows, end;
   const int32_t* list;
 };
 
 __device__ __forceinline__ TileRows tile_rows(const PagedAttn& p, const Unit& u) {
   TileRows t{};
   if (p.idx == nullptr) {
-    t.row0 = u.tile * kRows;
-    const int left = u.w.n * p.G - t.row0;
-    t.rows = left < kRows ? left : kRows;
-    return t;
+    // The last tiles see the most keys: they come first.
+    const int tiles = u.stride / p.Hkv;
+    t.row0 = (tiles - 1 - u.tile) * u.rows;
+    const int left = u.n * p.G - t.row0;
+    t.rows = left < u.rows ? left : u.rows;
+  } else {
+    const int bi = u.tile / u.sub, sub = u.tile - bi * u.sub;
+    const int64_t lo = (((u.pos0 >> 6) + bi) << 6) - u.pos0;
+    const int t0 = lo < 0 ? 0 : (int)lo;
+    const int t1 = lo + kBlock < u.n ? (int)(lo + kBlock) : u.n;
+    t.row0 = t0 * p.G + sub * u.rows;
+    const int left = t1 * p.G - t.row0;
+    t.rows = left < 0 ? 0 : (left < u.rows ? left : u.rows);
+    t.list = bi < p.Qc ? p.idx + (int64_t)u.s * p.is[0] + (int64_t)u.g * p.is[1] + (int64_t)bi * p.is[2] : nullptr;
   }
-  const int bi = u.tile / u.w.sub, sub = u.tile - bi * u.w.sub;
-  const int64_t lo = (((u.w.pos0 >> 6) + bi) << 6) - u.w.pos0;
-  const int t0 = lo < 0 ? 0 : (int)lo;
-  const int t1 = lo + kBlock < u.w.n ? (int)(lo + kBlock) : u.w.n;
-  t.row0 = t0 * p.G + sub * kRows;
-  const int left = t1 * p.G - t.row0;
-  t.rows = left < 0 ? 0 : (left < kRows ? left : kRows);
-  t.list = bi < p.Qc ? p.idx + (int64_t)u.s * p.is[0] + (int64_t)u.g * p.is[1] + (int64_t)bi * p.is[2] : nullptr;
+  const int64_t last = u.pos0 + (t.row0 + t.rows - 1) / p.G;
+  t.end = last < 0 || p.batch.pages == 0 ? 0 : (last + 1 < p.batch.cap ? (int)(last + 1) : p.batch.cap);
   return t;
+}
+
+// The first keys of the tiles of KEYS keys that a wave (or a workgroup) takes,
+// in order: items base, base + stride .. below hi of the row's keys, or of its
+// list's blocks without those that are padding or in every row's future.  64
+// items are looked up at once, one a lane.
+template <int KEYS>
+struct KeyWalk {
+  const int32_t* list;
+  int base, stride, hi, end, lane, found;
+  bool lists;
+  uint64_t bits;
+  __device__ __forceinline__ void init(const PagedAttn& p, const TileRows& t, int base_, int stride_, int hi_, int lane_) {
+    lists = p.idx != nullptr;
+    list = t.list;
+    base = base_;
+    stride = stride_;
+    hi = lists && list == nullptr ? 0 : hi_;
+    end = t.end;
+    lane = lane_;
+    bits = 0;
+    found = -1;
+  }
+  __device__ __forceinline__ int next() {
+    while (bits == 0) {
+      if (base >= hi) return -1;
+      const int item = base + stride * lane;
+      int64_t key = (int64_t)item * KEYS;
+      if (lists && item < hi) {
+        const int id = list[KEYS == kBlock ? item : item >> 1];
+        key = id < 0 ? end : (int64_t)id * kBlock + (KEYS == kBlock ? 0 : (item & 1) * KEYS);
+      }
+      const bool ok = item < hi && key < end;
+      found = ok ? (int)key : -1;
+      bits = __ballot(ok);
+      base += 64 * stride;
+    }
+    const int l = __builtin_ctzll(bits);
+    bits &= bits - 1;
+    return __builtin_amdgcn_readlane(found, l);
+  }
+};
+
+// Where element (row, d) of a unit's 32-row group lies in its partial sums.
+__device__ __forceinline__ int part_at(int row, int d) {
+  return ((d >> 3) * 64 + row + 32 * ((d >> 2) & 1)) * 4 + (d & 3);
 }
 
 // x combined over the lanes l, l ^ 16, l ^ 32, l ^ 48.
@@ -200,95 +332,91 @@ __device__ __forceinline__ float quad_sum(float x) {
   return half_sum(__builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1));
 }
 
-// One unit: up to 32 packed rows against a range of 32-key tiles, the four
-// waves taking every fourth tile each without a barrier between them.
-// Memory bounds it: a key's 256 + 256 bytes meet at most 32 rows.  A wave's
-// K rows go from memory straight into the A operand of S^T = K Q^T (lane: key
-// l % 16, 16 bytes of d at 8 (l / 16) + 32 kk, so a load takes 64 bytes of each of 16
-// rows); V rows, loaded alike, pass through the wave's own LDS, whose
-// transposing read gives the A operand of O^T = V^T P^T; P^T, the B operand,
-// is S^T's accumulator as it lies (keys 4 (l / 16) + r).  The next tile's K
-// is in flight from the last S^T on, its V from the LDS write on.
+// Orders a wave's own LDS accesses, for the compiler; the hardware keeps them in order.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Zero, unknown to the compiler.
+__device__ __forceinline__ int opaque_zero() {
+  int z = 0;
+  asm volatile("" : "+v"(z));
+  return z;
+}
+
+template <int D>
+constexpr int few_lds_bytes() {
+  // The waves' V rows, or their O rows, 16 at a time; then maxima and sums.
+  constexpr int v = kWaves * 32 * (D + 8) * 2, o = kWaves * 16 * (D + 4) * 4;
+  return (v > o ? v : o) + kWaves * 2 * 32 * 4;
+}
+template <int D>
+constexpr int many_lds_bytes() {
+  return 2 * kBlock * ((D + 8) + (D + 32)) * 2;
+}
+
+// A few-row unit.  Memory bounds it: a key's 4 D bytes meet at most 32 rows.
+// A wave's K rows go from memory straight into the A operand of S^T = K Q^T
+// (lane: key l % 16, 16 bytes of d at 8 (l / 16) + 32 kk, so a load takes 64
+// bytes of each of 16 rows); V rows, loaded alike, pass through the wave's own
+// LDS, whose transposing read gives the A operand of O^T = V^T P^T; P^T, the B
+// operand, is S^T's accumulator as it lies (keys 4 (l / 16) + r).  The next
+// tile's K is in flight from the last S^T on, its V from the LDS write on.
 template <int D, bool F16>
-__global__ __launch_bounds__(kWaves * 64, 2) void paged_rows_kernel(const PagedAttn p) {
+__device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int unit, int per, char* smem) {
   constexpr int KK = D / 32;   // steps of S^T over d
   constexpr int DT = D / 16;   // 16-row tiles of O^T
   constexpr int VSTR = D + 8;  // V rows in LDS, 16-bit elements
   constexpr int OSTR = D + 4;  // O rows in LDS, floats
-  constexpr int kVBytes = kWaves * kKeys * VSTR * 2, kOBytes = kWaves * 16 * OSTR * 4;
-  __shared__ __attribute__((aligned(16))) char smem[kVBytes > kOBytes ? kVBytes : kOBytes];
-  __shared__ float ml[kWaves][2][kRows];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int l16 = lane & 15, g4 = lane >> 4;
+  float* ml = reinterpret_cast<float*>(smem + few_lds_bytes<D>() - kWaves * 2 * 32 * 4);  // [wave][2][32]
 
-  Unit u;
-  const int per = steps_per_unit(p, lane);
-  if (!find_unit<false>(p, blockIdx.x, per, lane, u)) return;  // uniform: before any barrier
   const TileRows tr = tile_rows(p, u);
-  if (tr.rows == 0) return;
+  if (tr.rows == 0) return;  // uniform: before any barrier
   const int token0 = uniform(start_at(p.batch, u.s));
   const bool two = tr.rows > 16;  // the second 16 columns hold rows
 
-  // This lane's two rows: token, position (-1: no row) and query fragment.
-  int64_t qpos[2];
-  uint4 qf[2][KK];
+  // This lane's two rows: position and query fragment.  Columns past the last
+  // row repeat it, and keys past the last seen one below: every load has an
+  // address, none is under a branch.
+  int qpos[2];
+  u32x4 qf[2][KK];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const int r = tr.row0 + 16 * c + l16;
-    const bool have = 16 * c + l16 < tr.rows;
+    const int r = tr.row0 + (16 * c + l16 < tr.rows ? 16 * c + l16 : tr.rows - 1);
     const int t = r / p.G, h = r - t * p.G;
-    qpos[c] = have ? u.w.pos0 + t : -1;
+    qpos[c] = clip(u.pos0 + t);
     const uint16_t* src = static_cast<const uint16_t*>(p.q) + (int64_t)(token0 + t) * p.qs[0] +
                           (int64_t)(u.g * p.G + h) * p.qs[1] + 8 * g4;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
-      qf[c][kk] = have ? *reinterpret_cast<const uint4*>(src + 32 * kk) : uint4{0u, 0u, 0u, 0u};
+      qf[c][kk] = load16(src + 32 * kk);
   }
-  // Keys below `end` are read: up to the last row's position.
-  const int64_t first_pos = u.w.pos0 + tr.row0 / p.G, last_pos = u.w.pos0 + (tr.row0 + tr.rows - 1) / p.G;
-  const int end = last_pos + 1 < p.batch.cap ? (last_pos < 0 ? 0 : (int)(last_pos + 1)) : p.batch.cap;
-  // Tiles of this split: of the sequence's positions, or of its list's blocks.
-  const int tiles = p.idx ? 2 * p.K : (end + kKeys - 1) / kKeys;
+  const int first_pos = uniform(clip(u.pos0 + tr.row0 / p.G));
+  const int items = p.idx ? 2 * p.K : (tr.end + 31) / 32;
   const int lo = u.split * per * kWaves;
-  const int hi = tiles < lo + per * kWaves ? tiles : lo + per * kWaves;
+  const int hi = (int64_t)lo + (int64_t)per * kWaves < items ? lo + per * kWaves : items;
 
   const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)u.g * p.ks[1] + 8 * g4;
   const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1] + 8 * g4;
-  uint16_t* vl = reinterpret_cast<uint16_t*>(smem) + wave * kKeys * VSTR;
+  uint16_t* vl = reinterpret_cast<uint16_t*>(smem) + wave * 32 * VSTR;
 
-  // First key of tile t, -1 for none: a listed block that is padding or in
-  // the future of every row.
-  auto key_of = [&](int t) -> int {
-    if (t >= hi) return -1;
-    if (p.idx == nullptr) return t * kKeys;
-    const int id = tr.list != nullptr ? __builtin_amdgcn_readfirstlane(tr.list[t >> 1]) : -1;
-    if (id < 0 || (int64_t)id * kBlock >= end) return -1;
-    return id * kBlock + (t & 1) * kKeys;
-  };
-  auto next_key = [&](int& t) -> int {
-    for (t += kWaves; t < hi; t += kWaves) {
-      const int k = key_of(t);
-      if (k >= 0 && k < end) return k;
-    }
-    return -1;
-  };
-  // Pages of the keys key0 + l16 and key0 + 16 + l16.
+  // Pages of the keys key0 + l16 and key0 + 16 + l16, -1 for none.
   auto pages_of = [&](int key0, int (&pg)[2]) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int key = key0 + 16 * c + l16;
-      pg[c] = key0 >= 0 && key < end ? page_id(p.batch, u.s, key) : -1;
-    }
+    for (int c = 0; c < 2; ++c) pg[c] = page_id(p.batch, u.s, nearest(key0 + 16 * c + l16, tr.end));
   };
-  auto load = [&](const uint16_t* base, const int64_t* st, int key0, const int (&pg)[2], uint4 (&x)[2][KK]) {
+  auto load = [&](const uint16_t* base, const int64_t* st, int key0, const int (&pg)[2], u32x4 (&x)[2][KK]) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int key = key0 + 16 * c + l16;
+      const int key = nearest(key0 + 16 * c + l16, tr.end);
       const int slot = key - page_of(p.batch, key) * p.batch.page;
-      const uint16_t* src = base + (int64_t)pg[c] * st[0] + (int64_t)slot * st[2];
+      const uint16_t* src = base + (int64_t)(pg[c] < 0 ? 0 : pg[c]) * st[0] + (int64_t)slot * st[2];
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-        x[c][kk] = pg[c] >= 0 ? *reinterpret_cast<const uint4*>(src + 32 * kk) : uint4{0u, 0u, 0u, 0u};
+      for (int kk = 0; kk < KK; ++kk) x[c][kk] = load16(src + 32 * kk);
     }
   };
 
@@ -305,18 +433,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_rows_kernel(const PagedA
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) acc[c][dt] = f32x4v{};
     }
-    int t = lo + wave - kWaves, pg[2], pn[2];
-    uint4 kx[2][KK], vx[2][KK];
-    int key0 = next_key(t);
-    pages_of(key0, pg);
+    KeyWalk<32> walk;
+    walk.init(p, tr, lo + wave, kWaves, hi, lane);
+    int pg[2], pn[2];
+    u32x4 kx[2][KK], vx[2][KK];
+    int key0 = walk.next();
     if (key0 >= 0) {
+      pages_of(key0, pg);
       load(kbase, p.ks, key0, pg, kx);
       load(vbase, p.vs, key0, pg, vx);
     }
     while (key0 >= 0) {
-      const int nkey = next_key(t);
-      pages_of(nkey, pn);
-      const uint32_t have = (uint32_t)(__ballot(pg[0] >= 0) & 0xffffu) | (uint32_t)(__ballot(pg[1] >= 0) << 16);
+      const int nkey = walk.next();
+      if (nkey >= 0) pages_of(nkey, pn);
+      // Bits of the keys with a page and a position below the end.
+      uint32_t have = (uint32_t)(__ballot(pg[0] >= 0) & 0xffffu) | (uint32_t)(__ballot(pg[1] >= 0) << 16);
+      if (tr.end - key0 < 32) have &= (1u << (tr.end - key0)) - 1;
       f32x4v s[2][2];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
@@ -328,19 +460,19 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_rows_kernel(const PagedA
             for (int kk = 0; kk < KK; ++kk) s[c][kt] = mfma16x16x32<F16>(kx[kt][kk], qf[c][kk], s[c][kt]);
         }
       if (nkey >= 0) load(kbase, p.ks, nkey, pn, kx);
-      const bool part = have != 0xffffffffu || key0 + kKeys - 1 > first_pos;
-      uint4 pk[2];
+      const bool part = have != 0xffffffffu || key0 + 31 > first_pos;
+      u32x4 pk[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (c == 1 && !two) break;
         if (part) {
+          const uint32_t mine = have >> (4 * g4);
+          const int rel = qpos[c] - key0 - 4 * g4;
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int kr = 16 * kt + 4 * g4 + r;
-              if (!((have >> kr) & 1u) || key0 + kr > qpos[c]) s[c][kt][r] = -INFINITY;
-            }
+            for (int r = 0; r < 4; ++r)
+              if (!(mine & (1u << (16 * kt + r))) || 16 * kt + r > rel) s[c][kt][r] = -INFINITY;
         }
         float mx = fmaxf(fmaxf(fmaxf(s[c][0][0], s[c][0][1]), fmaxf(s[c][0][2], s[c][0][3])),
                          fmaxf(fmaxf(s[c][1][0], s[c][1][1]), fmaxf(s[c][1][2], s[c][1][3])));
@@ -360,7 +492,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_rows_kernel(const PagedA
           x[i] = fast_exp2(fmaf(s[c][i >> 2][i & 3], p.cs, nm));
           l[c] += x[i];
         }
-        pk[c] = uint4{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]), pack2<F16>(x[6], x[7])};
+        pk[c] = u32x4{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]), pack2<F16>(x[6], x[7])};
       }
       // V through the wave's LDS rows; the previous tile's reads of them
       // come before these writes in the wave's own order.
@@ -368,33 +500,32 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_rows_kernel(const PagedA
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
-          *reinterpret_cast<uint4*>(vl + (16 * kt + l16) * VSTR + 32 * kk + 8 * g4) = vx[kt][kk];
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+          *reinterpret_cast<u32x4*>(vl + (16 * kt + l16) * VSTR + 32 * kk + 8 * g4) = vx[kt][kk];
+      wave_lds_fence();
       if (nkey >= 0) load(vbase, p.vs, nkey, pn, vx);
       const uint16_t* vt = vl + (4 * g4 + (l16 >> 2)) * VSTR + 4 * (l16 & 3);
       if (careful && part) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (c == 1 && !two) break;
-          const int64_t off = qpos[c] - key0;
-          const int rel = off < -1 ? -1 : (off > kKeys ? kKeys : (int)off);
+          const int rel = qpos[c] < key0 ? -1 : qpos[c] - key0;  // last key that the row sees
 #pragma unroll 1
           for (int q = 0; q < 16; ++q) {
             // Column q alone, with the value rows that it does not see as zeros.
             const int seen = __builtin_amdgcn_readlane(rel, q);
+            const uint16_t* vq = vt + opaque_zero();  // reads it again for every column, not 64 registers ahead
+            const uint32_t mine = (seen < 31 ? have & ((2u << seen) - 1) : have) >> (4 * g4);
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int kr = 16 * (i >> 1) + 4 * g4 + 2 * (i & 1);
-              w[i] = (((have >> kr) & 1u) && kr <= seen ? 0xffffu : 0u) |
-                     (((have >> (kr + 1)) & 1u) && kr + 1 <= seen ? 0xffff0000u : 0u);
+              const int b = 16 * (i >> 1) + 2 * (i & 1);
+              w[i] = (mine & (1u << b) ? 0xffffu : 0u) | (mine & (2u << b) ? 0xffff0000u : 0u);
             }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-              const uint2 a = lds_read_tr16(vt + 16 * dt), b = lds_read_tr16(vt + 16 * VSTR + 16 * dt);
-              const f32x4v one = mfma16x16x32<F16>(uint4{a.x & w[0], a.y & w[1], b.x & w[2], b.y & w[3]}, pk[c], f32x4v{});
+              const uint2 a = lds_read_tr16(vq + 16 * dt), b = lds_read_tr16(vq + 16 * VSTR + 16 * dt);
+              const f32x4v one =
+                  mfma16x16x32<F16>(u32x4{a.x & w[0], a.y & w[1], b.x & w[2], b.y & w[3]}, pk[c], f32x4v{});
               if (l16 == q) acc[c][dt] += one;
             }
           }
@@ -403,14 +534,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_rows_kernel(const PagedA
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const uint2 a = lds_read_tr16(vt + 16 * dt), b = lds_read_tr16(vt + 16 * VSTR + 16 * dt);
-          const uint4 va = {a.x, a.y, b.x, b.y};
+          const u32x4 va = {a.x, a.y, b.x, b.y};
           acc[0][dt] = mfma16x16x32<F16>(va, pk[0], acc[0][dt]);
           if (two) acc[1][dt] = mfma16x16x32<F16>(va, pk[1], acc[1][dt]);
         }
       }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      wave_lds_fence();
       key0 = nkey;
       pg[0] = pn[0];
       pg[1] = pn[1];
@@ -429,12 +558,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_rows_kernel(const PagedA
   for (int c = 0; c < 2; ++c) {
     l[c] = quad_sum(l[c]);
     if (g4 == 0) {
-      ml[wave][0][16 * c + l16] = m[c];
-      ml[wave][1][16 * c + l16] = l[c];
+      ml[wave * 64 + 16 * c + l16] = m[c];
+      ml[wave * 64 + 32 + 16 * c + l16] = l[c];
     }
   }
   // The waves' sums joined through LDS, 16 rows at a time: thread t takes
-  // D / 16 values of row t / 16.
+  // D / 32 values of row t / 32.
   float* ol = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -444,30 +573,31 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_rows_kernel(const PagedA
     for (int dt = 0; dt < DT; ++dt)
       *reinterpret_cast<f32x4v*>(ol + (wave * 16 + l16) * OSTR + 16 * dt + 4 * g4) = acc[c][dt];
     __syncthreads();
-    constexpr int PER = D / 16;
-    const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER, row = 16 * c + r;
+    constexpr int PER = D / 32;
+    const int r = threadIdx.x >> 5, d0 = (threadIdx.x & 31) * PER, row = 16 * c + r;
     if (row >= tr.rows) continue;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml[w][0][row]);
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml[w * 64 + row]);
     const float nm = top == -INFINITY ? 0.f : -top;
     float sum = 0.f, o[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) o[i] = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float f = fast_exp2(ml[w][0][row] + nm);
-      sum += f * ml[w][1][row];
+      const float f = fast_exp2(ml[w * 64 + row] + nm);
+      sum += f * ml[w * 64 + 32 + row];
 #pragma unroll
       for (int i = 0; i < PER; ++i) o[i] += f * ol[(w * 16 + r) * OSTR + d0 + i];
     }
     if (u.splits > 1) {
-      float* po = p.part_o + ((int64_t)blockIdx.x * kRows + row) * D + d0;
+      const int64_t group = (int64_t)p.many_units * kWaves + unit;
+      float* po = p.part_o + group * 32 * D + part_at(row, d0);
 #pragma unroll
       for (int i = 0; i < PER; ++i) po[i] = o[i];
       if (d0 == 0) {
-        p.part_ml[(int64_t)blockIdx.x * 2 * kRows + row] = top;
-        p.part_ml[(int64_t)blockIdx.x * 2 * kRows + kRows + row] = sum;
+        p.part_ml[group * 64 + row] = top;
+        p.part_ml[group * 64 + 32 + row] = sum;
       }
       continue;
     }
@@ -481,58 +611,441 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_rows_kernel(const PagedA
   }
 }
 
-// Joins the splits of one (tile, head): a wave takes every fourth row.
-template <int D, bool F16>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn p) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Unit u;
-  const int per = steps_per_unit(p, lane);
-  if (!find_unit<true>(p, blockIdx.x, per, lane, u) || u.splits == 1) return;
+// A many-row unit.  The matrix cores bound it, with the softmax's VALU work
+// and the LDS reads beside them, so it is laid out like the block-sparse
+// prefill: S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 with one query row a
+// lane column, 64-key blocks double-buffered in LDS by way of registers, the
+// next block's loads in flight under the present one's products.  The pages of
+// the block after that are looked up meanwhile, one key a lane.  ALIGNED: a
+// page holds whole blocks, so a block is one piece of memory behind one buffer
+// descriptor; otherwise every row finds its own page.
+template <int D, bool F16, bool ALIGNED>
+__device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int unit, int per, char* smem) {
+  constexpr int NTHR = kWaves * 64;
+  constexpr int KSTR = D + 8, VSTR = D + 32;  // LDS rows; V rows start 16 banks apart
+  constexpr int KTILE = kBlock * KSTR, BUF = KTILE + kBlock * VSTR;
+  constexpr int ROWCH = D / 8, KCH = kBlock * ROWCH / NTHR;  // 16-byte pieces of a row, and of a thread
+  constexpr int DT = D / 32, KS = D / 16;
+  uint16_t* lds = reinterpret_cast<uint16_t*>(smem);
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int l32 = lane & 31, hl = lane >> 5;
+
   const TileRows tr = tile_rows(p, u);
-  const int token0 = start_at(p.batch, u.s), stride = u.w.tiles * p.Hkv;
-  if (u.first + (int64_t)(u.splits - 1) * stride >= p.grid) return;  // starts that overlap
-  constexpr int PER = D / 64;
-  for (int row = wave; row < tr.rows; row += 4) {
-    float best = -INFINITY;
-    for (int i = lane; i < u.splits; i += 64)
-      best = fmaxf(best, p.part_ml[((int64_t)u.first + (int64_t)i * stride) * 2 * kRows + row]);
+  if (tr.rows == 0) return;  // uniform: before any barrier
+  const int token0 = uniform(start_at(p.batch, u.s));
+  const int left = tr.rows - 32 * wave;
+  const int nrow = left < 0 ? 0 : (left < 32 ? left : 32);  // this wave's rows
+  // Columns past the last row repeat it; a wave without rows has the unit's first.
+  const int row = tr.row0 + (nrow == 0 ? 0 : 32 * wave + (l32 < nrow ? l32 : nrow - 1));
+  const int tok = row / p.G, head = u.g * p.G + row - tok * p.G;
+  const int qpos = clip(u.pos0 + tok);
+  // Positions of the wave's first and last row.
+  const int pos_lo = uniform(clip(u.pos0 + (tr.row0 + 32 * wave) / p.G));
+  const int pos_hi = uniform(clip(u.pos0 + (tr.row0 + 32 * wave + (nrow > 0 ? nrow - 1 : 0)) / p.G));
+
+  uint4 qf[KS];
+  {
+    const uint16_t* src =
+        static_cast<const uint16_t*>(p.q) + (int64_t)(token0 + tok) * p.qs[0] + (int64_t)head * p.qs[1] + 8 * hl;
 #pragma unroll
-    for (int mm = 1; mm < 64; mm *= 2) best = fmaxf(best, __shfl_xor(best, mm));
-    const float nm = best == -INFINITY ? 0.f : -best;
-    float sum = 0.f, o[PER] = {};
-    for (int i = 0; i < u.splits; ++i) {
-      const int64_t slot = (int64_t)u.first + (int64_t)i * stride;
-      const float f = fast_exp2(p.part_ml[slot * 2 * kRows + row] + nm);
-      sum += f * p.part_ml[slot * 2 * kRows + kRows + row];
+    for (int kk = 0; kk < KS; ++kk)
+      qf[kk] = *reinterpret_cast<const uint4*>(src + 16 * kk);
+  }
+  const int items = p.idx ? p.K : (tr.end + kBlock - 1) / kBlock;
+  const int64_t lo64 = (int64_t)u.split * per;
+  const int lo = lo64 < items ? (int)lo64 : items;
+  const int hi = lo64 + per < items ? (int)(lo64 + per) : items;
+
+  const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)u.g * p.ks[1];
+  const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1];
+  const int srow = tid / ROWCH, scol = (tid % ROWCH) * 8;  // this thread's pieces: rows srow + i NTHR / ROWCH
+  constexpr int SSTEP = NTHR / ROWCH;
+  int koff[KCH], voff[KCH];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) o[j] += f * p.part_o[(slot * kRows + row) * D + PER * lane + j];
+  for (int i = 0; i < KCH; ++i) {
+    koff[i] = ((srow + i * SSTEP) * (int)p.ks[2] + scol) * 2;
+    voff[i] = ((srow + i * SSTEP) * (int)p.vs[2] + scol) * 2;
+  }
+  u32x4 kst[KCH], vst[KCH];
+  // The page of key0 + lane, -1 for none.
+  auto page_at = [&](int key0) -> int {
+    return key0 < 0 ? -1 : page_id(p.batch, u.s, ALIGNED ? key0 : nearest(key0 + lane, tr.end));
+  };
+  auto load_block = [&](int key0, int pg) {
+    if constexpr (ALIGNED) {
+      const int page = uniform(pg);  // not negative: such blocks are not taken
+      const int slot = key0 - page_of(p.batch, key0) * p.batch.page;
+      int nk = tr.end - key0;
+      nk = nk > kBlock ? kBlock : nk;
+      const __amdgpu_buffer_rsrc_t rk =
+          make_rsrc(kbase + (int64_t)page * p.ks[0] + (int64_t)slot * p.ks[2], (uint32_t)(nk * (int)p.ks[2] * 2));
+      const __amdgpu_buffer_rsrc_t rv =
+          make_rsrc(vbase + (int64_t)page * p.vs[0] + (int64_t)slot * p.vs[2], (uint32_t)(nk * (int)p.vs[2] * 2));
+#pragma unroll
+      for (int i = 0; i < KCH; ++i)
+        kst[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, koff[i], 0, 0));
+#pragma unroll
+      for (int i = 0; i < KCH; ++i)
+        vst[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, voff[i], 0, 0));
+    } else {
+#pragma unroll
+      for (int i = 0; i < KCH; ++i) {
+        const int r = srow + i * SSTEP, page = __shfl(pg < 0 ? 0 : pg, r);
+        const int key = nearest(key0 + r, tr.end), slot = key - page_of(p.batch, key) * p.batch.page;
+        kst[i] = load16(kbase + (int64_t)page * p.ks[0] + (int64_t)slot * p.ks[2] + scol);
+        vst[i] = load16(vbase + (int64_t)page * p.vs[0] + (int64_t)slot * p.vs[2] + scol);
+      }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int t = (tr.row0 + row) / p.G, h = tr.row0 + row - t * p.G;
-    uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(token0 + t) * p.os[0] +
-                    (int64_t)(u.g * p.G + h) * p.os[1] + PER * lane;
-    if constexpr (PER == 2)
-      *reinterpret_cast<uint32_t*>(dst) = pack2<F16>(o[0] * inv, o[1] * inv);
-    else
-      *dst = (uint16_t)pack2<F16>(o[0] * inv, 0.f);
+  };
+  auto store_block = [&](int buf) {
+    uint16_t* ks = lds + buf * BUF;
+#pragma unroll
+    for (int i = 0; i < KCH; ++i) {
+      *reinterpret_cast<u32x4*>(ks + (srow + i * SSTEP) * KSTR + scol) = kst[i];
+      *reinterpret_cast<u32x4*>(ks + KTILE + (srow + i * SSTEP) * VSTR + scol) = vst[i];
+    }
+  };
+
+  float m = -INFINITY, l = 0.f;
+  f32x16_t acc[DT];
+  uint4 pk[2][2];
+  auto scores = [&](const uint16_t* ks, f32x16_t& s0, f32x16_t& s1) {
+    const uint16_t* kp = ks + l32 * KSTR + 8 * hl;
+    uint4 a0[KS], a1[KS];
+    auto rd = [&](int kk) {
+      a0[kk] = *reinterpret_cast<const uint4*>(kp + 16 * kk);
+      a1[kk] = *reinterpret_cast<const uint4*>(kp + 32 * KSTR + 16 * kk);
+    };
+#pragma unroll
+    for (int kk = 0; kk < kLookahead; ++kk) rd(kk);
+    s0 = f32x16_t{};
+    s1 = f32x16_t{};
+    // The reads of step kk + kLookahead are issued before the products of
+    // step kk; without the barriers one register quad serves all reads.
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      if (kk + kLookahead < KS) rd(kk + kLookahead);
+      __builtin_amdgcn_sched_barrier(0);
+      s0 = mfma32x32x16<F16>(a0[kk], qf[kk], s0);
+      s1 = mfma32x32x16<F16>(a1[kk], qf[kk], s1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Register r of key half c holds key 32 c + 8 (r / 4) + 4 (lane / 32) + r % 4.
+  auto softmax = [&](f32x16_t& s0, f32x16_t& s1, bool part, int rel, uint64_t there) {
+    if (part) {
+      const uint32_t lo_bits = (uint32_t)there >> (4 * hl), hi_bits = (uint32_t)(there >> 32) >> (4 * hl);
+      const int thr = rel - 4 * hl;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int kr = 8 * (r >> 2) + (r & 3);
+        if (kr > thr || !(lo_bits & (1u << kr))) s0[r] = -INFINITY;
+        if (32 + kr > thr || !(hi_bits & (1u << kr))) s1[r] = -INFINITY;
+      }
+    }
+    float mx = fmaxf(s0[0], s0[1]);
+#pragma unroll
+    for (int r = 2; r < 16; ++r) mx = fmaxf(mx, s0[r]);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s1[r]);
+    mx = half_max(mx) * p.cs;
+    if (__ballot(mx > m + kRescaleThreshold) != 0) {
+      const float mn = fmaxf(m, mx);
+      const float alpha = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[dt][r] *= alpha;
+    }
+    const float nm = m == -INFINITY ? 0.f : -m;
+    float sum = 0.f;
+#pragma unroll
+    for (int h2 = 0; h2 < 2; ++h2) {
+      uint32_t w0[4], w1[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x0 = fast_exp2(fmaf(s0[8 * h2 + 2 * e], p.cs, nm));
+        const float x1 = fast_exp2(fmaf(s0[8 * h2 + 2 * e + 1], p.cs, nm));
+        const float y0 = fast_exp2(fmaf(s1[8 * h2 + 2 * e], p.cs, nm));
+        const float y1 = fast_exp2(fmaf(s1[8 * h2 + 2 * e + 1], p.cs, nm));
+        sum += (x0 + x1) + (y0 + y1);
+        w0[e] = pack2<F16>(x0, x1);
+        w1[e] = pack2<F16>(y0, y1);
+      }
+      pk[0][h2] = uint4{w0[0], w0[1], w0[2], w0[3]};
+      pk[1][h2] = uint4{w1[0], w1[1], w1[2], w1[3]};
+    }
+    l += sum;
+  };
+  // P^T fragment pk[c][h2] holds keys K0 + 4 hl + 0..3 and K0 + 8 + 4 hl + 0..3,
+  // K0 = 32 c + 16 h2; the V^T fragment of d = 32 dt + l32 is two transposing reads of 4 keys each.
+  const int vlane = (4 * hl + ((lane & 15) >> 2)) * VSTR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  auto value = [&](const uint16_t* vp, int dt, int ch) {
+    const uint16_t* a = vp + 16 * ch * VSTR + 32 * dt;
+    const uint2 x = lds_read_tr16(a), y = lds_read_tr16(a + 8 * VSTR);
+    return uint4{x.x, x.y, y.x, y.y};
+  };
+  auto pv = [&](const uint16_t* vs) {
+    const uint16_t* vp = vs + vlane;
+    uint4 va[DT * 4];
+#pragma unroll
+    for (int i = 0; i < DT * 4; ++i) va[i] = value(vp, i % DT, i / DT);
+    __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 4 * kLookahead, 0);
+#pragma unroll
+    for (int i = 0; i < DT * 4 - 2 * kLookahead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kSchedMfma, 2 * kLookahead, 0);
+#pragma unroll
+    for (int i = 0; i < DT * 4; ++i)
+      acc[i % DT] = mfma32x32x16<F16>(va[i], pk[(i / DT) >> 1][(i / DT) & 1], acc[i % DT]);
+  };
+  // The same for one column at a time, with the value rows that it does not
+  // see as zeros: 0 times a NaN or infinity there would be NaN.
+  auto pv_careful = [&](const uint16_t* vs, int rel, uint64_t there) {
+    const uint16_t* vp = vs + vlane;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+      for (int q = 0; q < 32; ++q) {
+        const int seen = __builtin_amdgcn_readlane(rel, q);
+        const uint64_t mine = seen < 63 ? there & ((2ull << seen) - 1) : there;
+        const uint16_t* vq = vp + opaque_zero();  // as above
+        f32x16_t one = f32x16_t{};
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          const uint4 a = value(vq, dt, ch);
+          const uint32_t bits = (uint32_t)(mine >> (16 * ch + 4 * hl));
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int b = 8 * (i >> 1) + 2 * (i & 1);
+            w[i] = (bits & (1u << b) ? 0xffffu : 0u) | (bits & (2u << b) ? 0xffff0000u : 0u);
+          }
+          one = mfma32x32x16<F16>(uint4{a.x & w[0], a.y & w[1], a.z & w[2], a.w & w[3]}, pk[ch >> 1][ch & 1], one);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (l32 == q) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[dt][r] += one[r];
+        }
+      }
+    }
+  };
+
+  for (bool careful = false;; careful = true) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16_t{};
+    KeyWalk<kBlock> walk;
+    walk.init(p, tr, lo, 1, hi, lane);
+    // The next block that is taken, with the pages of its keys; those without
+    // a page are passed over.
+    auto take = [&](int& key0, int& pg) {
+      do {
+        key0 = walk.next();
+        pg = page_at(key0);
+      } while (ALIGNED && key0 >= 0 && uniform(pg) < 0);
+    };
+    int key0, pg, nkey, npg;
+    take(key0, pg);
+    int buf = 0;
+    if (key0 >= 0) {
+      load_block(key0, pg);
+      take(nkey, npg);
+      store_block(0);
+      __syncthreads();
+      while (true) {
+        if (nkey >= 0) load_block(nkey, npg);
+        int akey = -1, apg = -1;
+        if (nkey >= 0) take(akey, apg);
+        if (nrow > 0 && key0 <= pos_hi) {
+          const uint16_t* ks = lds + buf * BUF;
+          // Bits of the keys with a page and a position below the end.
+          uint64_t there = ALIGNED ? ~0ull : __ballot(pg >= 0);
+          if (tr.end - key0 < kBlock) there &= (1ull << (tr.end - key0)) - 1;
+          const bool part = there != ~0ull || key0 + kBlock - 1 > pos_lo;
+          const int rel = qpos < key0 ? -1 : qpos - key0;
+          f32x16_t s0, s1;
+          scores(ks, s0, s1);
+          softmax(s0, s1, part, rel, there);
+          if (careful && part)
+            pv_careful(ks + KTILE, rel, there);
+          else
+            pv(ks + KTILE);
+        }
+        if (nkey < 0) break;
+        store_block(buf ^ 1);
+        __syncthreads();
+        buf ^= 1;
+        key0 = nkey;
+        pg = npg;
+        nkey = akey;
+        npg = apg;
+      }
+    }
+    if (careful) break;
+    bool odd = false;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) odd |= !(fabsf(acc[dt][r]) < INFINITY);
+    if (!uniform(__syncthreads_or(odd))) break;
+  }
+
+  l = half_sum(l);
+  if (u.splits > 1) {
+    const int64_t group = (int64_t)unit * kWaves + wave;
+    if (nrow == 0) return;
+    float* po = p.part_o + group * 32 * D + lane * 4;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4*>(po + (dt * 4 + j) * 256) =
+            float4{acc[dt][4 * j], acc[dt][4 * j + 1], acc[dt][4 * j + 2], acc[dt][4 * j + 3]};
+    if (hl == 0) {
+      p.part_ml[group * 64 + l32] = m;
+      p.part_ml[group * 64 + 32 + l32] = l;
+    }
+    return;
+  }
+  // Through LDS, so that every store writes 16-byte pieces of whole rows; the
+  // vote above was the last barrier that readers of the tiles passed.
+  constexpr int OSTR = D + 8;
+  static_assert(kWaves * 32 * OSTR <= 2 * BUF, "output staging must fit the K/V tiles");
+  if (nrow == 0) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* ot = lds + wave * 32 * OSTR;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint2*>(ot + l32 * OSTR + dt * 32 + 8 * j + 4 * hl) =
+          uint2{pack2<F16>(acc[dt][4 * j] * inv, acc[dt][4 * j + 1] * inv),
+                pack2<F16>(acc[dt][4 * j + 2] * inv, acc[dt][4 * j + 3] * inv)};
+  wave_lds_fence();
+  const int64_t at = (int64_t)(token0 + tok) * p.os[0] + (int64_t)head * p.os[1];  // of row l32
+#pragma unroll
+  for (int i = 0; i < 32 * ROWCH / 64; ++i) {
+    const int c = i * 64 + lane, r = c / ROWCH, ch = c % ROWCH;
+    const int lo32 = __shfl((int)at, r), hi32 = __shfl((int)(at >> 32), r);
+    if (r < nrow)
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
+                                (int64_t)(((uint64_t)(uint32_t)hi32 << 32) | (uint32_t)lo32) + ch * 8) =
+          *reinterpret_cast<const uint4*>(ot + r * OSTR + ch * 8);
   }
 }
 
-// Tiles of a (ragged) batch with N new tokens: sequences round up one each.
-int64_t tile_bound(int64_t N, int64_t S, int64_t G, bool lists) {
-  if (!lists) return (N * G + kRows - 1) / kRows + S;
-  // Listed rows also break at every 64 positions.
-  const int64_t blocks = N / kBlock + 2 * S < N + S ? N / kBlock + 2 * S : N + S;
-  return blocks * ((kBlock * G + kRows - 1) / kRows);
+template <int D, bool F16, bool ALIGNED>
+__global__ __launch_bounds__(kWaves * 64, 2) void paged_attention_kernel(const PagedAttn p) {
+  constexpr int kLds = few_lds_bytes<D>() > many_lds_bytes<D>() ? few_lds_bytes<D>() : many_lds_bytes<D>();
+  __shared__ __attribute__((aligned(16))) char smem[kLds];
+  const int lane = threadIdx.x & 63;
+  const Pace pace = choose_pace(p, lane);
+  int want = blockIdx.x;
+  Unit u;
+  if (find_unit<true, false>(p, want, pace.many, lane, u)) {
+    if (u.splits > 1 && want >= p.many_units) return;  // starts that overlap
+    many_rows<D, F16, ALIGNED>(p, u, want, pace.many, smem);
+  } else if (find_unit<false, false>(p, want, pace.few, lane, u)) {
+    if (u.splits > 1 && want >= p.few_units) return;
+    few_rows<D, F16>(p, u, want, pace.few, smem);
+  }
+}
+
+// Joins the splits of one 32-row group: every thread takes 4 values of its
+// row from every eighth of d.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn p) {
+  const int lane = threadIdx.x & 63;
+  const Pace pace = choose_pace(p, lane);
+  // Groups in order: eight to a many-row tile, then one to a few-row tile.
+  int want = blockIdx.x / kWaves, sub = blockIdx.x % kWaves;
+  Unit u;
+  const bool many = find_unit<true, true>(p, want, pace.many, lane, u);
+  if (!many) {
+    want = want * kWaves + sub;
+    sub = 0;
+    if (!find_unit<false, true>(p, want, pace.few, lane, u)) return;
+  }
+  if (u.splits == 1) return;
+  if (u.first + (int64_t)(u.splits - 1) * u.stride >= (many ? p.many_units : p.few_units)) return;  // starts that overlap
+  const TileRows tr = tile_rows(p, u);
+  const int row = lane & 31, hl = lane >> 5, wave = threadIdx.x >> 6;
+  const int r = sub * 32 + row;
+  if (r >= tr.rows) return;
+  const int64_t group0 = many ? (int64_t)u.first * kWaves + sub : (int64_t)p.many_units * kWaves + u.first;
+  const int64_t step = many ? (int64_t)u.stride * kWaves : u.stride;
+  float top = -INFINITY;
+  for (int i = 0; i < u.splits; ++i) top = fmaxf(top, p.part_ml[(group0 + i * step) * 64 + row]);
+  const float nm = top == -INFINITY ? 0.f : -top;
+  constexpr int PIECES = D / 32;  // of 4 values: pieces wave, wave + 4 ..
+  float sum = 0.f;
+  f32x4v o[PIECES] = {};
+  for (int i = 0; i < u.splits; ++i) {
+    const int64_t group = group0 + i * step;
+    const float f = fast_exp2(p.part_ml[group * 64 + row] + nm);
+    sum += f * p.part_ml[group * 64 + 32 + row];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j)
+      o[j] += f * *reinterpret_cast<const f32x4v*>(p.part_o + group * 32 * D + (wave + 4 * j) * 256 + lane * 4);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int at = tr.row0 + r, t = at / p.G, h = at - t * p.G;
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(start_at(p.batch, u.s) + t) * p.os[0] +
+                  (int64_t)(u.g * p.G + h) * p.os[1] + 4 * hl;
+#pragma unroll
+  for (int j = 0; j < PIECES; ++j)
+    *reinterpret_cast<uint2*>(dst + 8 * (wave + 4 * j)) =
+        uint2{pack2<F16>(o[j][0] * inv, o[j][1] * inv), pack2<F16>(o[j][2] * inv, o[j][3] * inv)};
+}
+
+// Bounds of what a batch with N new tokens of S sequences can hold of either
+// kind, whatever its lengths are: (tile, head) pairs and units.
+struct Bounds {
+  int64_t many_tiles, many_units, few_tiles, few_units;
+};
+
+Bounds bounds_of(int64_t N, int64_t S, int64_t G, int64_t Hkv, bool lists) {
+  Bounds b{};
+  const int64_t rows = N * G;
+  if (rows > kFewRows) {
+    // A many-row sequence has more than kFewRows rows, so there are few of them.
+    const int64_t seqs = S < rows / (kFewRows + 1) ? S : rows / (kFewRows + 1);
+    // Listed rows break at every 64 positions too.
+    b.many_tiles = !lists ? rows / Many::rows + seqs
+                          : (N / kBlock + 2 * seqs) * ((kBlock * G + Many::rows - 1) / Many::rows);
+    b.many_tiles *= Hkv;
+    b.many_units = b.many_tiles + (b.many_tiles < kManySlots ? kManySlots : b.many_tiles);
+  }
+  // Few-row tiles: up to kFewRows rows a sequence, each of whose tokens may
+  // stand in one of two blocks.
+  const int64_t seqs = S < N ? S : N;
+  const int64_t most = (N < kFewRows / G ? N : kFewRows / G) * G;  // rows of one of them
+  b.few_tiles = most == 0 ? 0 : seqs * ((most + Few::rows - 1) / Few::rows) * (lists && most > G ? 2 : 1) * Hkv;
+  b.few_units = b.few_tiles == 0 ? 0 : b.few_tiles + kFewSlots;
+  return b;
+}
+
+int64_t workspace_of(const Bounds& b, int64_t D) {
+  // Splitting stops where there are units enough, so only the first many-row
+  // units can be split ones.
+  const int64_t many = b.many_units < 2 * kManySlots ? b.many_units : 2 * kManySlots;
+  return (many * kWaves + b.few_units) * 32 * (D + 2) * 4;
 }
 
 }  // namespace
 
 extern "C" int64_t spruce_paged_attention_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
                                                           int64_t K) {
-  if (N < 1 || S < 1 || Hkv < 1 || Hq < Hkv || N >= (int64_t)1 << 30 || S >= (int64_t)1 << 20) return 0;
-  const int64_t units = tile_bound(N, S, Hq / Hkv, K > 0) * Hkv + kSlots;
-  return units * kRows * (D + 2) * 4;
+  if (N < 1 || S < 1 || Hkv < 1 || Hq < Hkv || N >= (int64_t)1 << 30 || S >= (int64_t)1 << 20 || Hq >= 1 << 16) return 0;
+  return workspace_of(bounds_of(N, S, Hq / Hkv, Hkv, K > 0), D);
 }
 
 extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const void* k_pages, const int64_t kps[4],
@@ -568,7 +1081,8 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
   SPRUCE_REQUIRE(K >= 0 && K < (int64_t)1 << 24, "invalid list width %lld", (long long)K);
   SPRUCE_REQUIRE(K == 0 || (idx && is && Qc >= 0), "indices must be a non-null device pointer");
   SPRUCE_REQUIRE(K == 0 || is[3] == 1, "indices must have a contiguous final dimension");
-  const int64_t need = spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D, K);
+  const Bounds bounds = bounds_of(N, S, Hq / Hkv, Hkv, K > 0);
+  const int64_t need = workspace_of(bounds, D);
   SPRUCE_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
                  (long long)workspace_bytes, (long long)need);
   SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
@@ -593,27 +1107,33 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
     p.Qc = (int)(Qc < (int64_t)1 << 30 ? Qc : (int64_t)1 << 30);
     p.K = (int)K;
   }
-  const int64_t tiles = tile_bound(N, S, p.G, K > 0) * Hkv;
-  SPRUCE_REQUIRE(tiles + kSlots < (int64_t)1 << 24, "too many tokens for one call");
-  p.grid = (int)(tiles + kSlots);
+  const int64_t units = bounds.many_units + bounds.few_units;
+  const int64_t groups = bounds.many_tiles * kWaves + bounds.few_tiles;
+  SPRUCE_REQUIRE(units < (int64_t)1 << 22 && groups < (int64_t)1 << 23, "too many tokens for one call");
+  p.many_units = (int)(bounds.many_units < 2 * kManySlots ? bounds.many_units : 2 * kManySlots);
+  p.few_units = (int)bounds.few_units;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + (int64_t)p.grid * kRows * D;
+  p.part_ml = p.part_o + ((int64_t)p.many_units * kWaves + p.few_units) * 32 * D;
+  // Rows of a page's block behind one 32-bit buffer offset.
+  const bool aligned = page_size % kBlock == 0 && kps[2] > 0 && vps[2] > 0 && kps[2] < 1 << 22 && vps[2] < 1 << 22;
   const hipStream_t st = (hipStream_t)stream;
-  const int64_t most = K > 0 ? K * kBlock : p.batch.cap;  // keys of a row at most
-  const bool join = most > kMinSteps * kStep;
-#define SPRUCE_PAGED(KERNEL, GRID)                                                                    \
-  do {                                                                                                \
-    const dim3 g((unsigned)(GRID));                                                                   \
-    if (D == 128 && dtype == SPRUCE_DTYPE_BF16)                                                       \
-      hipLaunchKernelGGL((KERNEL<128, false>), g, dim3(256), 0, st, p);                               \
-    else if (D == 128) hipLaunchKernelGGL((KERNEL<128, true>), g, dim3(256), 0, st, p);               \
-    else if (dtype == SPRUCE_DTYPE_BF16) hipLaunchKernelGGL((KERNEL<64, false>), g, dim3(256), 0, st, p); \
-    else hipLaunchKernelGGL((KERNEL<64, true>), g, dim3(256), 0, st, p);                              \
-    const int e = check_launch(#KERNEL);                                                              \
-    if (e) return e;                                                                                  \
+#define SPRUCE_PAGED(D_, F16_)                                                                                    \
+  do {                                                                                                            \
+    if (aligned)                                                                                                  \
+      hipLaunchKernelGGL((paged_attention_kernel<D_, F16_, true>), dim3((unsigned)units), dim3(kWaves * 64), 0, st, p);  \
+    else                                                                                                          \
+      hipLaunchKernelGGL((paged_attention_kernel<D_, F16_, false>), dim3((unsigned)units), dim3(kWaves * 64), 0, st, p); \
+    const int e = check_launch("paged_attention_kernel");                                                         \
+    if (e) return e;                                                                                              \
+    hipLaunchKernelGGL((paged_join_kernel<D_, F16_>), dim3((unsigned)groups), dim3(256), 0, st, p);               \
   } while (0)
-  SPRUCE_PAGED(paged_rows_kernel, join ? p.grid : tiles);
-  if (join) SPRUCE_PAGED(paged_join_kernel, tiles);
+  if (D == 128) {
+    if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_PAGED(128, false);
+    else SPRUCE_PAGED(128, true);
+  } else {
+    if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_PAGED(64, false);
+    else SPRUCE_PAGED(64, true);
+  }
 #undef SPRUCE_PAGED
-  return SPRUCE_OK;
+  return check_launch("paged_join_kernel");
 }
