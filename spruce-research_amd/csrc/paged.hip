@@ -13,8 +13,7 @@
 //   few rows    32 rows; every wave takes 32 keys at a time of its own,
 //               without a barrier until the waves' sums are joined;
 //   many rows   256 rows, 32 a wave; all waves share each 64-key block in LDS.
-// One launch holds the units of both kinds, since the lengths that tell them
-// apart are on the device: a batch may mix them.
+// A batch may mix them.
 #include "attention_impl.h"
 #include "paged.h"
 
@@ -143,51 +142,50 @@ __device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
 
 // How many steps a unit takes of its row tile at most, for either kind; every
 // workgroup works this out from the lengths, 64 sequences at a time.
-struct Pace {
-  int many, few;
-};
-
-__device__ __forceinline__ Pace choose_pace(const PagedAttn& p, int lane) {
-  int64_t few = 0, many = 0, tiles = 0;
+// Few rows: about kFewSlots units of equal size.
+__device__ __forceinline__ int few_pace(const PagedAttn& p, int lane) {
+  int64_t work = 0;
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
     const SeqWork w = sequence_work(p, s0 + lane);
-    const int64_t work = (int64_t)w.tiles * w.steps;
-    few += w.many ? 0 : work;
-    many += w.many ? work : 0;
+    work += w.many ? 0 : (int64_t)w.tiles * w.steps;
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) work += __shfl_xor(work, m);
+  const int64_t per = (work * p.Hkv + kFewSlots - 1) / kFewSlots;
+  return uniform((int)(per < 1 ? 1 : (per < (1 << 30) ? per : 1 << 30)));
+}
+
+// Many rows: lane l weighs l + 1 splits of the average tile.  A split costs
+// its blocks and a fixed part worth about eight more (first loads, last
+// reduction, store) and four for its part in the join; CUs take one unit at a
+// time.
+__device__ __forceinline__ int many_pace(const PagedAttn& p, int lane) {
+  int64_t work = 0, tiles = 0;
+  for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
+    const SeqWork w = sequence_work(p, s0 + lane);
+    work += w.many ? (int64_t)w.tiles * w.steps : 0;
     tiles += w.many ? w.tiles : 0;
   }
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) {
-    few += __shfl_xor(few, m);
-    many += __shfl_xor(many, m);
+    work += __shfl_xor(work, m);
     tiles += __shfl_xor(tiles, m);
   }
-  Pace pace;
-  // Few rows: about kFewSlots units of equal size.
-  const int64_t per = (few * p.Hkv + kFewSlots - 1) / kFewSlots;
-  pace.few = uniform((int)(per < 1 ? 1 : (per < (1 << 30) ? per : 1 << 30)));
-  // Many rows: lane l weighs l + 1 splits of the average tile.  A split costs
-  // its blocks and a fixed part worth about eight more (first loads, last
-  // reduction, store) and four for its part in the join; CUs take one unit
-  // at a time.
   const int64_t units = tiles * p.Hkv;
-  pace.many = 1 << 30;
-  if (units > 0 && units * 2 <= kManySlots) {
-    const int avg = (int)(many / tiles);
-    const int ns = lane + 1, part = (avg + ns - 1) / ns;
-    const int rounds = (int)((units * ns + kCus - 1) / kCus);
-    uint32_t cost = (uint32_t)rounds * (uint32_t)(part + 8 + (ns > 1 ? 4 : 0));
-    if (units * ns > kManySlots || ns > avg || cost >= 1u << 25) cost = (1u << 25) - 1;
-    uint32_t best = cost << 6 | (uint32_t)lane;
+  if (units == 0 || units * 2 > kManySlots) return 1 << 30;
+  const int avg = (int)(work / tiles);
+  const int ns = lane + 1, part = (avg + ns - 1) / ns;
+  const int rounds = (int)((units * ns + kCus - 1) / kCus);
+  uint32_t cost = (uint32_t)rounds * (uint32_t)(part + 8 + (ns > 1 ? 4 : 0));
+  if (units * ns > kManySlots || ns > avg || cost >= 1u << 25) cost = (1u << 25) - 1;
+  uint32_t best = cost << 6 | (uint32_t)lane;
 #pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-      const uint32_t o = (uint32_t)__shfl_xor((int)best, m);
-      best = o < best ? o : best;
-    }
-    const int n = (int)(best & 63) + 1;
-    pace.many = uniform(n == 1 ? 1 << 30 : (avg + n - 1) / n);
+  for (int m = 1; m < 64; m *= 2) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)best, m);
+    best = o < best ? o : best;
   }
-  return pace;
+  const int n = (int)(best & 63) + 1;
+  return uniform(n == 1 ? 1 << 30 : (avg + n - 1) / n);
 }
 
 struct Unit {
@@ -227,9 +225,9 @@ __device__ __forceinline__ bool find_unit(const PagedAttn& p, int& want, int per
       if (th <= 0 || in < 0 || in >= th * (BY_TILE ? 1 : u.splits)) return false;  // starts that overlap
       // Within a sequence: split slowest, then tile, head fastest: the eight
       // XCDs take units in turn, so each L2 serves one head where Hkv divides 8.
-      u.split = BY_TILE ? 0 : in / th;
+      u.split = BY_TILE ? 0 : uniform(in / th);
       const int r = in - u.split * th;
-      u.tile = r / p.Hkv;
+      u.tile = uniform(r / p.Hkv);
       u.g = r - u.tile * p.Hkv;
       u.first = before + r;
       u.stride = th;
@@ -268,7 +266,9 @@ __device__ __forceinline__ TileRows tile_rows(const PagedAttn& p, const Unit& u)
     t.list = bi < p.Qc ? p.idx + (int64_t)u.s * p.is[0] + (int64_t)u.g * p.is[1] + (int64_t)bi * p.is[2] : nullptr;
   }
   const int64_t last = u.pos0 + (t.row0 + t.rows - 1) / p.G;
-  t.end = last < 0 || p.batch.pages == 0 ? 0 : (last + 1 < p.batch.cap ? (int)(last + 1) : p.batch.cap);
+  t.end = uniform(last < 0 || p.batch.pages == 0 ? 0 : (last + 1 < p.batch.cap ? (int)(last + 1) : p.batch.cap));
+  t.row0 = uniform(t.row0);
+  t.rows = uniform(t.rows);
   return t;
 }
 
@@ -285,9 +285,9 @@ struct KeyWalk {
   __device__ __forceinline__ void init(const PagedAttn& p, const TileRows& t, int base_, int stride_, int hi_, int lane_) {
     lists = p.idx != nullptr;
     list = t.list;
-    base = base_;
+    base = uniform(base_);
     stride = stride_;
-    hi = lists && list == nullptr ? 0 : hi_;
+    hi = uniform(lists && list == nullptr ? 0 : hi_);
     end = t.end;
     lane = lane_;
     bits = 0;
@@ -424,8 +424,10 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
   f32x4v acc[2][DT];
   // A masked key has p = 0, but 0 times a NaN or infinity in its value row is
   // NaN: where the sums come out non-finite, the keys are walked once more
-  // with the partly masked tiles taken one column at a time.
-  for (bool careful = false;; careful = true) {
+  // (CAREFUL) with the partly masked tiles taken one column at a time.  Two
+  // copies of the loop: a branch in one costs the usual case its registers.
+  auto walk_keys = [&](auto careful_tag) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful_tag)::value;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       m[c] = -INFINITY;
@@ -504,7 +506,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
       wave_lds_fence();
       if (nkey >= 0) load(vbase, p.vs, nkey, pn, vx);
       const uint16_t* vt = vl + (4 * g4 + (l16 >> 2)) * VSTR + 4 * (l16 & 3);
-      if (careful && part) {
+      if (CAREFUL && part) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (c == 1 && !two) break;
@@ -530,13 +532,19 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
             }
           }
         }
-      } else {
+      } else if (two) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const uint2 a = lds_read_tr16(vt + 16 * dt), b = lds_read_tr16(vt + 16 * VSTR + 16 * dt);
           const u32x4 va = {a.x, a.y, b.x, b.y};
           acc[0][dt] = mfma16x16x32<F16>(va, pk[0], acc[0][dt]);
-          if (two) acc[1][dt] = mfma16x16x32<F16>(va, pk[1], acc[1][dt]);
+          acc[1][dt] = mfma16x16x32<F16>(va, pk[1], acc[1][dt]);
+        }
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const uint2 a = lds_read_tr16(vt + 16 * dt), b = lds_read_tr16(vt + 16 * VSTR + 16 * dt);
+          acc[0][dt] = mfma16x16x32<F16>(u32x4{a.x, a.y, b.x, b.y}, pk[0], acc[0][dt]);
         }
       }
       wave_lds_fence();
@@ -544,7 +552,9 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
       pg[0] = pn[0];
       pg[1] = pn[1];
     }
-    if (careful) break;
+  };
+  walk_keys(std::false_type{});
+  {
     bool odd = false;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
@@ -552,7 +562,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) odd |= !(fabsf(acc[c][dt][r]) < INFINITY);
-    if (!__ballot(odd)) break;
+    if (__ballot(odd)) walk_keys(std::true_type{});
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -673,7 +683,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
   };
   auto load_block = [&](int key0, int pg) {
     if constexpr (ALIGNED) {
-      const int page = uniform(pg);  // not negative: such blocks are not taken
+      const int page = uniform(pg < 0 ? 0 : pg);
       const int slot = key0 - page_of(p.batch, key0) * p.batch.page;
       int nk = tr.end - key0;
       nk = nk > kBlock ? kBlock : nk;
@@ -837,20 +847,17 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
     }
   };
 
-  for (bool careful = false;; careful = true) {
+  auto walk_keys = [&](auto careful_tag) __attribute__((always_inline)) {  // as in few_rows
+    constexpr bool CAREFUL = decltype(careful_tag)::value;
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16_t{};
     KeyWalk<kBlock> walk;
     walk.init(p, tr, lo, 1, hi, lane);
-    // The next block that is taken, with the pages of its keys; those without
-    // a page are passed over.
     auto take = [&](int& key0, int& pg) {
-      do {
-        key0 = walk.next();
-        pg = page_at(key0);
-      } while (ALIGNED && key0 >= 0 && uniform(pg) < 0);
+      key0 = walk.next();
+      pg = page_at(key0);
     };
     int key0, pg, nkey, npg;
     take(key0, pg);
@@ -867,14 +874,14 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
         if (nrow > 0 && key0 <= pos_hi) {
           const uint16_t* ks = lds + buf * BUF;
           // Bits of the keys with a page and a position below the end.
-          uint64_t there = ALIGNED ? ~0ull : __ballot(pg >= 0);
+          uint64_t there = ALIGNED ? (uniform(pg) < 0 ? 0 : ~0ull) : __ballot(pg >= 0);
           if (tr.end - key0 < kBlock) there &= (1ull << (tr.end - key0)) - 1;
           const bool part = there != ~0ull || key0 + kBlock - 1 > pos_lo;
           const int rel = qpos < key0 ? -1 : qpos - key0;
           f32x16_t s0, s1;
           scores(ks, s0, s1);
           softmax(s0, s1, part, rel, there);
-          if (careful && part)
+          if (CAREFUL && part)
             pv_careful(ks + KTILE, rel, there);
           else
             pv(ks + KTILE);
@@ -889,13 +896,18 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
         npg = apg;
       }
     }
-    if (careful) break;
+  };
+  walk_keys(std::false_type{});
+  {
     bool odd = false;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) odd |= !(fabsf(acc[dt][r]) < INFINITY);
-    if (!uniform(__syncthreads_or(odd))) break;
+    if (uniform(__syncthreads_or(odd))) {
+      walk_keys(std::true_type{});
+      __syncthreads();
+    }
   }
 
   l = half_sum(l);
@@ -915,8 +927,8 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
     }
     return;
   }
-  // Through LDS, so that every store writes 16-byte pieces of whole rows; the
-  // vote above was the last barrier that readers of the tiles passed.
+  // Through LDS, so that every store writes 16-byte pieces of whole rows; all
+  // readers of the tiles have passed the barrier above.
   constexpr int OSTR = D + 8;
   static_assert(kWaves * 32 * OSTR <= 2 * BUF, "output staging must fit the K/V tiles");
   if (nrow == 0) return;
@@ -942,21 +954,31 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
   }
 }
 
-template <int D, bool F16, bool ALIGNED>
-__global__ __launch_bounds__(kWaves * 64, 2) void paged_attention_kernel(const PagedAttn p) {
-  constexpr int kLds = few_lds_bytes<D>() > many_lds_bytes<D>() ? few_lds_bytes<D>() : many_lds_bytes<D>();
-  __shared__ __attribute__((aligned(16))) char smem[kLds];
+// A launch for either kind: the lengths that tell them apart are on the
+// device, so the workgroups of a kind that the batch does not hold find no
+// unit and end.  (Both in one kernel needed more registers than there are.)
+template <int D, bool F16>
+__global__ __launch_bounds__(kWaves * 64, 2) void paged_few_kernel(const PagedAttn p) {
+  __shared__ __attribute__((aligned(16))) char smem[few_lds_bytes<D>()];
   const int lane = threadIdx.x & 63;
-  const Pace pace = choose_pace(p, lane);
+  const int per = few_pace(p, lane);
   int want = blockIdx.x;
   Unit u;
-  if (find_unit<true, false>(p, want, pace.many, lane, u)) {
-    if (u.splits > 1 && want >= p.many_units) return;  // starts that overlap
-    many_rows<D, F16, ALIGNED>(p, u, want, pace.many, smem);
-  } else if (find_unit<false, false>(p, want, pace.few, lane, u)) {
-    if (u.splits > 1 && want >= p.few_units) return;
-    few_rows<D, F16>(p, u, want, pace.few, smem);
-  }
+  if (!find_unit<false, false>(p, want, per, lane, u)) return;
+  if (u.splits > 1 && want >= p.few_units) return;  // starts that overlap
+  few_rows<D, F16>(p, u, want, per, smem);
+}
+
+template <int D, bool F16, bool ALIGNED>
+__global__ __launch_bounds__(kWaves * 64, 2) void paged_many_kernel(const PagedAttn p) {
+  __shared__ __attribute__((aligned(16))) char smem[many_lds_bytes<D>()];
+  const int lane = threadIdx.x & 63;
+  const int per = many_pace(p, lane);
+  int want = blockIdx.x;
+  Unit u;
+  if (!find_unit<true, false>(p, want, per, lane, u)) return;
+  if (u.splits > 1 && want >= p.many_units) return;  // starts that overlap
+  many_rows<D, F16, ALIGNED>(p, u, want, per, smem);
 }
 
 // Joins the splits of one 32-row group: every thread takes 4 values of its
@@ -964,15 +986,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attention_kernel(const P
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn p) {
   const int lane = threadIdx.x & 63;
-  const Pace pace = choose_pace(p, lane);
   // Groups in order: eight to a many-row tile, then one to a few-row tile.
   int want = blockIdx.x / kWaves, sub = blockIdx.x % kWaves;
   Unit u;
-  const bool many = find_unit<true, true>(p, want, pace.many, lane, u);
+  const bool many = find_unit<true, true>(p, want, many_pace(p, lane), lane, u);
   if (!many) {
     want = want * kWaves + sub;
     sub = 0;
-    if (!find_unit<false, true>(p, want, pace.few, lane, u)) return;
+    if (!find_unit<false, true>(p, want, few_pace(p, lane), lane, u)) return;
   }
   if (u.splits == 1) return;
   if (u.first + (int64_t)(u.splits - 1) * u.stride >= (many ? p.many_units : p.few_units)) return;  // starts that overlap
@@ -1107,9 +1128,8 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
     p.Qc = (int)(Qc < (int64_t)1 << 30 ? Qc : (int64_t)1 << 30);
     p.K = (int)K;
   }
-  const int64_t units = bounds.many_units + bounds.few_units;
   const int64_t groups = bounds.many_tiles * kWaves + bounds.few_tiles;
-  SPRUCE_REQUIRE(units < (int64_t)1 << 22 && groups < (int64_t)1 << 23, "too many tokens for one call");
+  SPRUCE_REQUIRE(bounds.many_units < (int64_t)1 << 22 && bounds.few_units < (int64_t)1 << 22 && groups < (int64_t)1 << 23, "too many tokens for one call");
   p.many_units = (int)(bounds.many_units < 2 * kManySlots ? bounds.many_units : 2 * kManySlots);
   p.few_units = (int)bounds.few_units;
   p.part_o = static_cast<float*>(workspace);
@@ -1117,15 +1137,23 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
   // Rows of a page's block behind one 32-bit buffer offset.
   const bool aligned = page_size % kBlock == 0 && kps[2] > 0 && vps[2] > 0 && kps[2] < 1 << 22 && vps[2] < 1 << 22;
   const hipStream_t st = (hipStream_t)stream;
-#define SPRUCE_PAGED(D_, F16_)                                                                                    \
-  do {                                                                                                            \
-    if (aligned)                                                                                                  \
-      hipLaunchKernelGGL((paged_attention_kernel<D_, F16_, true>), dim3((unsigned)units), dim3(kWaves * 64), 0, st, p);  \
-    else                                                                                                          \
-      hipLaunchKernelGGL((paged_attention_kernel<D_, F16_, false>), dim3((unsigned)units), dim3(kWaves * 64), 0, st, p); \
-    const int e = check_launch("paged_attention_kernel");                                                         \
-    if (e) return e;                                                                                              \
-    hipLaunchKernelGGL((paged_join_kernel<D_, F16_>), dim3((unsigned)groups), dim3(256), 0, st, p);               \
+#define SPRUCE_LAUNCH(KERNEL, GRID, THREADS)                                                  \
+  do {                                                                                        \
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)(GRID)), dim3(THREADS), 0, st, p);              \
+    const int e = check_launch("paged attention");                                            \
+    if (e) return e;                                                                          \
+  } while (0)
+#define SPRUCE_PAGED(D_, F16_)                                                                \
+  do {                                                                                        \
+    if (bounds.many_units > 0) {                                                              \
+      if (aligned)                                                                            \
+        SPRUCE_LAUNCH((paged_many_kernel<D_, F16_, true>), bounds.many_units, kWaves * 64);   \
+      else                                                                                    \
+        SPRUCE_LAUNCH((paged_many_kernel<D_, F16_, false>), bounds.many_units, kWaves * 64);  \
+    }                                                                                         \
+    if (bounds.few_units > 0)                                                                 \
+      SPRUCE_LAUNCH((paged_few_kernel<D_, F16_>), bounds.few_units, kWaves * 64);             \
+    SPRUCE_LAUNCH((paged_join_kernel<D_, F16_>), groups, 256);                                \
   } while (0)
   if (D == 128) {
     if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_PAGED(128, false);
@@ -1135,5 +1163,6 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
     else SPRUCE_PAGED(64, true);
   }
 #undef SPRUCE_PAGED
-  return check_launch("paged_join_kernel");
+#undef SPRUCE_LAUNCH
+  return SPRUCE_OK;
 }
