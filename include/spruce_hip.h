@@ -758,11 +758,12 @@ int spruce_paged_append(const void* q, const int64_t qs[3], void* qo, const int6
  * included, reaches no row.  Rows of no sequence are left alone.
  *   q, out [N, Hq, D] (strides qs, os), bf16 / f16, D in {64, 128}, at most 64
  *   query heads per KV head, scale > 0; rows 16-byte aligned.
- *   workspace: spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D, K)
- *   bytes, 16-byte aligned, one call's own until it is done (long rows are
+ *   workspace: spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D,
+ *   table_width * page_size, K) bytes, 16-byte aligned, one call's own until it is done (long rows are
  *   split over workgroups and joined from there).
  */
-int64_t spruce_paged_attention_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t K);
+int64_t spruce_paged_attention_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                               int64_t keys, int64_t K);
 int spruce_paged_attention(const void* q, const int64_t qs[3], const void* k_pages, const int64_t kps[4],
                            const void* v_pages, const int64_t vps[4], int64_t pages, int64_t page_size,
                            const int32_t* page_table, int64_t table_stride, int64_t table_width,

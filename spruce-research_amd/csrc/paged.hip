@@ -34,25 +34,23 @@ struct PagedAttn {
   const int32_t* idx;  // block lists [S, Hkv, Qc, K], or null
   int64_t is[3];
   int Qc, K;
+  int few_limit;   // packed rows of a sequence up to which it goes the few-row way
+  bool whole[2];   // few, many: a workgroup takes one row tile whole
   float* part_o;   // [groups][32 * D], a 32 x 32 accumulator's order
   float* part_ml;  // [groups][2][32]
-  int many_units, few_units;  // units of either kind that have partial slots
 };
 
 constexpr int kWaves = 8;
-constexpr int kFewRows = 64;     // packed rows of a sequence up to which it takes the few-row way
-constexpr int kCus = 256;
-constexpr int kFewSlots = 512;   // few-row units that the splits aim at
-constexpr int kManySlots = 768;  // and the most many-row units that splitting may make
+constexpr int kFewRows = 64;    // packed rows of a sequence up to which memory bounds it
+constexpr int kGroups = 256;    // workgroups that share the keys out: one a CU, its registers' fill
+constexpr int kRowCost = 256;   // a row tile's fixed part (first loads, last sums, store), in keys
 
-// Unit shapes: rows of a unit, and keys of a step, its unit of work.
+// Unit shapes: packed rows of a tile.
 struct Few {
-  static constexpr bool many = false;
-  static constexpr int rows = 32, step = 32 * kWaves;
+  static constexpr int rows = 32;
 };
 struct Many {
-  static constexpr bool many = true;
-  static constexpr int rows = 32 * kWaves, step = kBlock;
+  static constexpr int rows = 32 * kWaves;
 };
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
@@ -76,16 +74,27 @@ __device__ __forceinline__ f32x4v mfma16x16x32(u32x4 a, u32x4 b, f32x4v c) {
 // scalar unit around matrix instructions, which run whatever EXEC holds.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Sum of v over the lanes up to this one (row shifts within 16 lanes, then
-// the rows' last lanes broadcast onward).
-__device__ __forceinline__ int wave_prefix(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+// The lane below's value by `n` (row shifts within 16 lanes, then the rows'
+// last lanes onward), zero from outside: the steps of a prefix sum.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t shifted(int64_t v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+// Sum of v over the lanes up to this one.
+__device__ __forceinline__ int64_t wave_prefix(int64_t v) {
+  v += shifted<0x111, 0xf>(v);
+  v += shifted<0x112, 0xf>(v);
+  v += shifted<0x114, 0xf>(v);
+  v += shifted<0x118, 0xf>(v);
+  v += shifted<0x142, 0xa>(v);
+  v += shifted<0x143, 0xc>(v);
   return v;
+}
+__device__ __forceinline__ int64_t lane_of(int64_t v, int l) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) |
+                   (uint32_t)__builtin_amdgcn_readlane((int)v, l));
 }
 
 // A key of a tile, or the last key below `end` where it lies past that.
@@ -96,148 +105,166 @@ __device__ __forceinline__ int clip(int64_t pos) {
   return pos < 0 ? -1 : (pos < 0x7fffffff ? (int)pos : 0x7fffffff);
 }
 
-// The work of one sequence: its kind, row tiles per KV head, and key steps of each.
+// The work of one sequence, of one kind: its row tiles per KV head, and how
+// they weigh.  Tile j weighs first + slope (j + 1): its keys, and kRowCost.
+// (An upper bound of the keys: what a tile does not have, nobody walks.)
 struct SeqWork {
   int n;         // new tokens
   int64_t pos0;  // position of the first
-  bool many;
-  int tiles, steps;
-  int sub, rows;  // with lists: tiles of one 64-position block, and rows of one
+  int tiles;     // 0 where the sequence is of the other kind
+  int per;       // tokens of a tile (0: a tile is a part of one token's heads)
+  int sub, rows;  // tiles of one token or listed block, and rows of one
+  int64_t first, slope;
+  __device__ __forceinline__ int64_t before(int64_t j) const { return first * j + slope * (j * (j + 1) / 2); }
 };
 
 template <typename SHAPE>
-__device__ __forceinline__ void tile_sequence(const PagedAttn& p, int s, SeqWork& w) {
+__device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
+  constexpr bool kMany = SHAPE::rows > Few::rows;
+  SeqWork w{};
+  if (s >= p.batch.S) return w;
+  const int a = start_at(p.batch, s), e = start_at(p.batch, s + 1);
+  w.n = e > a ? e - a : 0;
+  // Positions go by the lengths as given; only what they address is bounded.
+  const int starts = p.batch.q_starts[s], ends = p.batch.q_starts[s + 1], keys = p.batch.kv_lens[s];
+  w.pos0 = (int64_t)keys - ((int64_t)ends - starts) + ((int64_t)a - starts);
+  if (w.n == 0 || ((int64_t)w.n * p.G > p.few_limit) != kMany) return w;
+  int64_t base = w.pos0 < 0 ? 0 : (w.pos0 < p.batch.cap ? w.pos0 : p.batch.cap);
   if (p.idx != nullptr) {
     const int64_t b0 = w.pos0 >> 6, b1 = (w.pos0 + w.n - 1) >> 6;
     const int rows = (w.n < kBlock ? w.n : kBlock) * p.G;
     w.sub = (rows + SHAPE::rows - 1) / SHAPE::rows;
     w.rows = ((rows + 31) / 32 + w.sub - 1) / w.sub * 32;  // shared out evenly
     w.tiles = (int)(b1 - b0 + 1) * w.sub;
-    w.steps = (int)(((int64_t)p.K * kBlock + SHAPE::step - 1) / SHAPE::step);
+    base = (int64_t)p.K * kBlock;
+  } else if (p.G <= SHAPE::rows) {
+    // Whole tokens to a tile: what the tiles see then grows evenly.
+    w.per = SHAPE::rows / p.G;
+    w.rows = w.per * p.G;
+    w.tiles = (w.n + w.per - 1) / w.per;
+    w.slope = w.per;
   } else {
-    w.sub = 1;
+    w.sub = (p.G + SHAPE::rows - 1) / SHAPE::rows;
     w.rows = SHAPE::rows;
-    w.tiles = (int)(((int64_t)w.n * p.G + SHAPE::rows - 1) / SHAPE::rows);
-    w.steps = (keys_of(p.batch, s) + SHAPE::step - 1) / SHAPE::step;
+    w.tiles = w.n * w.sub;
+    base += w.n;
   }
-  if (w.steps < 1) w.steps = 1;
-}
-
-__device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
-  SeqWork w{};
-  if (s >= p.batch.S) return w;
-  const int a = start_at(p.batch, s), e = start_at(p.batch, s + 1);
-  w.n = e > a ? e - a : 0;
-  // Positions go by the lengths as given; only what they address is bounded.
-  w.pos0 = (int64_t)p.batch.kv_lens[s] - ((int64_t)p.batch.q_starts[s + 1] - p.batch.q_starts[s]) +
-           ((int64_t)a - p.batch.q_starts[s]);
-  if (w.n == 0) return w;
-  w.many = (int64_t)w.n * p.G > kFewRows;
-  if (w.many)
-    tile_sequence<Many>(p, s, w);
-  else
-    tile_sequence<Few>(p, s, w);
+  w.first = base + kRowCost;
+  if (p.whole[kMany]) {
+    w.first = 1;
+    w.slope = 0;
+  }
   return w;
 }
 
-// How many steps a unit takes of its row tile at most, for either kind; every
-// workgroup works this out from the lengths, 64 sequences at a time.
-// Few rows: about kFewSlots units of equal size.
-__device__ __forceinline__ int few_pace(const PagedAttn& p, int lane) {
-  int64_t work = 0;
-  for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
-    const SeqWork w = sequence_work(p, s0 + lane);
-    work += w.many ? 0 : (int64_t)w.tiles * w.steps;
-  }
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) work += __shfl_xor(work, m);
-  const int64_t per = (work * p.Hkv + kFewSlots - 1) / kFewSlots;
-  return uniform((int)(per < 1 ? 1 : (per < (1 << 30) ? per : 1 << 30)));
-}
+// What a workgroup works on: all tiles of all sequences of one kind stand in
+// one line, each as long as it weighs, sequence by sequence, head by head,
+// tile by tile, and the workgroups share the line out evenly, whatever the
+// lengths are.  A stretch may end within a tile; the sums of such parts go to
+// the workgroup's two slots and are joined afterwards.  (Whole tiles: each
+// weighs one, and each is a workgroup's stretch.)
+struct Line {
+  int64_t total, share;
+};
 
-// Many rows: lane l weighs l + 1 splits of the average tile.  A split costs
-// its blocks and a fixed part worth about eight more (first loads, last
-// reduction, store) and four for its part in the join; CUs take one unit at a
-// time.
-__device__ __forceinline__ int many_pace(const PagedAttn& p, int lane) {
-  int64_t work = 0, tiles = 0;
+template <typename SHAPE>
+__device__ __forceinline__ Line line_of(const PagedAttn& p, int lane) {
+  Line line{0, 1};
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
-    const SeqWork w = sequence_work(p, s0 + lane);
-    work += w.many ? (int64_t)w.tiles * w.steps : 0;
-    tiles += w.many ? w.tiles : 0;
+    const SeqWork w = sequence_work<SHAPE>(p, s0 + lane);
+    line.total += lane_of(wave_prefix(w.before(w.tiles) * p.Hkv), 63);
   }
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) {
-    work += __shfl_xor(work, m);
-    tiles += __shfl_xor(tiles, m);
+  if (!p.whole[SHAPE::rows > Few::rows]) {
+    // Parts below kRowCost + 256 keys cost more than they save.
+    line.share = (line.total + kGroups - 1) / kGroups;
+    if (line.share < kRowCost + 256) line.share = kRowCost + 256;
   }
-  const int64_t units = tiles * p.Hkv;
-  if (units == 0 || units * 2 > kManySlots) return 1 << 30;
-  const int avg = (int)(work / tiles);
-  const int ns = lane + 1, part = (avg + ns - 1) / ns;
-  const int rounds = (int)((units * ns + kCus - 1) / kCus);
-  uint32_t cost = (uint32_t)rounds * (uint32_t)(part + 8 + (ns > 1 ? 4 : 0));
-  if (units * ns > kManySlots || ns > avg || cost >= 1u << 25) cost = (1u << 25) - 1;
-  uint32_t best = cost << 6 | (uint32_t)lane;
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)best, m);
-    best = o < best ? o : best;
-  }
-  const int n = (int)(best & 63) + 1;
-  return uniform(n == 1 ? 1 << 30 : (avg + n - 1) / n);
+  return line;
 }
 
 struct Unit {
-  int s, tile, g, split, splits;
-  int first, stride;  // unit of split 0 of this tile and head, and from split to split
-  int n, steps, sub, rows;
-  int64_t pos0;
+  int s, tile, g;
+  int64_t start, end;  // of the tile in the line
+  SeqWork w;
 };
 
-// The unit `want` of one kind, counted with its splits (BY_TILE false), or
-// the (tile, head) `want` counted without.  Past the last: false, and `want`
-// less by how many there are.
-template <bool MANY, bool BY_TILE>
-__device__ __forceinline__ bool find_unit(const PagedAttn& p, int& want, int per, int lane, Unit& u) {
-  int units = 0, tiles = 0;
+// The tile at place `at` of the line, or the at-th tile (BY_TILE, `at` a count).  False
+// behind the last, with `at` less by how many there are.
+template <typename SHAPE, bool BY_TILE>
+__device__ __forceinline__ bool find_unit(const PagedAttn& p, int64_t& at, int lane, Unit& u) {
+  int64_t places = 0, count = 0;
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
-    const SeqWork w = sequence_work(p, s0 + lane);
-    const bool kind = w.many == MANY;
-    const int splits = (w.steps + per - 1) / per;
-    const int mt = kind ? w.tiles * p.Hkv : 0, mu = mt * splits;
-    const int pt = wave_prefix(mt), pu = wave_prefix(mu);
-    const int mine = BY_TILE ? tiles + pt : units + pu;
-    const uint64_t past = __ballot(mine > want);
+    const SeqWork w = sequence_work<SHAPE>(p, s0 + lane);
+    const int64_t head = w.before(w.tiles);  // one head's length
+    const int64_t pp = wave_prefix(head * p.Hkv), pc = BY_TILE ? wave_prefix((int64_t)w.tiles * p.Hkv) : 0;
+    const uint64_t past = __ballot((BY_TILE ? count + pc : places + pp) > at);
     if (past) {
       const int l = __builtin_ctzll(past);
-      const int th = __builtin_amdgcn_readlane(mt, l);
       u.s = s0 + l;
-      u.splits = __builtin_amdgcn_readlane(splits, l);
-      u.n = __builtin_amdgcn_readlane(w.n, l);
-      u.pos0 = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w.pos0 >> 32), l) << 32) |
-                         (uint32_t)__builtin_amdgcn_readlane((int)w.pos0, l));
-      u.steps = __builtin_amdgcn_readlane(w.steps, l);
-      u.sub = __builtin_amdgcn_readlane(w.sub, l);
-      u.rows = __builtin_amdgcn_readlane(w.rows, l);
-      const int before = units + __builtin_amdgcn_readlane(pu, l) - th * u.splits;
-      const int in = want - (BY_TILE ? tiles + __builtin_amdgcn_readlane(pt, l) - th : before);
-      if (th <= 0 || in < 0 || in >= th * (BY_TILE ? 1 : u.splits)) return false;  // starts that overlap
-      // Within a sequence: split slowest, then tile, head fastest: the eight
-      // XCDs take units in turn, so each L2 serves one head where Hkv divides 8.
-      u.split = BY_TILE ? 0 : uniform(in / th);
-      const int r = in - u.split * th;
-      u.tile = uniform(r / p.Hkv);
-      u.g = r - u.tile * p.Hkv;
-      u.first = before + r;
-      u.stride = th;
+      u.w.n = __builtin_amdgcn_readlane(w.n, l);
+      u.w.pos0 = lane_of(w.pos0, l);
+      u.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
+      u.w.per = __builtin_amdgcn_readlane(w.per, l);
+      u.w.sub = __builtin_amdgcn_readlane(w.sub, l);
+      u.w.rows = __builtin_amdgcn_readlane(w.rows, l);
+      u.w.first = lane_of(w.first, l);
+      u.w.slope = lane_of(w.slope, l);
+      const int64_t one = lane_of(head, l);
+      const int64_t origin = places + lane_of(pp, l) - one * p.Hkv;
+      if (u.w.tiles <= 0) return false;
+      if constexpr (BY_TILE) {
+        const int64_t in = at - (count + lane_of(pc, l) - (int64_t)u.w.tiles * p.Hkv);
+        u.g = uniform((int)(in / u.w.tiles));
+        u.tile = uniform((int)(in - (int64_t)u.g * u.w.tiles));
+      } else {
+        const int64_t in = at - origin;
+        u.g = uniform((int)(in / one));
+        const int64_t y = in - u.g * one;
+        // The tile j with before(j) <= y < before(j + 1).
+        int j;
+        if (u.w.slope == 0) {
+          j = (int)(y / u.w.first);
+        } else {
+          const double b = (double)u.w.first + 0.5 * (double)u.w.slope;
+          j = (int)((sqrt(b * b + 2.0 * (double)u.w.slope * (double)y) - b) / (double)u.w.slope);
+          j = j < 0 ? 0 : (j < u.w.tiles ? j : u.w.tiles - 1);
+          while (j > 0 && u.w.before(j) > y) --j;
+          while (j + 1 < u.w.tiles && u.w.before(j + 1) <= y) ++j;
+        }
+        u.tile = uniform(j);
+      }
+      if (u.g < 0 || u.g >= p.Hkv || u.tile < 0 || u.tile >= u.w.tiles) return false;  // starts that overlap
+      u.start = origin + u.g * one + u.w.before(u.tile);
+      u.end = origin + u.g * one + u.w.before(u.tile + 1);
       return true;
     }
-    tiles += __builtin_amdgcn_readlane(pt, 63);
-    units += __builtin_amdgcn_readlane(pu, 63);
+    places += lane_of(pp, 63);
+    if (BY_TILE) count += lane_of(pc, 63);
   }
-  want -= BY_TILE ? tiles : units;
+  at -= BY_TILE ? count : places;
   return false;
+}
+
+// A workgroup's part of a tile: tiles of KEYS keys [lo, hi) of the row's keys
+// or list, and its slot for the sums (-1: it holds the tile whole).
+struct Part {
+  int lo, hi, slot;
+};
+
+template <int KEYS>
+__device__ __forceinline__ Part part_of(const Line& line, const Unit& u, int64_t from, int64_t to, int64_t group) {
+  Part part{0, 0x7fffffff, -1};
+  if (from > u.start || to < u.end) {
+    // Neighbours round the border between them alike.
+    auto border = [&](int64_t at) {
+      const int64_t key = at - u.start - kRowCost;
+      return key <= 0 ? 0 : (int)((key + KEYS - 1) / KEYS);
+    };
+    part.lo = uniform(border(from));
+    if (to < u.end) part.hi = uniform(border(to));
+    part.slot = uniform((int)(2 * group + (from > group * line.share ? 1 : 0)));
+  }
+  return part;
 }
 
 // Rows [row0, row0 + rows) of a unit in the sequence's packed rows, the block
@@ -249,26 +276,27 @@ struct TileRows {
 
 __device__ __forceinline__ TileRows tile_rows(const PagedAttn& p, const Unit& u) {
   TileRows t{};
-  if (p.idx == nullptr) {
-    // The last tiles see the most keys: they come first.
-    const int tiles = u.stride / p.Hkv;
-    t.row0 = (tiles - 1 - u.tile) * u.rows;
-    const int left = u.n * p.G - t.row0;
-    t.rows = left < u.rows ? left : u.rows;
-  } else {
-    const int bi = u.tile / u.sub, sub = u.tile - bi * u.sub;
-    const int64_t lo = (((u.pos0 >> 6) + bi) << 6) - u.pos0;
+  int left;
+  if (p.idx != nullptr) {
+    const int bi = u.tile / u.w.sub, sub = u.tile - bi * u.w.sub;
+    const int64_t lo = (((u.w.pos0 >> 6) + bi) << 6) - u.w.pos0;
     const int t0 = lo < 0 ? 0 : (int)lo;
-    const int t1 = lo + kBlock < u.n ? (int)(lo + kBlock) : u.n;
-    t.row0 = t0 * p.G + sub * u.rows;
-    const int left = t1 * p.G - t.row0;
-    t.rows = left < 0 ? 0 : (left < u.rows ? left : u.rows);
+    const int t1 = lo + kBlock < u.w.n ? (int)(lo + kBlock) : u.w.n;
+    t.row0 = t0 * p.G + sub * u.w.rows;
+    left = t1 * p.G - t.row0;
     t.list = bi < p.Qc ? p.idx + (int64_t)u.s * p.is[0] + (int64_t)u.g * p.is[1] + (int64_t)bi * p.is[2] : nullptr;
+  } else if (u.w.per > 0) {
+    t.row0 = u.tile * u.w.rows;
+    left = u.w.n * p.G - t.row0;
+  } else {
+    const int token = u.tile / u.w.sub;
+    t.row0 = token * p.G + (u.tile - token * u.w.sub) * u.w.rows;
+    left = (token + 1) * p.G - t.row0;
   }
-  const int64_t last = u.pos0 + (t.row0 + t.rows - 1) / p.G;
-  t.end = uniform(last < 0 || p.batch.pages == 0 ? 0 : (last + 1 < p.batch.cap ? (int)(last + 1) : p.batch.cap));
+  t.rows = uniform(left < 0 ? 0 : (left < u.w.rows ? left : u.w.rows));
   t.row0 = uniform(t.row0);
-  t.rows = uniform(t.rows);
+  const int64_t last = u.w.pos0 + (t.row0 + t.rows - 1) / p.G;
+  t.end = uniform(last < 0 || p.batch.pages == 0 ? 0 : (last + 1 < p.batch.cap ? (int)(last + 1) : p.batch.cap));
   return t;
 }
 
@@ -365,7 +393,7 @@ constexpr int many_lds_bytes() {
 // operand, is S^T's accumulator as it lies (keys 4 (l / 16) + r).  The next
 // tile's K is in flight from the last S^T on, its V from the LDS write on.
 template <int D, bool F16>
-__device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int unit, int per, char* smem) {
+__device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, const Part& part, char* smem) {
   constexpr int KK = D / 32;   // steps of S^T over d
   constexpr int DT = D / 16;   // 16-row tiles of O^T
   constexpr int VSTR = D + 8;  // V rows in LDS, 16-bit elements
@@ -388,17 +416,16 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
   for (int c = 0; c < 2; ++c) {
     const int r = tr.row0 + (16 * c + l16 < tr.rows ? 16 * c + l16 : tr.rows - 1);
     const int t = r / p.G, h = r - t * p.G;
-    qpos[c] = clip(u.pos0 + t);
+    qpos[c] = clip(u.w.pos0 + t);
     const uint16_t* src = static_cast<const uint16_t*>(p.q) + (int64_t)(token0 + t) * p.qs[0] +
                           (int64_t)(u.g * p.G + h) * p.qs[1] + 8 * g4;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
       qf[c][kk] = load16(src + 32 * kk);
   }
-  const int first_pos = uniform(clip(u.pos0 + tr.row0 / p.G));
+  const int first_pos = uniform(clip(u.w.pos0 + tr.row0 / p.G));
   const int items = p.idx ? 2 * p.K : (tr.end + 31) / 32;
-  const int lo = u.split * per * kWaves;
-  const int hi = (int64_t)lo + (int64_t)per * kWaves < items ? lo + per * kWaves : items;
+  const int hi = part.hi < items ? part.hi : items;
 
   const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)u.g * p.ks[1] + 8 * g4;
   const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1] + 8 * g4;
@@ -436,7 +463,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
       for (int dt = 0; dt < DT; ++dt) acc[c][dt] = f32x4v{};
     }
     KeyWalk<32> walk;
-    walk.init(p, tr, lo + wave, kWaves, hi, lane);
+    walk.init(p, tr, part.lo + wave, kWaves, hi, lane);
     int pg[2], pn[2];
     u32x4 kx[2][KK], vx[2][KK];
     int key0 = walk.next();
@@ -462,12 +489,12 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
             for (int kk = 0; kk < KK; ++kk) s[c][kt] = mfma16x16x32<F16>(kx[kt][kk], qf[c][kk], s[c][kt]);
         }
       if (nkey >= 0) load(kbase, p.ks, nkey, pn, kx);
-      const bool part = have != 0xffffffffu || key0 + 31 > first_pos;
+      const bool masked = have != 0xffffffffu || key0 + 31 > first_pos;
       u32x4 pk[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (c == 1 && !two) break;
-        if (part) {
+        if (masked) {
           const uint32_t mine = have >> (4 * g4);
           const int rel = qpos[c] - key0 - 4 * g4;
 #pragma unroll
@@ -506,7 +533,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
       wave_lds_fence();
       if (nkey >= 0) load(vbase, p.vs, nkey, pn, vx);
       const uint16_t* vt = vl + (4 * g4 + (l16 >> 2)) * VSTR + 4 * (l16 & 3);
-      if (CAREFUL && part) {
+      if (CAREFUL && masked) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (c == 1 && !two) break;
@@ -600,8 +627,8 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
 #pragma unroll
       for (int i = 0; i < PER; ++i) o[i] += f * ol[(w * 16 + r) * OSTR + d0 + i];
     }
-    if (u.splits > 1) {
-      const int64_t group = (int64_t)p.many_units * kWaves + unit;
+    if (part.slot >= 0) {
+      const int64_t group = part.slot;
       float* po = p.part_o + group * 32 * D + part_at(row, d0);
 #pragma unroll
       for (int i = 0; i < PER; ++i) po[i] = o[i];
@@ -630,7 +657,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, int 
 // page holds whole blocks, so a block is one piece of memory behind one buffer
 // descriptor; otherwise every row finds its own page.
 template <int D, bool F16, bool ALIGNED>
-__device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int unit, int per, char* smem) {
+__device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, const Part& part, char* smem) {
   constexpr int NTHR = kWaves * 64;
   constexpr int KSTR = D + 8, VSTR = D + 32;  // LDS rows; V rows start 16 banks apart
   constexpr int KTILE = kBlock * KSTR, BUF = KTILE + kBlock * VSTR;
@@ -648,10 +675,10 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
   // Columns past the last row repeat it; a wave without rows has the unit's first.
   const int row = tr.row0 + (nrow == 0 ? 0 : 32 * wave + (l32 < nrow ? l32 : nrow - 1));
   const int tok = row / p.G, head = u.g * p.G + row - tok * p.G;
-  const int qpos = clip(u.pos0 + tok);
+  const int qpos = clip(u.w.pos0 + tok);
   // Positions of the wave's first and last row.
-  const int pos_lo = uniform(clip(u.pos0 + (tr.row0 + 32 * wave) / p.G));
-  const int pos_hi = uniform(clip(u.pos0 + (tr.row0 + 32 * wave + (nrow > 0 ? nrow - 1 : 0)) / p.G));
+  const int pos_lo = uniform(clip(u.w.pos0 + (tr.row0 + 32 * wave) / p.G));
+  const int pos_hi = uniform(clip(u.w.pos0 + (tr.row0 + 32 * wave + (nrow > 0 ? nrow - 1 : 0)) / p.G));
 
   uint4 qf[KS];
   {
@@ -662,9 +689,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
       qf[kk] = *reinterpret_cast<const uint4*>(src + 16 * kk);
   }
   const int items = p.idx ? p.K : (tr.end + kBlock - 1) / kBlock;
-  const int64_t lo64 = (int64_t)u.split * per;
-  const int lo = lo64 < items ? (int)lo64 : items;
-  const int hi = lo64 + per < items ? (int)(lo64 + per) : items;
+  const int hi = part.hi < items ? part.hi : items;
 
   const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)u.g * p.ks[1];
   const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1];
@@ -742,8 +767,8 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
     }
   };
   // Register r of key half c holds key 32 c + 8 (r / 4) + 4 (lane / 32) + r % 4.
-  auto softmax = [&](f32x16_t& s0, f32x16_t& s1, bool part, int rel, uint64_t there) {
-    if (part) {
+  auto softmax = [&](f32x16_t& s0, f32x16_t& s1, bool masked, int rel, uint64_t there) {
+    if (masked) {
       const uint32_t lo_bits = (uint32_t)there >> (4 * hl), hi_bits = (uint32_t)(there >> 32) >> (4 * hl);
       const int thr = rel - 4 * hl;
 #pragma unroll
@@ -854,7 +879,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16_t{};
     KeyWalk<kBlock> walk;
-    walk.init(p, tr, lo, 1, hi, lane);
+    walk.init(p, tr, part.lo, 1, hi, lane);
     auto take = [&](int& key0, int& pg) {
       key0 = walk.next();
       pg = page_at(key0);
@@ -876,12 +901,12 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
           // Bits of the keys with a page and a position below the end.
           uint64_t there = ALIGNED ? (uniform(pg) < 0 ? 0 : ~0ull) : __ballot(pg >= 0);
           if (tr.end - key0 < kBlock) there &= (1ull << (tr.end - key0)) - 1;
-          const bool part = there != ~0ull || key0 + kBlock - 1 > pos_lo;
+          const bool masked = there != ~0ull || key0 + kBlock - 1 > pos_lo;
           const int rel = qpos < key0 ? -1 : qpos - key0;
           f32x16_t s0, s1;
           scores(ks, s0, s1);
-          softmax(s0, s1, part, rel, there);
-          if (CAREFUL && part)
+          softmax(s0, s1, masked, rel, there);
+          if (CAREFUL && masked)
             pv_careful(ks + KTILE, rel, there);
           else
             pv(ks + KTILE);
@@ -911,8 +936,8 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
   }
 
   l = half_sum(l);
-  if (u.splits > 1) {
-    const int64_t group = (int64_t)unit * kWaves + wave;
+  if (part.slot >= 0) {
+    const int64_t group = (int64_t)part.slot * kWaves + wave;
     if (nrow == 0) return;
     float* po = p.part_o + group * 32 * D + lane * 4;
 #pragma unroll
@@ -956,66 +981,72 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, int
 
 // A launch for either kind: the lengths that tell them apart are on the
 // device, so the workgroups of a kind that the batch does not hold find no
-// unit and end.  (Both in one kernel needed more registers than there are.)
+// tile and end.  (Both in one kernel needed more registers than there are.)
+// Workgroups go to the eight XCDs in turn; the line is dealt so that each XCD
+// has one stretch of it, and mostly one head's keys, in its L2.
+template <typename SHAPE, int KEYS, typename BODY>
+__device__ __forceinline__ void walk_line(const PagedAttn& p, BODY body) {
+  const int lane = threadIdx.x & 63;
+  const Line line = line_of<SHAPE>(p, lane);
+  int64_t group = blockIdx.x;
+  if (!p.whole[SHAPE::rows > Few::rows]) group = (group & 7) * (kGroups / 8) + (group >> 3);
+  int64_t at = group * line.share;
+  const int64_t end = at + line.share < line.total ? at + line.share : line.total;
+  while (at < end) {
+    Unit u;
+    int64_t place = at;
+    if (!find_unit<SHAPE, false>(p, place, lane, u)) return;
+    const int64_t to = u.end < end ? u.end : end;
+    body(u, part_of<KEYS>(line, u, at, to, group));
+    at = to;
+    if (at < end) __syncthreads();  // the tile's LDS is free
+  }
+}
+
 template <int D, bool F16>
 __global__ __launch_bounds__(kWaves * 64, 2) void paged_few_kernel(const PagedAttn p) {
   __shared__ __attribute__((aligned(16))) char smem[few_lds_bytes<D>()];
-  const int lane = threadIdx.x & 63;
-  const int per = few_pace(p, lane);
-  int want = blockIdx.x;
-  Unit u;
-  if (!find_unit<false, false>(p, want, per, lane, u)) return;
-  if (u.splits > 1 && want >= p.few_units) return;  // starts that overlap
-  few_rows<D, F16>(p, u, want, per, smem);
+  walk_line<Few, 32>(p, [&](const Unit& u, const Part& part) { few_rows<D, F16>(p, u, part, smem); });
 }
 
 template <int D, bool F16, bool ALIGNED>
 __global__ __launch_bounds__(kWaves * 64, 2) void paged_many_kernel(const PagedAttn p) {
   __shared__ __attribute__((aligned(16))) char smem[many_lds_bytes<D>()];
-  const int lane = threadIdx.x & 63;
-  const int per = many_pace(p, lane);
-  int want = blockIdx.x;
-  Unit u;
-  if (!find_unit<true, false>(p, want, per, lane, u)) return;
-  if (u.splits > 1 && want >= p.many_units) return;  // starts that overlap
-  many_rows<D, F16, ALIGNED>(p, u, want, per, smem);
+  walk_line<Many, kBlock>(p, [&](const Unit& u, const Part& part) { many_rows<D, F16, ALIGNED>(p, u, part, smem); });
 }
 
-// Joins the splits of one 32-row group: every thread takes 4 values of its
+// Joins the parts of one 32-row group of a tile: every thread takes 4 values of its
 // row from every eighth of d.
-template <int D, bool F16>
+template <typename SHAPE, int D, bool F16>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn p) {
+  constexpr int kTileGroups = SHAPE::rows / 32;
   const int lane = threadIdx.x & 63;
-  // Groups in order: eight to a many-row tile, then one to a few-row tile.
-  int want = blockIdx.x / kWaves, sub = blockIdx.x % kWaves;
+  const Line line = line_of<SHAPE>(p, lane);
+  int64_t tile = blockIdx.x / kTileGroups;
+  const int sub = blockIdx.x % kTileGroups;
   Unit u;
-  const bool many = find_unit<true, true>(p, want, many_pace(p, lane), lane, u);
-  if (!many) {
-    want = want * kWaves + sub;
-    sub = 0;
-    if (!find_unit<false, true>(p, want, few_pace(p, lane), lane, u)) return;
-  }
-  if (u.splits == 1) return;
-  if (u.first + (int64_t)(u.splits - 1) * u.stride >= (many ? p.many_units : p.few_units)) return;  // starts that overlap
+  if (!find_unit<SHAPE, true>(p, tile, lane, u)) return;
+  const int64_t g0 = u.start / line.share, g1 = (u.end - 1) / line.share;
+  if (g0 == g1 || g1 >= kGroups) return;  // held whole (or starts that overlap)
   const TileRows tr = tile_rows(p, u);
   const int row = lane & 31, hl = lane >> 5, wave = threadIdx.x >> 6;
   const int r = sub * 32 + row;
   if (r >= tr.rows) return;
-  const int64_t group0 = many ? (int64_t)u.first * kWaves + sub : (int64_t)p.many_units * kWaves + u.first;
-  const int64_t step = many ? (int64_t)u.stride * kWaves : u.stride;
+  // The part of group g: the one that starts its stretch, or the one behind.
+  auto part = [&](int64_t g) { return (2 * g + (g == g0 && u.start > g0 * line.share ? 1 : 0)) * kTileGroups + sub; };
   float top = -INFINITY;
-  for (int i = 0; i < u.splits; ++i) top = fmaxf(top, p.part_ml[(group0 + i * step) * 64 + row]);
+  for (int64_t g = g0; g <= g1; ++g) top = fmaxf(top, p.part_ml[part(g) * 64 + row]);
   const float nm = top == -INFINITY ? 0.f : -top;
   constexpr int PIECES = D / 32;  // of 4 values: pieces wave, wave + 4 ..
   float sum = 0.f;
   f32x4v o[PIECES] = {};
-  for (int i = 0; i < u.splits; ++i) {
-    const int64_t group = group0 + i * step;
-    const float f = fast_exp2(p.part_ml[group * 64 + row] + nm);
-    sum += f * p.part_ml[group * 64 + 32 + row];
+  for (int64_t g = g0; g <= g1; ++g) {
+    const int64_t at = part(g);
+    const float f = fast_exp2(p.part_ml[at * 64 + row] + nm);
+    sum += f * p.part_ml[at * 64 + 32 + row];
 #pragma unroll
     for (int j = 0; j < PIECES; ++j)
-      o[j] += f * *reinterpret_cast<const f32x4v*>(p.part_o + group * 32 * D + (wave + 4 * j) * 256 + lane * 4);
+      o[j] += f * *reinterpret_cast<const f32x4v*>(p.part_o + at * 32 * D + (wave + 4 * j) * 256 + lane * 4);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int at = tr.row0 + r, t = at / p.G, h = at - t * p.G;
@@ -1027,46 +1058,61 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn p) {
         uint2{pack2<F16>(o[j][0] * inv, o[j][1] * inv), pack2<F16>(o[j][2] * inv, o[j][3] * inv)};
 }
 
-// Bounds of what a batch with N new tokens of S sequences can hold of either
-// kind, whatever its lengths are: (tile, head) pairs and units.
-struct Bounds {
-  int64_t many_tiles, many_units, few_tiles, few_units;
+// How a call is launched, and the most row tiles that a batch with N new
+// tokens of S sequences can hold of either kind, whatever its lengths are.
+struct Plan {
+  bool few, many, few_whole, many_whole;
+  int few_limit;
+  int64_t few_tiles, many_tiles;
 };
 
-Bounds bounds_of(int64_t N, int64_t S, int64_t G, int64_t Hkv, bool lists) {
-  Bounds b{};
-  const int64_t rows = N * G;
-  if (rows > kFewRows) {
-    // A many-row sequence has more than kFewRows rows, so there are few of them.
-    const int64_t seqs = S < rows / (kFewRows + 1) ? S : rows / (kFewRows + 1);
-    // Listed rows break at every 64 positions too.
-    b.many_tiles = !lists ? rows / Many::rows + seqs
-                          : (N / kBlock + 2 * seqs) * ((kBlock * G + Many::rows - 1) / Many::rows);
-    b.many_tiles *= Hkv;
-    b.many_units = b.many_tiles + (b.many_tiles < kManySlots ? kManySlots : b.many_tiles);
-  }
-  // Few-row tiles: up to kFewRows rows a sequence, each of whose tokens may
-  // stand in one of two blocks.
+template <typename SHAPE>
+int64_t tiles_bound(int64_t N, int64_t S, int64_t G, int64_t most, bool lists) {
+  // `most`: packed rows of one sequence at most; a sequence rounds up by one tile.
   const int64_t seqs = S < N ? S : N;
-  const int64_t most = (N < kFewRows / G ? N : kFewRows / G) * G;  // rows of one of them
-  b.few_tiles = most == 0 ? 0 : seqs * ((most + Few::rows - 1) / Few::rows) * (lists && most > G ? 2 : 1) * Hkv;
-  b.few_units = b.few_tiles == 0 ? 0 : b.few_tiles + kFewSlots;
-  return b;
+  if (lists) {
+    // Rows break at every 64 positions too.
+    const int64_t rows = most < kBlock * G ? most : kBlock * G;
+    return (N / kBlock + 2 * seqs) * ((rows + SHAPE::rows - 1) / SHAPE::rows);
+  }
+  if (G > SHAPE::rows) return N * ((G + SHAPE::rows - 1) / SHAPE::rows);
+  return N / (SHAPE::rows / G) + seqs;
 }
 
-int64_t workspace_of(const Bounds& b, int64_t D) {
-  // Splitting stops where there are units enough, so only the first many-row
-  // units can be split ones.
-  const int64_t many = b.many_units < 2 * kManySlots ? b.many_units : 2 * kManySlots;
-  return (many * kWaves + b.few_units) * 32 * (D + 2) * 4;
+Plan plan_of(int64_t N, int64_t S, int64_t G, int64_t Hkv, int64_t keys, bool lists) {
+  Plan plan{};
+  // The lengths are not known here, but every sequence has a new token in all
+  // but odd batches: where even one that has all others' is few rows, the
+  // few-row way is launched alone and takes whatever there is; likewise the
+  // many-row way where one sequence has all tokens.  (An idle launch is 5 to 15 us.)
+  const int64_t longest = N > S ? N - S + 1 : 1;
+  plan.few = S > 1 || N * G <= kFewRows;
+  plan.many = longest * G > kFewRows;
+  if (!plan.few && !plan.many) plan.few = true;
+  plan.few_limit = !plan.many ? 0x7fffffff : (plan.few ? kFewRows : -1);
+  if (plan.few) plan.few_tiles = tiles_bound<Few>(N, S, G, plan.many ? kFewRows : N * G, lists) * Hkv;
+  if (plan.many) plan.many_tiles = tiles_bound<Many>(N, S, G, N * G, lists) * Hkv;
+  // Rows of few keys are not worth a join, many tiles not a split.
+  plan.few_whole = keys <= 1024 || plan.few_tiles > 64 * kGroups;
+  plan.many_whole = keys <= 1024 || plan.many_tiles > 16 * kGroups;
+  return plan;
+}
+
+int64_t workspace_of(const Plan& plan, int64_t D) {
+  int64_t groups = 0;
+  if (plan.few && !plan.few_whole) groups = 2 * kGroups;
+  if (plan.many && !plan.many_whole) groups = 2 * kGroups * kWaves;
+  return (groups > 0 ? groups : 1) * 32 * (D + 2) * 4;
 }
 
 }  // namespace
 
 extern "C" int64_t spruce_paged_attention_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
-                                                          int64_t K) {
-  if (N < 1 || S < 1 || Hkv < 1 || Hq < Hkv || N >= (int64_t)1 << 30 || S >= (int64_t)1 << 20 || Hq >= 1 << 16) return 0;
-  return workspace_of(bounds_of(N, S, Hq / Hkv, Hkv, K > 0), D);
+                                                          int64_t keys, int64_t K) {
+  if (N < 1 || S < 1 || Hkv < 1 || Hq < Hkv || N >= (int64_t)1 << 30 || S >= (int64_t)1 << 20 || Hq >= 1 << 16 ||
+      D < 1 || D > 128)
+    return 0;
+  return workspace_of(plan_of(N, S, Hq / Hkv, Hkv, K > 0 ? K * kBlock : keys, K > 0), D);
 }
 
 extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const void* k_pages, const int64_t kps[4],
@@ -1102,8 +1148,8 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
   SPRUCE_REQUIRE(K >= 0 && K < (int64_t)1 << 24, "invalid list width %lld", (long long)K);
   SPRUCE_REQUIRE(K == 0 || (idx && is && Qc >= 0), "indices must be a non-null device pointer");
   SPRUCE_REQUIRE(K == 0 || is[3] == 1, "indices must have a contiguous final dimension");
-  const Bounds bounds = bounds_of(N, S, Hq / Hkv, Hkv, K > 0);
-  const int64_t need = workspace_of(bounds, D);
+  const Plan plan = plan_of(N, S, Hq / Hkv, Hkv, K > 0 ? K * kBlock : p.batch.cap, K > 0);
+  const int64_t need = workspace_of(plan, D);
   SPRUCE_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
                  (long long)workspace_bytes, (long long)need);
   SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
@@ -1128,12 +1174,13 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
     p.Qc = (int)(Qc < (int64_t)1 << 30 ? Qc : (int64_t)1 << 30);
     p.K = (int)K;
   }
-  const int64_t groups = bounds.many_tiles * kWaves + bounds.few_tiles;
-  SPRUCE_REQUIRE(bounds.many_units < (int64_t)1 << 22 && bounds.few_units < (int64_t)1 << 22 && groups < (int64_t)1 << 23, "too many tokens for one call");
-  p.many_units = (int)(bounds.many_units < 2 * kManySlots ? bounds.many_units : 2 * kManySlots);
-  p.few_units = (int)bounds.few_units;
+  SPRUCE_REQUIRE(plan.few_tiles < (int64_t)1 << 22 && plan.many_tiles < (int64_t)1 << 19, "too many tokens for one call");
+  p.few_limit = plan.few_limit;
+  p.whole[0] = plan.few_whole;
+  p.whole[1] = plan.many_whole;
+  // The kinds' launches follow one another, so they share the slots.
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + ((int64_t)p.many_units * kWaves + p.few_units) * 32 * D;
+  p.part_ml = p.part_o + need / (32 * (D + 2) * 4) * 32 * D;
   // Rows of a page's block behind one 32-bit buffer offset.
   const bool aligned = page_size % kBlock == 0 && kps[2] > 0 && vps[2] > 0 && kps[2] < 1 << 22 && vps[2] < 1 << 22;
   const hipStream_t st = (hipStream_t)stream;
@@ -1145,15 +1192,21 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
   } while (0)
 #define SPRUCE_PAGED(D_, F16_)                                                                \
   do {                                                                                        \
-    if (bounds.many_units > 0) {                                                              \
+    if (plan.many) {                                                                          \
+      const int64_t grid = plan.many_whole ? plan.many_tiles : kGroups;                       \
       if (aligned)                                                                            \
-        SPRUCE_LAUNCH((paged_many_kernel<D_, F16_, true>), bounds.many_units, kWaves * 64);   \
+        SPRUCE_LAUNCH((paged_many_kernel<D_, F16_, true>), grid, kWaves * 64);                \
       else                                                                                    \
-        SPRUCE_LAUNCH((paged_many_kernel<D_, F16_, false>), bounds.many_units, kWaves * 64);  \
+        SPRUCE_LAUNCH((paged_many_kernel<D_, F16_, false>), grid, kWaves * 64);               \
+      if (!plan.many_whole)                                                                   \
+        SPRUCE_LAUNCH((paged_join_kernel<Many, D_, F16_>), plan.many_tiles * kWaves, 256);    \
     }                                                                                         \
-    if (bounds.few_units > 0)                                                                 \
-      SPRUCE_LAUNCH((paged_few_kernel<D_, F16_>), bounds.few_units, kWaves * 64);             \
-    SPRUCE_LAUNCH((paged_join_kernel<D_, F16_>), groups, 256);                                \
+    if (plan.few) {                                                                           \
+      const int64_t grid = plan.few_whole ? plan.few_tiles : kGroups;                         \
+      SPRUCE_LAUNCH((paged_few_kernel<D_, F16_>), grid, kWaves * 64);                         \
+      if (!plan.few_whole)                                                                    \
+        SPRUCE_LAUNCH((paged_join_kernel<Few, D_, F16_>), plan.few_tiles, 256);               \
+    }                                                                                         \
   } while (0)
   if (D == 128) {
     if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_PAGED(128, false);

@@ -167,7 +167,7 @@ def paged_chunk_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, sc
     if out is None:
         out = torch.empty((N, Hq, D), device=q.device, dtype=q.dtype)
     lib = spruce_hip.lib()
-    need = lib.spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D, K)
+    need = lib.spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D, page_table.shape[1] * page_size, K)
     work = torch.empty(need, device=q.device, dtype=torch.uint8)
     with spruce_hip.on_device(q.device):
         rc = lib.spruce_paged_attention(

@@ -158,7 +158,7 @@ def lib():
         handle.spruce_select_flat_workspace_bytes.restype = _i64
         handle.spruce_select_flat_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64]
         handle.spruce_paged_attention_workspace_bytes.restype = _i64
-        handle.spruce_paged_attention_workspace_bytes.argtypes = [_i64] * 6
+        handle.spruce_paged_attention_workspace_bytes.argtypes = [_i64] * 7
         _lib = handle
     return _lib
 

@@ -208,7 +208,7 @@ def test_attention_refusals():
 
 def test_attention_entry_point_refuses_before_the_launch():
     lib, fake = spruce_hip.lib(), ctypes.c_void_p(1 << 20)
-    need = lib.spruce_paged_attention_workspace_bytes(8, 2, 4, 2, 128, 0)
+    need = lib.spruce_paged_attention_workspace_bytes(8, 2, 4, 2, 128, 64, 0)
     assert need > 0 and need % 16 == 0
 
     def call(D=128, dtype=0, Hq=4, scale=0.1, qs=(512, 128, 1), K=0, idx=None, is_=(1, 1, 1, 1), Qc=1, ws=fake,
