@@ -69,12 +69,13 @@ __device__ __forceinline__ int keys_of(const PagedBatch& b, int s) {
   return v < 0 ? 0 : (v > b.cap ? b.cap : v);
 }
 
-// The page that holds position pos (0 <= pos < cap) of sequence s, -1 where
-// the table names none.
-__device__ __forceinline__ int page_id(const PagedBatch& b, int s, int pos) {
-  const int v = b.table[(int64_t)s * b.table_stride + page_of(b, pos)];
-  return v >= 0 && v < b.pages ? v : -1;
+// The table's entry for position pos (0 <= pos < cap) of sequence s, and
+// whether it names a page: apart, so that a caller can look entries up ahead
+// and wait for them where it uses them.
+__device__ __forceinline__ int page_entry(const PagedBatch& b, int s, int pos) {
+  return b.table[(int64_t)s * b.table_stride + page_of(b, pos)];
 }
+__device__ __forceinline__ bool is_page(const PagedBatch& b, int entry) { return (uint32_t)entry < (uint32_t)b.pages; }
 
 // The sequence of packed row n, wave-uniform: the starts at or below n are
 // counted 64 at a time.  -1 for rows before the first or behind the last.

@@ -70,6 +70,30 @@ __device__ __forceinline__ f32x4v mfma16x16x32(u32x4 a, u32x4 b, f32x4v c) {
                                                    0, 0, 0);
 }
 
+// The kernel's arguments, read from memory again where they are next used:
+// kept in scalar registers over a loop that does not need them, they push out
+// what it does need.  (PagedAttn is the kernels' only argument.)
+template <typename T>
+__device__ __forceinline__ T* global(T* p) {
+  return (T*)(__attribute__((address_space(1))) T*)p;
+}
+__device__ __forceinline__ PagedAttn arguments(uintptr_t k) {
+  asm volatile("" : "+s"(k));
+  PagedAttn p = *(const PagedAttn*)(const __attribute__((address_space(4))) PagedAttn*)k;
+  // Pointers read from memory might point anywhere; these are global.
+  p.q = global(p.q);
+  p.out = global(p.out);
+  p.k = global(p.k);
+  p.v = global(p.v);
+  p.idx = global(p.idx);
+  p.part_o = global(p.part_o);
+  p.part_ml = global(p.part_ml);
+  p.batch.table = global(p.batch.table);
+  p.batch.q_starts = global(p.batch.q_starts);
+  p.batch.kv_lens = global(p.batch.kv_lens);
+  return p;
+}
+
 // The same value in every lane, for the compiler too: it must branch on the
 // scalar unit around matrix instructions, which run whatever EXEC holds.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -218,6 +242,17 @@ __device__ __forceinline__ bool find_unit(const PagedAttn& p, int64_t& at, int l
         u.tile = uniform((int)(in - (int64_t)u.g * u.w.tiles));
       } else {
         const int64_t in = at - origin;
+        if (p.whole[SHAPE::rows > Few::rows]) {
+          // The last tiles see the most keys and come first; heads in turn, so
+          // that each XCD's L2 serves one head where their number divides 8.
+          const int tile = (int)(in / p.Hkv);
+          u.g = uniform((int)(in - (int64_t)tile * p.Hkv));
+          u.tile = uniform(u.w.tiles - 1 - tile);
+          if (u.tile < 0) return false;  // starts that overlap
+          u.start = at;
+          u.end = at + 1;
+          return true;
+        }
         u.g = uniform((int)(in / one));
         const int64_t y = in - u.g * one;
         // The tile j with before(j) <= y < before(j + 1).
@@ -392,8 +427,14 @@ constexpr int many_lds_bytes() {
 // LDS, whose transposing read gives the A operand of O^T = V^T P^T; P^T, the B
 // operand, is S^T's accumulator as it lies (keys 4 (l / 16) + r).  The next
 // tile's K is in flight from the last S^T on, its V from the LDS write on.
-template <int D, bool F16>
-__device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, const Part& part, char* smem) {
+//
+// A masked key has p = 0, but 0 times a NaN or infinity in its value row is
+// NaN.  Where sums come out non-finite nothing is written and the result is
+// true: the unit is then done again, CAREFUL, with the partly masked tiles
+// taken one column at a time.
+template <int D, bool F16, bool CAREFUL>
+__device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Part& part, char* smem) {
+  const PagedAttn p = arguments(args);
   constexpr int KK = D / 32;   // steps of S^T over d
   constexpr int DT = D / 16;   // 16-row tiles of O^T
   constexpr int VSTR = D + 8;  // V rows in LDS, 16-bit elements
@@ -403,7 +444,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, cons
   float* ml = reinterpret_cast<float*>(smem + few_lds_bytes<D>() - kWaves * 2 * 32 * 4);  // [wave][2][32]
 
   const TileRows tr = tile_rows(p, u);
-  if (tr.rows == 0) return;  // uniform: before any barrier
+  if (tr.rows == 0) return false;  // uniform: before any barrier
   const int token0 = uniform(start_at(p.batch, u.s));
   const bool two = tr.rows > 16;  // the second 16 columns hold rows
 
@@ -431,17 +472,17 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, cons
   const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1] + 8 * g4;
   uint16_t* vl = reinterpret_cast<uint16_t*>(smem) + wave * 32 * VSTR;
 
-  // Pages of the keys key0 + l16 and key0 + 16 + l16, -1 for none.
+  // Table entries of the keys key0 + l16 and key0 + 16 + l16.
   auto pages_of = [&](int key0, int (&pg)[2]) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) pg[c] = page_id(p.batch, u.s, nearest(key0 + 16 * c + l16, tr.end));
+    for (int c = 0; c < 2; ++c) pg[c] = page_entry(p.batch, u.s, nearest(key0 + 16 * c + l16, tr.end));
   };
   auto load = [&](const uint16_t* base, const int64_t* st, int key0, const int (&pg)[2], u32x4 (&x)[2][KK]) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int key = nearest(key0 + 16 * c + l16, tr.end);
       const int slot = key - page_of(p.batch, key) * p.batch.page;
-      const uint16_t* src = base + (int64_t)(pg[c] < 0 ? 0 : pg[c]) * st[0] + (int64_t)slot * st[2];
+      const uint16_t* src = base + (int64_t)(is_page(p.batch, pg[c]) ? pg[c] : 0) * st[0] + (int64_t)slot * st[2];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) x[c][kk] = load16(src + 32 * kk);
     }
@@ -449,12 +490,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, cons
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   f32x4v acc[2][DT];
-  // A masked key has p = 0, but 0 times a NaN or infinity in its value row is
-  // NaN: where the sums come out non-finite, the keys are walked once more
-  // (CAREFUL) with the partly masked tiles taken one column at a time.  Two
-  // copies of the loop: a branch in one costs the usual case its registers.
-  auto walk_keys = [&](auto careful_tag) __attribute__((always_inline)) {
-    constexpr bool CAREFUL = decltype(careful_tag)::value;
+  {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       m[c] = -INFINITY;
@@ -476,7 +512,8 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, cons
       const int nkey = walk.next();
       if (nkey >= 0) pages_of(nkey, pn);
       // Bits of the keys with a page and a position below the end.
-      uint32_t have = (uint32_t)(__ballot(pg[0] >= 0) & 0xffffu) | (uint32_t)(__ballot(pg[1] >= 0) << 16);
+      uint32_t have = (uint32_t)(__ballot(is_page(p.batch, pg[0])) & 0xffffu) |
+                      (uint32_t)(__ballot(is_page(p.batch, pg[1])) << 16);
       if (tr.end - key0 < 32) have &= (1u << (tr.end - key0)) - 1;
       f32x4v s[2][2];
 #pragma unroll
@@ -579,9 +616,8 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, cons
       pg[0] = pn[0];
       pg[1] = pn[1];
     }
-  };
-  walk_keys(std::false_type{});
-  {
+  }
+  if constexpr (!CAREFUL) {
     bool odd = false;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
@@ -589,7 +625,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, cons
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) odd |= !(fabsf(acc[c][dt][r]) < INFINITY);
-    if (__ballot(odd)) walk_keys(std::true_type{});
+    if (uniform(__syncthreads_or(odd))) return true;
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -599,6 +635,7 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, cons
       ml[wave * 64 + 32 + 16 * c + l16] = l[c];
     }
   }
+  const PagedAttn pe = arguments(args);
   // The waves' sums joined through LDS, 16 rows at a time: thread t takes
   // D / 32 values of row t / 32.
   float* ol = reinterpret_cast<float*>(smem);
@@ -629,23 +666,24 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, cons
     }
     if (part.slot >= 0) {
       const int64_t group = part.slot;
-      float* po = p.part_o + group * 32 * D + part_at(row, d0);
+      float* po = pe.part_o + group * 32 * D + part_at(row, d0);
 #pragma unroll
       for (int i = 0; i < PER; ++i) po[i] = o[i];
       if (d0 == 0) {
-        p.part_ml[group * 64 + row] = top;
-        p.part_ml[group * 64 + 32 + row] = sum;
+        pe.part_ml[group * 64 + row] = top;
+        pe.part_ml[group * 64 + 32 + row] = sum;
       }
       continue;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int t = (tr.row0 + row) / p.G, h = tr.row0 + row - t * p.G;
-    uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(token0 + t) * p.os[0] +
-                    (int64_t)(u.g * p.G + h) * p.os[1] + d0;
+    const int t = (tr.row0 + row) / pe.G, h = tr.row0 + row - t * pe.G;
+    uint16_t* dst = static_cast<uint16_t*>(pe.out) + (int64_t)(token0 + t) * pe.os[0] +
+                    (int64_t)(u.g * pe.G + h) * pe.os[1] + d0;
 #pragma unroll
     for (int i = 0; i < PER; i += 2)
       reinterpret_cast<uint32_t*>(dst)[i / 2] = pack2<F16>(o[i] * inv, o[i + 1] * inv);
   }
+  return false;
 }
 
 // A many-row unit.  The matrix cores bound it, with the softmax's VALU work
@@ -656,8 +694,9 @@ __device__ __forceinline__ void few_rows(const PagedAttn& p, const Unit& u, cons
 // the block after that are looked up meanwhile, one key a lane.  ALIGNED: a
 // page holds whole blocks, so a block is one piece of memory behind one buffer
 // descriptor; otherwise every row finds its own page.
-template <int D, bool F16, bool ALIGNED>
-__device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, const Part& part, char* smem) {
+template <int D, bool F16, bool ALIGNED, bool CAREFUL>
+__device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const Part& part, char* smem) {
+  const PagedAttn p = arguments(args);
   constexpr int NTHR = kWaves * 64;
   constexpr int KSTR = D + 8, VSTR = D + 32;  // LDS rows; V rows start 16 banks apart
   constexpr int KTILE = kBlock * KSTR, BUF = KTILE + kBlock * VSTR;
@@ -668,7 +707,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
   const int l32 = lane & 31, hl = lane >> 5;
 
   const TileRows tr = tile_rows(p, u);
-  if (tr.rows == 0) return;  // uniform: before any barrier
+  if (tr.rows == 0) return false;  // uniform: before any barrier
   const int token0 = uniform(start_at(p.batch, u.s));
   const int left = tr.rows - 32 * wave;
   const int nrow = left < 0 ? 0 : (left < 32 ? left : 32);  // this wave's rows
@@ -702,13 +741,13 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
     voff[i] = ((srow + i * SSTEP) * (int)p.vs[2] + scol) * 2;
   }
   u32x4 kst[KCH], vst[KCH];
-  // The page of key0 + lane, -1 for none.
+  // The table's entry of key0 + lane.
   auto page_at = [&](int key0) -> int {
-    return key0 < 0 ? -1 : page_id(p.batch, u.s, ALIGNED ? key0 : nearest(key0 + lane, tr.end));
+    return page_entry(p.batch, u.s, ALIGNED ? key0 : nearest(key0 + lane, tr.end));
   };
   auto load_block = [&](int key0, int pg) {
     if constexpr (ALIGNED) {
-      const int page = uniform(pg < 0 ? 0 : pg);
+      const int page = uniform(is_page(p.batch, pg) ? pg : 0);
       const int slot = key0 - page_of(p.batch, key0) * p.batch.page;
       int nk = tr.end - key0;
       nk = nk > kBlock ? kBlock : nk;
@@ -725,7 +764,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
     } else {
 #pragma unroll
       for (int i = 0; i < KCH; ++i) {
-        const int r = srow + i * SSTEP, page = __shfl(pg < 0 ? 0 : pg, r);
+        const int r = srow + i * SSTEP, page = __shfl(is_page(p.batch, pg) ? pg : 0, r);
         const int key = nearest(key0 + r, tr.end), slot = key - page_of(p.batch, key) * p.batch.page;
         kst[i] = load16(kbase + (int64_t)page * p.ks[0] + (int64_t)slot * p.ks[2] + scol);
         vst[i] = load16(vbase + (int64_t)page * p.vs[0] + (int64_t)slot * p.vs[2] + scol);
@@ -872,8 +911,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
     }
   };
 
-  auto walk_keys = [&](auto careful_tag) __attribute__((always_inline)) {  // as in few_rows
-    constexpr bool CAREFUL = decltype(careful_tag)::value;
+  {
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
@@ -882,7 +920,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
     walk.init(p, tr, part.lo, 1, hi, lane);
     auto take = [&](int& key0, int& pg) {
       key0 = walk.next();
-      pg = page_at(key0);
+      pg = key0 < 0 ? 0 : page_at(key0);
     };
     int key0, pg, nkey, npg;
     take(key0, pg);
@@ -899,7 +937,7 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
         if (nrow > 0 && key0 <= pos_hi) {
           const uint16_t* ks = lds + buf * BUF;
           // Bits of the keys with a page and a position below the end.
-          uint64_t there = ALIGNED ? (uniform(pg) < 0 ? 0 : ~0ull) : __ballot(pg >= 0);
+          uint64_t there = __ballot(is_page(p.batch, pg));
           if (tr.end - key0 < kBlock) there &= (1ull << (tr.end - key0)) - 1;
           const bool masked = there != ~0ull || key0 + kBlock - 1 > pos_lo;
           const int rel = qpos < key0 ? -1 : qpos - key0;
@@ -921,25 +959,24 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
         npg = apg;
       }
     }
-  };
-  walk_keys(std::false_type{});
-  {
+  }
+  if constexpr (!CAREFUL) {
     bool odd = false;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) odd |= !(fabsf(acc[dt][r]) < INFINITY);
-    if (uniform(__syncthreads_or(odd))) {
-      walk_keys(std::true_type{});
-      __syncthreads();
-    }
+    if (uniform(__syncthreads_or(odd))) return true;  // as in few_rows
+  } else {
+    __syncthreads();
   }
 
   l = half_sum(l);
+  const PagedAttn pe = arguments(args);
   if (part.slot >= 0) {
     const int64_t group = (int64_t)part.slot * kWaves + wave;
-    if (nrow == 0) return;
-    float* po = p.part_o + group * 32 * D + lane * 4;
+    if (nrow == 0) return false;
+    float* po = pe.part_o + group * 32 * D + lane * 4;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -947,16 +984,16 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
         *reinterpret_cast<float4*>(po + (dt * 4 + j) * 256) =
             float4{acc[dt][4 * j], acc[dt][4 * j + 1], acc[dt][4 * j + 2], acc[dt][4 * j + 3]};
     if (hl == 0) {
-      p.part_ml[group * 64 + l32] = m;
-      p.part_ml[group * 64 + 32 + l32] = l;
+      pe.part_ml[group * 64 + l32] = m;
+      pe.part_ml[group * 64 + 32 + l32] = l;
     }
-    return;
+    return false;
   }
   // Through LDS, so that every store writes 16-byte pieces of whole rows; all
   // readers of the tiles have passed the barrier above.
   constexpr int OSTR = D + 8;
   static_assert(kWaves * 32 * OSTR <= 2 * BUF, "output staging must fit the K/V tiles");
-  if (nrow == 0) return;
+  if (nrow == 0) return false;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* ot = lds + wave * 32 * OSTR;
 #pragma unroll
@@ -967,16 +1004,63 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
           uint2{pack2<F16>(acc[dt][4 * j] * inv, acc[dt][4 * j + 1] * inv),
                 pack2<F16>(acc[dt][4 * j + 2] * inv, acc[dt][4 * j + 3] * inv)};
   wave_lds_fence();
-  const int64_t at = (int64_t)(token0 + tok) * p.os[0] + (int64_t)head * p.os[1];  // of row l32
+  const int64_t at = (int64_t)(token0 + tok) * pe.os[0] + (int64_t)head * pe.os[1];  // of row l32
 #pragma unroll
   for (int i = 0; i < 32 * ROWCH / 64; ++i) {
     const int c = i * 64 + lane, r = c / ROWCH, ch = c % ROWCH;
     const int lo32 = __shfl((int)at, r), hi32 = __shfl((int)(at >> 32), r);
     if (r < nrow)
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(pe.out) +
                                 (int64_t)(((uint64_t)(uint32_t)hi32 << 32) | (uint32_t)lo32) + ch * 8) =
           *reinterpret_cast<const uint4*>(ot + r * OSTR + ch * 8);
   }
+  return false;
+}
+
+// What the two kinds have for a unit: its shape, the keys of a step, its LDS,
+// and the body.
+template <int D, bool F16>
+struct FewBody {
+  typedef Few Shape;
+  static constexpr int keys = 32, lds = few_lds_bytes<D>();
+  template <bool CAREFUL>
+  static __device__ __forceinline__ bool run(uintptr_t args, const Unit& u, const Part& part, char* smem) {
+    return few_rows<D, F16, CAREFUL>(args, u, part, smem);
+  }
+};
+template <int D, bool F16, bool ALIGNED>
+struct ManyBody {
+  typedef Many Shape;
+  static constexpr int keys = kBlock, lds = many_lds_bytes<D>();
+  template <bool CAREFUL>
+  static __device__ __forceinline__ bool run(uintptr_t args, const Unit& u, const Part& part, char* smem) {
+    return many_rows<D, F16, ALIGNED, CAREFUL>(args, u, part, smem);
+  }
+};
+
+// The stretch [at, end) of workgroup `group`, as far as its first unit.
+struct Stretch {
+  int64_t at, end, group;
+};
+
+template <typename BODY, bool CAREFUL>
+__device__ __forceinline__ bool run_unit(uintptr_t args, const Line& line, const Stretch& st, char* smem, int64_t& to) {
+  Unit u;
+  int64_t place = st.at;
+  if (!find_unit<typename BODY::Shape, false>(arguments(args), place, threadIdx.x & 63, u)) return false;
+  to = u.end < st.end ? u.end : st.end;
+  return BODY::template run<CAREFUL>(args, u, part_of<BODY::keys>(line, u, st.at, to, st.group), smem);
+}
+
+// The careful way, looking its unit up again, is a function of its own: what
+// it would keep in registers pushed the usual way's out of them.
+template <typename BODY>
+__device__ __attribute__((noinline)) void run_again(uint64_t args, int64_t share, int64_t at, int64_t end, int64_t group,
+                                                    __attribute__((address_space(3))) char* smem) {
+  auto same = [](int64_t x) { return lane_of(x, 0); };
+  int64_t to;
+  run_unit<BODY, true>((uintptr_t)same((int64_t)args), Line{0, same(share)}, Stretch{same(at), same(end), same(group)},
+                       (char*)smem, to);
 }
 
 // A launch for either kind: the lengths that tell them apart are on the
@@ -984,35 +1068,28 @@ __device__ __forceinline__ void many_rows(const PagedAttn& p, const Unit& u, con
 // tile and end.  (Both in one kernel needed more registers than there are.)
 // Workgroups go to the eight XCDs in turn; the line is dealt so that each XCD
 // has one stretch of it, and mostly one head's keys, in its L2.
-template <typename SHAPE, int KEYS, typename BODY>
-__device__ __forceinline__ void walk_line(const PagedAttn& p, BODY body) {
-  const int lane = threadIdx.x & 63;
-  const Line line = line_of<SHAPE>(p, lane);
-  int64_t group = blockIdx.x;
-  if (!p.whole[SHAPE::rows > Few::rows]) group = (group & 7) * (kGroups / 8) + (group >> 3);
-  int64_t at = group * line.share;
-  const int64_t end = at + line.share < line.total ? at + line.share : line.total;
-  while (at < end) {
-    Unit u;
-    int64_t place = at;
-    if (!find_unit<SHAPE, false>(p, place, lane, u)) return;
-    const int64_t to = u.end < end ? u.end : end;
-    body(u, part_of<KEYS>(line, u, at, to, group));
-    at = to;
-    if (at < end) __syncthreads();  // the tile's LDS is free
+template <typename BODY>
+__global__ __launch_bounds__(kWaves * 64, 2) void paged_attention_kernel(const PagedAttn) {
+  typedef typename BODY::Shape SHAPE;
+  __shared__ __attribute__((aligned(16))) char smem[BODY::lds];
+  const uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+  Line line;
+  Stretch st;
+  {
+    const PagedAttn p = arguments(args);
+    line = line_of<SHAPE>(p, threadIdx.x & 63);
+    st.group = blockIdx.x;
+    if (!p.whole[SHAPE::rows > Few::rows]) st.group = (st.group & 7) * (kGroups / 8) + (st.group >> 3);
   }
-}
-
-template <int D, bool F16>
-__global__ __launch_bounds__(kWaves * 64, 2) void paged_few_kernel(const PagedAttn p) {
-  __shared__ __attribute__((aligned(16))) char smem[few_lds_bytes<D>()];
-  walk_line<Few, 32>(p, [&](const Unit& u, const Part& part) { few_rows<D, F16>(p, u, part, smem); });
-}
-
-template <int D, bool F16, bool ALIGNED>
-__global__ __launch_bounds__(kWaves * 64, 2) void paged_many_kernel(const PagedAttn p) {
-  __shared__ __attribute__((aligned(16))) char smem[many_lds_bytes<D>()];
-  walk_line<Many, kBlock>(p, [&](const Unit& u, const Part& part) { many_rows<D, F16, ALIGNED>(p, u, part, smem); });
+  st.at = st.group * line.share;
+  st.end = st.at + line.share < line.total ? st.at + line.share : line.total;
+  while (st.at < st.end) {
+    int64_t to = st.end;
+    if (run_unit<BODY, false>(args, line, st, smem, to))
+      run_again<BODY>(args, line.share, st.at, st.end, st.group, (__attribute__((address_space(3))) char*)smem);
+    st.at = to;
+    if (st.at < st.end) __syncthreads();  // the unit's LDS is free
+  }
 }
 
 // Joins the parts of one 32-row group of a tile: every thread takes 4 values of its
@@ -1094,7 +1171,7 @@ Plan plan_of(int64_t N, int64_t S, int64_t G, int64_t Hkv, int64_t keys, bool li
   if (plan.many) plan.many_tiles = tiles_bound<Many>(N, S, G, N * G, lists) * Hkv;
   // Rows of few keys are not worth a join, many tiles not a split.
   plan.few_whole = keys <= 1024 || plan.few_tiles > 64 * kGroups;
-  plan.many_whole = keys <= 1024 || plan.many_tiles > 16 * kGroups;
+  plan.many_whole = keys <= 1024 || plan.many_tiles >= 2 * kGroups;
   return plan;
 }
 
@@ -1195,15 +1272,15 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
     if (plan.many) {                                                                          \
       const int64_t grid = plan.many_whole ? plan.many_tiles : kGroups;                       \
       if (aligned)                                                                            \
-        SPRUCE_LAUNCH((paged_many_kernel<D_, F16_, true>), grid, kWaves * 64);                \
+        SPRUCE_LAUNCH((paged_attention_kernel<ManyBody<D_, F16_, true>>), grid, kWaves * 64);                \
       else                                                                                    \
-        SPRUCE_LAUNCH((paged_many_kernel<D_, F16_, false>), grid, kWaves * 64);               \
+        SPRUCE_LAUNCH((paged_attention_kernel<ManyBody<D_, F16_, false>>), grid, kWaves * 64);               \
       if (!plan.many_whole)                                                                   \
         SPRUCE_LAUNCH((paged_join_kernel<Many, D_, F16_>), plan.many_tiles * kWaves, 256);    \
     }                                                                                         \
     if (plan.few) {                                                                           \
       const int64_t grid = plan.few_whole ? plan.few_tiles : kGroups;                         \
-      SPRUCE_LAUNCH((paged_few_kernel<D_, F16_>), grid, kWaves * 64);                         \
+      SPRUCE_LAUNCH((paged_attention_kernel<FewBody<D_, F16_>>), grid, kWaves * 64);                         \
       if (!plan.few_whole)                                                                    \
         SPRUCE_LAUNCH((paged_join_kernel<Few, D_, F16_>), plan.few_tiles, 256);               \
     }                                                                                         \

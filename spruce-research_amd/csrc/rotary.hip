@@ -92,7 +92,8 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(const RotaryParams p) 
     position = (int64_t)p.batch.kv_lens[s] - p.batch.q_starts[s + 1] + t;
     if (position >= 0 && position < p.batch.cap) {
       const int at = (int)position;
-      page = page_id(p.batch, s, at);
+      page = page_entry(p.batch, s, at);
+      if (!is_page(p.batch, page)) page = -1;
       slot = at - page_of(p.batch, at) * p.batch.page;
     }
   }
