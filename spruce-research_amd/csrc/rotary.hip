@@ -12,199 +12,241 @@
 // t_i / (2 pi) is formed in 64 bits and its fraction alone goes to 32; all
 // else is 32-bit, rounded once.
 //
-// Bytes bound it (each value read and written once).  A wave owns one token:
-// its lanes work out one pair's sine and cosine each, once for all heads, and
-// hand them over through LDS; then D/16 lanes take a head row, 16 values a
-// lane chosen so that both members of every pair are in the lane.
+// Bytes bound it (each value read and written once).  A wave owns one token,
+// or some of its heads where tokens are few: its lanes work out one pair's sine
+// and cosine each, once for all heads, and hand them over through LDS; then
+// D/16 lanes take a head row, 16 values a lane chosen so that both members of
+// every pair are in the lane.  The rows of four passes (two of float32) are in
+// flight before the look-ups (sequence, position, page) and the sines begin.
 #include "paged.h"
 
 using namespace spruce;
 
 namespace {
 
+struct RotaryRows {
+  const void* src;
+  void* dst;
+  int64_t ss[3], ds[3];  // batch, head, token strides; of pages: page, head, slot
+  int heads;
+};
+
 struct RotaryParams {
-  const void* src[3];    // q, k, v rows; v only with PAGED
-  void* dst[3];          // q and k rows, or the key and value pages
-  int64_t ss[3][3];      // batch, head, token strides of src
-  int64_t ds[3][3];      // the same of dst; for pages: page, head, slot
+  RotaryRows q, k, v;    // v only with PAGED, whose k and v go to the pages
   const void* positions;  // int32 or int64
   int64_t pos_stride;    // per batch
   int pos64;
   const double* inv_freq;
   int rot, interleaved;
   float factor;
-  const void* weight[2];
+  const void* q_weight;
+  const void* k_weight;
   int weight_f32;
   float eps;
-  int heads[3];
-  int tokens;   // per batch
+  int tokens;    // per batch
   int64_t rows;  // batches * tokens
-  int groups, passes;  // passes over the heads, and in how many waves' hands
+  int groups;    // waves that share a token's passes
   PagedBatch batch;
 };
 
 constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Eight values as they lie in memory.
+template <int EB>
+struct Raw8 {
+  u32x4 w[EB / 2];
+};
+template <int EB>
+__device__ __forceinline__ Raw8<EB> raw8(const char* p) {
+  Raw8<EB> r;
+#pragma unroll
+  for (int i = 0; i < EB / 2; ++i) r.w[i] = reinterpret_cast<const u32x4*>(p)[i];
+  return r;
+}
+
 template <int EB, bool F16>
-__device__ __forceinline__ void widen8(const char* p, float (&v)[8]) {
+__device__ __forceinline__ void widen8(const Raw8<EB>& r, float* v) {
   if constexpr (EB == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, (uint32_t)r.w[i >> 2][i & 3]);
   } else {
-    const uint4 r = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] = unpack1<F16>(w[i] & 0xffffu);
-      v[2 * i + 1] = unpack1<F16>(w[i] >> 16);
+      v[2 * i] = unpack1<F16>(r.w[0][i] & 0xffffu);
+      v[2 * i + 1] = unpack1<F16>(r.w[0][i] >> 16);
     }
   }
 }
 
 template <int EB, bool F16>
-__device__ __forceinline__ void narrow8(char* p, const float (&v)[8]) {
+__device__ __forceinline__ void store8(char* p, const float* v) {
   if constexpr (EB == 4) {
     reinterpret_cast<float4*>(p)[0] = float4{v[0], v[1], v[2], v[3]};
     reinterpret_cast<float4*>(p)[1] = float4{v[4], v[5], v[6], v[7]};
   } else {
-    *reinterpret_cast<uint4*>(p) =
-        uint4{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]), pack2<F16>(v[4], v[5]), pack2<F16>(v[6], v[7])};
+    *reinterpret_cast<u32x4*>(p) =
+        u32x4{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]), pack2<F16>(v[4], v[5]), pack2<F16>(v[6], v[7])};
   }
 }
 
 template <int EB, bool F16, int D, bool PAGED>
-__global__ __launch_bounds__(256) void head_rotary_kernel(const RotaryParams p) {
+__global__ __launch_bounds__(256, 4) void head_rotary_kernel(const RotaryParams p) {
   constexpr int LPH = D / 16, HPW = 64 / LPH;  // lanes of a head row, head rows of a pass
+  constexpr int kFlight = 8 / EB;              // passes in flight: 32 registers
   __shared__ float2 turns[4][D / 2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t item = (int64_t)flat_block() * 4 + wave;
-  const int64_t row = item / p.groups;
-  const int grp = (int)(item - row * p.groups);
+  int64_t row = item;
+  int grp = 0;
+  if (p.groups > 1) {  // few tokens: the product fits 32 bits
+    row = (uint32_t)item / (uint32_t)p.groups;
+    grp = (int)((uint32_t)item - (uint32_t)row * (uint32_t)p.groups);
+  }
   if (row >= p.rows) return;  // no barrier below
-  const int b = (int)(row / p.tokens), t = (int)(row - (int64_t)b * p.tokens);
-
-  int64_t position;
-  int page = -1, slot = 0;
-  if constexpr (PAGED) {
-    const int s = sequence_of(p.batch, t, lane);
-    if (s < 0) return;
-    position = (int64_t)p.batch.kv_lens[s] - p.batch.q_starts[s + 1] + t;
-    if (position >= 0 && position < p.batch.cap) {
-      const int at = (int)position;
-      page = page_entry(p.batch, s, at);
-      if (!is_page(p.batch, page)) page = -1;
-      slot = at - page_of(p.batch, at) * p.batch.page;
-    }
+  int b = 0, t = (int)row;
+  if (!PAGED && p.rows > p.tokens) {
+    b = (int)(row / p.tokens);
+    t = (int)(row - (int64_t)b * p.tokens);
   }
-  if (!PAGED || p.positions != nullptr) {
-    const int64_t i = (int64_t)b * p.pos_stride + t;
-    position = p.pos64 ? static_cast<const int64_t*>(p.positions)[i] : static_cast<const int32_t*>(p.positions)[i];
-  }
-  if (lane < p.rot / 2) {
-    double turn = (double)position * p.inv_freq[lane] * kTurn;
-    turn -= rint(turn);
-    float s, c;
-    sincospif(2.f * (float)turn, &s, &c);
-    turns[wave][lane] = float2{c * p.factor, s * p.factor};
-  }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-
   const int j = lane % LPH;
   const bool turned = j < p.rot / 16;
   const int e0 = turned && !p.interleaved ? 8 * j : 16 * j;
   const int e1 = turned && !p.interleaved ? 8 * j + p.rot / 2 : 16 * j + 8;
-  float cs[8], sn[8];
-  if (turned) {
+
+  // Passes of HPW heads each: the queries', the keys', the values'.
+  const int nq = (p.q.heads + HPW - 1) / HPW, nk = (p.k.heads + HPW - 1) / HPW;
+  const int passes = nq + nk + (PAGED ? nk : 0);
+  const int per = (passes + p.groups - 1) / p.groups;
+  const int first = grp * per, last = first + per < passes ? first + per : passes;
+  auto rows_of = [&](int pass) -> const RotaryRows& { return pass < nq ? p.q : (pass < nq + nk ? p.k : p.v); };
+  auto head_of = [&](int pass) {
+    return (pass < nq ? pass : (pass < nq + nk ? pass - nq : pass - nq - nk)) * HPW + lane / LPH;
+  };
+
+  float cs[8], sn[8], qw[16], kw[16];
+  int64_t position = 0;
+  int page = -1, slot = 0;
+  for (int base = first; base < last; base += kFlight) {
+    Raw8<EB> x[kFlight][2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 x = turns[wave][8 * j + i];
-      cs[i] = x.x;
-      sn[i] = x.y;
-    }
-  }
-  const int total = p.heads[0] + p.heads[1] + (PAGED ? p.heads[2] : 0);
-  const int per = (p.passes + p.groups - 1) / p.groups;
-  for (int pass = grp * per; pass < (grp + 1) * per && pass < p.passes; ++pass) {
-    int h = pass * HPW + lane / LPH;
-    if (h >= total) continue;
-    int what = 0;
-    if (h >= p.heads[0]) {
-      h -= p.heads[0];
-      what = 1;
-      if (PAGED && h >= p.heads[1]) {
-        h -= p.heads[1];
-        what = 2;
+    for (int i = 0; i < kFlight; ++i) {
+      if (base + i < last) {
+        const RotaryRows& r = rows_of(base + i);
+        int h = head_of(base + i);
+        h = h < r.heads ? h : r.heads - 1;  // lanes without a head repeat the last
+        const char* src = static_cast<const char*>(r.src) +
+                          ((int64_t)b * r.ss[0] + (int64_t)h * r.ss[1] + (int64_t)t * r.ss[2]) * EB;
+        x[i][0] = raw8<EB>(src + e0 * EB);
+        x[i][1] = raw8<EB>(src + e1 * EB);
       }
     }
-    if (PAGED && what > 0 && page < 0) continue;
-    const char* src = static_cast<const char*>(p.src[what]) +
-                      ((int64_t)b * p.ss[what][0] + (int64_t)h * p.ss[what][1] + (int64_t)t * p.ss[what][2]) * EB;
-    const bool paged = PAGED && what > 0;
-    char* dst = static_cast<char*>(p.dst[what]) +
-                ((int64_t)(paged ? page : b) * p.ds[what][0] + (int64_t)h * p.ds[what][1] +
-                 (int64_t)(paged ? slot : t) * p.ds[what][2]) * EB;
-    float x[8], y[8];
-    widen8<EB, F16>(src + e0 * EB, x);
-    widen8<EB, F16>(src + e1 * EB, y);
-    if (what < 2) {
-      const void* weight = p.weight[what];
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
-      // Every lane of the row takes part; rows of one pass may differ in
-      // `what`, so the sums are formed before the branch on the weight.
-#pragma unroll
-      for (int m = 1; m < LPH; m *= 2) ss += __shfl_xor(ss, m);
-      if (weight != nullptr) {
-        const float r = 1.f / sqrtf(ss * (1.f / D) + p.eps);
-        float w0[8], w1[8];
+    if (base == first) {
+      auto weights = [&](const void* w, float* out) {
+        if (w == nullptr) return;
         if (p.weight_f32) {
-          widen8<4, false>(static_cast<const char*>(weight) + e0 * 4, w0);
-          widen8<4, false>(static_cast<const char*>(weight) + e1 * 4, w1);
+          widen8<4, false>(raw8<4>(static_cast<const char*>(w) + e0 * 4), out);
+          widen8<4, false>(raw8<4>(static_cast<const char*>(w) + e1 * 4), out + 8);
         } else {
-          widen8<EB, F16>(static_cast<const char*>(weight) + e0 * EB, w0);
-          widen8<EB, F16>(static_cast<const char*>(weight) + e1 * EB, w1);
+          widen8<EB, F16>(raw8<EB>(static_cast<const char*>(w) + e0 * EB), out);
+          widen8<EB, F16>(raw8<EB>(static_cast<const char*>(w) + e1 * EB), out + 8);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = x[i] * r * w0[i];
-          y[i] = y[i] * r * w1[i];
+      };
+      weights(p.q_weight, qw);
+      weights(p.k_weight, kw);
+      double freq = 0.0;
+      if (lane < p.rot / 2) freq = p.inv_freq[lane];
+      if constexpr (PAGED) {
+        const int s = sequence_of(p.batch, t, lane);
+        if (s < 0) return;
+        position = (int64_t)p.batch.kv_lens[s] - p.batch.q_starts[s + 1] + t;
+        if (position >= 0 && position < p.batch.cap) {
+          const int at = (int)position;
+          page = page_entry(p.batch, s, at);
+          if (!is_page(p.batch, page)) page = -1;
+          slot = at - page_of(p.batch, at) * p.batch.page;
         }
       }
-      if (turned) {
-        if (p.interleaved) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = x[2 * i], c = x[2 * i + 1], d = y[2 * i], f = y[2 * i + 1];
-            x[2 * i] = a * cs[i] - c * sn[i];
-            x[2 * i + 1] = c * cs[i] + a * sn[i];
-            y[2 * i] = d * cs[4 + i] - f * sn[4 + i];
-            y[2 * i + 1] = f * cs[4 + i] + d * sn[4 + i];
-          }
-        } else {
+      if (!PAGED || p.positions != nullptr) {
+        const int64_t i = (int64_t)b * p.pos_stride + t;
+        position = p.pos64 ? static_cast<const int64_t*>(p.positions)[i] : static_cast<const int32_t*>(p.positions)[i];
+      }
+      if (p.rot > 0) {
+        if (lane < p.rot / 2) {
+          double turn = (double)position * freq * kTurn;
+          turn -= rint(turn);
+          float s, c;
+          sincospif(2.f * (float)turn, &s, &c);
+          turns[wave][lane] = float2{c * p.factor, s * p.factor};
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (turned) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float a = x[i], c = y[i];
-            x[i] = a * cs[i] - c * sn[i];
-            y[i] = c * cs[i] + a * sn[i];
+            const float2 y = turns[wave][8 * j + i];
+            cs[i] = y.x;
+            sn[i] = y.y;
           }
         }
       }
     }
-    narrow8<EB, F16>(dst + e0 * EB, x);
-    narrow8<EB, F16>(dst + e1 * EB, y);
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int pass = base + i;
+      if (pass >= last) break;
+      const RotaryRows& r = rows_of(pass);
+      const int h = head_of(pass);
+      float v[16];
+      widen8<EB, F16>(x[i][0], v);
+      widen8<EB, F16>(x[i][1], v + 8);
+      if (pass < nq + nk) {
+        const bool is_q = pass < nq;
+        if ((is_q ? p.q_weight : p.k_weight) != nullptr) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ss += v[e] * v[e];
+#pragma unroll
+          for (int m = 1; m < LPH; m *= 2) ss += __shfl_xor(ss, m);
+          const float rn = 1.f / sqrtf(ss * (1.f / D) + p.eps);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = v[e] * rn * (is_q ? qw[e] : kw[e]);
+        }
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            // Pairs: (v[e], v[e + 8]), or neighbours.
+            float& a = p.interleaved ? v[2 * e] : v[e];
+            float& c = p.interleaved ? v[2 * e + 1] : v[e + 8];
+            const float a0 = a, c0 = c;
+            a = a0 * cs[e] - c0 * sn[e];
+            c = c0 * cs[e] + a0 * sn[e];
+          }
+        }
+      }
+      const bool paged = PAGED && pass >= nq;
+      if (h >= r.heads || (paged && page < 0)) continue;
+      char* dst = static_cast<char*>(r.dst) +
+                  ((int64_t)(paged ? page : b) * r.ds[0] + (int64_t)h * r.ds[1] + (int64_t)(paged ? slot : t) * r.ds[2]) *
+                      EB;
+      store8<EB, F16>(dst + e0 * EB, v);
+      store8<EB, F16>(dst + e1 * EB, v + 8);
+    }
   }
 }
 
 template <bool PAGED>
 int launch_rotary(RotaryParams& p, int64_t D, int dtype, hipStream_t stream) {
-  const int total = p.heads[0] + p.heads[1] + (PAGED ? p.heads[2] : 0);
   const int hpw = D == 128 ? 8 : 16;
-  p.passes = (total + hpw - 1) / hpw;
+  const int nk = (p.k.heads + hpw - 1) / hpw, passes = (p.q.heads + hpw - 1) / hpw + nk + (PAGED ? nk : 0);
+  // Few tokens: their heads are shared out until 4096 waves (four a SIMD) are up.
   p.groups = 1;
+  if (p.rows < 4096) {
+    const int64_t g = 4096 / p.rows;
+    p.groups = g < passes ? (int)g : passes;
+  }
   const int64_t blocks = (p.rows * p.groups + 3) / 4;
   SPRUCE_REQUIRE(blocks < (int64_t)1 << 31, "too many tokens");
   const dim3 grid = flat_grid(blocks);
@@ -250,8 +292,8 @@ int set_rotary(RotaryParams& p, int64_t D, int dtype, const double* inv_freq, in
   p.rot = (int)rotary_dim;
   p.interleaved = layout == SPRUCE_ROTARY_INTERLEAVED;
   p.factor = factor;
-  p.weight[0] = q_weight;
-  p.weight[1] = k_weight;
+  p.q_weight = q_weight;
+  p.k_weight = k_weight;
   p.weight_f32 = weight_dtype == SPRUCE_DTYPE_F32;
   p.eps = eps;
   return SPRUCE_OK;
@@ -278,21 +320,20 @@ extern "C" int spruce_rotate_heads(const void* q, const int64_t qs[4], const voi
   const int eb = dtype == SPRUCE_DTYPE_F32 ? 4 : 2;
   SPRUCE_REQUIRE(rows16(q, qs, eb) && rows16(k, ks, eb) && rows16(qo, qos, eb) && rows16(ko, kos, eb),
                  "q, k and the outputs must be 16-byte aligned with strides that keep rows 16-byte aligned");
-  p.src[0] = q;
-  p.src[1] = k;
-  p.dst[0] = qo;
-  p.dst[1] = ko;
-  for (int i = 0; i < 3; ++i) {
-    p.ss[0][i] = qs[i];
-    p.ss[1][i] = ks[i];
-    p.ds[0][i] = qos[i];
-    p.ds[1][i] = kos[i];
-  }
+  auto rows = [](RotaryRows& r, const void* src, const int64_t* ss, void* dst, const int64_t* ds, int64_t heads) {
+    r.src = src;
+    r.dst = dst;
+    for (int i = 0; i < 3; ++i) {
+      r.ss[i] = ss[i];
+      r.ds[i] = ds[i];
+    }
+    r.heads = (int)heads;
+  };
+  rows(p.q, q, qs, qo, qos, Hq);
+  rows(p.k, k, ks, ko, kos, Hkv);
   p.positions = positions;
   p.pos_stride = pos_stride;
   p.pos64 = pos64;
-  p.heads[0] = (int)Hq;
-  p.heads[1] = (int)Hkv;
   p.tokens = (int)T;
   p.rows = B * T;
   return launch_rotary<false>(p, D, dtype, (hipStream_t)stream);
@@ -320,36 +361,27 @@ extern "C" int spruce_paged_append(const void* q, const int64_t qs[3], void* qo,
   if (N == 0) return SPRUCE_OK;
   SPRUCE_REQUIRE(k && v && (pages == 0 || (k_pages && v_pages)), "k, v and the pages must be non-null device pointers");
   SPRUCE_REQUIRE(Hq == 0 || (q && qo), "q and its output must be non-null device pointers");
-  // Packed [N, H, D] rows: batch stride 0, head, token.
-  const int64_t* packed[3] = {qs, ks, vs};
-  for (int i = 0; i < 3; ++i) {
-    if (i == 0 && Hq == 0) continue;
-    p.ss[i][1] = packed[i][1];
-    p.ss[i][2] = packed[i][0];
-  }
-  if (Hq) {
-    p.ds[0][1] = qos[1];
-    p.ds[0][2] = qos[0];
-  }
-  for (int i = 0; i < 3; ++i) {
-    p.ds[1][i] = kps[i];
-    p.ds[2][i] = vps[i];
-  }
-  p.src[0] = q;
-  p.src[1] = k;
-  p.src[2] = v;
-  p.dst[0] = qo;
-  p.dst[1] = k_pages;
-  p.dst[2] = v_pages;
+  // Packed [N, H, D] rows as one batch; the pages' strides as they are.
+  auto rows = [&](RotaryRows& r, const void* src, const int64_t* ss, void* dst, const int64_t* ds, bool paged, int64_t heads) {
+    r.src = src;
+    r.dst = dst;
+    r.ss[1] = ss[1];
+    r.ss[2] = ss[0];
+    r.ds[0] = paged ? ds[0] : 0;
+    r.ds[1] = ds[1];
+    r.ds[2] = paged ? ds[2] : ds[0];
+    r.heads = (int)heads;
+  };
   const int eb = dtype == SPRUCE_DTYPE_F32 ? 4 : 2;
-  for (int i = Hq ? 0 : 1; i < 3; ++i)
-    SPRUCE_REQUIRE(rows16(p.src[i], p.ss[i], eb) && rows16(p.dst[i], p.ds[i], eb),
-                   "q, k, v, the pages and the output must be 16-byte aligned with strides that keep rows 16-byte "
-                   "aligned");
+  if (Hq) rows(p.q, q, qs, qo, qos, false, Hq);
+  rows(p.k, k, ks, k_pages, kps, true, Hkv);
+  rows(p.v, v, vs, v_pages, vps, true, Hkv);
+  auto fits = [&](const RotaryRows& r) { return rows16(r.src, r.ss, eb) && rows16(r.dst, r.ds, eb); };
+  SPRUCE_REQUIRE((Hq == 0 || fits(p.q)) && fits(p.k) && fits(p.v),
+                 "q, k, v, the pages and the output must be 16-byte aligned with strides that keep rows 16-byte "
+                 "aligned");
   p.positions = positions;
   p.pos64 = pos64;
-  p.heads[0] = (int)Hq;
-  p.heads[1] = p.heads[2] = (int)Hkv;
   p.tokens = (int)N;
   p.rows = N;
   return launch_rotary<true>(p, D, dtype, (hipStream_t)stream);
