@@ -92,7 +92,7 @@ __device__ __forceinline__ void store8(char* p, const float* v) {
 }
 
 template <int EB, bool F16, int D, bool PAGED>
-__global__ __launch_bounds__(256, 4) void head_rotary_kernel(const RotaryParams p) {
+__global__ __launch_bounds__(256, EB == 4 ? 5 : 4) void head_rotary_kernel(const RotaryParams p) {
   constexpr int LPH = D / 16, HPW = 64 / LPH;  // lanes of a head row, head rows of a pass
   constexpr int kFlight = 8 / EB;              // passes in flight: 32 registers
   __shared__ float2 turns[4][D / 2];
