@@ -696,6 +696,10 @@ int spruce_kernel_metadata(int variant, int64_t Hq, int64_t Hkv, int64_t D,
  * these are read on the device: a captured launch takes the values they hold
  * at replay.  Ids outside [0, pages) and positions past the table name no
  * slot.
+ *
+ * These calls take their arguments as one block of 8-byte fields, which is
+ * read before they return: a token's step is a few microseconds on the device,
+ * and marshalling forty arguments one by one takes a Python caller as long.
  * ---------------------------------------------------------------------- */
 
 /* Pairs (x_i, x_{i + R/2}) or (x_{2i}, x_{2i+1}) of the R rotated dims. */
@@ -720,11 +724,27 @@ int spruce_kernel_metadata(int variant, int64_t Hq, int64_t Hkv, int64_t D,
  *   inv_freq float64 [rotary_dim / 2].  weight_dtype: SPRUCE_DTYPE_F32 or
  *   dtype.
  */
-int spruce_rotate_heads(const void* q, const int64_t qs[4], const void* k, const int64_t ks[4], int64_t B,
-                        int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int dtype, const void* positions,
-                        int64_t pos_stride, int pos64, const double* inv_freq, int64_t rotary_dim, int layout,
-                        float factor, const void* q_weight, const void* k_weight, int weight_dtype, float eps,
-                        void* qo, const int64_t qos[4], void* ko, const int64_t kos[4], void* stream);
+typedef struct spruce_rotate_heads_args {
+  const void* q;
+  int64_t qs[4];
+  const void* k;
+  int64_t ks[4];
+  int64_t B, Hq, Hkv, T, D, dtype;
+  const void* positions;
+  int64_t pos_stride, pos64;
+  const double* inv_freq;
+  int64_t rotary_dim, layout;
+  double factor;
+  const void* q_weight;
+  const void* k_weight;
+  int64_t weight_dtype;
+  double eps;
+  void* q_out;
+  int64_t qos[4];
+  void* k_out;
+  int64_t kos[4];
+} spruce_rotate_heads_args;
+int spruce_rotate_heads(const spruce_rotate_heads_args* args, void* stream);
 
 /*
  * Writes the new tokens' keys and values (k, v [N, Hkv, D], strides ks, vs)
@@ -735,14 +755,37 @@ int spruce_rotate_heads(const void* q, const int64_t qs[4], const void* k, const
  * behind q_starts[S] are left alone, in qo too, and a token without a slot
  * writes no key and value.  Two tokens with one slot leave either's values.
  */
-int spruce_paged_append(const void* q, const int64_t qs[3], void* qo, const int64_t qos[3], const void* k,
-                        const int64_t ks[3], const void* v, const int64_t vs[3], int64_t N, int64_t Hq, int64_t Hkv,
-                        int64_t D, int dtype, void* k_pages, const int64_t kps[4], void* v_pages,
-                        const int64_t vps[4], int64_t pages, int64_t page_size, const int32_t* page_table,
-                        int64_t table_stride, int64_t table_width, const int32_t* q_starts, const int32_t* kv_lens,
-                        int64_t S, const void* positions, int pos64, const double* inv_freq, int64_t rotary_dim,
-                        int layout, float factor, const void* q_weight, const void* k_weight, int weight_dtype,
-                        float eps, void* stream);
+typedef struct spruce_paged_append_args {
+  const void* q;
+  int64_t qs[3];
+  void* q_out;
+  int64_t qos[3];
+  const void* k;
+  int64_t ks[3];
+  const void* v;
+  int64_t vs[3];
+  int64_t N, Hq, Hkv, D, dtype;
+  void* k_pages;
+  int64_t kps[4];
+  void* v_pages;
+  int64_t vps[4];
+  int64_t pages, page_size;
+  const int32_t* page_table;
+  int64_t table_stride, table_width;
+  const int32_t* q_starts;
+  const int32_t* kv_lens;
+  int64_t S;
+  const void* positions;
+  int64_t pos64;
+  const double* inv_freq;
+  int64_t rotary_dim, layout;
+  double factor;
+  const void* q_weight;
+  const void* k_weight;
+  int64_t weight_dtype;
+  double eps;
+} spruce_paged_append_args;
+int spruce_paged_append(const spruce_paged_append_args* args, void* stream);
 
 /*
  * Attention of the new tokens over the cache: token n at position p attends
@@ -764,13 +807,29 @@ int spruce_paged_append(const void* q, const int64_t qs[3], void* qo, const int6
  */
 int64_t spruce_paged_attention_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
                                                int64_t keys, int64_t K);
-int spruce_paged_attention(const void* q, const int64_t qs[3], const void* k_pages, const int64_t kps[4],
-                           const void* v_pages, const int64_t vps[4], int64_t pages, int64_t page_size,
-                           const int32_t* page_table, int64_t table_stride, int64_t table_width,
-                           const int32_t* q_starts, const int32_t* kv_lens, int64_t S, int64_t N, int64_t Hq,
-                           int64_t Hkv, int64_t D, float scale, int dtype, const int32_t* idx, const int64_t is[4],
-                           int64_t Qc, int64_t K, void* out, const int64_t os[3], void* workspace,
-                           int64_t workspace_bytes, void* stream);
+typedef struct spruce_paged_attention_args {
+  const void* q;
+  int64_t qs[3];
+  const void* k_pages;
+  int64_t kps[4];
+  const void* v_pages;
+  int64_t vps[4];
+  int64_t pages, page_size;
+  const int32_t* page_table;
+  int64_t table_stride, table_width;
+  const int32_t* q_starts;
+  const int32_t* kv_lens;
+  int64_t S, N, Hq, Hkv, D, dtype;
+  double scale;
+  const int32_t* idx;
+  int64_t is[4];
+  int64_t Qc, K;
+  void* out;
+  int64_t os[3];
+  void* workspace;
+  int64_t workspace_bytes;
+} spruce_paged_attention_args;
+int spruce_paged_attention(const spruce_paged_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

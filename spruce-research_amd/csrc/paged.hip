@@ -1192,14 +1192,12 @@ extern "C" int64_t spruce_paged_attention_workspace_bytes(int64_t N, int64_t S, 
   return workspace_of(plan_of(N, S, Hq / Hkv, Hkv, K > 0 ? K * kBlock : keys, K > 0), D);
 }
 
-extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const void* k_pages, const int64_t kps[4],
-                                      const void* v_pages, const int64_t vps[4], int64_t pages, int64_t page_size,
-                                      const int32_t* page_table, int64_t table_stride, int64_t table_width,
-                                      const int32_t* q_starts, const int32_t* kv_lens, int64_t S, int64_t N,
-                                      int64_t Hq, int64_t Hkv, int64_t D, float scale, int dtype, const int32_t* idx,
-                                      const int64_t is[4], int64_t Qc, int64_t K, void* out, const int64_t os[3],
-                                      void* workspace, int64_t workspace_bytes, void* stream) {
-  SPRUCE_REQUIRE(qs && kps && vps && os, "stride arrays must be non-null");
+extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, void* stream) {
+  SPRUCE_REQUIRE(args != nullptr, "args must be non-null");
+  const spruce_paged_attention_args& a = *args;
+  const int64_t N = a.N, S = a.S, Hq = a.Hq, Hkv = a.Hkv, D = a.D, K = a.K;
+  const int dtype = (int)a.dtype;
+  const float scale = (float)a.scale;
   SPRUCE_REQUIRE(D == 64 || D == 128, "kernel supports head_dim 64 or 128, got %lld", (long long)D);
   SPRUCE_REQUIRE(dtype == SPRUCE_DTYPE_BF16 || dtype == SPRUCE_DTYPE_F16,
                  "the paged attention takes bf16 or f16, got dtype code %d", dtype);
@@ -1207,48 +1205,50 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
                  "query heads (%lld) must be divisible by KV heads (%lld)", (long long)Hq, (long long)Hkv);
   SPRUCE_REQUIRE(Hq / Hkv <= 64, "at most 64 query heads per KV head are supported");
   SPRUCE_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
-  SPRUCE_REQUIRE(qs[2] == 1 && kps[3] == 1 && vps[3] == 1 && os[2] == 1,
+  SPRUCE_REQUIRE(a.qs[2] == 1 && a.kps[3] == 1 && a.vps[3] == 1 && a.os[2] == 1,
                  "q, the pages and out must have a contiguous final dimension");
   PagedAttn p{};
-  const int rc = prepare_batch(p.batch, page_table, table_stride, table_width, q_starts, kv_lens, S, N, page_size, pages);
+  const int rc = prepare_batch(p.batch, a.page_table, a.table_stride, a.table_width, a.q_starts, a.kv_lens, S, N,
+                               a.page_size, a.pages);
   if (rc) return rc;
   if (N == 0) return SPRUCE_OK;
-  SPRUCE_REQUIRE(q && out && (pages == 0 || (k_pages && v_pages)), "q, the pages and out must be non-null device pointers");
+  SPRUCE_REQUIRE(a.q && a.out && (a.pages == 0 || (a.k_pages && a.v_pages)),
+                 "q, the pages and out must be non-null device pointers");
   auto rows16 = [](const void* ptr, const int64_t* s, int n) {
     if (reinterpret_cast<uintptr_t>(ptr) % 16) return false;
     for (int i = 0; i < n; ++i)
       if (s[i] % 8) return false;
     return true;
   };
-  SPRUCE_REQUIRE(rows16(q, qs, 2) && rows16(k_pages, kps, 3) && rows16(v_pages, vps, 3) && rows16(out, os, 2),
+  SPRUCE_REQUIRE(rows16(a.q, a.qs, 2) && rows16(a.k_pages, a.kps, 3) && rows16(a.v_pages, a.vps, 3) && rows16(a.out, a.os, 2),
                  "q, the pages and out must be 16-byte aligned with strides that keep rows 16-byte aligned");
   SPRUCE_REQUIRE(K >= 0 && K < (int64_t)1 << 24, "invalid list width %lld", (long long)K);
-  SPRUCE_REQUIRE(K == 0 || (idx && is && Qc >= 0), "indices must be a non-null device pointer");
-  SPRUCE_REQUIRE(K == 0 || is[3] == 1, "indices must have a contiguous final dimension");
+  SPRUCE_REQUIRE(K == 0 || (a.idx && a.Qc >= 0), "indices must be a non-null device pointer");
+  SPRUCE_REQUIRE(K == 0 || a.is[3] == 1, "indices must have a contiguous final dimension");
   const Plan plan = plan_of(N, S, Hq / Hkv, Hkv, K > 0 ? K * kBlock : p.batch.cap, K > 0);
   const int64_t need = workspace_of(plan, D);
-  SPRUCE_REQUIRE(workspace && workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
-                 (long long)workspace_bytes, (long long)need);
-  SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
-  p.q = q;
-  p.out = out;
-  p.k = k_pages;
-  p.v = v_pages;
+  SPRUCE_REQUIRE(a.workspace && a.workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
+                 (long long)a.workspace_bytes, (long long)need);
+  SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0, "workspace must be 16-byte aligned");
+  p.q = a.q;
+  p.out = a.out;
+  p.k = a.k_pages;
+  p.v = a.v_pages;
   for (int i = 0; i < 2; ++i) {
-    p.qs[i] = qs[i];
-    p.os[i] = os[i];
+    p.qs[i] = a.qs[i];
+    p.os[i] = a.os[i];
   }
   for (int i = 0; i < 3; ++i) {
-    p.ks[i] = kps[i];
-    p.vs[i] = vps[i];
+    p.ks[i] = a.kps[i];
+    p.vs[i] = a.vps[i];
   }
   p.Hkv = (int)Hkv;
   p.G = (int)(Hq / Hkv);
   p.cs = scale * 1.4426950408889634f;
   if (K > 0) {
-    p.idx = idx;
-    for (int i = 0; i < 3; ++i) p.is[i] = is[i];
-    p.Qc = (int)(Qc < (int64_t)1 << 30 ? Qc : (int64_t)1 << 30);
+    p.idx = a.idx;
+    for (int i = 0; i < 3; ++i) p.is[i] = a.is[i];
+    p.Qc = (int)(a.Qc < (int64_t)1 << 30 ? a.Qc : (int64_t)1 << 30);
     p.K = (int)K;
   }
   SPRUCE_REQUIRE(plan.few_tiles < (int64_t)1 << 22 && plan.many_tiles < (int64_t)1 << 19, "too many tokens for one call");
@@ -1256,10 +1256,11 @@ extern "C" int spruce_paged_attention(const void* q, const int64_t qs[3], const 
   p.whole[0] = plan.few_whole;
   p.whole[1] = plan.many_whole;
   // The kinds' launches follow one another, so they share the slots.
-  p.part_o = static_cast<float*>(workspace);
+  p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = p.part_o + need / (32 * (D + 2) * 4) * 32 * D;
   // Rows of a page's block behind one 32-bit buffer offset.
-  const bool aligned = page_size % kBlock == 0 && kps[2] > 0 && vps[2] > 0 && kps[2] < 1 << 22 && vps[2] < 1 << 22;
+  const bool aligned = a.page_size % kBlock == 0 && a.kps[2] > 0 && a.vps[2] > 0 && a.kps[2] < 1 << 22 &&
+                       a.vps[2] < 1 << 22;
   const hipStream_t st = (hipStream_t)stream;
 #define SPRUCE_LAUNCH(KERNEL, GRID, THREADS)                                                  \
   do {                                                                                        \

@@ -273,52 +273,52 @@ bool rows16(const void* p, const int64_t s[3], int eb) {
   return true;
 }
 
-int set_rotary(RotaryParams& p, int64_t D, int dtype, const double* inv_freq, int64_t rotary_dim, int layout,
-               float factor, const void* q_weight, const void* k_weight, int weight_dtype, float eps) {
+int set_rotary(RotaryParams& p, int64_t D, int dtype, const double* inv_freq, int64_t rotary_dim, int64_t layout,
+               double factor, const void* q_weight, const void* k_weight, int64_t weight_dtype, double eps) {
   SPRUCE_REQUIRE(D == 64 || D == 128, "kernel supports head_dim 64 or 128, got %lld", (long long)D);
   SPRUCE_REQUIRE(dtype == SPRUCE_DTYPE_BF16 || dtype == SPRUCE_DTYPE_F16 || dtype == SPRUCE_DTYPE_F32,
                  "unsupported dtype code %d", dtype);
   SPRUCE_REQUIRE(rotary_dim >= 0 && rotary_dim <= D && rotary_dim % 16 == 0,
                  "rotary_dim must be a multiple of 16 up to head_dim, got %lld", (long long)rotary_dim);
   SPRUCE_REQUIRE(rotary_dim == 0 || inv_freq != nullptr, "inv_freq must be a non-null device pointer");
-  SPRUCE_REQUIRE(layout == SPRUCE_ROTARY_HALF || layout == SPRUCE_ROTARY_INTERLEAVED, "unknown rotary layout %d",
-                 layout);
+  SPRUCE_REQUIRE(layout == SPRUCE_ROTARY_HALF || layout == SPRUCE_ROTARY_INTERLEAVED, "unknown rotary layout %lld",
+                 (long long)layout);
   SPRUCE_REQUIRE(weight_dtype == SPRUCE_DTYPE_F32 || weight_dtype == dtype,
-                 "norm weights must be float32 or the input dtype (code %d), got code %d", dtype, weight_dtype);
+                 "norm weights must be float32 or the input dtype (code %d), got code %d", dtype, (int)weight_dtype);
   SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(q_weight) % 16 == 0 && reinterpret_cast<uintptr_t>(k_weight) % 16 == 0,
                  "norm weights must be 16-byte aligned");
   SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(inv_freq) % 8 == 0, "inv_freq must be 8-byte aligned");
   p.inv_freq = inv_freq;
   p.rot = (int)rotary_dim;
   p.interleaved = layout == SPRUCE_ROTARY_INTERLEAVED;
-  p.factor = factor;
+  p.factor = (float)factor;
   p.q_weight = q_weight;
   p.k_weight = k_weight;
   p.weight_f32 = weight_dtype == SPRUCE_DTYPE_F32;
-  p.eps = eps;
+  p.eps = (float)eps;
   return SPRUCE_OK;
 }
 
 }  // namespace
 
-extern "C" int spruce_rotate_heads(const void* q, const int64_t qs[4], const void* k, const int64_t ks[4], int64_t B,
-                                   int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int dtype, const void* positions,
-                                   int64_t pos_stride, int pos64, const double* inv_freq, int64_t rotary_dim,
-                                   int layout, float factor, const void* q_weight, const void* k_weight,
-                                   int weight_dtype, float eps, void* qo, const int64_t qos[4], void* ko,
-                                   const int64_t kos[4], void* stream) {
-  SPRUCE_REQUIRE(qs && ks && qos && kos, "stride arrays must be non-null");
+extern "C" int spruce_rotate_heads(const spruce_rotate_heads_args* args, void* stream) {
+  SPRUCE_REQUIRE(args != nullptr, "args must be non-null");
+  const spruce_rotate_heads_args& a = *args;
+  const int64_t B = a.B, Hq = a.Hq, Hkv = a.Hkv, T = a.T, D = a.D;
+  const int dtype = (int)a.dtype;
   SPRUCE_REQUIRE(B >= 0 && T >= 0 && Hq >= 1 && Hkv >= 1 && Hq < 1 << 16 && Hkv < 1 << 16, "invalid shape");
   SPRUCE_REQUIRE(T < (int64_t)1 << 30 && B < (int64_t)1 << 30, "too many tokens");
-  SPRUCE_REQUIRE(qs[3] == 1 && ks[3] == 1 && qos[3] == 1 && kos[3] == 1,
+  SPRUCE_REQUIRE(a.qs[3] == 1 && a.ks[3] == 1 && a.qos[3] == 1 && a.kos[3] == 1,
                  "q, k and the outputs must have a contiguous final dimension");
   RotaryParams p{};
-  const int rc = set_rotary(p, D, dtype, inv_freq, rotary_dim, layout, factor, q_weight, k_weight, weight_dtype, eps);
+  const int rc = set_rotary(p, D, dtype, a.inv_freq, a.rotary_dim, a.layout, a.factor, a.q_weight, a.k_weight,
+                            a.weight_dtype, a.eps);
   if (rc) return rc;
   if (B == 0 || T == 0) return SPRUCE_OK;
-  SPRUCE_REQUIRE(q && k && qo && ko && positions, "q, k, positions and the outputs must be non-null device pointers");
+  SPRUCE_REQUIRE(a.q && a.k && a.q_out && a.k_out && a.positions, "q, k, positions and the outputs must be non-null device pointers");
   const int eb = dtype == SPRUCE_DTYPE_F32 ? 4 : 2;
-  SPRUCE_REQUIRE(rows16(q, qs, eb) && rows16(k, ks, eb) && rows16(qo, qos, eb) && rows16(ko, kos, eb),
+  SPRUCE_REQUIRE(rows16(a.q, a.qs, eb) && rows16(a.k, a.ks, eb) && rows16(a.q_out, a.qos, eb) &&
+                     rows16(a.k_out, a.kos, eb),
                  "q, k and the outputs must be 16-byte aligned with strides that keep rows 16-byte aligned");
   auto rows = [](RotaryRows& r, const void* src, const int64_t* ss, void* dst, const int64_t* ds, int64_t heads) {
     r.src = src;
@@ -329,38 +329,36 @@ extern "C" int spruce_rotate_heads(const void* q, const int64_t qs[4], const voi
     }
     r.heads = (int)heads;
   };
-  rows(p.q, q, qs, qo, qos, Hq);
-  rows(p.k, k, ks, ko, kos, Hkv);
-  p.positions = positions;
-  p.pos_stride = pos_stride;
-  p.pos64 = pos64;
+  rows(p.q, a.q, a.qs, a.q_out, a.qos, Hq);
+  rows(p.k, a.k, a.ks, a.k_out, a.kos, Hkv);
+  p.positions = a.positions;
+  p.pos_stride = a.pos_stride;
+  p.pos64 = a.pos64 != 0;
   p.tokens = (int)T;
   p.rows = B * T;
   return launch_rotary<false>(p, D, dtype, (hipStream_t)stream);
 }
 
-extern "C" int spruce_paged_append(const void* q, const int64_t qs[3], void* qo, const int64_t qos[3], const void* k,
-                                   const int64_t ks[3], const void* v, const int64_t vs[3], int64_t N, int64_t Hq,
-                                   int64_t Hkv, int64_t D, int dtype, void* k_pages, const int64_t kps[4],
-                                   void* v_pages, const int64_t vps[4], int64_t pages, int64_t page_size,
-                                   const int32_t* page_table, int64_t table_stride, int64_t table_width,
-                                   const int32_t* q_starts, const int32_t* kv_lens, int64_t S, const void* positions,
-                                   int pos64, const double* inv_freq, int64_t rotary_dim, int layout, float factor,
-                                   const void* q_weight, const void* k_weight, int weight_dtype, float eps,
-                                   void* stream) {
-  SPRUCE_REQUIRE(ks && vs && kps && vps, "stride arrays must be non-null");
-  SPRUCE_REQUIRE(Hq == 0 || (qs && qos), "stride arrays must be non-null");
+extern "C" int spruce_paged_append(const spruce_paged_append_args* args, void* stream) {
+  SPRUCE_REQUIRE(args != nullptr, "args must be non-null");
+  const spruce_paged_append_args& a = *args;
+  const int64_t N = a.N, Hq = a.Hq, Hkv = a.Hkv, D = a.D;
+  const int dtype = (int)a.dtype;
   SPRUCE_REQUIRE(Hq >= 0 && Hkv >= 1 && Hq < 1 << 16 && Hkv < 1 << 16, "invalid shape");
-  SPRUCE_REQUIRE((Hq == 0 || (qs[2] == 1 && qos[2] == 1)) && ks[2] == 1 && vs[2] == 1 && kps[3] == 1 && vps[3] == 1,
+  SPRUCE_REQUIRE((Hq == 0 || (a.qs[2] == 1 && a.qos[2] == 1)) && a.ks[2] == 1 && a.vs[2] == 1 && a.kps[3] == 1 &&
+                     a.vps[3] == 1,
                  "q, k, v, the pages and the output must have a contiguous final dimension");
   RotaryParams p{};
-  int rc = set_rotary(p, D, dtype, inv_freq, rotary_dim, layout, factor, q_weight, k_weight, weight_dtype, eps);
+  int rc = set_rotary(p, D, dtype, a.inv_freq, a.rotary_dim, a.layout, a.factor, a.q_weight, a.k_weight, a.weight_dtype,
+                      a.eps);
   if (rc) return rc;
-  rc = prepare_batch(p.batch, page_table, table_stride, table_width, q_starts, kv_lens, S, N, page_size, pages);
+  rc = prepare_batch(p.batch, a.page_table, a.table_stride, a.table_width, a.q_starts, a.kv_lens, a.S, N, a.page_size,
+                     a.pages);
   if (rc) return rc;
   if (N == 0) return SPRUCE_OK;
-  SPRUCE_REQUIRE(k && v && (pages == 0 || (k_pages && v_pages)), "k, v and the pages must be non-null device pointers");
-  SPRUCE_REQUIRE(Hq == 0 || (q && qo), "q and its output must be non-null device pointers");
+  SPRUCE_REQUIRE(a.k && a.v && (a.pages == 0 || (a.k_pages && a.v_pages)),
+                 "k, v and the pages must be non-null device pointers");
+  SPRUCE_REQUIRE(Hq == 0 || (a.q && a.q_out), "q and its output must be non-null device pointers");
   // Packed [N, H, D] rows as one batch; the pages' strides as they are.
   auto rows = [&](RotaryRows& r, const void* src, const int64_t* ss, void* dst, const int64_t* ds, bool paged, int64_t heads) {
     r.src = src;
@@ -373,15 +371,15 @@ extern "C" int spruce_paged_append(const void* q, const int64_t qs[3], void* qo,
     r.heads = (int)heads;
   };
   const int eb = dtype == SPRUCE_DTYPE_F32 ? 4 : 2;
-  if (Hq) rows(p.q, q, qs, qo, qos, false, Hq);
-  rows(p.k, k, ks, k_pages, kps, true, Hkv);
-  rows(p.v, v, vs, v_pages, vps, true, Hkv);
+  if (Hq) rows(p.q, a.q, a.qs, a.q_out, a.qos, false, Hq);
+  rows(p.k, a.k, a.ks, a.k_pages, a.kps, true, Hkv);
+  rows(p.v, a.v, a.vs, a.v_pages, a.vps, true, Hkv);
   auto fits = [&](const RotaryRows& r) { return rows16(r.src, r.ss, eb) && rows16(r.dst, r.ds, eb); };
   SPRUCE_REQUIRE((Hq == 0 || fits(p.q)) && fits(p.k) && fits(p.v),
                  "q, k, v, the pages and the output must be 16-byte aligned with strides that keep rows 16-byte "
                  "aligned");
-  p.positions = positions;
-  p.pos64 = pos64;
+  p.positions = a.positions;
+  p.pos64 = a.pos64 != 0;
   p.tokens = (int)N;
   p.rows = N;
   return launch_rotary<true>(p, D, dtype, (hipStream_t)stream);

@@ -20,39 +20,47 @@ Calls run on the current stream of the tensors' device, wait for nothing and
 can be captured; a replay goes by what the three tensors then hold.  Inference
 only: inputs that need gradients are refused.
 """
-import ctypes
+import functools
+import struct
 
 import torch
 
 import spruce_hip
-from kernels.rotary import _positions, _refuse_grad, _rotation, _weights
+from kernels.rotary import _needs_grad, _positions, _refuse_grad, _rotation, _weights
 
 __all__ = ["append_paged_kv", "paged_chunk_attention"]
 
-_I64X3 = ctypes.c_int64 * 3
+# struct spruce_paged_append_args and spruce_paged_attention_args, field by field.
+_APPEND_ARGS = struct.Struct("=q3qq3qq3qq3q5qq4qq4qqqqqqqqqqqqqqdqqqd")
+_ATTENTION_ARGS = struct.Struct("=q3qq4qq4qqqqqqqq6qdq4qqqq3qqq")
 
 
-def _check_cache(k_pages, v_pages, page_table, q_starts, kv_lens, like):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+def _check_cache(k_pages, v_pages, page_table, q_starts, kv_lens, dtype, device):
+    """The packed fields of a checked cache and batch (pages to sequences), and its shape."""
+    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must match as [pages, Hkv, page_size, D]")
-    if k_pages.dtype != like.dtype or v_pages.dtype != like.dtype:
+    if k_pages.dtype != dtype or v_pages.dtype != dtype:
         raise ValueError("the pages must have the dtype of the new tokens")
-    if k_pages.stride(-1) != 1 or v_pages.stride(-1) != 1:
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError("k_pages and v_pages must have a contiguous final dimension")
     if page_table.dim() != 2 or page_table.dtype != torch.int32:
         raise ValueError("page_table must be int32 [S, W]")
-    S = page_table.shape[0]
-    if S < 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    S, W = page_table.shape
+    ts, step = page_table.stride()
+    if S < 1 or (W > 1 and step != 1):
         raise ValueError("page_table needs a sequence and a contiguous final dimension")
     if q_starts.dtype != torch.int32 or q_starts.shape != (S + 1,) or not q_starts.is_contiguous():
         raise ValueError(f"q_starts must be contiguous int32 [S + 1] = [{S + 1}]")
     if kv_lens.dtype != torch.int32 or kv_lens.shape != (S,) or not kv_lens.is_contiguous():
         raise ValueError(f"kv_lens must be contiguous int32 [S] = [{S}]")
-    device = like.device
     if (k_pages.device != device or v_pages.device != device or page_table.device != device
             or q_starts.device != device or kv_lens.device != device):
         raise ValueError("the cache and the batch's tensors must be on the same device as the new tokens")
-    return S
+    # One sequence's row has no stride that matters.
+    fields = (k_pages.data_ptr(), *ks, v_pages.data_ptr(), *vs, shape[0], shape[2], page_table.data_ptr(),
+              ts if S > 1 else W, W, q_starts.data_ptr(), kv_lens.data_ptr(), S)
+    return fields, shape
 
 
 def append_paged_kv(k, v, k_pages, v_pages, page_table, q_starts, kv_lens, *, query=None, inv_freq=None,
@@ -69,48 +77,53 @@ def append_paged_kv(k, v, k_pages, v_pages, page_table, q_starts, kv_lens, *, qu
     page is not written.  Two tokens must not share a slot: which of them it then
     holds is unspecified.
     """
-    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+    device, dtype = k.device, k.dtype
+    if k.dim() != 3 or k.shape != v.shape or v.dtype != dtype or v.device != device:
         raise ValueError("k and v must match as [N, Hkv, D]")
     N, Hkv, D = k.shape
-    if D not in (64, 128):
+    if D != 128 and D != 64:
         raise ValueError(f"kernel supports head_dim 64 or 128, got {D}")
-    S = _check_cache(k_pages, v_pages, page_table, q_starts, kv_lens, k)
-    if k_pages.shape[1] != Hkv or k_pages.shape[3] != D:
+    cache, pages = _check_cache(k_pages, v_pages, page_table, q_starts, kv_lens, dtype, device)
+    if pages[1] != Hkv or pages[3] != D:
         raise ValueError("the pages and the new tokens must match in KV heads and head_dim")
-    if k.stride(-1) != 1 or v.stride(-1) != 1:
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1 or vs[2] != 1:
         raise ValueError("k and v must have a contiguous final dimension")
-    Hq, out = 0, None
+    Hq, qs, out = 0, (0, 0, 0), None
     if query is not None:
-        if query.dim() != 3 or query.shape[0] != N or query.shape[2] != D or query.dtype != k.dtype:
+        if query.dim() != 3 or query.shape[0] != N or query.shape[2] != D or query.dtype != dtype:
             raise ValueError("query must be [N, Hq, D] in the dtype of k")
-        if query.device != k.device:
+        if query.device != device:
             raise ValueError("query must be on the same device as k")
-        if query.stride(-1) != 1:
+        Hq, qs = query.shape[1], query.stride()
+        if qs[2] != 1:
             raise ValueError("query must have a contiguous final dimension")
-        Hq = query.shape[1]
         if Hq < 1:
             raise ValueError("query must have a head")
-    rotary_dim, code = _rotation(inv_freq, layout, D, k.device)
-    weight_code = _weights(q_weight, k_weight, D, k)
-    pos64 = 0 if positions is None else _positions(positions, ((N,),), k.device)
-    _refuse_grad(k, v, query, k_pages, v_pages, q_weight, k_weight, inv_freq)
+    rotation = _rotation(inv_freq, layout, D, device)
+    weights = _weights(q_weight, k_weight, D, dtype, device)
+    place = (0, 0, False) if positions is None else _positions(positions, ((N,),), device)
+    if torch.is_grad_enabled() and (
+            k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+            or (query is not None and query.requires_grad) or _needs_grad(q_weight, k_weight, inv_freq)):
+        _refuse_grad()
     if not k.is_cuda:
         raise RuntimeError("the paged HIP backend requires GPU tensors")
-    if query is not None:
-        out = torch.empty((N, Hq, D), device=k.device, dtype=k.dtype)
-    with spruce_hip.on_device(k.device):
-        rc = spruce_hip.lib().spruce_paged_append(
-            spruce_hip.ptr(query), _I64X3(*query.stride()) if Hq else None, spruce_hip.ptr(out),
-            _I64X3(*out.stride()) if Hq else None,
-            spruce_hip.ptr(k), _I64X3(*k.stride()), spruce_hip.ptr(v), _I64X3(*v.stride()),
-            N, Hq, Hkv, D, spruce_hip.dtype_code(k),
-            spruce_hip.ptr(k_pages), spruce_hip.strides(k_pages), spruce_hip.ptr(v_pages), spruce_hip.strides(v_pages),
-            k_pages.shape[0], k_pages.shape[2], spruce_hip.ptr(page_table), page_table.stride(0), page_table.shape[1],
-            spruce_hip.ptr(q_starts), spruce_hip.ptr(kv_lens), S, spruce_hip.ptr(positions), pos64,
-            spruce_hip.ptr(inv_freq), rotary_dim, code, factor, spruce_hip.ptr(q_weight), spruce_hip.ptr(k_weight),
-            weight_code, eps, spruce_hip.stream_of(k))
-    spruce_hip.check(rc, "spruce_paged_append")
+    if Hq:
+        out = torch.empty((N, Hq, D), device=device, dtype=dtype)
+    with spruce_hip.on_device(device):
+        rc = spruce_hip.lib().spruce_paged_append(_APPEND_ARGS.pack(
+            query.data_ptr() if Hq else 0, *qs, out.data_ptr() if Hq else 0, Hq * D, D, 1,
+            k.data_ptr(), *ks, v.data_ptr(), *vs, N, Hq, Hkv, D, spruce_hip.dtype_code(k), *cache, place[0], place[2],
+            *rotation, factor, *weights, eps), spruce_hip.raw_stream(device.index))
+    if rc:
+        spruce_hip.check(rc, "spruce_paged_append")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*shape):
+    return spruce_hip.lib().spruce_paged_attention_workspace_bytes(*shape)
 
 
 def paged_chunk_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, scale, *, indices=None, out=None):
@@ -130,52 +143,53 @@ def paged_chunk_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, sc
     were).  A token that attends no key gets zeros, a key without a page no
     weight, and what masked keys and values hold reaches no row.
     """
-    if q.dim() != 3 or k_pages.dim() != 4:
+    device, dtype = q.device, q.dtype
+    if q.dim() != 3:
         raise ValueError("q must be [N, Hq, D] and the pages [pages, Hkv, page_size, D]")
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"the paged attention takes bfloat16 or float16, got {q.dtype}")
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise ValueError(f"the paged attention takes bfloat16 or float16, got {dtype}")
     N, Hq, D = q.shape
-    S = _check_cache(k_pages, v_pages, page_table, q_starts, kv_lens, q)
-    pages, Hkv, page_size, _ = k_pages.shape
-    if D not in (64, 128):
+    cache, (_, Hkv, page_size, Dk) = _check_cache(k_pages, v_pages, page_table, q_starts, kv_lens, dtype, device)
+    S, W = page_table.shape
+    if D != 128 and D != 64:
         raise ValueError(f"kernel supports head_dim 64 or 128, got {D}")
-    if k_pages.shape[3] != D:
+    if Dk != D:
         raise ValueError("q and the pages must match in head_dim")
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError("query heads must be divisible by KV heads")
-    if q.stride(-1) != 1:
+    qs = q.stride()
+    if qs[2] != 1:
         raise ValueError("q must have a contiguous final dimension")
     if not 0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    Qc = K = 0
+    lists, K = (0, 0, 0, 0, 1, 0, 0), 0
     if indices is not None:
         if indices.dim() != 4 or tuple(indices.shape[:2]) != (S, Hkv) or indices.dtype != torch.int32:
             raise ValueError("indices must be int32 [S,Hkv,Qc,K]")
         Qc, K = indices.shape[2:]
         if Qc < 1 or K < 1:
             raise ValueError("indices must hold a row and a column")
-        if indices.stride(-1) != 1 and K > 1:
+        strides = indices.stride()
+        if strides[3] != 1 and K > 1:
             raise ValueError("indices must have a contiguous final dimension")
-        if indices.device != q.device:
+        if indices.device != device:
             raise ValueError("indices must be on the same device as q")
-    if out is not None:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1:
-            raise ValueError("out must match q in shape, dtype and device, with a contiguous final dimension")
-    _refuse_grad(q, k_pages, v_pages, out)
+        lists = (indices.data_ptr(), *strides[:3], 1, Qc, K)
+    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.device != device or out.stride(-1) != 1):
+        raise ValueError("out must match q in shape, dtype and device, with a contiguous final dimension")
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad
+                                    or (out is not None and out.requires_grad)):
+        _refuse_grad()
     if not q.is_cuda:
         raise RuntimeError("the paged HIP backend requires GPU tensors")
     if out is None:
-        out = torch.empty((N, Hq, D), device=q.device, dtype=q.dtype)
-    lib = spruce_hip.lib()
-    need = lib.spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D, page_table.shape[1] * page_size, K)
-    work = torch.empty(need, device=q.device, dtype=torch.uint8)
-    with spruce_hip.on_device(q.device):
-        rc = lib.spruce_paged_attention(
-            spruce_hip.ptr(q), _I64X3(*q.stride()), spruce_hip.ptr(k_pages), spruce_hip.strides(k_pages),
-            spruce_hip.ptr(v_pages), spruce_hip.strides(v_pages), pages, page_size,
-            spruce_hip.ptr(page_table), page_table.stride(0), page_table.shape[1], spruce_hip.ptr(q_starts),
-            spruce_hip.ptr(kv_lens), S, N, Hq, Hkv, D, scale, spruce_hip.DTYPE_CODES[q.dtype],
-            spruce_hip.ptr(indices), None if indices is None else spruce_hip.strides(indices), Qc, K,
-            spruce_hip.ptr(out), _I64X3(*out.stride()), spruce_hip.ptr(work), need, spruce_hip.stream_of(q))
-    spruce_hip.check(rc, "spruce_paged_attention")
+        out = torch.empty((N, Hq, D), device=device, dtype=dtype)
+    need = _workspace_bytes(N, S, Hq, Hkv, D, W * page_size, K)
+    work = torch.empty(need, device=device, dtype=torch.uint8)
+    with spruce_hip.on_device(device):
+        rc = spruce_hip.lib().spruce_paged_attention(_ATTENTION_ARGS.pack(
+            q.data_ptr(), *qs, *cache, N, Hq, Hkv, D, spruce_hip.DTYPE_CODES[dtype], scale, *lists,
+            out.data_ptr(), *out.stride(), work.data_ptr(), need), spruce_hip.raw_stream(device.index))
+    if rc:
+        spruce_hip.check(rc, "spruce_paged_attention")
     return out

@@ -8,6 +8,7 @@ attention: inputs that need gradients are refused.  (The reference leaves this
 step to Transformers' model code.)
 """
 import math
+import struct
 
 import torch
 
@@ -65,52 +66,66 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, or
     return inv_freq.to(device), attention
 
 
-def _refuse_grad(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the HIP rotary and paged operators compute no gradients; run them under torch.no_grad()")
+def _refuse_grad():
+    raise RuntimeError("the HIP rotary and paged operators compute no gradients; run them under torch.no_grad()")
+
+
+_LAYOUT_CODES = {name: code for code, name in enumerate(ROTARY_LAYOUTS)}
 
 
 def _rotation(inv_freq, layout, head_dim, device):
-    """(rotary_dim, layout code) of checked angles (None: no rotation)."""
-    if layout not in ROTARY_LAYOUTS:
+    """(pointer, rotary_dim, layout code) of checked angles (None: no rotation)."""
+    code = _LAYOUT_CODES.get(layout)
+    if code is None:
         raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
     if inv_freq is None:
-        return 0, 0
+        return 0, 0, 0
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be contiguous float64 [rotary_dim / 2]")
     if inv_freq.device != device:
         raise ValueError("inv_freq must be on the same device as q and k")
-    rotary_dim = 2 * inv_freq.shape[0]
+    rotary_dim = 2 * len(inv_freq)
     if rotary_dim > head_dim or rotary_dim % 16:
         raise ValueError(f"rotary_dim must be a multiple of 16 up to head_dim {head_dim}, got {rotary_dim}")
-    return rotary_dim, ROTARY_LAYOUTS.index(layout)
+    return inv_freq.data_ptr(), rotary_dim, code
 
 
-def _weights(q_weight, k_weight, head_dim, like):
-    """The norm weights' shared dtype code, after their checks."""
-    dtype = None
+def _weights(q_weight, k_weight, head_dim, dtype, device):
+    """(pointers of the norm weights, their shared dtype code), after their checks."""
+    shared = None
     for w in (q_weight, k_weight):
         if w is None:
             continue
         if w.shape != (head_dim,) or not w.is_contiguous():
             raise ValueError(f"norm weights must be contiguous [{head_dim}]")
-        if w.device != like.device:
+        if w.device != device:
             raise ValueError("norm weights must be on the same device as q and k")
-        if w.dtype not in (like.dtype, torch.float32) or dtype not in (None, w.dtype):
+        if w.dtype not in (dtype, torch.float32) or shared not in (None, w.dtype):
             raise ValueError("norm weights must share one dtype: float32 or the inputs'")
-        dtype = w.dtype
-    return spruce_hip.DTYPE_CODES[dtype or torch.float32]
+        shared = w.dtype
+    return (0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+            2 if shared is None else spruce_hip.DTYPE_CODES[shared])
 
 
-def _positions(positions, shape, device):
+def _positions(positions, shapes, device):
+    """(pointer, row stride, 64 bits or not) of checked positions."""
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be int32 or int64")
     if positions.device != device:
         raise ValueError("positions must be on the same device as q and k")
-    if tuple(positions.shape) not in shape or (positions.shape[-1] > 1 and positions.stride(-1) != 1):
-        raise ValueError(f"positions must be {' or '.join(map(str, shape))} with contiguous tokens, "
-                         f"got {tuple(positions.shape)}")
-    return int(positions.dtype == torch.int64)
+    shape, stride = tuple(positions.shape), positions.stride()
+    if shape not in shapes or (shape[-1] > 1 and stride[-1] != 1):
+        raise ValueError(f"positions must be {' or '.join(map(str, shapes))} with contiguous tokens, got {shape}")
+    return positions.data_ptr(), stride[0] if len(shape) == 2 else 0, positions.dtype == torch.int64
+
+
+def _needs_grad(q_weight, k_weight, inv_freq):
+    return ((q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)
+            or (inv_freq is not None and inv_freq.requires_grad))
+
+
+# struct spruce_rotate_heads_args, field by field.
+_ROTATE_ARGS = struct.Struct("=q4qq4q6qqqqqqqdqqqdq4qq4q")
 
 
 def rotate_heads(q, k, positions, inv_freq, *, layout="half", factor=1.0, q_weight=None, k_weight=None, eps=1e-6):
@@ -129,32 +144,36 @@ def rotate_heads(q, k, positions, inv_freq, *, layout="half", factor=1.0, q_weig
     the rest in 32, rounded once.  Returns (q, k) of the same shapes and dtype,
     as views of contiguous ``[B,T,H,D]`` tensors.
     """
-    if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+    device, dtype = q.device, q.dtype
+    if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q and k must be [B,H,T,D] and match in batch, tokens, and head_dim")
-    if q.dtype != k.dtype:
-        raise ValueError("q and k must share one dtype")
-    if k.device != q.device:
-        raise ValueError("q and k must be on the same device")
     B, Hq, T, D = q.shape
-    if D not in (64, 128):
+    Bk, Hkv, Tk, Dk = k.shape
+    if Bk != B or Tk != T or Dk != D:
+        raise ValueError("q and k must be [B,H,T,D] and match in batch, tokens, and head_dim")
+    if k.dtype != dtype:
+        raise ValueError("q and k must share one dtype")
+    if k.device != device:
+        raise ValueError("q and k must be on the same device")
+    if D != 128 and D != 64:
         raise ValueError(f"kernel supports head_dim 64 or 128, got {D}")
-    if q.stride(-1) != 1 or k.stride(-1) != 1:
+    qs, ks = q.stride(), k.stride()
+    if qs[3] != 1 or ks[3] != 1:
         raise ValueError("q and k must have a contiguous final dimension")
-    rotary_dim, code = _rotation(inv_freq, layout, D, q.device)
-    weight_code = _weights(q_weight, k_weight, D, q)
-    pos64 = _positions(positions, ((B, T), (T,)), q.device)
-    _refuse_grad(q, k, q_weight, k_weight, inv_freq)
+    rotation = _rotation(inv_freq, layout, D, device)
+    weights = _weights(q_weight, k_weight, D, dtype, device)
+    place = _positions(positions, ((B, T), (T,)), device)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or _needs_grad(q_weight, k_weight, inv_freq)):
+        _refuse_grad()
     if not q.is_cuda:
         raise RuntimeError("the rotary HIP backend requires GPU tensors")
-    qo = torch.empty((B, T, Hq, D), device=q.device, dtype=q.dtype).transpose(1, 2)
-    ko = torch.empty((B, T, k.shape[1], D), device=q.device, dtype=q.dtype).transpose(1, 2)
-    with spruce_hip.on_device(q.device):
-        rc = spruce_hip.lib().spruce_rotate_heads(
-            spruce_hip.ptr(q), spruce_hip.strides(q), spruce_hip.ptr(k), spruce_hip.strides(k),
-            B, Hq, k.shape[1], T, D, spruce_hip.dtype_code(q), spruce_hip.ptr(positions),
-            positions.stride(0) if positions.dim() == 2 else 0, pos64, spruce_hip.ptr(inv_freq), rotary_dim, code,
-            factor, spruce_hip.ptr(q_weight), spruce_hip.ptr(k_weight), weight_code, eps,
-            spruce_hip.ptr(qo), spruce_hip.strides(qo), spruce_hip.ptr(ko), spruce_hip.strides(ko),
-            spruce_hip.stream_of(q))
-    spruce_hip.check(rc, "spruce_rotate_heads")
-    return qo, ko
+    qo = torch.empty((B, T, Hq, D), device=device, dtype=dtype)
+    ko = torch.empty((B, T, Hkv, D), device=device, dtype=dtype)
+    with spruce_hip.on_device(device):
+        rc = spruce_hip.lib().spruce_rotate_heads(_ROTATE_ARGS.pack(
+            q.data_ptr(), *qs, k.data_ptr(), *ks, B, Hq, Hkv, T, D, spruce_hip.dtype_code(q), *place, *rotation, factor,
+            *weights, eps, qo.data_ptr(), T * Hq * D, D, Hq * D, 1, ko.data_ptr(), T * Hkv * D, D, Hkv * D, 1),
+            spruce_hip.raw_stream(device.index))
+    if rc:
+        spruce_hip.check(rc, "spruce_rotate_heads")
+    return qo.transpose(1, 2), ko.transpose(1, 2)

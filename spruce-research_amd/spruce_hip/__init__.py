@@ -108,16 +108,10 @@ _SIGNATURES = {
     "spruce_tree_traverse": [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _i64,
                              ctypes.c_int, _p],
     "spruce_gate_candidate_scores": [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _p],
-    "spruce_rotate_heads": [
-        _p, _STRIDES, _p, _STRIDES, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, _p, _i64, ctypes.c_int, _p, _i64,
-        ctypes.c_int, ctypes.c_float, _p, _p, ctypes.c_int, ctypes.c_float, _p, _STRIDES, _p, _STRIDES, _p],
-    "spruce_paged_append": [
-        _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _i64, _i64, _i64, _i64, ctypes.c_int,
-        _p, _STRIDES, _p, _STRIDES, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p, ctypes.c_int, _p, _i64,
-        ctypes.c_int, ctypes.c_float, _p, _p, ctypes.c_int, ctypes.c_float, _p],
-    "spruce_paged_attention": [
-        _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64,
-        ctypes.c_float, ctypes.c_int, _p, _STRIDES, _i64, _i64, _p, _STRIDES, _p, _i64, _p],
+    # The paged serving step: the arguments in one block (``struct`` packs it), and the stream.
+    "spruce_rotate_heads": [ctypes.c_char_p, _p],
+    "spruce_paged_append": [ctypes.c_char_p, _p],
+    "spruce_paged_attention": [ctypes.c_char_p, _p],
     "spruce_sparse_prefill_mask": [
         _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _i64,
         _i64, _i64, _i64, _i64, _i64, ctypes.c_float, ctypes.c_int, ctypes.c_int,
@@ -204,6 +198,15 @@ def ptr(t):
 def stream_of(t):
     return torch.cuda.current_stream(t.device).cuda_stream
 
+
+def raw_stream(index):
+    """The hipStream_t of the current stream of device ``index``: ``stream_of`` without
+    the stream object it makes on the way (2 us of a call of 15)."""
+    return _raw_stream(index)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 _SAME_DEVICE = contextlib.nullcontext()
 

@@ -1,12 +1,14 @@
 """Rotary frequencies and the refusals of the rotary and append calls: the
 checks come before the GPU is touched, so these run without one."""
-import ctypes
 import math
+import os
+import re
 
 import pytest
 import torch
 
 import spruce_hip
+from kernels import paged, rotary
 from kernels.paged import append_paged_kv, paged_chunk_attention
 from kernels.rotary import rotary_frequencies, rotate_heads
 
@@ -126,39 +128,57 @@ def test_append_refusals():
         _append(k=torch.zeros(3, 2, 64, dtype=bf, requires_grad=True))
 
 
-def _st(*s):
-    return (ctypes.c_int64 * len(s))(*s)
+FAKE = 1 << 20  # never dereferenced: validation fails first
+
+
+def _call(entry, layout, fields):
+    return getattr(spruce_hip.lib(), entry)(layout.pack(*fields), None)
 
 
 def test_entry_points_refuse_before_the_launch():
-    lib, fake = spruce_hip.lib(), ctypes.c_void_p(1 << 20)
-
-    def rotate(D=128, dtype=0, R=128, layout=0, wd=2, qs=(0, 128, 512, 1), B=1, q=fake, freq=fake, w=None):
-        return lib.spruce_rotate_heads(q, _st(*qs), fake, _st(0, 128, 256, 1), B, 4, 2, 8, D, dtype, fake, 0, 0, freq,
-                                       R, layout, 1.0, w, None, wd, 1e-6, fake, _st(0, 128, 512, 1), fake,
-                                       _st(0, 128, 256, 1), None)
+    def rotate(D=128, dtype=0, R=128, layout=0, wd=2, qs=(0, 128, 512, 1), B=1, q=FAKE, freq=FAKE, w=0):
+        return _call("spruce_rotate_heads", rotary._ROTATE_ARGS, (
+            q, *qs, FAKE, 0, 128, 256, 1, B, 4, 2, 8, D, dtype, FAKE, 0, 0, freq, R, layout, 1.0, w, 0, wd, 1e-6,
+            FAKE, 0, 128, 512, 1, FAKE, 0, 128, 256, 1))
     for kwargs, message in ((dict(D=96), "head_dim 64 or 128"), (dict(dtype=3), "dtype"), (dict(R=24), "rotary_dim"),
                             (dict(R=144), "rotary_dim"), (dict(layout=2), "layout"), (dict(wd=1), "norm weights"),
-                            (dict(w=ctypes.c_void_p((1 << 20) + 4)), "norm weights must be 16-byte"),
+                            (dict(w=FAKE + 4), "norm weights must be 16-byte"),
                             (dict(qs=(0, 128, 512, 2)), "contiguous final"), (dict(qs=(0, 100, 512, 1)), "16-byte"),
-                            (dict(q=ctypes.c_void_p((1 << 20) + 2)), "16-byte"), (dict(q=None), "non-null"),
-                            (dict(freq=None), "inv_freq"), (dict(B=-1), "invalid shape")):
+                            (dict(q=FAKE + 2), "16-byte"), (dict(q=0), "non-null"),
+                            (dict(freq=0), "inv_freq"), (dict(B=-1), "invalid shape")):
         assert rotate(**kwargs) == -1, kwargs
         assert message in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
     assert rotate(B=0) == 0
+    assert spruce_hip.lib().spruce_rotate_heads(None, None) == -1
 
-    def append(N=8, Hq=4, page=16, pages=9, width=4, stride=4, S=2, table=fake, q=fake, kps=(4096, 2048, 128, 1)):
-        return lib.spruce_paged_append(q, _st(512, 128, 1), fake, _st(512, 128, 1), fake, _st(256, 128, 1), fake,
-                                       _st(256, 128, 1), N, Hq, 2, 128, 0, fake, _st(*kps), fake,
-                                       _st(4096, 2048, 128, 1), pages, page, table, stride, width, fake, fake, S, None,
-                                       0, None, 0, 0, 1.0, None, None, 2, 1e-6, None)
+    def append(N=8, Hq=4, page=16, pages=9, width=4, stride=4, S=2, table=FAKE, q=FAKE, kps=(4096, 2048, 128, 1)):
+        return _call("spruce_paged_append", paged._APPEND_ARGS, (
+            q, 512, 128, 1, FAKE, 512, 128, 1, FAKE, 256, 128, 1, FAKE, 256, 128, 1, N, Hq, 2, 128, 0, FAKE, *kps,
+            FAKE, 4096, 2048, 128, 1, pages, page, table, stride, width, FAKE, FAKE, S, 0, 0, 0, 0, 0, 1.0, 0, 0, 2,
+            1e-6))
     for kwargs, message in ((dict(page=0), "page size"), (dict(S=0), "sequences"), (dict(stride=3), "overlap"),
                             (dict(width=1 << 28, stride=1 << 28), "2^31"), (dict(pages=-1), "page count"),
-                            (dict(N=-1), "token count"), (dict(table=None), "non-null"), (dict(q=None), "non-null"),
+                            (dict(N=-1), "token count"), (dict(table=0), "non-null"), (dict(q=0), "non-null"),
                             (dict(kps=(4096, 2048, 100, 1)), "16-byte")):
         assert append(**kwargs) == -1, kwargs
         assert message in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
     assert append(N=0) == 0
+    assert spruce_hip.lib().spruce_paged_append(None, None) == -1
+
+
+def test_argument_blocks_match_the_header():
+    # The packed fields, in order: pointers, integers and arrays are 8 bytes each, doubles "d".
+    text = open(os.path.join(os.path.dirname(spruce_hip.LIB_PATH), "..", "..", "include", "spruce_hip.h")).read()
+    for name, layout in (("rotate_heads", rotary._ROTATE_ARGS), ("paged_append", paged._APPEND_ARGS),
+                         ("paged_attention", paged._ATTENTION_ARGS)):
+        body = re.search(r"typedef struct spruce_%s_args \{(.*?)\} spruce" % name, text, re.S).group(1)
+        kinds = ""
+        for line in body.strip().split(";"):
+            for field in filter(None, (f.strip() for f in line.split(","))):
+                size = re.search(r"\[(\d)\]", field)
+                kinds += ("d" if line.strip().startswith("double") else "q") * (int(size.group(1)) if size else 1)
+        code = re.sub(r"(\d)q", lambda m: "q" * int(m.group(1)), layout.format.lstrip("="))
+        assert code == kinds, name
 
 
 def test_page_division_by_multiplication():
@@ -207,23 +227,23 @@ def test_attention_refusals():
 
 
 def test_attention_entry_point_refuses_before_the_launch():
-    lib, fake = spruce_hip.lib(), ctypes.c_void_p(1 << 20)
-    need = lib.spruce_paged_attention_workspace_bytes(8, 2, 4, 2, 128, 64, 0)
+    need = spruce_hip.lib().spruce_paged_attention_workspace_bytes(8, 2, 4, 2, 128, 64, 0)
     assert need > 0 and need % 16 == 0
 
-    def call(D=128, dtype=0, Hq=4, scale=0.1, qs=(512, 128, 1), K=0, idx=None, is_=(1, 1, 1, 1), Qc=1, ws=fake,
-             ws_bytes=need, width=4, N=8, q=fake):
-        return lib.spruce_paged_attention(q, _st(*qs), fake, _st(4096, 2048, 128, 1), fake, _st(4096, 2048, 128, 1), 9,
-                                          16, fake, 4, width, fake, fake, 2, N, Hq, 2, D, scale, dtype, idx, _st(*is_),
-                                          Qc, K, fake, _st(512, 128, 1), ws, ws_bytes, None)
+    def call(D=128, dtype=0, Hq=4, scale=0.1, qs=(512, 128, 1), K=0, idx=0, is_=(1, 1, 1, 1), Qc=1, ws=FAKE,
+             ws_bytes=need, width=4, N=8, q=FAKE):
+        return _call("spruce_paged_attention", paged._ATTENTION_ARGS, (
+            q, *qs, FAKE, 4096, 2048, 128, 1, FAKE, 4096, 2048, 128, 1, 9, 16, FAKE, 4, width, FAKE, FAKE, 2, N, Hq, 2, D,
+            dtype, scale, idx, *is_, Qc, K, FAKE, 512, 128, 1, ws, ws_bytes))
     for kwargs, message in ((dict(D=96), "head_dim 64 or 128"), (dict(dtype=2), "bf16 or f16"),
                             (dict(Hq=5), "divisible"), (dict(Hq=130), "at most 64"), (dict(scale=0.0), "scale"),
                             (dict(scale=float("inf")), "scale"), (dict(qs=(512, 128, 2)), "contiguous final"),
                             (dict(qs=(500, 128, 1)), "16-byte"), (dict(K=4), "indices"),
-                            (dict(K=4, idx=fake, is_=(1, 1, 1, 2)), "contiguous final"), (dict(K=-1), "list width"),
-                            (dict(ws=None), "workspace"), (dict(ws_bytes=need - 4), "workspace too small"),
-                            (dict(ws=ctypes.c_void_p((1 << 20) + 4)), "workspace must be 16-byte"),
-                            (dict(width=5), "overlap"), (dict(N=-1), "token count"), (dict(q=None), "non-null")):
+                            (dict(K=4, idx=FAKE, is_=(1, 1, 1, 2)), "contiguous final"), (dict(K=-1), "list width"),
+                            (dict(ws=0), "workspace"), (dict(ws_bytes=need - 4), "workspace too small"),
+                            (dict(ws=FAKE + 4), "workspace must be 16-byte"),
+                            (dict(width=5), "overlap"), (dict(N=-1), "token count"), (dict(q=0), "non-null")):
         assert call(**kwargs) == -1, kwargs
         assert message in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
     assert call(N=0) == 0
+    assert spruce_hip.lib().spruce_paged_attention(None, None) == -1
