@@ -36,21 +36,22 @@ struct PagedAttn {
   int Qc, K;
   int few_limit;   // packed rows of a sequence up to which it goes the few-row way
   bool whole[2];   // few, many: a workgroup takes one row tile whole
+  int groups;      // workgroups of a head that share its keys out, where they are not
   float* part_o;   // [groups][32 * D], a 32 x 32 accumulator's order
   float* part_ml;  // [groups][2][32]
 };
 
 constexpr int kWaves = 8;
 constexpr int kFewRows = 64;    // packed rows of a sequence up to which memory bounds it
-constexpr int kGroups = 256;    // workgroups that share the keys out: one a CU, its registers' fill
-constexpr int kRowCost = 256;   // a row tile's fixed part (first loads, last sums, store), in keys
+constexpr int kCus = 256;       // a workgroup fills a CU's registers
 
-// Unit shapes: packed rows of a tile.
+// Unit shapes: packed rows of a tile, and its fixed part (look-ups, first loads,
+// last sums, store) in keys.
 struct Few {
-  static constexpr int rows = 32;
+  static constexpr int rows = 32, cost = 768;
 };
 struct Many {
-  static constexpr int rows = 32 * kWaves;
+  static constexpr int rows = 32 * kWaves, cost = 512;
 };
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
@@ -121,6 +122,12 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int l) {
                    (uint32_t)__builtin_amdgcn_readlane((int)v, l));
 }
 
+// a / b of no negative numbers, by way of 32 bits where both fit.
+__device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
+
 // A key of a tile, or the last key below `end` where it lies past that.
 __device__ __forceinline__ int nearest(int key, int end) { return key < end ? key : end - 1; }
 
@@ -130,14 +137,15 @@ __device__ __forceinline__ int clip(int64_t pos) {
 }
 
 // The work of one sequence, of one kind: its row tiles per KV head, and how
-// they weigh.  Tile j weighs first + slope (j + 1): its keys, and kRowCost.
-// (An upper bound of the keys: what a tile does not have, nobody walks.)
+// they weigh.  Tile j weighs first + slope (j + 1), G to a key: its keys, and
+// its fixed part.  (An upper bound of the keys: what a tile does not have,
+// nobody walks.)
 struct SeqWork {
   int n;         // new tokens
   int64_t pos0;  // position of the first
   int tiles;     // 0 where the sequence is of the other kind
-  int per;       // tokens of a tile (0: a tile is a part of one token's heads)
-  int sub, rows;  // tiles of one token or listed block, and rows of one
+  int rows;      // packed rows of a tile
+  int sub;       // with lists: tiles of one 64-position block
   int64_t first, slope;
   __device__ __forceinline__ int64_t before(int64_t j) const { return first * j + slope * (j * (j + 1) / 2); }
 };
@@ -147,13 +155,15 @@ __device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
   constexpr bool kMany = SHAPE::rows > Few::rows;
   SeqWork w{};
   if (s >= p.batch.S) return w;
+  const int starts = p.batch.q_starts[s], ends = p.batch.q_starts[s + 1], keys = p.batch.kv_lens[s];
   const int a = start_at(p.batch, s), e = start_at(p.batch, s + 1);
   w.n = e > a ? e - a : 0;
   // Positions go by the lengths as given; only what they address is bounded.
-  const int starts = p.batch.q_starts[s], ends = p.batch.q_starts[s + 1], keys = p.batch.kv_lens[s];
   w.pos0 = (int64_t)keys - ((int64_t)ends - starts) + ((int64_t)a - starts);
-  if (w.n == 0 || ((int64_t)w.n * p.G > p.few_limit) != kMany) return w;
+  const int64_t packed = (int64_t)w.n * p.G;
+  if (w.n == 0 || (packed > p.few_limit) != kMany) return w;
   int64_t base = w.pos0 < 0 ? 0 : (w.pos0 < p.batch.cap ? w.pos0 : p.batch.cap);
+  w.rows = SHAPE::rows;
   if (p.idx != nullptr) {
     const int64_t b0 = w.pos0 >> 6, b1 = (w.pos0 + w.n - 1) >> 6;
     const int rows = (w.n < kBlock ? w.n : kBlock) * p.G;
@@ -161,19 +171,12 @@ __device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
     w.rows = ((rows + 31) / 32 + w.sub - 1) / w.sub * 32;  // shared out evenly
     w.tiles = (int)(b1 - b0 + 1) * w.sub;
     base = (int64_t)p.K * kBlock;
-  } else if (p.G <= SHAPE::rows) {
-    // Whole tokens to a tile: what the tiles see then grows evenly.
-    w.per = SHAPE::rows / p.G;
-    w.rows = w.per * p.G;
-    w.tiles = (w.n + w.per - 1) / w.per;
-    w.slope = w.per;
   } else {
-    w.sub = (p.G + SHAPE::rows - 1) / SHAPE::rows;
-    w.rows = SHAPE::rows;
-    w.tiles = w.n * w.sub;
-    base += w.n;
+    w.tiles = (int)((packed + SHAPE::rows - 1) / SHAPE::rows);
+    w.slope = SHAPE::rows;  // the last row of tile j is of token rows (j + 1) / G at most
+    base += 1;
   }
-  w.first = base + kRowCost;
+  w.first = (base + SHAPE::cost) * p.G;
   if (p.whole[kMany]) {
     w.first = 1;
     w.slope = 0;
@@ -182,27 +185,30 @@ __device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
 }
 
 // What a workgroup works on: all tiles of all sequences of one kind stand in
-// one line, each as long as it weighs, sequence by sequence, head by head,
-// tile by tile, and the workgroups share the line out evenly, whatever the
-// lengths are.  A stretch may end within a tile; the sums of such parts go to
-// the workgroup's two slots and are joined afterwards.  (Whole tiles: each
-// weighs one, and each is a workgroup's stretch.)
+// one line per head, each as long as it weighs, and a head's workgroups share
+// its line out evenly, whatever the lengths are.  A stretch may end within a
+// tile; the sums of such parts go to the workgroup's two slots and are joined
+// afterwards.  (Whole tiles: each is a workgroup's stretch, the line is not
+// measured.)  The heads' workgroups alternate: those of all heads are at the
+// same keys at a time, which lie together in memory, and as workgroups go to
+// the eight XCDs in turn, each L2 serves one head where their number divides 8.
 struct Line {
   int64_t total, share;
 };
 
+// `w0`: the work of sequence `lane`, which most batches need no more than.
 template <typename SHAPE>
-__device__ __forceinline__ Line line_of(const PagedAttn& p, int lane) {
+__device__ __forceinline__ Line line_of(const PagedAttn& p, const SeqWork& w0, int lane) {
+  if (p.whole[SHAPE::rows > Few::rows]) return Line{(int64_t)1 << 62, 1};
   Line line{0, 1};
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
-    const SeqWork w = sequence_work<SHAPE>(p, s0 + lane);
-    line.total += lane_of(wave_prefix(w.before(w.tiles) * p.Hkv), 63);
+    const SeqWork w = s0 == 0 ? w0 : sequence_work<SHAPE>(p, s0 + lane);
+    line.total += lane_of(wave_prefix(w.before(w.tiles)), 63);
   }
-  if (!p.whole[SHAPE::rows > Few::rows]) {
-    // Parts below kRowCost + 256 keys cost more than they save.
-    line.share = (line.total + kGroups - 1) / kGroups;
-    if (line.share < kRowCost + 256) line.share = kRowCost + 256;
-  }
+  // Parts of fewer than 256 keys cost more than they save.
+  line.share = divided(line.total + p.groups - 1, p.groups);
+  const int64_t least = (int64_t)(SHAPE::cost + 256) * p.G;
+  if (line.share < least) line.share = least;
   return line;
 }
 
@@ -212,71 +218,54 @@ struct Unit {
   SeqWork w;
 };
 
-// The tile at place `at` of the line, or the at-th tile (BY_TILE, `at` a count).  False
-// behind the last, with `at` less by how many there are.
+// The tile of head g at place `at` of the line, or the at-th tile (BY_TILE).  False
+// behind the last.
 template <typename SHAPE, bool BY_TILE>
-__device__ __forceinline__ bool find_unit(const PagedAttn& p, int64_t& at, int lane, Unit& u) {
+__device__ __forceinline__ bool find_unit(const PagedAttn& p, const SeqWork& w0, int64_t at, int g, int lane, Unit& u) {
+  const bool whole = p.whole[SHAPE::rows > Few::rows];
   int64_t places = 0, count = 0;
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
-    const SeqWork w = sequence_work<SHAPE>(p, s0 + lane);
-    const int64_t head = w.before(w.tiles);  // one head's length
-    const int64_t pp = wave_prefix(head * p.Hkv), pc = BY_TILE ? wave_prefix((int64_t)w.tiles * p.Hkv) : 0;
+    const SeqWork w = s0 == 0 ? w0 : sequence_work<SHAPE>(p, s0 + lane);
+    const int64_t pp = wave_prefix(w.before(w.tiles)), pc = BY_TILE ? wave_prefix((int64_t)w.tiles) : 0;
     const uint64_t past = __ballot((BY_TILE ? count + pc : places + pp) > at);
     if (past) {
       const int l = __builtin_ctzll(past);
       u.s = s0 + l;
+      u.g = g;
       u.w.n = __builtin_amdgcn_readlane(w.n, l);
       u.w.pos0 = lane_of(w.pos0, l);
       u.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
-      u.w.per = __builtin_amdgcn_readlane(w.per, l);
       u.w.sub = __builtin_amdgcn_readlane(w.sub, l);
       u.w.rows = __builtin_amdgcn_readlane(w.rows, l);
       u.w.first = lane_of(w.first, l);
       u.w.slope = lane_of(w.slope, l);
-      const int64_t one = lane_of(head, l);
-      const int64_t origin = places + lane_of(pp, l) - one * p.Hkv;
       if (u.w.tiles <= 0) return false;
+      const int64_t origin = places + lane_of(pp, l) - u.w.before(u.w.tiles);
+      int64_t j;
       if constexpr (BY_TILE) {
-        const int64_t in = at - (count + lane_of(pc, l) - (int64_t)u.w.tiles * p.Hkv);
-        u.g = uniform((int)(in / u.w.tiles));
-        u.tile = uniform((int)(in - (int64_t)u.g * u.w.tiles));
+        j = at - (count + lane_of(pc, l) - u.w.tiles);
+      } else if (whole) {
+        j = u.w.tiles - 1 - (at - origin);  // the last tiles see the most keys and come first
+      } else if (u.w.slope == 0) {
+        j = divided(at - origin, u.w.first);
       } else {
-        const int64_t in = at - origin;
-        if (p.whole[SHAPE::rows > Few::rows]) {
-          // The last tiles see the most keys and come first; heads in turn, so
-          // that each XCD's L2 serves one head where their number divides 8.
-          const int tile = (int)(in / p.Hkv);
-          u.g = uniform((int)(in - (int64_t)tile * p.Hkv));
-          u.tile = uniform(u.w.tiles - 1 - tile);
-          if (u.tile < 0) return false;  // starts that overlap
-          u.start = at;
-          u.end = at + 1;
-          return true;
-        }
-        u.g = uniform((int)(in / one));
-        const int64_t y = in - u.g * one;
         // The tile j with before(j) <= y < before(j + 1).
-        int j;
-        if (u.w.slope == 0) {
-          j = (int)(y / u.w.first);
-        } else {
-          const double b = (double)u.w.first + 0.5 * (double)u.w.slope;
-          j = (int)((sqrt(b * b + 2.0 * (double)u.w.slope * (double)y) - b) / (double)u.w.slope);
-          j = j < 0 ? 0 : (j < u.w.tiles ? j : u.w.tiles - 1);
-          while (j > 0 && u.w.before(j) > y) --j;
-          while (j + 1 < u.w.tiles && u.w.before(j + 1) <= y) ++j;
-        }
-        u.tile = uniform(j);
+        const int64_t y = at - origin;
+        const double b = (double)u.w.first + 0.5 * (double)u.w.slope;
+        j = (int64_t)((sqrt(b * b + 2.0 * (double)u.w.slope * (double)y) - b) / (double)u.w.slope);
+        j = j < 0 ? 0 : (j < u.w.tiles ? j : u.w.tiles - 1);
+        while (j > 0 && u.w.before(j) > y) --j;
+        while (j + 1 < u.w.tiles && u.w.before(j + 1) <= y) ++j;
       }
-      if (u.g < 0 || u.g >= p.Hkv || u.tile < 0 || u.tile >= u.w.tiles) return false;  // starts that overlap
-      u.start = origin + u.g * one + u.w.before(u.tile);
-      u.end = origin + u.g * one + u.w.before(u.tile + 1);
+      if (j < 0 || j >= u.w.tiles) return false;  // starts that overlap
+      u.tile = uniform((int)j);
+      u.start = whole ? at : origin + u.w.before(u.tile);
+      u.end = whole ? at + 1 : origin + u.w.before(u.tile + 1);
       return true;
     }
     places += lane_of(pp, 63);
     if (BY_TILE) count += lane_of(pc, 63);
   }
-  at -= BY_TILE ? count : places;
   return false;
 }
 
@@ -286,18 +275,18 @@ struct Part {
   int lo, hi, slot;
 };
 
-template <int KEYS>
-__device__ __forceinline__ Part part_of(const Line& line, const Unit& u, int64_t from, int64_t to, int64_t group) {
+template <typename SHAPE, int KEYS>
+__device__ __forceinline__ Part part_of(const Line& line, const Unit& u, int G, int64_t from, int64_t to, int64_t turn) {
   Part part{0, 0x7fffffff, -1};
   if (from > u.start || to < u.end) {
     // Neighbours round the border between them alike.
     auto border = [&](int64_t at) {
-      const int64_t key = at - u.start - kRowCost;
-      return key <= 0 ? 0 : (int)((key + KEYS - 1) / KEYS);
+      const int64_t key = at - u.start - (int64_t)SHAPE::cost * G;
+      return key <= 0 ? 0 : (int)divided(key + KEYS * G - 1, KEYS * G);
     };
     part.lo = uniform(border(from));
     if (to < u.end) part.hi = uniform(border(to));
-    part.slot = uniform((int)(2 * group + (from > group * line.share ? 1 : 0)));
+    part.slot = uniform((int)(2 * blockIdx.x + (from > turn * line.share ? 1 : 0)));
   }
   return part;
 }
@@ -320,13 +309,9 @@ __device__ __forceinline__ TileRows tile_rows(const PagedAttn& p, const Unit& u)
     t.row0 = t0 * p.G + sub * u.w.rows;
     left = t1 * p.G - t.row0;
     t.list = bi < p.Qc ? p.idx + (int64_t)u.s * p.is[0] + (int64_t)u.g * p.is[1] + (int64_t)bi * p.is[2] : nullptr;
-  } else if (u.w.per > 0) {
+  } else {
     t.row0 = u.tile * u.w.rows;
     left = u.w.n * p.G - t.row0;
-  } else {
-    const int token = u.tile / u.w.sub;
-    t.row0 = token * p.G + (u.tile - token * u.w.sub) * u.w.rows;
-    left = (token + 1) * p.G - t.row0;
   }
   t.rows = uniform(left < 0 ? 0 : (left < u.w.rows ? left : u.w.rows));
   t.row0 = uniform(t.row0);
@@ -410,9 +395,13 @@ __device__ __forceinline__ int opaque_zero() {
 }
 
 template <int D>
+constexpr int few_keys() {
+  return 32;  // keys of a wave's tile
+}
+template <int D>
 constexpr int few_lds_bytes() {
   // The waves' V rows, or their O rows, 16 at a time; then maxima and sums.
-  constexpr int v = kWaves * 32 * (D + 8) * 2, o = kWaves * 16 * (D + 4) * 4;
+  constexpr int v = kWaves * few_keys<D>() * (D + 8) * 2, o = kWaves * 16 * (D + 4) * 4;
   return (v > o ? v : o) + kWaves * 2 * 32 * 4;
 }
 template <int D>
@@ -435,6 +424,7 @@ constexpr int many_lds_bytes() {
 template <int D, bool F16, bool CAREFUL>
 __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Part& part, char* smem) {
   const PagedAttn p = arguments(args);
+  constexpr int KEYS = few_keys<D>(), KT = KEYS / 16, KH = KEYS / 32;  // 16- and 32-key pieces of a tile
   constexpr int KK = D / 32;   // steps of S^T over d
   constexpr int DT = D / 16;   // 16-row tiles of O^T
   constexpr int VSTR = D + 8;  // V rows in LDS, 16-bit elements
@@ -465,21 +455,21 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
       qf[c][kk] = load16(src + 32 * kk);
   }
   const int first_pos = uniform(clip(u.w.pos0 + tr.row0 / p.G));
-  const int items = p.idx ? 2 * p.K : (tr.end + 31) / 32;
+  const int items = p.idx ? kBlock / KEYS * p.K : (tr.end + KEYS - 1) / KEYS;
   const int hi = part.hi < items ? part.hi : items;
 
   const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)u.g * p.ks[1] + 8 * g4;
   const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1] + 8 * g4;
-  uint16_t* vl = reinterpret_cast<uint16_t*>(smem) + wave * 32 * VSTR;
+  uint16_t* vl = reinterpret_cast<uint16_t*>(smem) + wave * KEYS * VSTR;
 
-  // Table entries of the keys key0 + l16 and key0 + 16 + l16.
-  auto pages_of = [&](int key0, int (&pg)[2]) {
+  // Table entries of the keys key0 + 16 c + l16.
+  auto pages_of = [&](int key0, int (&pg)[KT]) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) pg[c] = page_entry(p.batch, u.s, nearest(key0 + 16 * c + l16, tr.end));
+    for (int c = 0; c < KT; ++c) pg[c] = page_entry(p.batch, u.s, nearest(key0 + 16 * c + l16, tr.end));
   };
-  auto load = [&](const uint16_t* base, const int64_t* st, int key0, const int (&pg)[2], u32x4 (&x)[2][KK]) {
+  auto load = [&](const uint16_t* base, const int64_t* st, int key0, const int (&pg)[KT], u32x4 (&x)[KT][KK]) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < KT; ++c) {
       const int key = nearest(key0 + 16 * c + l16, tr.end);
       const int slot = key - page_of(p.batch, key) * p.batch.page;
       const uint16_t* src = base + (int64_t)(is_page(p.batch, pg[c]) ? pg[c] : 0) * st[0] + (int64_t)slot * st[2];
@@ -490,58 +480,73 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   f32x4v acc[2][DT];
+  // Zeros that are no constant: constant ones are kept in registers, or worse,
+  // for every later use of a zero.
+  const float zero = __builtin_bit_cast(float, opaque_zero());
   {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       m[c] = -INFINITY;
       l[c] = 0.f;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[c][dt] = f32x4v{};
+      for (int dt = 0; dt < DT; ++dt) acc[c][dt] = f32x4v{zero, zero, zero, zero};
     }
-    KeyWalk<32> walk;
+    KeyWalk<KEYS> walk;
     walk.init(p, tr, part.lo + wave, kWaves, hi, lane);
-    int pg[2], pn[2];
-    u32x4 kx[2][KK], vx[2][KK];
-    int key0 = walk.next();
+    // Keys and table entries of this tile, the next and the one after: entries
+    // are looked up a tile before the loads that they address are issued.
+    int pg[KT], pn[KT], pa[KT];
+    u32x4 kx[KT][KK], vx[KT][KK];
+    int key0 = walk.next(), nkey = -1;
     if (key0 >= 0) {
       pages_of(key0, pg);
+      nkey = walk.next();
+      if (nkey >= 0) pages_of(nkey, pn);
       load(kbase, p.ks, key0, pg, kx);
       load(vbase, p.vs, key0, pg, vx);
     }
     while (key0 >= 0) {
-      const int nkey = walk.next();
-      if (nkey >= 0) pages_of(nkey, pn);
+      const int akey = nkey >= 0 ? walk.next() : -1;
+      if (akey >= 0) pages_of(akey, pa);
       // Bits of the keys with a page and a position below the end.
-      uint32_t have = (uint32_t)(__ballot(is_page(p.batch, pg[0])) & 0xffffu) |
-                      (uint32_t)(__ballot(is_page(p.batch, pg[1])) << 16);
-      if (tr.end - key0 < 32) have &= (1u << (tr.end - key0)) - 1;
-      f32x4v s[2][2];
+      uint32_t have[KH];
+      bool masked = key0 + KEYS - 1 > first_pos;
+#pragma unroll
+      for (int i = 0; i < KH; ++i) {
+        have[i] = (uint32_t)(__ballot(is_page(p.batch, pg[2 * i])) & 0xffffu) |
+                  (uint32_t)(__ballot(is_page(p.batch, pg[2 * i + 1])) << 16);
+        const int left = tr.end - key0 - 32 * i;
+        if (left < 32) have[i] &= left <= 0 ? 0u : (1u << left) - 1;
+        masked |= have[i] != 0xffffffffu;
+      }
+      f32x4v s[2][KT];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < KT; ++kt) {
           s[c][kt] = f32x4v{};
           if (c == 0 || two)
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) s[c][kt] = mfma16x16x32<F16>(kx[kt][kk], qf[c][kk], s[c][kt]);
         }
       if (nkey >= 0) load(kbase, p.ks, nkey, pn, kx);
-      const bool masked = have != 0xffffffffu || key0 + 31 > first_pos;
-      u32x4 pk[2];
+      u32x4 pk[2][KH];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (c == 1 && !two) break;
         if (masked) {
-          const uint32_t mine = have >> (4 * g4);
           const int rel = qpos[c] - key0 - 4 * g4;
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
+          for (int kt = 0; kt < KT; ++kt) {
+            const uint32_t mine = have[kt >> 1] >> (4 * g4);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (!(mine & (1u << (16 * kt + r))) || 16 * kt + r > rel) s[c][kt][r] = -INFINITY;
+              if (!(mine & (1u << (16 * (kt & 1) + r))) || 16 * kt + r > rel) s[c][kt][r] = -INFINITY;
+          }
         }
-        float mx = fmaxf(fmaxf(fmaxf(s[c][0][0], s[c][0][1]), fmaxf(s[c][0][2], s[c][0][3])),
-                         fmaxf(fmaxf(s[c][1][0], s[c][1][1]), fmaxf(s[c][1][2], s[c][1][3])));
+        float mx = s[c][0][0];
+#pragma unroll
+        for (int i = 1; i < 4 * KT; ++i) mx = fmaxf(mx, s[c][i >> 2][i & 3]);
         mx = quad_max(mx) * p.cs;
         if (__ballot(mx > m[c] + kRescaleThreshold)) {
           const float mn = fmaxf(m[c], mx);
@@ -552,18 +557,22 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
           for (int dt = 0; dt < DT; ++dt) acc[c][dt] *= alpha;
         }
         const float nm = m[c] == -INFINITY ? 0.f : -m[c];
-        float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = fast_exp2(fmaf(s[c][i >> 2][i & 3], p.cs, nm));
-          l[c] += x[i];
+        for (int h2 = 0; h2 < KH; ++h2) {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] = fast_exp2(fmaf(s[c][2 * h2 + (i >> 2)][i & 3], p.cs, nm));
+            l[c] += x[i];
+          }
+          pk[c][h2] =
+              u32x4{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]), pack2<F16>(x[6], x[7])};
         }
-        pk[c] = u32x4{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]), pack2<F16>(x[6], x[7])};
       }
       // V through the wave's LDS rows; the previous tile's reads of them
       // come before these writes in the wave's own order.
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
           *reinterpret_cast<u32x4*>(vl + (16 * kt + l16) * VSTR + 32 * kk + 8 * g4) = vx[kt][kk];
@@ -580,41 +589,57 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
             // Column q alone, with the value rows that it does not see as zeros.
             const int seen = __builtin_amdgcn_readlane(rel, q);
             const uint16_t* vq = vt + opaque_zero();  // reads it again for every column, not 64 registers ahead
-            const uint32_t mine = (seen < 31 ? have & ((2u << seen) - 1) : have) >> (4 * g4);
-            uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int b = 16 * (i >> 1) + 2 * (i & 1);
-              w[i] = (mine & (1u << b) ? 0xffffu : 0u) | (mine & (2u << b) ? 0xffff0000u : 0u);
-            }
+            for (int h2 = 0; h2 < KH; ++h2) {
+              const int s2 = seen - 32 * h2;
+              const uint32_t mine = (s2 < 0 ? 0u : (s2 < 31 ? have[h2] & ((2u << s2) - 1) : have[h2])) >> (4 * g4);
+              uint32_t w[4];
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-              const uint2 a = lds_read_tr16(vq + 16 * dt), b = lds_read_tr16(vq + 16 * VSTR + 16 * dt);
-              const f32x4v one =
-                  mfma16x16x32<F16>(u32x4{a.x & w[0], a.y & w[1], b.x & w[2], b.y & w[3]}, pk[c], f32x4v{});
-              if (l16 == q) acc[c][dt] += one;
+              for (int i = 0; i < 4; ++i) {
+                const int b = 16 * (i >> 1) + 2 * (i & 1);
+                w[i] = (mine & (1u << b) ? 0xffffu : 0u) | (mine & (2u << b) ? 0xffff0000u : 0u);
+              }
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt) {
+                const uint2 a = lds_read_tr16(vq + 32 * h2 * VSTR + 16 * dt),
+                            b = lds_read_tr16(vq + (32 * h2 + 16) * VSTR + 16 * dt);
+                const f32x4v one =
+                    mfma16x16x32<F16>(u32x4{a.x & w[0], a.y & w[1], b.x & w[2], b.y & w[3]}, pk[c][h2], f32x4v{});
+                if (l16 == q) acc[c][dt] += one;
+              }
             }
           }
         }
-      } else if (two) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const uint2 a = lds_read_tr16(vt + 16 * dt), b = lds_read_tr16(vt + 16 * VSTR + 16 * dt);
-          const u32x4 va = {a.x, a.y, b.x, b.y};
-          acc[0][dt] = mfma16x16x32<F16>(va, pk[0], acc[0][dt]);
-          acc[1][dt] = mfma16x16x32<F16>(va, pk[1], acc[1][dt]);
-        }
       } else {
+        auto values = [&](int h2, int dt) {
+          const uint2 a = lds_read_tr16(vt + 32 * h2 * VSTR + 16 * dt),
+                      b = lds_read_tr16(vt + (32 * h2 + 16) * VSTR + 16 * dt);
+          return u32x4{a.x, a.y, b.x, b.y};
+        };
+        if (two) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const uint2 a = lds_read_tr16(vt + 16 * dt), b = lds_read_tr16(vt + 16 * VSTR + 16 * dt);
-          acc[0][dt] = mfma16x16x32<F16>(u32x4{a.x, a.y, b.x, b.y}, pk[0], acc[0][dt]);
+          for (int h2 = 0; h2 < KH; ++h2)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              const u32x4 va = values(h2, dt);
+              acc[0][dt] = mfma16x16x32<F16>(va, pk[0][h2], acc[0][dt]);
+              acc[1][dt] = mfma16x16x32<F16>(va, pk[1][h2], acc[1][dt]);
+            }
+        } else {
+#pragma unroll
+          for (int h2 = 0; h2 < KH; ++h2)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[0][dt] = mfma16x16x32<F16>(values(h2, dt), pk[0][h2], acc[0][dt]);
         }
       }
       wave_lds_fence();
       key0 = nkey;
-      pg[0] = pn[0];
-      pg[1] = pn[1];
+      nkey = akey;
+#pragma unroll
+      for (int c = 0; c < KT; ++c) {
+        pg[c] = pn[c];
+        pn[c] = pa[c];
+      }
     }
   }
   if constexpr (!CAREFUL) {
@@ -914,8 +939,11 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
   {
     m = -INFINITY;
     l = 0.f;
+    const float zero = __builtin_bit_cast(float, opaque_zero());
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16_t{};
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[dt][r] = zero;
     KeyWalk<kBlock> walk;
     walk.init(p, tr, part.lo, 1, hi, lane);
     auto take = [&](int& key0, int& pg) {
@@ -1022,7 +1050,7 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
 template <int D, bool F16>
 struct FewBody {
   typedef Few Shape;
-  static constexpr int keys = 32, lds = few_lds_bytes<D>();
+  static constexpr int keys = few_keys<D>(), lds = few_lds_bytes<D>();
   template <bool CAREFUL>
   static __device__ __forceinline__ bool run(uintptr_t args, const Unit& u, const Part& part, char* smem) {
     return few_rows<D, F16, CAREFUL>(args, u, part, smem);
@@ -1038,36 +1066,41 @@ struct ManyBody {
   }
 };
 
-// The stretch [at, end) of workgroup `group`, as far as its first unit.
+// The stretch [at, end) of head g's line, the turn-th, as far as its first unit.
 struct Stretch {
-  int64_t at, end, group;
+  int64_t at, end, turn;
+  int g;
 };
 
 template <typename BODY, bool CAREFUL>
 __device__ __forceinline__ bool run_unit(uintptr_t args, const Line& line, const Stretch& st, char* smem, int64_t& to) {
   Unit u;
-  int64_t place = st.at;
-  if (!find_unit<typename BODY::Shape, false>(arguments(args), place, threadIdx.x & 63, u)) return false;
+  int G;
+  {
+    const PagedAttn p = arguments(args);
+    const SeqWork w0 = sequence_work<typename BODY::Shape>(p, threadIdx.x & 63);
+    if (!find_unit<typename BODY::Shape, false>(p, w0, st.at, st.g, threadIdx.x & 63, u)) return false;
+    G = p.G;
+  }
   to = u.end < st.end ? u.end : st.end;
-  return BODY::template run<CAREFUL>(args, u, part_of<BODY::keys>(line, u, st.at, to, st.group), smem);
+  const Part part = part_of<typename BODY::Shape, BODY::keys>(line, u, G, st.at, to, st.turn);
+  return BODY::template run<CAREFUL>(args, u, part, smem);
 }
 
 // The careful way, looking its unit up again, is a function of its own: what
 // it would keep in registers pushed the usual way's out of them.
 template <typename BODY>
-__device__ __attribute__((noinline)) void run_again(uint64_t args, int64_t share, int64_t at, int64_t end, int64_t group,
-                                                    __attribute__((address_space(3))) char* smem) {
+__device__ __attribute__((noinline)) void run_again(uint64_t args, int64_t share, int64_t at, int64_t end, int64_t turn,
+                                                    int g, __attribute__((address_space(3))) char* smem) {
   auto same = [](int64_t x) { return lane_of(x, 0); };
   int64_t to;
-  run_unit<BODY, true>((uintptr_t)same((int64_t)args), Line{0, same(share)}, Stretch{same(at), same(end), same(group)},
-                       (char*)smem, to);
+  run_unit<BODY, true>((uintptr_t)same((int64_t)args), Line{0, same(share)},
+                       Stretch{same(at), same(end), same(turn), uniform(g)}, (char*)smem, to);
 }
 
 // A launch for either kind: the lengths that tell them apart are on the
 // device, so the workgroups of a kind that the batch does not hold find no
 // tile and end.  (Both in one kernel needed more registers than there are.)
-// Workgroups go to the eight XCDs in turn; the line is dealt so that each XCD
-// has one stretch of it, and mostly one head's keys, in its L2.
 template <typename BODY>
 __global__ __launch_bounds__(kWaves * 64, 2) void paged_attention_kernel(const PagedAttn) {
   typedef typename BODY::Shape SHAPE;
@@ -1077,16 +1110,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attention_kernel(const P
   Stretch st;
   {
     const PagedAttn p = arguments(args);
-    line = line_of<SHAPE>(p, threadIdx.x & 63);
-    st.group = blockIdx.x;
-    if (!p.whole[SHAPE::rows > Few::rows]) st.group = (st.group & 7) * (kGroups / 8) + (st.group >> 3);
+    line = line_of<SHAPE>(p, sequence_work<SHAPE>(p, threadIdx.x & 63), threadIdx.x & 63);
+    const int turn = uniform((int)blockIdx.x / p.Hkv);
+    st.turn = turn;
+    st.g = (int)blockIdx.x - turn * p.Hkv;
   }
-  st.at = st.group * line.share;
+  st.at = st.turn * line.share;
   st.end = st.at + line.share < line.total ? st.at + line.share : line.total;
   while (st.at < st.end) {
     int64_t to = st.end;
     if (run_unit<BODY, false>(args, line, st, smem, to))
-      run_again<BODY>(args, line.share, st.at, st.end, st.group, (__attribute__((address_space(3))) char*)smem);
+      run_again<BODY>(args, line.share, st.at, st.end, st.turn, st.g, (__attribute__((address_space(3))) char*)smem);
     st.at = to;
     if (st.at < st.end) __syncthreads();  // the unit's LDS is free
   }
@@ -1098,32 +1132,52 @@ template <typename SHAPE, int D, bool F16>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn p) {
   constexpr int kTileGroups = SHAPE::rows / 32;
   const int lane = threadIdx.x & 63;
-  const Line line = line_of<SHAPE>(p, lane);
-  int64_t tile = blockIdx.x / kTileGroups;
-  const int sub = blockIdx.x % kTileGroups;
+  const SeqWork w0 = sequence_work<SHAPE>(p, lane);
+  const Line line = line_of<SHAPE>(p, w0, lane);
+  const int sub = blockIdx.x % kTileGroups, index = blockIdx.x / kTileGroups;
   Unit u;
-  if (!find_unit<SHAPE, true>(p, tile, lane, u)) return;
-  const int64_t g0 = u.start / line.share, g1 = (u.end - 1) / line.share;
-  if (g0 == g1 || g1 >= kGroups) return;  // held whole (or starts that overlap)
+  if (!find_unit<SHAPE, true>(p, w0, index / p.Hkv, index % p.Hkv, lane, u)) return;
+  const int64_t t0 = divided(u.start, line.share), t1 = divided(u.end - 1, line.share);
+  if (t0 == t1 || t1 >= p.groups) return;  // held whole (or starts that overlap)
   const TileRows tr = tile_rows(p, u);
   const int row = lane & 31, hl = lane >> 5, wave = threadIdx.x >> 6;
   const int r = sub * 32 + row;
   if (r >= tr.rows) return;
-  // The part of group g: the one that starts its stretch, or the one behind.
-  auto part = [&](int64_t g) { return (2 * g + (g == g0 && u.start > g0 * line.share ? 1 : 0)) * kTileGroups + sub; };
-  float top = -INFINITY;
-  for (int64_t g = g0; g <= g1; ++g) top = fmaxf(top, p.part_ml[part(g) * 64 + row]);
-  const float nm = top == -INFINITY ? 0.f : -top;
+  // The part of a turn: the one that starts its stretch, or the one behind.
+  auto part = [&](int64_t t) {
+    return (2 * (t * p.Hkv + u.g) + (t == t0 && u.start > t0 * line.share ? 1 : 0)) * kTileGroups + sub;
+  };
   constexpr int PIECES = D / 32;  // of 4 values: pieces wave, wave + 4 ..
-  float sum = 0.f;
+  float top = -INFINITY, sum = 0.f;
   f32x4v o[PIECES] = {};
-  for (int64_t g = g0; g <= g1; ++g) {
-    const int64_t at = part(g);
-    const float f = fast_exp2(p.part_ml[at * 64 + row] + nm);
-    sum += f * p.part_ml[at * 64 + 32 + row];
+  // Two parts at a time, all their loads in flight (a second one behind the
+  // last is the last again and weighs nothing).
+  for (int64_t t = t0; t <= t1; t += 2) {
+    float m[2], l[2];
+    f32x4v x[2][PIECES];
 #pragma unroll
-    for (int j = 0; j < PIECES; ++j)
-      o[j] += f * *reinterpret_cast<const f32x4v*>(p.part_o + at * 32 * D + (wave + 4 * j) * 256 + lane * 4);
+    for (int i = 0; i < 2; ++i) {
+      const int64_t at = part(t + i < t1 ? t + i : t1);
+      m[i] = p.part_ml[at * 64 + row];
+      l[i] = p.part_ml[at * 64 + 32 + row];
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j)
+        x[i][j] = *reinterpret_cast<const f32x4v*>(p.part_o + at * 32 * D + (wave + 4 * j) * 256 + lane * 4);
+    }
+    if (t + 1 > t1) {
+      m[1] = -INFINITY;
+      l[1] = 0.f;
+    }
+    const float now = fmaxf(top, fmaxf(m[0], m[1]));
+    const float nm = now == -INFINITY ? 0.f : -now;
+    const float f = fast_exp2(top + nm), f0 = fast_exp2(m[0] + nm), f1 = fast_exp2(m[1] + nm);
+    sum = f * sum + f0 * l[0] + f1 * l[1];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      o[j] = f * o[j] + f0 * x[0][j];
+      if (t + 1 <= t1) o[j] += f1 * x[1][j];
+    }
+    top = now;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int at = tr.row0 + r, t = at / p.G, h = at - t * p.G;
@@ -1140,20 +1194,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn p) {
 struct Plan {
   bool few, many, few_whole, many_whole;
   int few_limit;
-  int64_t few_tiles, many_tiles;
+  int64_t few_tiles, many_tiles, groups;
 };
 
 template <typename SHAPE>
 int64_t tiles_bound(int64_t N, int64_t S, int64_t G, int64_t most, bool lists) {
   // `most`: packed rows of one sequence at most; a sequence rounds up by one tile.
   const int64_t seqs = S < N ? S : N;
-  if (lists) {
-    // Rows break at every 64 positions too.
-    const int64_t rows = most < kBlock * G ? most : kBlock * G;
-    return (N / kBlock + 2 * seqs) * ((rows + SHAPE::rows - 1) / SHAPE::rows);
-  }
-  if (G > SHAPE::rows) return N * ((G + SHAPE::rows - 1) / SHAPE::rows);
-  return N / (SHAPE::rows / G) + seqs;
+  if (!lists) return N * G / SHAPE::rows + seqs;
+  // Rows break at every 64 positions too.
+  const int64_t rows = most < kBlock * G ? most : kBlock * G;
+  return (N / kBlock + 2 * seqs) * ((rows + SHAPE::rows - 1) / SHAPE::rows);
 }
 
 Plan plan_of(int64_t N, int64_t S, int64_t G, int64_t Hkv, int64_t keys, bool lists) {
@@ -1170,15 +1221,18 @@ Plan plan_of(int64_t N, int64_t S, int64_t G, int64_t Hkv, int64_t keys, bool li
   if (plan.few) plan.few_tiles = tiles_bound<Few>(N, S, G, plan.many ? kFewRows : N * G, lists) * Hkv;
   if (plan.many) plan.many_tiles = tiles_bound<Many>(N, S, G, N * G, lists) * Hkv;
   // Rows of few keys are not worth a join, many tiles not a split.
-  plan.few_whole = keys <= 1024 || plan.few_tiles > 64 * kGroups;
-  plan.many_whole = keys <= 1024 || plan.many_tiles >= 2 * kGroups;
+  plan.few_whole = keys <= 1024 || plan.few_tiles > 64 * kCus;
+  plan.many_whole = keys <= 1024 || plan.many_tiles >= 2 * kCus;
+  // A CU each; with many heads, whose number may not divide the CUs', in rounds.
+  plan.groups = (Hkv <= 32 ? kCus : 4 * kCus) / Hkv;
+  if (plan.groups < 1) plan.groups = 1;
   return plan;
 }
 
-int64_t workspace_of(const Plan& plan, int64_t D) {
+int64_t workspace_of(const Plan& plan, int64_t Hkv, int64_t D) {
   int64_t groups = 0;
-  if (plan.few && !plan.few_whole) groups = 2 * kGroups;
-  if (plan.many && !plan.many_whole) groups = 2 * kGroups * kWaves;
+  if (plan.few && !plan.few_whole) groups = 2 * plan.groups * Hkv;
+  if (plan.many && !plan.many_whole) groups = 2 * plan.groups * Hkv * kWaves;
   return (groups > 0 ? groups : 1) * 32 * (D + 2) * 4;
 }
 
@@ -1189,7 +1243,7 @@ extern "C" int64_t spruce_paged_attention_workspace_bytes(int64_t N, int64_t S, 
   if (N < 1 || S < 1 || Hkv < 1 || Hq < Hkv || N >= (int64_t)1 << 30 || S >= (int64_t)1 << 20 || Hq >= 1 << 16 ||
       D < 1 || D > 128)
     return 0;
-  return workspace_of(plan_of(N, S, Hq / Hkv, Hkv, K > 0 ? K * kBlock : keys, K > 0), D);
+  return workspace_of(plan_of(N, S, Hq / Hkv, Hkv, K > 0 ? K * kBlock : keys, K > 0), Hkv, D);
 }
 
 extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, void* stream) {
@@ -1226,7 +1280,7 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
   SPRUCE_REQUIRE(K == 0 || (a.idx && a.Qc >= 0), "indices must be a non-null device pointer");
   SPRUCE_REQUIRE(K == 0 || a.is[3] == 1, "indices must have a contiguous final dimension");
   const Plan plan = plan_of(N, S, Hq / Hkv, Hkv, K > 0 ? K * kBlock : p.batch.cap, K > 0);
-  const int64_t need = workspace_of(plan, D);
+  const int64_t need = workspace_of(plan, Hkv, D);
   SPRUCE_REQUIRE(a.workspace && a.workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
                  (long long)a.workspace_bytes, (long long)need);
   SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0, "workspace must be 16-byte aligned");
@@ -1255,6 +1309,7 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
   p.few_limit = plan.few_limit;
   p.whole[0] = plan.few_whole;
   p.whole[1] = plan.many_whole;
+  p.groups = (int)plan.groups;
   // The kinds' launches follow one another, so they share the slots.
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = p.part_o + need / (32 * (D + 2) * 4) * 32 * D;
@@ -1271,7 +1326,7 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
 #define SPRUCE_PAGED(D_, F16_)                                                                \
   do {                                                                                        \
     if (plan.many) {                                                                          \
-      const int64_t grid = plan.many_whole ? plan.many_tiles : kGroups;                       \
+      const int64_t grid = plan.many_whole ? plan.many_tiles : plan.groups * Hkv;                       \
       if (aligned)                                                                            \
         SPRUCE_LAUNCH((paged_attention_kernel<ManyBody<D_, F16_, true>>), grid, kWaves * 64);                \
       else                                                                                    \
@@ -1280,7 +1335,7 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
         SPRUCE_LAUNCH((paged_join_kernel<Many, D_, F16_>), plan.many_tiles * kWaves, 256);    \
     }                                                                                         \
     if (plan.few) {                                                                           \
-      const int64_t grid = plan.few_whole ? plan.few_tiles : kGroups;                         \
+      const int64_t grid = plan.few_whole ? plan.few_tiles : plan.groups * Hkv;                         \
       SPRUCE_LAUNCH((paged_attention_kernel<FewBody<D_, F16_>>), grid, kWaves * 64);                         \
       if (!plan.few_whole)                                                                    \
         SPRUCE_LAUNCH((paged_join_kernel<Few, D_, F16_>), plan.few_tiles, 256);               \
