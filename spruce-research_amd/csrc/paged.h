@@ -6,6 +6,21 @@
 
 namespace spruce {
 
+// x / d == (x * magic) >> shift for 0 <= x < 2^31.  With l = ceil(log2(d)),
+// magic = floor(2^(31 + l) / d) + 1 exceeds 2^(31 + l) / d by at most 1, so
+// x * magic / 2^(31 + l) exceeds x / d by less than 2^-l <= 1 / d: the floor is
+// the same.
+struct Divisor {
+  uint32_t magic;
+  int shift;
+  __device__ __forceinline__ int of(int x) const { return (int)(((uint64_t)(uint32_t)x * magic) >> shift); }
+};
+inline Divisor divisor(int64_t d) {  // 1 <= d < 2^31
+  int l = 0;
+  while (((int64_t)1 << l) < d) ++l;
+  return Divisor{(uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)d) + 1), 31 + l};
+}
+
 // Sequences s = 0..S-1 with their new tokens at rows q_starts[s] ..
 // q_starts[s + 1) of the packed tensors and kv_lens[s] cached keys, those of
 // the new tokens included: new token i stands at position kv_lens[s] - n + i
@@ -19,14 +34,10 @@ struct PagedBatch {
   const int32_t* q_starts;
   const int32_t* kv_lens;
   int S, N, page, pages;
-  int cap;         // positions the table holds: width * page
-  uint32_t magic;  // p / page == (p * magic) >> shift for p < 2^31
-  int shift;
+  int cap;  // positions the table holds: width * page
+  Divisor by_page;
 };
 
-// With l = ceil(log2(page)), magic = floor(2^(31 + l) / page) + 1 exceeds
-// 2^(31 + l) / page by at most 1, so p * magic / 2^(31 + l) exceeds p / page
-// by less than 2^-l <= 1 / page for p < 2^31: the floor is the same.
 inline int prepare_batch(PagedBatch& b, const int32_t* table, int64_t table_stride, int64_t width,
                          const int32_t* q_starts, const int32_t* kv_lens, int64_t S, int64_t N, int64_t page,
                          int64_t pages) {
@@ -48,22 +59,15 @@ inline int prepare_batch(PagedBatch& b, const int32_t* table, int64_t table_stri
   b.page = (int)page;
   b.pages = (int)pages;
   b.cap = (int)(width * page);
-  int l = 0;
-  while (((int64_t)1 << l) < page) ++l;
-  b.magic = (uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)page) + 1);
-  b.shift = 31 + l;
+  b.by_page = divisor(page);
   return SPRUCE_OK;
 }
 
-__device__ __forceinline__ int page_of(const PagedBatch& b, int pos) {
-  return (int)(((uint64_t)(uint32_t)pos * b.magic) >> b.shift);
-}
+__device__ __forceinline__ int page_of(const PagedBatch& b, int pos) { return b.by_page.of(pos); }
 
 // q_starts[s] and kv_lens[s] brought into range.
-__device__ __forceinline__ int start_at(const PagedBatch& b, int s) {
-  const int v = b.q_starts[s];
-  return v < 0 ? 0 : (v > b.N ? b.N : v);
-}
+__device__ __forceinline__ int clamp_start(const PagedBatch& b, int v) { return v < 0 ? 0 : (v > b.N ? b.N : v); }
+__device__ __forceinline__ int start_at(const PagedBatch& b, int s) { return clamp_start(b, b.q_starts[s]); }
 __device__ __forceinline__ int keys_of(const PagedBatch& b, int s) {
   const int v = b.kv_lens[s];
   return v < 0 ? 0 : (v > b.cap ? b.cap : v);

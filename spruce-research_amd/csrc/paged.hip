@@ -30,13 +30,13 @@ struct PagedAttn {
   int64_t ks[3], vs[3];  // page, head, slot strides
   PagedBatch batch;
   int Hkv, G;
+  Divisor by_heads, by_group;  // by Hkv and G
   float cs;  // scale * log2 e
   const int32_t* idx;  // block lists [S, Hkv, Qc, K], or null
   int64_t is[3];
   int Qc, K;
   int few_limit;   // packed rows of a sequence up to which it goes the few-row way
-  bool whole[2];   // few, many: a workgroup takes one row tile whole
-  int groups;      // workgroups of a head that share its keys out, where they are not
+  int groups;      // workgroups of a head that share its keys out
   float* part_o;   // [groups][32 * D], a 32 x 32 accumulator's order
   float* part_ml;  // [groups][2][32]
 };
@@ -102,13 +102,17 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // The lane below's value by `n` (row shifts within 16 lanes, then the rows'
 // last lanes onward), zero from outside: the steps of a prefix sum.
 template <int CTRL, int ROWS>
+__device__ __forceinline__ int shifted(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
 __device__ __forceinline__ int64_t shifted(int64_t v) {
-  const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
-  const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  const int lo = shifted<CTRL, ROWS>((int)v), hi = shifted<CTRL, ROWS>((int)(v >> 32));
   return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
 }
 // Sum of v over the lanes up to this one.
-__device__ __forceinline__ int64_t wave_prefix(int64_t v) {
+template <typename T>
+__device__ __forceinline__ T wave_prefix(T v) {
   v += shifted<0x111, 0xf>(v);
   v += shifted<0x112, 0xf>(v);
   v += shifted<0x114, 0xf>(v);
@@ -141,7 +145,7 @@ __device__ __forceinline__ int clip(int64_t pos) {
 // its fixed part.  (An upper bound of the keys: what a tile does not have,
 // nobody walks.)
 struct SeqWork {
-  int n;         // new tokens
+  int start, n;  // first packed row, new tokens
   int64_t pos0;  // position of the first
   int tiles;     // 0 where the sequence is of the other kind
   int rows;      // packed rows of a tile
@@ -150,16 +154,24 @@ struct SeqWork {
   __device__ __forceinline__ int64_t before(int64_t j) const { return first * j + slope * (j * (j + 1) / 2); }
 };
 
+// A sequence's lengths as the caller gives them.
+struct Lengths {
+  int starts, ends, keys;
+};
+__device__ __forceinline__ Lengths lengths_of(const PagedAttn& p, int s) {
+  if (s >= p.batch.S) return Lengths{0, 0, 0};
+  return Lengths{p.batch.q_starts[s], p.batch.q_starts[s + 1], p.batch.kv_lens[s]};
+}
+
 template <typename SHAPE>
-__device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
+__device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, const Lengths& len) {
   constexpr bool kMany = SHAPE::rows > Few::rows;
   SeqWork w{};
-  if (s >= p.batch.S) return w;
-  const int starts = p.batch.q_starts[s], ends = p.batch.q_starts[s + 1], keys = p.batch.kv_lens[s];
-  const int a = start_at(p.batch, s), e = start_at(p.batch, s + 1);
+  const int a = clamp_start(p.batch, len.starts), e = clamp_start(p.batch, len.ends);
+  w.start = a;
   w.n = e > a ? e - a : 0;
   // Positions go by the lengths as given; only what they address is bounded.
-  w.pos0 = (int64_t)keys - ((int64_t)ends - starts) + ((int64_t)a - starts);
+  w.pos0 = (int64_t)len.keys - ((int64_t)len.ends - len.starts) + ((int64_t)a - len.starts);
   const int64_t packed = (int64_t)w.n * p.G;
   if (w.n == 0 || (packed > p.few_limit) != kMany) return w;
   int64_t base = w.pos0 < 0 ? 0 : (w.pos0 < p.batch.cap ? w.pos0 : p.batch.cap);
@@ -177,10 +189,6 @@ __device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
     base += 1;
   }
   w.first = (base + SHAPE::cost) * p.G;
-  if (p.whole[kMany]) {
-    w.first = 1;
-    w.slope = 0;
-  }
   return w;
 }
 
@@ -188,8 +196,7 @@ __device__ __forceinline__ SeqWork sequence_work(const PagedAttn& p, int s) {
 // one line per head, each as long as it weighs, and a head's workgroups share
 // its line out evenly, whatever the lengths are.  A stretch may end within a
 // tile; the sums of such parts go to the workgroup's two slots and are joined
-// afterwards.  (Whole tiles: each is a workgroup's stretch, the line is not
-// measured.)  The heads' workgroups alternate: those of all heads are at the
+// afterwards.  The heads' workgroups alternate: those of all heads are at the
 // same keys at a time, which lie together in memory, and as workgroups go to
 // the eight XCDs in turn, each L2 serves one head where their number divides 8.
 struct Line {
@@ -199,10 +206,9 @@ struct Line {
 // `w0`: the work of sequence `lane`, which most batches need no more than.
 template <typename SHAPE>
 __device__ __forceinline__ Line line_of(const PagedAttn& p, const SeqWork& w0, int lane) {
-  if (p.whole[SHAPE::rows > Few::rows]) return Line{(int64_t)1 << 62, 1};
   Line line{0, 1};
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
-    const SeqWork w = s0 == 0 ? w0 : sequence_work<SHAPE>(p, s0 + lane);
+    const SeqWork w = s0 == 0 ? w0 : sequence_work<SHAPE>(p, lengths_of(p, s0 + lane));
     line.total += lane_of(wave_prefix(w.before(w.tiles)), 63);
   }
   // Parts of fewer than 256 keys cost more than they save.
@@ -218,34 +224,59 @@ struct Unit {
   SeqWork w;
 };
 
+__device__ __forceinline__ void take_sequence(Unit& u, const SeqWork& w, int s0, int l) {
+  u.s = s0 + l;
+  u.w.start = __builtin_amdgcn_readlane(w.start, l);
+  u.w.n = __builtin_amdgcn_readlane(w.n, l);
+  u.w.pos0 = lane_of(w.pos0, l);
+  u.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
+  u.w.rows = __builtin_amdgcn_readlane(w.rows, l);
+  u.w.sub = __builtin_amdgcn_readlane(w.sub, l);
+  u.w.first = lane_of(w.first, l);
+  u.w.slope = lane_of(w.slope, l);
+}
+
+// The at-th of the row tiles, of a sequence the last first: they see the most
+// keys.  False behind the last.  (The line is not measured.)
+template <typename SHAPE>
+__device__ __forceinline__ bool find_tile(const PagedAttn& p, int at, int g, int lane, Unit& u) {
+  constexpr int kMost = 1 << 24;  // a call has fewer; starts that overlap may claim any number
+  int count = 0;
+  for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
+    const SeqWork w = sequence_work<SHAPE>(p, lengths_of(p, s0 + lane));
+    const int pc = count + wave_prefix(w.tiles < kMost ? w.tiles : kMost);
+    const uint64_t past = __ballot(pc > at);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      take_sequence(u, w, s0, l);
+      u.g = g;
+      u.tile = __builtin_amdgcn_readlane(pc, l) - 1 - at;
+      u.start = u.end = 0;
+      return u.tile < u.w.tiles;
+    }
+    count = __builtin_amdgcn_readlane(pc, 63);
+  }
+  return false;
+}
+
 // The tile of head g at place `at` of the line, or the at-th tile (BY_TILE).  False
 // behind the last.
 template <typename SHAPE, bool BY_TILE>
 __device__ __forceinline__ bool find_unit(const PagedAttn& p, const SeqWork& w0, int64_t at, int g, int lane, Unit& u) {
-  const bool whole = p.whole[SHAPE::rows > Few::rows];
   int64_t places = 0, count = 0;
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
-    const SeqWork w = s0 == 0 ? w0 : sequence_work<SHAPE>(p, s0 + lane);
+    const SeqWork w = s0 == 0 ? w0 : sequence_work<SHAPE>(p, lengths_of(p, s0 + lane));
     const int64_t pp = wave_prefix(w.before(w.tiles)), pc = BY_TILE ? wave_prefix((int64_t)w.tiles) : 0;
     const uint64_t past = __ballot((BY_TILE ? count + pc : places + pp) > at);
     if (past) {
       const int l = __builtin_ctzll(past);
-      u.s = s0 + l;
+      take_sequence(u, w, s0, l);
       u.g = g;
-      u.w.n = __builtin_amdgcn_readlane(w.n, l);
-      u.w.pos0 = lane_of(w.pos0, l);
-      u.w.tiles = __builtin_amdgcn_readlane(w.tiles, l);
-      u.w.sub = __builtin_amdgcn_readlane(w.sub, l);
-      u.w.rows = __builtin_amdgcn_readlane(w.rows, l);
-      u.w.first = lane_of(w.first, l);
-      u.w.slope = lane_of(w.slope, l);
       if (u.w.tiles <= 0) return false;
       const int64_t origin = places + lane_of(pp, l) - u.w.before(u.w.tiles);
       int64_t j;
       if constexpr (BY_TILE) {
         j = at - (count + lane_of(pc, l) - u.w.tiles);
-      } else if (whole) {
-        j = u.w.tiles - 1 - (at - origin);  // the last tiles see the most keys and come first
       } else if (u.w.slope == 0) {
         j = divided(at - origin, u.w.first);
       } else {
@@ -259,8 +290,8 @@ __device__ __forceinline__ bool find_unit(const PagedAttn& p, const SeqWork& w0,
       }
       if (j < 0 || j >= u.w.tiles) return false;  // starts that overlap
       u.tile = uniform((int)j);
-      u.start = whole ? at : origin + u.w.before(u.tile);
-      u.end = whole ? at + 1 : origin + u.w.before(u.tile + 1);
+      u.start = origin + u.w.before(u.tile);
+      u.end = origin + u.w.before(u.tile + 1);
       return true;
     }
     places += lane_of(pp, 63);
@@ -274,10 +305,11 @@ __device__ __forceinline__ bool find_unit(const PagedAttn& p, const SeqWork& w0,
 struct Part {
   int lo, hi, slot;
 };
+constexpr Part kWhole{0, 0x7fffffff, -1};
 
 template <typename SHAPE, int KEYS>
 __device__ __forceinline__ Part part_of(const Line& line, const Unit& u, int G, int64_t from, int64_t to, int64_t turn) {
-  Part part{0, 0x7fffffff, -1};
+  Part part = kWhole;
   if (from > u.start || to < u.end) {
     // Neighbours round the border between them alike.
     auto border = [&](int64_t at) {
@@ -315,7 +347,7 @@ __device__ __forceinline__ TileRows tile_rows(const PagedAttn& p, const Unit& u)
   }
   t.rows = uniform(left < 0 ? 0 : (left < u.w.rows ? left : u.w.rows));
   t.row0 = uniform(t.row0);
-  const int64_t last = u.w.pos0 + (t.row0 + t.rows - 1) / p.G;
+  const int64_t last = u.w.pos0 + p.by_group.of(t.row0 + t.rows - 1);
   t.end = uniform(last < 0 || p.batch.pages == 0 ? 0 : (last + 1 < p.batch.cap ? (int)(last + 1) : p.batch.cap));
   return t;
 }
@@ -323,7 +355,7 @@ __device__ __forceinline__ TileRows tile_rows(const PagedAttn& p, const Unit& u)
 // The first keys of the tiles of KEYS keys that a wave (or a workgroup) takes,
 // in order: items base, base + stride .. below hi of the row's keys, or of its
 // list's blocks without those that are padding or in every row's future.  64
-// items are looked up at once, one a lane.
+// items of a list are looked up at once, one a lane.
 template <int KEYS>
 struct KeyWalk {
   const int32_t* list;
@@ -342,15 +374,21 @@ struct KeyWalk {
     found = -1;
   }
   __device__ __forceinline__ int next() {
+    if (!lists) {  // hi is at most the tiles below `end`
+      if (base >= hi) return -1;
+      const int key = base * KEYS;
+      base += stride;
+      return key;
+    }
     while (bits == 0) {
       if (base >= hi) return -1;
       const int item = base + stride * lane;
-      int64_t key = (int64_t)item * KEYS;
-      if (lists && item < hi) {
+      int64_t key = end;
+      if (item < hi) {
         const int id = list[KEYS == kBlock ? item : item >> 1];
-        key = id < 0 ? end : (int64_t)id * kBlock + (KEYS == kBlock ? 0 : (item & 1) * KEYS);
+        if (id >= 0) key = (int64_t)id * kBlock + (KEYS == kBlock ? 0 : (item & 1) * KEYS);
       }
-      const bool ok = item < hi && key < end;
+      const bool ok = key < end;
       found = ok ? (int)key : -1;
       bits = __ballot(ok);
       base += 64 * stride;
@@ -394,15 +432,13 @@ __device__ __forceinline__ int opaque_zero() {
   return z;
 }
 
-template <int D>
-constexpr int few_keys() {
-  return 32;  // keys of a wave's tile
-}
+constexpr int kFewKeys = 32;  // keys of a wave's tile
 template <int D>
 constexpr int few_lds_bytes() {
-  // The waves' V rows, or their O rows, 16 at a time; then maxima and sums.
-  constexpr int v = kWaves * few_keys<D>() * (D + 8) * 2, o = kWaves * 16 * (D + 4) * 4;
-  return (v > o ? v : o) + kWaves * 2 * 32 * 4;
+  // Every wave's V rows, or later its O rows, 16 at a time; then the waves'
+  // maxima and sums, and which of the waves has a sum that is not finite.
+  static_assert(16 * (D + 4) * 4 <= kFewKeys * (D + 8) * 2, "a wave's O rows must fit its V rows");
+  return kWaves * (kFewKeys * (D + 8) * 2 + 2 * 32 * 4 + 4);
 }
 template <int D>
 constexpr int many_lds_bytes() {
@@ -424,18 +460,19 @@ constexpr int many_lds_bytes() {
 template <int D, bool F16, bool CAREFUL>
 __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Part& part, char* smem) {
   const PagedAttn p = arguments(args);
-  constexpr int KEYS = few_keys<D>(), KT = KEYS / 16, KH = KEYS / 32;  // 16- and 32-key pieces of a tile
+  constexpr int KEYS = kFewKeys, KT = KEYS / 16, KH = KEYS / 32;  // 16- and 32-key pieces of a tile
   constexpr int KK = D / 32;   // steps of S^T over d
   constexpr int DT = D / 16;   // 16-row tiles of O^T
   constexpr int VSTR = D + 8;  // V rows in LDS, 16-bit elements
   constexpr int OSTR = D + 4;  // O rows in LDS, floats
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int l16 = lane & 15, g4 = lane >> 4;
-  float* ml = reinterpret_cast<float*>(smem + few_lds_bytes<D>() - kWaves * 2 * 32 * 4);  // [wave][2][32]
+  float* ml = reinterpret_cast<float*>(smem + kWaves * kFewKeys * VSTR * 2);  // [wave][2][32]
+  int* odds = reinterpret_cast<int*>(ml + kWaves * 64);                     // [wave]
 
   const TileRows tr = tile_rows(p, u);
   if (tr.rows == 0) return false;  // uniform: before any barrier
-  const int token0 = uniform(start_at(p.batch, u.s));
+  const int token0 = u.w.start;
   const bool two = tr.rows > 16;  // the second 16 columns hold rows
 
   // This lane's two rows: position and query fragment.  Columns past the last
@@ -446,7 +483,7 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int r = tr.row0 + (16 * c + l16 < tr.rows ? 16 * c + l16 : tr.rows - 1);
-    const int t = r / p.G, h = r - t * p.G;
+    const int t = p.by_group.of(r), h = r - t * p.G;
     qpos[c] = clip(u.w.pos0 + t);
     const uint16_t* src = static_cast<const uint16_t*>(p.q) + (int64_t)(token0 + t) * p.qs[0] +
                           (int64_t)(u.g * p.G + h) * p.qs[1] + 8 * g4;
@@ -454,7 +491,7 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
     for (int kk = 0; kk < KK; ++kk)
       qf[c][kk] = load16(src + 32 * kk);
   }
-  const int first_pos = uniform(clip(u.w.pos0 + tr.row0 / p.G));
+  const int first_pos = uniform(clip(u.w.pos0 + p.by_group.of(tr.row0)));
   const int items = p.idx ? kBlock / KEYS * p.K : (tr.end + KEYS - 1) / KEYS;
   const int hi = part.hi < items ? part.hi : items;
 
@@ -650,7 +687,7 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) odd |= !(fabsf(acc[c][dt][r]) < INFINITY);
-    if (uniform(__syncthreads_or(odd))) return true;
+    odds[wave] = __ballot(odd) != 0;
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -661,17 +698,24 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
     }
   }
   const PagedAttn pe = arguments(args);
-  // The waves' sums joined through LDS, 16 rows at a time: thread t takes
-  // D / 32 values of row t / 32.
+  // The waves' sums joined through LDS, 16 rows at a time, each wave's where
+  // its V rows were: thread t takes D / 32 values of row t / 32.
+  constexpr int OWAVE = kFewKeys * VSTR / 2;  // floats from wave to wave
   float* ol = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (c == 1 && !two) break;
-    __syncthreads();
+    if (c == 1) __syncthreads();
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
-      *reinterpret_cast<f32x4v*>(ol + (wave * 16 + l16) * OSTR + 16 * dt + 4 * g4) = acc[c][dt];
+      *reinterpret_cast<f32x4v*>(ol + wave * OWAVE + l16 * OSTR + 16 * dt + 4 * g4) = acc[c][dt];
     __syncthreads();
+    if (!CAREFUL && c == 0) {
+      int any = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) any |= odds[w];
+      if (uniform(any)) return true;
+    }
     constexpr int PER = D / 32;
     const int r = threadIdx.x >> 5, d0 = (threadIdx.x & 31) * PER, row = 16 * c + r;
     if (row >= tr.rows) continue;
@@ -687,7 +731,7 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
       const float f = fast_exp2(ml[w * 64 + row] + nm);
       sum += f * ml[w * 64 + 32 + row];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) o[i] += f * ol[(w * 16 + r) * OSTR + d0 + i];
+      for (int i = 0; i < PER; ++i) o[i] += f * ol[w * OWAVE + r * OSTR + d0 + i];
     }
     if (part.slot >= 0) {
       const int64_t group = part.slot;
@@ -701,7 +745,7 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
       continue;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int t = (tr.row0 + row) / pe.G, h = tr.row0 + row - t * pe.G;
+    const int t = pe.by_group.of(tr.row0 + row), h = tr.row0 + row - t * pe.G;
     uint16_t* dst = static_cast<uint16_t*>(pe.out) + (int64_t)(token0 + t) * pe.os[0] +
                     (int64_t)(u.g * pe.G + h) * pe.os[1] + d0;
 #pragma unroll
@@ -733,16 +777,16 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
 
   const TileRows tr = tile_rows(p, u);
   if (tr.rows == 0) return false;  // uniform: before any barrier
-  const int token0 = uniform(start_at(p.batch, u.s));
+  const int token0 = u.w.start;
   const int left = tr.rows - 32 * wave;
   const int nrow = left < 0 ? 0 : (left < 32 ? left : 32);  // this wave's rows
   // Columns past the last row repeat it; a wave without rows has the unit's first.
   const int row = tr.row0 + (nrow == 0 ? 0 : 32 * wave + (l32 < nrow ? l32 : nrow - 1));
-  const int tok = row / p.G, head = u.g * p.G + row - tok * p.G;
+  const int tok = p.by_group.of(row), head = u.g * p.G + row - tok * p.G;
   const int qpos = clip(u.w.pos0 + tok);
   // Positions of the wave's first and last row.
-  const int pos_lo = uniform(clip(u.w.pos0 + (tr.row0 + 32 * wave) / p.G));
-  const int pos_hi = uniform(clip(u.w.pos0 + (tr.row0 + 32 * wave + (nrow > 0 ? nrow - 1 : 0)) / p.G));
+  const int pos_lo = uniform(clip(u.w.pos0 + p.by_group.of(tr.row0 + 32 * wave)));
+  const int pos_hi = uniform(clip(u.w.pos0 + p.by_group.of(tr.row0 + 32 * wave + (nrow > 0 ? nrow - 1 : 0))));
 
   uint4 qf[KS];
   {
@@ -1050,7 +1094,7 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
 template <int D, bool F16>
 struct FewBody {
   typedef Few Shape;
-  static constexpr int keys = few_keys<D>(), lds = few_lds_bytes<D>();
+  static constexpr int keys = kFewKeys, lds = few_lds_bytes<D>();
   template <bool CAREFUL>
   static __device__ __forceinline__ bool run(uintptr_t args, const Unit& u, const Part& part, char* smem) {
     return few_rows<D, F16, CAREFUL>(args, u, part, smem);
@@ -1072,19 +1116,48 @@ struct Stretch {
   int g;
 };
 
+// Every wave keeps the lengths of the first 64 sequences behind the body's LDS.
+template <typename BODY>
+constexpr int lds_bytes() {
+  return BODY::lds + kWaves * 64 * (int)sizeof(Lengths);
+}
+template <typename BODY>
+__device__ __forceinline__ Lengths& kept_lengths(char* smem) {
+  return reinterpret_cast<Lengths*>(smem + BODY::lds)[threadIdx.x];
+}
+
+// The turn of a workgroup among those of its head, and the head.
+__device__ __forceinline__ int turn_of(const PagedAttn& p, int& g) {
+  const int turn = uniform(p.by_heads.of((int)blockIdx.x));
+  g = (int)blockIdx.x - turn * p.Hkv;
+  return turn;
+}
+
 template <typename BODY, bool CAREFUL>
 __device__ __forceinline__ bool run_unit(uintptr_t args, const Line& line, const Stretch& st, char* smem, int64_t& to) {
   Unit u;
   int G;
   {
     const PagedAttn p = arguments(args);
-    const SeqWork w0 = sequence_work<typename BODY::Shape>(p, threadIdx.x & 63);
+    const SeqWork w0 = sequence_work<typename BODY::Shape>(p, kept_lengths<BODY>(smem));
     if (!find_unit<typename BODY::Shape, false>(p, w0, st.at, st.g, threadIdx.x & 63, u)) return false;
     G = p.G;
   }
   to = u.end < st.end ? u.end : st.end;
   const Part part = part_of<typename BODY::Shape, BODY::keys>(line, u, G, st.at, to, st.turn);
   return BODY::template run<CAREFUL>(args, u, part, smem);
+}
+
+template <typename BODY, bool CAREFUL>
+__device__ __forceinline__ bool run_tile(uintptr_t args, char* smem) {
+  Unit u;
+  {
+    const PagedAttn p = arguments(args);
+    int g;
+    const int turn = turn_of(p, g);
+    if (!find_tile<typename BODY::Shape>(p, turn, g, threadIdx.x & 63, u)) return false;
+  }
+  return BODY::template run<CAREFUL>(args, u, kWhole, smem);
 }
 
 // The careful way, looking its unit up again, is a function of its own: what
@@ -1097,23 +1170,30 @@ __device__ __attribute__((noinline)) void run_again(uint64_t args, int64_t share
   run_unit<BODY, true>((uintptr_t)same((int64_t)args), Line{0, same(share)},
                        Stretch{same(at), same(end), same(turn), uniform(g)}, (char*)smem, to);
 }
+template <typename BODY>
+__device__ __attribute__((noinline)) void run_tile_again(uint64_t args, __attribute__((address_space(3))) char* smem) {
+  run_tile<BODY, true>((uintptr_t)lane_of((int64_t)args, 0), (char*)smem);
+}
 
 // A launch for either kind: the lengths that tell them apart are on the
 // device, so the workgroups of a kind that the batch does not hold find no
 // tile and end.  (Both in one kernel needed more registers than there are.)
+// One kernel for shares of the line, one for a whole tile a workgroup, which
+// has none of the line's arithmetic before its first load.
 template <typename BODY>
 __global__ __launch_bounds__(kWaves * 64, 2) void paged_attention_kernel(const PagedAttn) {
   typedef typename BODY::Shape SHAPE;
-  __shared__ __attribute__((aligned(16))) char smem[BODY::lds];
+  __shared__ __attribute__((aligned(16))) char smem[lds_bytes<BODY>()];
   const uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
   Line line;
   Stretch st;
   {
     const PagedAttn p = arguments(args);
-    line = line_of<SHAPE>(p, sequence_work<SHAPE>(p, threadIdx.x & 63), threadIdx.x & 63);
-    const int turn = uniform((int)blockIdx.x / p.Hkv);
-    st.turn = turn;
-    st.g = (int)blockIdx.x - turn * p.Hkv;
+    const int lane = threadIdx.x & 63;
+    const Lengths len = lengths_of(p, lane);
+    kept_lengths<BODY>(smem) = len;
+    line = line_of<SHAPE>(p, sequence_work<SHAPE>(p, len), lane);
+    st.turn = turn_of(p, st.g);
   }
   st.at = st.turn * line.share;
   st.end = st.at + line.share < line.total ? st.at + line.share : line.total;
@@ -1121,9 +1201,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attention_kernel(const P
     int64_t to = st.end;
     if (run_unit<BODY, false>(args, line, st, smem, to))
       run_again<BODY>(args, line.share, st.at, st.end, st.turn, st.g, (__attribute__((address_space(3))) char*)smem);
+    if (to <= st.at) break;  // lines past 64 bits, of starts that overlap, lead back
     st.at = to;
     if (st.at < st.end) __syncthreads();  // the unit's LDS is free
   }
+}
+
+template <typename BODY>
+__global__ __launch_bounds__(kWaves * 64, 2) void paged_tile_kernel(const PagedAttn) {
+  __shared__ __attribute__((aligned(16))) char smem[BODY::lds];
+  const uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+  if (run_tile<BODY, false>(args, smem)) run_tile_again<BODY>(args, (__attribute__((address_space(3))) char*)smem);
 }
 
 // Joins the parts of one 32-row group of a tile: every thread takes 4 values of its
@@ -1132,11 +1220,12 @@ template <typename SHAPE, int D, bool F16>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn p) {
   constexpr int kTileGroups = SHAPE::rows / 32;
   const int lane = threadIdx.x & 63;
-  const SeqWork w0 = sequence_work<SHAPE>(p, lane);
+  const SeqWork w0 = sequence_work<SHAPE>(p, lengths_of(p, lane));
   const Line line = line_of<SHAPE>(p, w0, lane);
   const int sub = blockIdx.x % kTileGroups, index = blockIdx.x / kTileGroups;
   Unit u;
-  if (!find_unit<SHAPE, true>(p, w0, index / p.Hkv, index % p.Hkv, lane, u)) return;
+  const int at_tile = p.by_heads.of(index);
+  if (!find_unit<SHAPE, true>(p, w0, at_tile, index - at_tile * p.Hkv, lane, u)) return;
   const int64_t t0 = divided(u.start, line.share), t1 = divided(u.end - 1, line.share);
   if (t0 == t1 || t1 >= p.groups) return;  // held whole (or starts that overlap)
   const TileRows tr = tile_rows(p, u);
@@ -1180,8 +1269,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttn p) {
     top = now;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int at = tr.row0 + r, t = at / p.G, h = at - t * p.G;
-  uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(start_at(p.batch, u.s) + t) * p.os[0] +
+  const int at = tr.row0 + r, t = p.by_group.of(at), h = at - t * p.G;
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(u.w.start + t) * p.os[0] +
                   (int64_t)(u.g * p.G + h) * p.os[1] + 4 * hl;
 #pragma unroll
   for (int j = 0; j < PIECES; ++j)
@@ -1297,6 +1386,8 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
     p.vs[i] = a.vps[i];
   }
   p.Hkv = (int)Hkv;
+  p.by_heads = divisor(Hkv);
+  p.by_group = divisor(Hq / Hkv);
   p.G = (int)(Hq / Hkv);
   p.cs = scale * 1.4426950408889634f;
   if (K > 0) {
@@ -1307,8 +1398,6 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
   }
   SPRUCE_REQUIRE(plan.few_tiles < (int64_t)1 << 22 && plan.many_tiles < (int64_t)1 << 19, "too many tokens for one call");
   p.few_limit = plan.few_limit;
-  p.whole[0] = plan.few_whole;
-  p.whole[1] = plan.many_whole;
   p.groups = (int)plan.groups;
   // The kinds' launches follow one another, so they share the slots.
   p.part_o = static_cast<float*>(a.workspace);
@@ -1323,23 +1412,26 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
     const int e = check_launch("paged attention");                                            \
     if (e) return e;                                                                          \
   } while (0)
+#define SPRUCE_PAGED_KIND(BODY_, JOIN_, WHOLE_, TILES_, JOINS_)                               \
+  do {                                                                                        \
+    if (WHOLE_) {                                                                             \
+      SPRUCE_LAUNCH((paged_tile_kernel<BODY_>), TILES_, kWaves * 64);                         \
+    } else {                                                                                  \
+      SPRUCE_LAUNCH((paged_attention_kernel<BODY_>), plan.groups * Hkv, kWaves * 64);         \
+      SPRUCE_LAUNCH((JOIN_), (TILES_) * (JOINS_), 256);                                       \
+    }                                                                                         \
+  } while (0)
 #define SPRUCE_PAGED(D_, F16_)                                                                \
   do {                                                                                        \
-    if (plan.many) {                                                                          \
-      const int64_t grid = plan.many_whole ? plan.many_tiles : plan.groups * Hkv;                       \
-      if (aligned)                                                                            \
-        SPRUCE_LAUNCH((paged_attention_kernel<ManyBody<D_, F16_, true>>), grid, kWaves * 64);                \
-      else                                                                                    \
-        SPRUCE_LAUNCH((paged_attention_kernel<ManyBody<D_, F16_, false>>), grid, kWaves * 64);               \
-      if (!plan.many_whole)                                                                   \
-        SPRUCE_LAUNCH((paged_join_kernel<Many, D_, F16_>), plan.many_tiles * kWaves, 256);    \
-    }                                                                                         \
-    if (plan.few) {                                                                           \
-      const int64_t grid = plan.few_whole ? plan.few_tiles : plan.groups * Hkv;                         \
-      SPRUCE_LAUNCH((paged_attention_kernel<FewBody<D_, F16_>>), grid, kWaves * 64);                         \
-      if (!plan.few_whole)                                                                    \
-        SPRUCE_LAUNCH((paged_join_kernel<Few, D_, F16_>), plan.few_tiles, 256);               \
-    }                                                                                         \
+    typedef FewBody<D_, F16_> FewOf;                                                          \
+    typedef ManyBody<D_, F16_, true> ManyOf;                                                  \
+    typedef ManyBody<D_, F16_, false> ScatteredOf;                                            \
+    if (plan.many && aligned)                                                                 \
+      SPRUCE_PAGED_KIND(ManyOf, (paged_join_kernel<Many, D_, F16_>), plan.many_whole, plan.many_tiles, kWaves); \
+    if (plan.many && !aligned)                                                                \
+      SPRUCE_PAGED_KIND(ScatteredOf, (paged_join_kernel<Many, D_, F16_>), plan.many_whole, plan.many_tiles, kWaves); \
+    if (plan.few)                                                                             \
+      SPRUCE_PAGED_KIND(FewOf, (paged_join_kernel<Few, D_, F16_>), plan.few_whole, plan.few_tiles, 1); \
   } while (0)
   if (D == 128) {
     if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_PAGED(128, false);
@@ -1349,6 +1441,7 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
     else SPRUCE_PAGED(64, true);
   }
 #undef SPRUCE_PAGED
+#undef SPRUCE_PAGED_KIND
 #undef SPRUCE_LAUNCH
   return SPRUCE_OK;
 }
