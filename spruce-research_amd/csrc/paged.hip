@@ -94,6 +94,7 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
   };
   SPRUCE_REQUIRE(rows16(a.q, a.qs, 2) && rows16(a.k_pages, a.kps, 3) && rows16(a.v_pages, a.vps, 3) && rows16(a.out, a.os, 2),
                  "q, the pages and out must be 16-byte aligned with strides that keep rows 16-byte aligned");
+  SPRUCE_REQUIRE((N == 1 || a.os[0] >= D) && (Hq == 1 || a.os[1] >= D), "the rows of out overlap");
   SPRUCE_REQUIRE(K >= 0 && K < (int64_t)1 << 24, "invalid list width %lld", (long long)K);
   SPRUCE_REQUIRE(K == 0 || (a.idx && a.Qc >= 0), "indices must be a non-null device pointer");
   SPRUCE_REQUIRE(K == 0 || a.is[3] == 1, "indices must have a contiguous final dimension");
@@ -125,15 +126,18 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
     p.Qc = (int)(a.Qc < (int64_t)1 << 30 ? a.Qc : (int64_t)1 << 30);
     p.K = (int)K;
   }
-  SPRUCE_REQUIRE(plan.few_tiles < (int64_t)1 << 22 && plan.many_tiles < (int64_t)1 << 19, "too many tokens for one call");
+  // Grids of fewer than 2^32 threads, rows of a sequence in 32 bits with room for the tiles' ends.
+  SPRUCE_REQUIRE(N * (Hq / Hkv) < (int64_t)1 << 28 && plan.few_tiles < (int64_t)1 << 23 &&
+                     plan.many_tiles < (int64_t)1 << 23,
+                 "too many tokens for one call");
   p.few_limit = plan.few_limit;
   p.groups = (int)plan.groups;
   // The kinds' launches follow one another, so they share the slots.
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = p.part_o + plan.slots * 32 * D;
   p.begun = reinterpret_cast<int4*>(p.part_ml + plan.slots * 64);
-  // Rows of a page's block behind one 32-bit buffer offset.
-  const bool aligned = a.page_size % kBlock == 0 && a.kps[2] > 0 && a.vps[2] > 0 && a.kps[2] < 1 << 22 &&
+  // Rows of a page's block behind one 32-bit buffer offset, bounded by the last row's end.
+  const bool aligned = a.page_size % kBlock == 0 && a.kps[2] >= D && a.vps[2] >= D && a.kps[2] < 1 << 22 &&
                        a.vps[2] < 1 << 22;
   const hipStream_t st = (hipStream_t)stream;
   const bool f16 = dtype == SPRUCE_DTYPE_F16;

@@ -318,7 +318,8 @@ __device__ __forceinline__ Part part_of(const Line& line, const Unit& u, int G, 
     // Neighbours round the border between them alike.
     auto border = [&](int64_t at) {
       const int64_t key = at - u.start - (int64_t)SHAPE::cost * G;
-      return key <= 0 ? 0 : (int)divided(key + KEYS * G - 1, KEYS * G);
+      const int64_t tiles = key <= 0 ? 0 : divided(key + KEYS * G - 1, KEYS * G);
+      return tiles < 1 << 30 ? (int)tiles : 1 << 30;
     };
     part.lo = uniform(border(from));
     if (to < u.end) {

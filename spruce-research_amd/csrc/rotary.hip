@@ -378,6 +378,10 @@ extern "C" int spruce_paged_append(const spruce_paged_append_args* args, void* s
   SPRUCE_REQUIRE((Hq == 0 || fits(p.q)) && fits(p.k) && fits(p.v),
                  "q, k, v, the pages and the output must be 16-byte aligned with strides that keep rows 16-byte "
                  "aligned");
+  auto apart = [&](const int64_t* s) {
+    return (a.pages < 2 || s[0] >= D) && (Hkv == 1 || s[1] >= D) && (a.page_size == 1 || s[2] >= D);
+  };
+  SPRUCE_REQUIRE(apart(a.kps) && apart(a.vps), "the rows of the pages overlap");
   p.positions = a.positions;
   p.pos64 = a.pos64 != 0;
   p.tokens = (int)N;

@@ -139,8 +139,8 @@ def paged_chunk_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, sc
     behind a token's own are ignored, duplicates attended as often as listed;
     tokens past row Qc attend nothing.
 
-    Returns ``[N,Hq,D]`` (``out`` when given; rows of no sequence are left as they
-    were).  A token that attends no key gets zeros, a key without a page no
+    Returns ``[N,Hq,D]`` (``out`` when given, which must share no memory with the
+    inputs; rows of no sequence are left as they were).  A token that attends no key gets zeros, a key without a page no
     weight, and what masked keys and values hold reaches no row.
     """
     device, dtype = q.device, q.dtype

@@ -331,3 +331,65 @@ def test_chunks_and_tokens_agree_with_the_whole_prompt():
     want, bar = attend64(qr[0].transpose(0, 1), kp, vp, table, [T], [T], D ** -0.5, idx.cpu())
     check(torch.cat(parts), want, bar)
     check(whole, want, bar)       # the dense operator's own sums obey the same bar
+
+
+@pytest.mark.parametrize("new,kv,page,Hq,Hkv,D", [
+    ([1] * 70, [1 + 13 * s for s in range(70)], 16, 8, 2, 128),                  # few keys: a tile a workgroup
+    ([33] * 66, [33 + 7 * s for s in range(66)], 32, 14, 2, 64),
+    ([33] * 66, [1500 - 20 * s for s in range(66)], 32, 14, 2, 64),              # many keys: shared out
+    ([33, 1] * 33, [1500 - 20 * s for s in range(66)], 48, 14, 2, 128),          # both kinds, page ends within tiles
+    ([1, 2, 5], [1500, 1100, 1300], 16, 40, 40, 64),                             # heads that do not divide the CUs
+    ([70], [1200], 64, 40, 40, 64),
+    ([1100], [1100], 64, 128, 2, 64),                                            # many tiles: each whole
+])
+def test_ways_to_share_the_work(new, kv, page, Hq, Hkv, D):
+    print(f"case new={new[:4]} kv={kv[:4]} page={page} {Hq}/{Hkv} D={D}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(sum(kv))
+    table, starts, lens, total = make_batch(7, new, kv, page)
+    kp, vp = make_cache(gen, total, Hkv, page, D, torch.bfloat16)
+    q = torch.randn(sum(new), Hq, D, generator=gen, device=DEV).to(torch.bfloat16)
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5)
+    want, bar = attend64(q, kp, vp, table, new, kv, D ** -0.5)
+    check(got, want, bar)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_sequences_of_many_heads(dtype):
+    # Enough row tiles that no sequence is split, of sequences that could be.
+    S, H, D, page = 130, 128, 64, 32
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    kv = [1100 - s for s in range(S)]
+    table, starts, lens, total = make_batch(5, [1] * S, kv, page)
+    kp, vp = make_cache(gen, total, H, page, D, dtype, False)
+    q = torch.randn(S, H, D, generator=gen, device=DEV).to(dtype)
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, 0.125).double()
+    half = torch.finfo(dtype).eps / 2
+    for s in range(S):
+        at = torch.arange(kv[s], device=DEV)
+        ids = table[s].long()[at // page]
+        k, v = (x[ids, :, at % page].double() for x in (kp, vp))       # [kv, H, D]
+        x = q[s].double()
+        score = 0.125 * (x * k).sum(-1)
+        p = torch.softmax(score, 0)[..., None]
+        want, away = (p * v).sum(0), (p * v.abs()).sum(0)
+        e = 2.0 ** -24 * (D + 4) * 0.125 * (x.abs() * k.abs()).sum(-1).amax(0)[:, None] + 2.0 ** -21
+        bar = half * want.abs() * (1 + half) + away * (half + 4 * e)
+        if dtype == torch.float16:
+            top = torch.exp(score - score.amax(0)).sum(0)[:, None]
+            bar = bar + 2.0 ** -25 * (1 + v.abs().sum(0) / top)
+        assert bool(((got[s] - want).abs() <= bar).all()), s
+
+
+@pytest.mark.parametrize("new", [3, 200])
+def test_pages_whose_rows_overlap(new):
+    # Slots 72 values apart with rows of 128: read as they lie.
+    page, Hkv, D, kv = 64, 2, 128, 1300
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    table, starts, lens, total = make_batch(2, [new], [kv], page)
+    span = page * 72 + D
+    kp, vp = (torch.randn(total * Hkv * span, generator=gen, device=DEV).to(torch.bfloat16)
+              .as_strided((total, Hkv, page, D), (Hkv * span, span, 72, 1)) for _ in range(2))
+    q = torch.randn(new, 8, D, generator=gen, device=DEV).to(torch.bfloat16)
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5)
+    want, bar = attend64(q, kp.contiguous(), vp.contiguous(), table, [new], [kv], D ** -0.5)
+    check(got, want, bar)

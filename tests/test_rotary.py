@@ -247,3 +247,22 @@ def test_attention_entry_point_refuses_before_the_launch():
         assert message in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
     assert call(N=0) == 0
     assert spruce_hip.lib().spruce_paged_attention(None, None) == -1
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    def append(kps=(4096, 2048, 128, 1), vps=(4096, 2048, 128, 1), pages=9, page=16):
+        return _call("spruce_paged_append", paged._APPEND_ARGS, (
+            0, 0, 0, 1, 0, 0, 0, 1, FAKE, 256, 128, 1, FAKE, 256, 128, 1, 8, 0, 2, 128, 0, FAKE, *kps, FAKE, *vps, pages,
+            page, FAKE, 4, 4, FAKE, FAKE, 2, 0, 0, 0, 0, 0, 1.0, 0, 0, 2, 1e-6))
+
+    need = spruce_hip.lib().spruce_paged_attention_workspace_bytes(8, 2, 4, 2, 128, 64, 0)
+
+    def attend(os=(512, 128, 1)):
+        return _call("spruce_paged_attention", paged._ATTENTION_ARGS, (
+            FAKE, 512, 128, 1, FAKE, 4096, 2048, 128, 1, FAKE, 4096, 2048, 128, 1, 9, 16, FAKE, 4, 4, FAKE, FAKE, 2, 8, 4,
+            2, 128, 0, 0.1, 0, 1, 1, 1, 1, 1, 0, FAKE, *os, FAKE, need))
+    for call, kwargs in ((append, dict(kps=(0, 2048, 128, 1))), (append, dict(kps=(4096, 0, 128, 1))),
+                         (append, dict(vps=(4096, 2048, 64, 1))), (attend, dict(os=(0, 128, 1))),
+                         (attend, dict(os=(512, 64, 1)))):
+        assert call(**kwargs) == -1, kwargs
+        assert "overlap" in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
