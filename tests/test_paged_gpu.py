@@ -393,3 +393,27 @@ def test_pages_whose_rows_overlap(new):
     got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5)
     want, bar = attend64(q, kp.contiguous(), vp.contiguous(), table, [new], [kv], D ** -0.5)
     check(got, want, bar)
+
+
+@pytest.mark.parametrize("page", [64, 48])
+def test_offsets_past_32_bits(page):
+    # The sequences' pages are the last of a cache of more than 2^31 elements.
+    Hkv, D, dtype = 2, 128, torch.bfloat16
+    total = (1 << 31) // (page * Hkv * D) + 200
+    gen = torch.Generator(device=DEV).manual_seed(page)
+    new, kv = [2, 170], [90, 1100]
+    table, starts, lens, used = make_batch(1, new, kv, page)
+    kp, vp = (torch.empty(total, page, Hkv, D, device=DEV, dtype=dtype).transpose(1, 2) for _ in range(2))
+    for x in (kp, vp):
+        x[-used:] = torch.randn(used, Hkv, page, D, generator=gen, device=DEV).to(dtype)
+    far = torch.where((table >= 0) & (table < used), table + (total - used), table)
+    N = sum(new)
+    q, k, v = (torch.randn(N, H, D, generator=gen, device=DEV).to(dtype) for H in (8, Hkv, Hkv))
+    near = [x[-used:].clone() for x in (kp, vp)]
+    append_paged_kv(k, v, *near, table, starts, lens)
+    append_paged_kv(k, v, kp, vp, far, starts, lens)
+    assert torch.equal(kp[-used:], near[0]) and torch.equal(vp[-used:], near[1])
+    got = paged_chunk_attention(q, kp, vp, far, starts, lens, D ** -0.5)
+    assert torch.equal(got, paged_chunk_attention(q, *near, table, starts, lens, D ** -0.5))
+    want, bar = attend64(q, *near, table, new, kv, D ** -0.5)
+    check(got, want, bar)

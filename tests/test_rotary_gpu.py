@@ -246,3 +246,16 @@ def test_append_lengths_that_do_not_fit():
                 want_k[table[s, p // 16], :, p % 16] = k[t]
                 want_v[table[s, p // 16], :, p % 16] = v[t]
     assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
+
+
+def test_rotate_offsets_past_32_bits():
+    # The last tokens of more than 2^31 elements, as those tokens alone.
+    T, H, D, last = (1 << 31) // (28 * 128) + 33, 28, 128, 40
+    q = torch.empty(1, T, H, D, device=DEV, dtype=torch.bfloat16).transpose(1, 2)
+    q[:, :, -last:] = torch.randn(1, H, last, D, device=DEV).to(torch.bfloat16)
+    k = torch.randn(1, 2, T, D, device=DEV).to(torch.bfloat16)
+    pos = torch.arange(T, device=DEV)
+    inv_freq = rotary_frequencies(D, device=DEV)[0]
+    qo, ko = rotate_heads(q, k, pos, inv_freq)
+    qs, ks = rotate_heads(q[:, :, -last:], k[:, :, -last:], pos[-last:], inv_freq)
+    assert torch.equal(qo[:, :, -last:], qs) and torch.equal(ko[:, :, -last:], ks)
