@@ -504,7 +504,10 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
   const int hi = part.hi < items ? part.hi : items;
 
   const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)u.g * p.ks[1] + 8 * g4;
-  const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1] + 8 * g4;
+  // V rows: lanes vr = 0 .. VROWS - 1 of rows at a time, 16 bytes of d at 8 vc.
+  constexpr int VROWS = 512 / D, VI = KEYS / VROWS;
+  const int vr = lane / (D / 8), vc = lane % (D / 8);
+  const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1] + 8 * vc;
   uint16_t* vl = reinterpret_cast<uint16_t*>(smem) + wave * KEYS * VSTR;
 
   // Table entries of the keys key0 + 16 c + l16.
@@ -520,6 +523,16 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
       const uint16_t* src = base + (int64_t)(is_page(p.batch, pg[c]) ? pg[c] : 0) * st[0] + (int64_t)slot * st[2];
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) x[c][kk] = load16(src + 32 * kk);
+    }
+  };
+
+  auto load_v = [&](int key0, const int (&pg)[KT], u32x4 (&x)[VI]) {
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      const int entry = __shfl(pg[i * VROWS / 16], i * VROWS % 16 + vr);
+      const int key = nearest(key0 + i * VROWS + vr, tr.end);
+      const int slot = key - page_of(p.batch, key) * p.batch.page;
+      x[i] = load16(vbase + (int64_t)(is_page(p.batch, entry) ? entry : 0) * p.vs[0] + (int64_t)slot * p.vs[2]);
     }
   };
 
@@ -541,14 +554,14 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
     // Keys and table entries of this tile, the next and the one after: entries
     // are looked up a tile before the loads that they address are issued.
     int pg[KT], pn[KT], pa[KT];
-    u32x4 kx[KT][KK], vx[KT][KK];
+    u32x4 kx[KT][KK], vx[VI];
     int key0 = walk.next(), nkey = -1;
     if (key0 >= 0) {
       pages_of(key0, pg);
       nkey = walk.next();
       if (nkey >= 0) pages_of(nkey, pn);
       load(kbase, p.ks, key0, pg, kx);
-      load(vbase, p.vs, key0, pg, vx);
+      load_v(key0, pg, vx);
     }
     while (key0 >= 0) {
       const int akey = nkey >= 0 ? walk.next() : -1;
@@ -617,12 +630,10 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
       // V through the wave's LDS rows; the previous tile's reads of them
       // come before these writes in the wave's own order.
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-          *reinterpret_cast<u32x4*>(vl + (16 * kt + l16) * VSTR + 32 * kk + 8 * g4) = vx[kt][kk];
+      for (int i = 0; i < VI; ++i)
+        *reinterpret_cast<u32x4*>(vl + (i * VROWS + vr) * VSTR + 8 * vc) = vx[i];
       wave_lds_fence();
-      if (nkey >= 0) load(vbase, p.vs, nkey, pn, vx);
+      if (nkey >= 0) load_v(nkey, pn, vx);
       const uint16_t* vt = vl + (4 * g4 + (l16 >> 2)) * VSTR + 4 * (l16 & 3);
       if (CAREFUL && masked) {
 #pragma unroll
