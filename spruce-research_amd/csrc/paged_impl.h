@@ -503,11 +503,11 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
   const int items = p.idx ? kBlock / KEYS * p.K : (tr.end + KEYS - 1) / KEYS;
   const int hi = part.hi < items ? part.hi : items;
 
-  const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)u.g * p.ks[1] + 8 * g4;
-  // V rows: lanes vr = 0 .. VROWS - 1 of rows at a time, 16 bytes of d at 8 vc.
-  constexpr int VROWS = 512 / D, VI = KEYS / VROWS;
-  const int vr = lane / (D / 8), vc = lane % (D / 8);
-  const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1] + 8 * vc;
+  // Rows as memory has them: LROWS at a time, this lane's lr-th of those, 16 bytes at 8 lc.
+  constexpr int LROWS = 512 / D, LI = KEYS / LROWS;
+  const int lr = lane / (D / 8), lc = lane % (D / 8);
+  const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)u.g * p.ks[1] + 8 * lc;
+  const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + (int64_t)u.g * p.vs[1] + 8 * lc;
   uint16_t* vl = reinterpret_cast<uint16_t*>(smem) + wave * KEYS * VSTR;
 
   // Table entries of the keys key0 + 16 c + l16.
@@ -515,25 +515,19 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
 #pragma unroll
     for (int c = 0; c < KT; ++c) pg[c] = page_entry(p.batch, u.s, nearest(key0 + 16 * c + l16, tr.end));
   };
-  auto load = [&](const uint16_t* base, const int64_t* st, int key0, const int (&pg)[KT], u32x4 (&x)[KT][KK]) {
+  auto load = [&](const uint16_t* base, const int64_t* st, int key0, const int (&pg)[KT], u32x4 (&x)[LI]) {
 #pragma unroll
-    for (int c = 0; c < KT; ++c) {
-      const int key = nearest(key0 + 16 * c + l16, tr.end);
+    for (int i = 0; i < LI; ++i) {
+      const int entry = __shfl(pg[i * LROWS / 16], i * LROWS % 16 + lr);
+      const int key = nearest(key0 + i * LROWS + lr, tr.end);
       const int slot = key - page_of(p.batch, key) * p.batch.page;
-      const uint16_t* src = base + (int64_t)(is_page(p.batch, pg[c]) ? pg[c] : 0) * st[0] + (int64_t)slot * st[2];
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) x[c][kk] = load16(src + 32 * kk);
+      x[i] = load16(base + (int64_t)(is_page(p.batch, entry) ? entry : 0) * st[0] + (int64_t)slot * st[2]);
     }
   };
-
-  auto load_v = [&](int key0, const int (&pg)[KT], u32x4 (&x)[VI]) {
+  auto keep = [&](const u32x4 (&x)[LI]) {
 #pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int entry = __shfl(pg[i * VROWS / 16], i * VROWS % 16 + vr);
-      const int key = nearest(key0 + i * VROWS + vr, tr.end);
-      const int slot = key - page_of(p.batch, key) * p.batch.page;
-      x[i] = load16(vbase + (int64_t)(is_page(p.batch, entry) ? entry : 0) * p.vs[0] + (int64_t)slot * p.vs[2]);
-    }
+    for (int i = 0; i < LI; ++i) *reinterpret_cast<u32x4*>(vl + (i * LROWS + lr) * VSTR + 8 * lc) = x[i];
+    wave_lds_fence();
   };
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -554,14 +548,14 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
     // Keys and table entries of this tile, the next and the one after: entries
     // are looked up a tile before the loads that they address are issued.
     int pg[KT], pn[KT], pa[KT];
-    u32x4 kx[KT][KK], vx[VI];
+    u32x4 kx[LI], vx[LI];
     int key0 = walk.next(), nkey = -1;
     if (key0 >= 0) {
       pages_of(key0, pg);
       nkey = walk.next();
       if (nkey >= 0) pages_of(nkey, pn);
       load(kbase, p.ks, key0, pg, kx);
-      load_v(key0, pg, vx);
+      load(vbase, p.vs, key0, pg, vx);
     }
     while (key0 >= 0) {
       const int akey = nkey >= 0 ? walk.next() : -1;
@@ -577,17 +571,23 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
         if (left < 32) have[i] &= left <= 0 ? 0u : (1u << left) - 1;
         masked |= have[i] != 0xffffffffu;
       }
+      keep(kx);
+      if (nkey >= 0) load(kbase, p.ks, nkey, pn, kx);
       f32x4v s[2][KT];
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int kt = 0; kt < KT; ++kt) {
+        s[0][kt] = f32x4v{};
+        s[1][kt] = f32x4v{};
+        u32x4 a[KK];
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          s[c][kt] = f32x4v{};
-          if (c == 0 || two)
+        for (int kk = 0; kk < KK; ++kk) a[kk] = load16(vl + (16 * kt + l16) * VSTR + 32 * kk + 8 * g4);
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) s[c][kt] = mfma16x16x32<F16>(kx[kt][kk], qf[c][kk], s[c][kt]);
-        }
-      if (nkey >= 0) load(kbase, p.ks, nkey, pn, kx);
+        for (int kk = 0; kk < KK; ++kk) s[0][kt] = mfma16x16x32<F16>(a[kk], qf[0][kk], s[0][kt]);
+        if (two)
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) s[1][kt] = mfma16x16x32<F16>(a[kk], qf[1][kk], s[1][kt]);
+      }
+      wave_lds_fence();
       u32x4 pk[2][KH];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -627,13 +627,8 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
               u32x4{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(x[4], x[5]), pack2<F16>(x[6], x[7])};
         }
       }
-      // V through the wave's LDS rows; the previous tile's reads of them
-      // come before these writes in the wave's own order.
-#pragma unroll
-      for (int i = 0; i < VI; ++i)
-        *reinterpret_cast<u32x4*>(vl + (i * VROWS + vr) * VSTR + 8 * vc) = vx[i];
-      wave_lds_fence();
-      if (nkey >= 0) load_v(nkey, pn, vx);
+      keep(vx);
+      if (nkey >= 0) load(vbase, p.vs, nkey, pn, vx);
       const uint16_t* vt = vl + (4 * g4 + (l16 >> 2)) * VSTR + 4 * (l16 & 3);
       if (CAREFUL && masked) {
 #pragma unroll
