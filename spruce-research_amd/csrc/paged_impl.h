@@ -62,6 +62,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ u32x4 load16(const uint16_t* p) { return *reinterpret_cast<const u32x4*>(p); }
 
+// The same of what is read but once: not kept in the caches, which a pass over
+// a large cache of keys would only fill in vain.
+__device__ __forceinline__ u32x4 load16_once(const uint16_t* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+}
+
 template <bool F16>
 __device__ __forceinline__ f32x4v mfma16x16x32(u32x4 a, u32x4 b, f32x4v c) {
   if constexpr (F16)
@@ -521,7 +527,7 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
       const int entry = __shfl(pg[i * LROWS / 16], i * LROWS % 16 + lr);
       const int key = nearest(key0 + i * LROWS + lr, tr.end);
       const int slot = key - page_of(p.batch, key) * p.batch.page;
-      x[i] = load16(base + (int64_t)(is_page(p.batch, entry) ? entry : 0) * st[0] + (int64_t)slot * st[2]);
+      x[i] = load16_once(base + (int64_t)(is_page(p.batch, entry) ? entry : 0) * st[0] + (int64_t)slot * st[2]);
     }
   };
   auto keep = [&](const u32x4 (&x)[LI]) {
