@@ -58,11 +58,14 @@ template <int EB>
 struct Raw8 {
   u32x4 w[EB / 2];
 };
-template <int EB>
+template <int EB, bool PAST = false>
 __device__ __forceinline__ Raw8<EB> raw8(const char* p) {
   Raw8<EB> r;
 #pragma unroll
-  for (int i = 0; i < EB / 2; ++i) r.w[i] = reinterpret_cast<const u32x4*>(p)[i];
+  for (int i = 0; i < EB / 2; ++i) {
+    const u32x4* at = reinterpret_cast<const u32x4*>(p) + i;
+    r.w[i] = PAST ? __builtin_nontemporal_load(at) : *at;
+  }
   return r;
 }
 
@@ -80,9 +83,14 @@ __device__ __forceinline__ void widen8(const Raw8<EB>& r, float* v) {
   }
 }
 
-template <int EB, bool F16>
+template <int EB, bool F16, bool PAST>
 __device__ __forceinline__ void store8(char* p, const float* v) {
-  if constexpr (EB == 4) {
+  if constexpr (PAST) {
+    static_assert(EB == 2, "16-byte pieces");
+    __builtin_nontemporal_store(
+        u32x4{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]), pack2<F16>(v[4], v[5]), pack2<F16>(v[6], v[7])},
+        reinterpret_cast<u32x4*>(p));
+  } else if constexpr (EB == 4) {
     reinterpret_cast<float4*>(p)[0] = float4{v[0], v[1], v[2], v[3]};
     reinterpret_cast<float4*>(p)[1] = float4{v[4], v[5], v[6], v[7]};
   } else {
@@ -91,7 +99,8 @@ __device__ __forceinline__ void store8(char* p, const float* v) {
   }
 }
 
-template <int EB, bool F16, int D, bool PAGED>
+// PAST: rows go past the caches (see launch_rotary).
+template <int EB, bool F16, int D, bool PAGED, bool PAST>
 __global__ __launch_bounds__(256, EB == 4 ? 5 : 4) void head_rotary_kernel(const RotaryParams p) {
   constexpr int LPH = D / 16, HPW = 64 / LPH;  // lanes of a head row, head rows of a pass
   constexpr int kFlight = 8 / EB;              // passes in flight: 32 registers
@@ -138,8 +147,8 @@ __global__ __launch_bounds__(256, EB == 4 ? 5 : 4) void head_rotary_kernel(const
         h = h < r.heads ? h : r.heads - 1;  // lanes without a head repeat the last
         const char* src = static_cast<const char*>(r.src) +
                           ((int64_t)b * r.ss[0] + (int64_t)h * r.ss[1] + (int64_t)t * r.ss[2]) * EB;
-        x[i][0] = raw8<EB>(src + e0 * EB);
-        x[i][1] = raw8<EB>(src + e1 * EB);
+        x[i][0] = raw8<EB, PAST>(src + e0 * EB);
+        x[i][1] = raw8<EB, PAST>(src + e1 * EB);
       }
     }
     if (base == first) {
@@ -231,8 +240,8 @@ __global__ __launch_bounds__(256, EB == 4 ? 5 : 4) void head_rotary_kernel(const
       char* dst = static_cast<char*>(r.dst) +
                   ((int64_t)(paged ? page : b) * r.ds[0] + (int64_t)h * r.ds[1] + (int64_t)(paged ? slot : t) * r.ds[2]) *
                       EB;
-      store8<EB, F16>(dst + e0 * EB, v);
-      store8<EB, F16>(dst + e1 * EB, v + 8);
+      store8<EB, F16, PAST>(dst + e0 * EB, v);
+      store8<EB, F16, PAST>(dst + e1 * EB, v + 8);
     }
   }
 }
@@ -250,16 +259,32 @@ int launch_rotary(RotaryParams& p, int64_t D, int dtype, hipStream_t stream) {
   const int64_t blocks = (p.rows * p.groups + 3) / 4;
   SPRUCE_REQUIRE(blocks < (int64_t)1 << 31, "too many tokens");
   const dim3 grid = flat_grid(blocks);
-#define SPRUCE_ROTARY(EB, F16, DD) \
-  hipLaunchKernelGGL((head_rotary_kernel<EB, F16, DD, PAGED>), grid, dim3(256), 0, stream, p)
-  if (D == 128) {
-    if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_ROTARY(2, false, 128);
-    else if (dtype == SPRUCE_DTYPE_F16) SPRUCE_ROTARY(2, true, 128);
-    else SPRUCE_ROTARY(4, false, 128);
+  // Rows that the 256 MB behind the L2s cannot hold until someone reads them
+  // again go past the caches, where the lanes of a head take 128 bytes at a
+  // time (a whole line): 32768 tokens of 28 + 4 heads of 128 in 102 us rather than 113, the append
+  // of 16384 tokens in 80 rather than 88.  Pieces of a line come from memory more than once so (8170
+  // tokens in float32 in 35 us rather than 25), and small outputs serve their readers from the caches.
+  auto lines = [](const RotaryRows& r) {
+    bool whole = (reinterpret_cast<uintptr_t>(r.src) | reinterpret_cast<uintptr_t>(r.dst)) % 128 == 0;
+    for (int i = 0; i < 3; ++i) whole = whole && (r.ss[i] | r.ds[i]) % 64 == 0;
+    return whole;  // (rows that are not there have zeros)
+  };
+  const int64_t values = p.rows * (p.q.heads + p.k.heads + (PAGED ? p.k.heads : 0)) * D;
+  const bool past = values * 4 > (int64_t)256 << 20 && dtype != SPRUCE_DTYPE_F32 && D == 128 && p.rot == D &&
+                    !p.interleaved && lines(p.q) && lines(p.k) && lines(p.v);
+#define SPRUCE_ROTARY(EB, F16, DD, PAST) \
+  hipLaunchKernelGGL((head_rotary_kernel<EB, F16, DD, PAGED, PAST>), grid, dim3(256), 0, stream, p)
+  if (past) {
+    if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_ROTARY(2, false, 128, true);
+    else SPRUCE_ROTARY(2, true, 128, true);
+  } else if (D == 128) {
+    if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_ROTARY(2, false, 128, false);
+    else if (dtype == SPRUCE_DTYPE_F16) SPRUCE_ROTARY(2, true, 128, false);
+    else SPRUCE_ROTARY(4, false, 128, false);
   } else {
-    if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_ROTARY(2, false, 64);
-    else if (dtype == SPRUCE_DTYPE_F16) SPRUCE_ROTARY(2, true, 64);
-    else SPRUCE_ROTARY(4, false, 64);
+    if (dtype == SPRUCE_DTYPE_BF16) SPRUCE_ROTARY(2, false, 64, false);
+    else if (dtype == SPRUCE_DTYPE_F16) SPRUCE_ROTARY(2, true, 64, false);
+    else SPRUCE_ROTARY(4, false, 64, false);
   }
 #undef SPRUCE_ROTARY
   return check_launch("head_rotary_kernel");

@@ -259,3 +259,28 @@ def test_rotate_offsets_past_32_bits():
     qo, ko = rotate_heads(q, k, pos, inv_freq)
     qs, ks = rotate_heads(q[:, :, -last:], k[:, :, -last:], pos[-last:], inv_freq)
     assert torch.equal(qo[:, :, -last:], qs) and torch.equal(ko[:, :, -last:], ks)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_calls_equal_their_parts(dtype):
+    # Rows that go past the caches hold the bits of those that do not.
+    T, Hq, Hkv, D, page = 20011, 28, 4, 128, 64
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    q, k, v = (torch.randn(1, T, H, D, generator=gen, device=DEV).to(dtype).transpose(1, 2) for H in (Hq, Hkv, Hkv))
+    w = (1 + 0.1 * torch.randn(D, generator=gen, device=DEV)).to(dtype)
+    inv_freq = rotary_frequencies(D, device=DEV)[0]
+    pos = torch.arange(T, device=DEV)
+    qo, ko = rotate_heads(q, k, pos, inv_freq, q_weight=w, k_weight=w)
+    parts = [rotate_heads(q[:, :, a:a + 5000], k[:, :, a:a + 5000], pos[a:a + 5000], inv_freq, q_weight=w, k_weight=w)
+             for a in range(0, T, 5000)]
+    assert torch.equal(qo, torch.cat([x for x, _ in parts], 2)) and torch.equal(ko, torch.cat([x for _, x in parts], 2))
+    pages = -(-T // page)
+    table = torch.randperm(pages, generator=gen, device=DEV).to(torch.int32)[None]
+    kp, vp = (torch.zeros(pages, Hkv, page, D, device=DEV, dtype=dtype) for _ in range(2))
+    turned = append_paged_kv(k[0].transpose(0, 1), v[0].transpose(0, 1), kp, vp, table,
+                             torch.tensor([0, T], dtype=torch.int32, device=DEV),
+                             torch.tensor([T], dtype=torch.int32, device=DEV), query=q[0].transpose(0, 1),
+                             inv_freq=inv_freq, q_weight=w, k_weight=w)
+    assert torch.equal(turned, qo[0].transpose(0, 1))
+    back = [x[table[0].long()].transpose(1, 2).reshape(-1, Hkv, D)[:T] for x in (kp, vp)]
+    assert torch.equal(back[0], ko[0].transpose(0, 1)) and torch.equal(back[1], v[0].transpose(0, 1))
