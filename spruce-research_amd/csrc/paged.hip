@@ -25,24 +25,42 @@ int64_t tiles_bound(int64_t N, int64_t S, int64_t G, int64_t most, bool lists) {
   return (N / kBlock + 2 * seqs) * ((rows + SHAPE::rows - 1) / SHAPE::rows);
 }
 
+// The rules below go by sizes that the host knows; figures are of bf16 and f16,
+// 28/4 heads of 128 and 16/8 heads of 64, keys between a fifth and the whole of
+// the table's.
 Plan plan_of(int64_t N, int64_t S, int64_t G, int64_t Hkv, int64_t keys, bool lists) {
   Plan plan{};
+  // Packed rows of a sequence up to which it goes the few-row way.  More than 32
+  // make a second tile, which reads every key again (64 sequences of 42 rows and
+  // 8000 keys: 358 us, 228 the many-row way; 16 of 4000: 63 and 54); where there
+  // are few workgroups that costs less than the many-row way's longer steps (one
+  // sequence of 35 rows: 13 us rather than 19 over 600 keys, 42 rather than 47
+  // over 32000).
+  const int64_t few_rows = S * Hkv >= 32 ? 32 : 64;
   // The lengths are not known here, but every sequence has a new token in all
-  // but odd batches: where even one that has all others' is few rows, the
-  // few-row way is launched alone and takes whatever there is; likewise the
-  // many-row way where one sequence has all tokens.  (An idle launch is 5 to 15 us.)
+  // but odd batches: where even one that has all others' is two tiles at most,
+  // the few-row way is launched alone and takes whatever there is; likewise the
+  // many-row way where one sequence has all tokens.  (An idle launch is 4 to 15
+  // us: 48 us rather than 44 for one to four tokens of each of 16 sequences.)
   const int64_t longest = N > S ? N - S + 1 : 1;
-  plan.few = S > 1 || N * G <= kFewRows;
-  plan.many = longest * G > kFewRows;
-  if (!plan.few && !plan.many) plan.few = true;
-  plan.few_limit = !plan.many ? 0x7fffffff : (plan.few ? kFewRows : -1);
-  if (plan.few) plan.few_tiles = tiles_bound<Few>(N, S, G, plan.many ? kFewRows : N * G, lists) * Hkv;
+  plan.few = S > 1 || N * G <= few_rows;
+  plan.many = !plan.few || longest * G > 64;
+  plan.few_limit = !plan.many ? 0x7fffffff : (plan.few ? (int)few_rows : -1);
+  if (plan.few) plan.few_tiles = tiles_bound<Few>(N, S, G, plan.many ? few_rows : N * G, lists) * Hkv;
   if (plan.many) plan.many_tiles = tiles_bound<Many>(N, S, G, N * G, lists) * Hkv;
-  // Rows of few keys are not worth a join, many tiles not a split.
-  plan.few_whole = keys <= 1024 || plan.few_tiles > 64 * kCus;
-  plan.many_whole = keys <= 1024 || plan.many_tiles >= 2 * kCus;
-  // A CU each; with many heads, whose number may not divide the CUs', in rounds.
-  plan.groups = (Hkv <= 32 ? kCus : 4 * kCus) / Hkv;
+  // Whole tiles save the line's arithmetic and the join, shares even the lengths
+  // out.  Few rows: 16 sequences, 1024 keys: 16 us whole, 25 shared; 2048: 27
+  // and 26; 4096: 50 and 28.  64 sequences (a tile a CU), 4096 keys: 66 and 75;
+  // 8192: 130 and 127; 16384: 254 and 233.  Many rows: 8 sequences of 256 tokens
+  // (224 tiles), 1536 keys: 59 and 67, 4096: 131 and 111; 32 of 128 tokens, 8192
+  // keys: 422 and 400.  Tiles of one sequence are alike: 4096 tokens (512 tiles)
+  // over 16384 keys 985 and 1018; but 2560 (320 tiles) 874 and 672.
+  plan.few_whole = keys <= 1024 || (plan.few_tiles >= kCus && keys <= 4096) || plan.few_tiles > 64 * kCus;
+  plan.many_whole =
+      keys <= 1024 || (plan.many_tiles >= kCus && keys <= 2048) || plan.many_tiles >= (S == 1 ? 2 : 16) * kCus;
+  // A workgroup fills a CU's registers.  (40 heads, 4 sequences of 4000 keys: six
+  // workgroups a head on 256 CUs 70 us, 25 a head in rounds 79.)
+  plan.groups = kCus / Hkv;
   if (plan.groups < 1) plan.groups = 1;
   if (plan.few && !plan.few_whole) plan.slots = 2 * plan.groups * Hkv;
   if (plan.many && !plan.many_whole) plan.slots = 2 * plan.groups * Hkv * kWaves;

@@ -1,19 +1,39 @@
 // Attention of a ragged batch's new tokens over a paged K/V cache:
 //   o_n = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q_n.k_j - m),
 // j over the cached positions up to the token's own, all of them or those of
-// the 64-key blocks listed for the token's 64-position block.
+// the 64-key blocks listed for the token's 64-position block; m a running
+// maximum, sums in 32 bits, p rounded to the matrix cores' 16 bits (an error of
+// half a step a weight, of the size of the output's own rounding).
 //
 // Rows of one (sequence, KV head) are packed token by token, head by head
 // (row r: token r / G, query head g G + r % G), so few tokens of a wide group
 // fill a matrix tile as many tokens of a narrow one do.  What bounds a row tile
-// turns with its height: up to 64 packed rows (a decoding step, a few drafted
+// turns with its height: up to 32 packed rows (a decoding step, a few drafted
 // tokens) each key is read for few products and memory is the bound; above,
-// the matrix cores are.  A workgroup of eight waves works on one unit (rows of
-// a sequence and KV head against a range of its keys) in one of two ways:
+// the matrix cores are.  A workgroup of eight waves works on one unit (a row
+// tile against a range of its keys) in one of two ways:
 //   few rows    32 rows; every wave takes 32 keys at a time of its own,
 //               without a barrier until the waves' sums are joined;
 //   many rows   256 rows, 32 a wave; all waves share each 64-key block in LDS.
-// A batch may mix them.
+// A batch may mix them: a launch each (both in one kernel needed more
+// registers than there are).
+//
+// How the units come about is decided on the host, from the sizes alone (the
+// lengths are on the device).  Where there are few keys, or tiles enough for
+// all CUs, a workgroup takes a tile whole.  Otherwise the tiles of a head stand
+// in one line, each as long as it has keys, and a fixed number of workgroups
+// shares the line out evenly, whatever the lengths are; tiles cut by a border
+// are joined by a second kernel, in the line's order, so results do not depend
+// on timing.  (Equal parts of each sequence instead: 64 sequences of 6 to 32
+// thousand keys 587 us rather than 511 at that stage.)
+//
+// Measured on one MI355X (bf16 but for the drafts, heads of 128 but for theirs):
+//   one token of each of 64 sequences of 6554 to 32768 keys, 28/4 heads, pages of 16: 440 us, 5.87 TB/s
+//   four drafted tokens of each of 16 sequences of 1800 to 9001 keys, 16/8 heads of 64: 44 us, 4.3 TB/s
+//   one token over 517 keys, 8/2 heads: 12 us
+//   512 tokens over 33000 keys, 28/4 heads: 252 us, 954 TFLOP/s
+//   4096 tokens over 32768 keys, 32/8 heads: 1903 us, 1080 TFLOP/s
+//   2048 tokens over 64 listed blocks each, 28/4 heads: 139 us, 858 TFLOP/s
 #pragma once
 
 #include "attention_impl.h"
@@ -43,7 +63,6 @@ struct PagedAttn {
 };
 
 constexpr int kWaves = 8;
-constexpr int kFewRows = 64;    // packed rows of a sequence up to which memory bounds it
 constexpr int kCus = 256;       // a workgroup fills a CU's registers
 
 // Unit shapes: packed rows of a tile, and its fixed part (look-ups, first loads,
@@ -460,12 +479,14 @@ constexpr int many_lds_bytes() {
 }
 
 // A few-row unit.  Memory bounds it: a key's 4 D bytes meet at most 32 rows.
-// A wave's K rows go from memory straight into the A operand of S^T = K Q^T
-// (lane: key l % 16, 16 bytes of d at 8 (l / 16) + 32 kk, so a load takes 64
-// bytes of each of 16 rows); V rows, loaded alike, pass through the wave's own
-// LDS, whose transposing read gives the A operand of O^T = V^T P^T; P^T, the B
-// operand, is S^T's accumulator as it lies (keys 4 (l / 16) + r).  The next
-// tile's K is in flight from the last S^T on, its V from the LDS write on.
+// A wave's K and V rows come from memory as whole rows (D / 8 lanes of 16 bytes
+// each; 64 bytes of 16 rows a load, the operands' own order, took 496 us where
+// this takes 470), past the caches (440), and go through the wave's own LDS,
+// K's first: read back row by row they are the A operand of S^T = K Q^T, V's by
+// the transposing read that of O^T = V^T P^T; P^T, the B operand, is S^T's
+// accumulator as it lies (keys 4 (l / 16) + r).  The next tile's K is in flight
+// from this one's LDS write on, its V likewise.  Tiles of 64 keys at D = 64: 57.6
+// us where 32 took 55.2 (four drafted tokens of 16 sequences).
 //
 // A masked key has p = 0, but 0 times a NaN or infinity in its value row is
 // NaN.  Where sums come out non-finite nothing is written and the result is
@@ -777,7 +798,8 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
 }
 
 // A many-row unit.  The matrix cores bound it, with the softmax's VALU work
-// and the LDS reads beside them, so it is laid out like the block-sparse
+// and the LDS reads beside them (each about 2050 cycles a block and SIMD at full
+// rate; the matrix cores are busy 48% of them), so it is laid out like the block-sparse
 // prefill: S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 with one query row a
 // lane column, 64-key blocks double-buffered in LDS by way of registers, the
 // next block's loads in flight under the present one's products.  The pages of
