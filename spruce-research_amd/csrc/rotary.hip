@@ -22,8 +22,7 @@
 // Measured on one MI355X: 32768 tokens of 28 + 4 heads of 128, normed, bf16, 102 us
 // (5.26 TB/s); the append of 16384 tokens of 32 + 8 + 8 heads 78 us (5.14 TB/s); 8170
 // tokens of 16 + 8 heads of 64 in float32, interleaved, 25 us (4.0 TB/s); one token of each of
-// 64 sequences 4.9 us of kernel.  (Weights kept in LDS instead of registers: 119 us for 114;
-// float32 at four waves a SIMD like the 16-bit types, rather than five, is slower.)
+// 64 sequences 4.9 us of kernel.  (Weights kept in LDS instead of registers: 119 us for 114.)
 #include "paged.h"
 
 using namespace spruce;

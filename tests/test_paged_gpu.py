@@ -341,6 +341,10 @@ def test_chunks_and_tokens_agree_with_the_whole_prompt():
     ([1, 2, 5], [1500, 1100, 1300], 16, 40, 40, 64),                             # heads that do not divide the CUs
     ([70], [1200], 64, 40, 40, 64),
     ([1100], [1100], 64, 128, 2, 64),                                            # many tiles: each whole
+    ([9], [300], 16, 8, 2, 128),                                                 # two tiles of few rows
+    ([9], [3001], 16, 8, 2, 64),
+    ([9, 6, 1, 8] * 4, [1100 + 61 * s for s in range(16)], 48, 28, 4, 128),      # a second tile would read the keys again
+    ([2, 4, 3] * 30, [1030 + 11 * s for s in range(90)], 16, 14, 2, 64),         # a whole tile for each of many sequences
 ])
 def test_ways_to_share_the_work(new, kv, page, Hq, Hkv, D):
     print(f"case new={new[:4]} kv={kv[:4]} page={page} {Hq}/{Hkv} D={D}", flush=True)
