@@ -799,7 +799,7 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
 
 // A many-row unit.  The matrix cores bound it, with the softmax's VALU work
 // and the LDS reads beside them (each about 2050 cycles a block and SIMD at full
-// rate; the matrix cores are busy 48% of them), so it is laid out like the block-sparse
+// rate; the matrix cores are busy 50% of the time), so it is laid out like the block-sparse
 // prefill: S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 with one query row a
 // lane column, 64-key blocks double-buffered in LDS by way of registers, the
 // next block's loads in flight under the present one's products.  The pages of
