@@ -110,7 +110,7 @@ def append_paged_kv(k, v, k_pages, v_pages, page_table, q_starts, kv_lens, *, qu
     if not k.is_cuda:
         raise RuntimeError("the paged HIP backend requires GPU tensors")
     if Hq:
-        out = torch.empty((N, Hq, D), device=device, dtype=dtype)
+        out = k.new_empty_strided((N, Hq, D), (Hq * D, D, 1))
     with spruce_hip.on_device(device):
         rc = spruce_hip.lib().spruce_paged_append(_APPEND_ARGS.pack(
             query.data_ptr() if Hq else 0, *qs, out.data_ptr() if Hq else 0, Hq * D, D, 1,
@@ -183,9 +183,9 @@ def paged_chunk_attention(q, k_pages, v_pages, page_table, q_starts, kv_lens, sc
     if not q.is_cuda:
         raise RuntimeError("the paged HIP backend requires GPU tensors")
     if out is None:
-        out = torch.empty((N, Hq, D), device=device, dtype=dtype)
+        out = q.new_empty_strided((N, Hq, D), (Hq * D, D, 1))
     need = _workspace_bytes(N, S, Hq, Hkv, D, W * page_size, K)
-    work = torch.empty(need, device=device, dtype=torch.uint8)
+    work = q.new_empty_strided((need,), (1,), dtype=torch.uint8)
     with spruce_hip.on_device(device):
         rc = spruce_hip.lib().spruce_paged_attention(_ATTENTION_ARGS.pack(
             q.data_ptr(), *qs, *cache, N, Hq, Hkv, D, spruce_hip.DTYPE_CODES[dtype], scale, *lists,

@@ -142,7 +142,7 @@ def rotate_heads(q, k, positions, inv_freq, *, layout="half", factor=1.0, q_weig
     over the pairs (y_i, y_{i+R/2}) of layout ``"half"`` or (y_2i, y_2i+1) of
     ``"interleaved"``; y_R.. stay as they are.  Angles are formed in 64 bits,
     the rest in 32, rounded once.  Returns (q, k) of the same shapes and dtype,
-    as views of contiguous ``[B,T,H,D]`` tensors.
+    laid out as contiguous ``[B,T,H,D]``.
     """
     device, dtype = q.device, q.dtype
     if q.dim() != 4 or k.dim() != 4:
@@ -167,13 +167,15 @@ def rotate_heads(q, k, positions, inv_freq, *, layout="half", factor=1.0, q_weig
         _refuse_grad()
     if not q.is_cuda:
         raise RuntimeError("the rotary HIP backend requires GPU tensors")
-    qo = torch.empty((B, T, Hq, D), device=device, dtype=dtype)
-    ko = torch.empty((B, T, Hkv, D), device=device, dtype=dtype)
+    # Laid out [B,T,H,D] from the start: a decoding step's call is host time, and a
+    # transposed torch.empty takes 2 us more.
+    qos, kos = (T * Hq * D, D, Hq * D, 1), (T * Hkv * D, D, Hkv * D, 1)
+    qo, ko = q.new_empty_strided((B, Hq, T, D), qos), q.new_empty_strided((B, Hkv, T, D), kos)
     with spruce_hip.on_device(device):
         rc = spruce_hip.lib().spruce_rotate_heads(_ROTATE_ARGS.pack(
             q.data_ptr(), *qs, k.data_ptr(), *ks, B, Hq, Hkv, T, D, spruce_hip.dtype_code(q), *place, *rotation, factor,
-            *weights, eps, qo.data_ptr(), T * Hq * D, D, Hq * D, 1, ko.data_ptr(), T * Hkv * D, D, Hkv * D, 1),
+            *weights, eps, qo.data_ptr(), *qos, ko.data_ptr(), *kos),
             spruce_hip.raw_stream(device.index))
     if rc:
         spruce_hip.check(rc, "spruce_rotate_heads")
-    return qo.transpose(1, 2), ko.transpose(1, 2)
+    return qo, ko
