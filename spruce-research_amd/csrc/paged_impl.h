@@ -999,7 +999,8 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
 #pragma unroll 1
       for (int q = 0; q < 32; ++q) {
         const int seen = __builtin_amdgcn_readlane(rel, q);
-        const uint64_t mine = seen < 63 ? there & ((2ull << seen) - 1) : there;
+        // (-1: a row before the block sees nothing of it.)
+        const uint64_t mine = seen < 0 ? 0ull : (seen < 63 ? there & ((2ull << seen) - 1) : there);
         const uint16_t* vq = vp + opaque_zero();  // as above
         f32x16_t one = f32x16_t{};
 #pragma unroll

@@ -421,3 +421,51 @@ def test_offsets_past_32_bits(page):
     assert torch.equal(got, paged_chunk_attention(q, *near, table, starts, lens, D ** -0.5))
     want, bar = attend64(q, *near, table, new, kv, D ** -0.5)
     check(got, want, bar)
+
+
+def check_exact(got, want, bar, what=""):
+    """As check, with rows that are finite, infinite or NaN wherever the 64-bit form's are."""
+    want_t = want.to(got.dtype).double()
+    finite = torch.isfinite(want)
+    off = (got.double() - want).abs()
+    fine = torch.where(finite, torch.isfinite(got) & (off <= bar),
+                       (torch.isnan(got) & torch.isnan(want)) | (got.double() == want_t))
+    assert bool(fine.all()), (what, int((~fine).sum()), (~fine).nonzero()[:4].tolist())
+
+
+def attend_with_bad_slots(new, kv, page, Hq, Hkv, D, dtype, bad, lists=None, width=None, nan_keys=()):
+    """Positions `bad` of every sequence hold infinite values, `nan_keys` NaN keys; slots of no token hold NaN."""
+    gen = torch.Generator(device=DEV).manual_seed(sum(new) + sum(kv) + page)
+    table, starts, lens, total = make_batch(page, new, kv, page, width=width)
+    kp, vp = make_cache(gen, total, Hkv, page, D, dtype)
+    q = torch.randn(sum(new), Hq, D, generator=gen, device=DEV).to(dtype)
+    used = torch.zeros(total, page, dtype=torch.bool, device=DEV)
+    for s, m in enumerate(kv):
+        at = torch.arange(m, device=DEV)
+        used[table[s].long()[at // page], at % page] = True
+        for j in bad:
+            if j < m:
+                vp[int(table[s, j // page]), :, j % page] = float("inf") if j % 2 else float("-inf")
+        for j in nan_keys:
+            if j < m:
+                kp[int(table[s, j // page]), :, j % page] = float("nan")
+    kp.transpose(1, 2)[~used] = float("nan")
+    vp.transpose(1, 2)[~used] = float("nan")
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5,
+                                indices=None if lists is None else lists.to(DEV))
+    want, bar = attend64(q, kp, vp, table, new, kv, D ** -0.5, lists)
+    check_exact(got, want, bar, (new, kv, page, D, dtype, bad))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new,kv,bad", [
+    (64, 66, [65]),         # a wave's rows stand on both sides of the block border at 64
+    (64, 66, [64, 65]),
+    (70, 66, [2]),          # the first rows have no position at all
+    (70, 66, [1, 65]),
+    (130, 1155, [1088, 1090, 1154]),
+])
+def test_values_of_the_next_block_reach_no_earlier_row(new, kv, bad, page, dtype):
+    print(f"case new={new} kv={kv} page={page} bad={bad} {dtype}", flush=True)
+    attend_with_bad_slots([new], [kv], page, 8, 2, 128, dtype, bad)
