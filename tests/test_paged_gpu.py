@@ -469,3 +469,59 @@ def attend_with_bad_slots(new, kv, page, Hq, Hkv, D, dtype, bad, lists=None, wid
 def test_values_of_the_next_block_reach_no_earlier_row(new, kv, bad, page, dtype):
     print(f"case new={new} kv={kv} page={page} bad={bad} {dtype}", flush=True)
     attend_with_bad_slots([new], [kv], page, 8, 2, 128, dtype, bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [16, 48, 64])
+@pytest.mark.parametrize("new,kv,bad,nan_keys,width", [
+    ([1, 3, 5], [700, 66, 1010], [63, 64, 65, 1008], [1009], 64),          # few rows, whole tiles
+    ([1, 3, 5], [700, 66, 1010], [0, 64, 1007], [], 130),                  # the same, shared out
+    ([5, 4, 1], [2000, 3, 1301], [1, 1995, 1997, 1300], [1999], 130),
+    ([70, 130], [200, 1000], [129, 192, 870, 960, 961], [999], 64),        # many rows, whole tiles
+    ([70, 130], [200, 1000], [130, 191, 193, 869, 999], [], 130),          # the same, shared out
+    ([131, 66], [1279, 64], [1149, 1151, 1152, 1216, 1217, 3], [1278], 130),
+])
+def test_bad_values_at_any_place(new, kv, bad, nan_keys, width, page, D, dtype):
+    # Seen, they show; unseen, they do not.  `width` pages of 16: up to 1024 positions tiles go whole.
+    print(f"case new={new} kv={kv} page={page} D={D} width={width} {dtype}", flush=True)
+    # (1008 positions are 21 pages of 48, and 1010 a page more: shared out there.)
+    pages = max(width * 16 // page, (max(kv) + page - 1) // page)
+    attend_with_bad_slots(new, kv, page, 8, 2, D, dtype, bad, width=pages, nan_keys=nan_keys)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new,kv,bad,K", [
+    ([1, 3], [700, 66], [63, 64, 699], 6),
+    ([1, 3], [700, 1366], [1, 640, 1363, 1364], 20),
+    ([70, 40], [200, 1000], [131, 191, 192, 961, 999], 6),
+    ([70, 40], [200, 1000], [129, 960, 961], 20),
+])
+def test_bad_values_in_listed_blocks(new, kv, bad, K, page, D, dtype):
+    print(f"case new={new} kv={kv} page={page} D={D} K={K} {dtype}", flush=True)
+    attend_with_bad_slots(new, kv, page, 8, 2, D, dtype, bad, lists=_lists(K + D, new, kv, 2, K))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("new,kv,page,Hq,Hkv,D,K", [
+    ([1, 2, 5], [700, 2000, 1300], 16, 8, 2, 128, 40),     # few rows, the lists shared out
+    ([1, 4], [1300, 3000], 32, 16, 8, 64, 300),            # more than 64 items a wave
+    ([3], [1000], 64, 14, 2, 64, 521),
+    ([70, 33], [1500, 3000], 64, 8, 2, 128, 90),           # many rows, more than 64 items
+    ([70, 33], [1500, 3000], 48, 28, 4, 64, 131),
+])
+def test_long_lists(new, kv, page, Hq, Hkv, D, K, dtype):
+    print(f"case new={new} kv={kv} page={page} {Hq}/{Hkv} D={D} K={K} {dtype}", flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(sum(new) + page)
+    table, starts, lens, total = make_batch(page, new, kv, page)
+    kp, vp = make_cache(gen, total, Hkv, page, D, dtype)
+    q = torch.randn(sum(new), Hq, D, generator=gen, device=DEV).to(dtype)
+    idx = _lists(K, new, kv, Hkv, K)
+    idx[:, :, :, K // 4:K // 2] = -1        # whole rounds of padding in the middle
+    idx[-1, -1, 0, :-1] = -1                # one entry, the last
+    idx[-1, -1, 0, -1] = 0
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5, indices=idx.to(DEV))
+    want, bar = attend64(q, kp, vp, table, new, kv, D ** -0.5, idx)
+    check(got, want, bar)
