@@ -700,6 +700,9 @@ int spruce_kernel_metadata(int variant, int64_t Hq, int64_t Hkv, int64_t D,
  * These calls take their arguments as one block of 8-byte fields, which is
  * read before they return: a token's step is a few microseconds on the device,
  * and marshalling forty arguments one by one takes a Python caller as long.
+ * Outputs (the pages of the append among them) have rows that share no memory,
+ * each dim stepping over all that those with smaller strides span; others are
+ * refused.
  * ---------------------------------------------------------------------- */
 
 /* Pairs (x_i, x_{i + R/2}) or (x_{2i}, x_{2i+1}) of the R rotated dims. */

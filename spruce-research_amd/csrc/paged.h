@@ -63,6 +63,30 @@ inline int prepare_batch(PagedBatch& b, const int32_t* table, int64_t table_stri
   return SPRUCE_OK;
 }
 
+// Whether no two of the rows of D values that a call writes share memory: `n`
+// dims of sizes[i] rows at strides[i], in whatever order; each dim of more than
+// one row has to step over all that those with smaller strides span.  (Dims that
+// interleave without meeting are taken for overlapping.)
+inline bool rows_apart(const int64_t* strides, const int64_t* sizes, int n, int64_t D) {
+  int order[4], dims = 0;
+  for (int i = 0; i < n; ++i) {
+    if (sizes[i] == 0) return true;
+    if (sizes[i] == 1) continue;
+    int at = dims++;
+    for (; at > 0 && strides[order[at - 1]] > strides[i]; --at) order[at] = order[at - 1];
+    order[at] = i;
+  }
+  int64_t span = D;
+  for (int i = 0; i < dims; ++i) {
+    const int64_t stride = strides[order[i]];
+    int64_t steps;
+    if (stride < span || __builtin_mul_overflow(sizes[order[i]] - 1, stride, &steps) ||
+        __builtin_add_overflow(steps, span, &span))
+      return false;
+  }
+  return true;
+}
+
 __device__ __forceinline__ int page_of(const PagedBatch& b, int pos) { return b.by_page.of(pos); }
 
 // q_starts[s] and kv_lens[s] brought into range.

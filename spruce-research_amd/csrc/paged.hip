@@ -112,7 +112,8 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
   };
   SPRUCE_REQUIRE(rows16(a.q, a.qs, 2) && rows16(a.k_pages, a.kps, 3) && rows16(a.v_pages, a.vps, 3) && rows16(a.out, a.os, 2),
                  "q, the pages and out must be 16-byte aligned with strides that keep rows 16-byte aligned");
-  SPRUCE_REQUIRE((N == 1 || a.os[0] >= D) && (Hq == 1 || a.os[1] >= D), "the rows of out overlap");
+  const int64_t rows[2] = {N, Hq};
+  SPRUCE_REQUIRE(rows_apart(a.os, rows, 2, D), "the rows of out overlap");
   SPRUCE_REQUIRE(K >= 0 && K < (int64_t)1 << 24, "invalid list width %lld", (long long)K);
   SPRUCE_REQUIRE(K == 0 || (a.idx && a.Qc >= 0), "indices must be a non-null device pointer");
   SPRUCE_REQUIRE(K == 0 || a.is[3] == 1, "indices must have a contiguous final dimension");

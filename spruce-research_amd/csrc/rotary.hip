@@ -350,6 +350,8 @@ extern "C" int spruce_rotate_heads(const spruce_rotate_heads_args* args, void* s
   SPRUCE_REQUIRE(rows16(a.q, a.qs, eb) && rows16(a.k, a.ks, eb) && rows16(a.q_out, a.qos, eb) &&
                      rows16(a.k_out, a.kos, eb),
                  "q, k and the outputs must be 16-byte aligned with strides that keep rows 16-byte aligned");
+  const int64_t q_rows[3] = {B, Hq, T}, k_rows[3] = {B, Hkv, T};
+  SPRUCE_REQUIRE(rows_apart(a.qos, q_rows, 3, D) && rows_apart(a.kos, k_rows, 3, D), "the rows of the outputs overlap");
   auto rows = [](RotaryRows& r, const void* src, const int64_t* ss, void* dst, const int64_t* ds, int64_t heads) {
     r.src = src;
     r.dst = dst;
@@ -408,10 +410,9 @@ extern "C" int spruce_paged_append(const spruce_paged_append_args* args, void* s
   SPRUCE_REQUIRE((Hq == 0 || fits(p.q)) && fits(p.k) && fits(p.v),
                  "q, k, v, the pages and the output must be 16-byte aligned with strides that keep rows 16-byte "
                  "aligned");
-  auto apart = [&](const int64_t* s) {
-    return (a.pages < 2 || s[0] >= D) && (Hkv == 1 || s[1] >= D) && (a.page_size == 1 || s[2] >= D);
-  };
-  SPRUCE_REQUIRE(apart(a.kps) && apart(a.vps), "the rows of the pages overlap");
+  const int64_t pages[3] = {a.pages, Hkv, a.page_size}, tokens[2] = {N, Hq};
+  SPRUCE_REQUIRE(rows_apart(a.kps, pages, 3, D) && rows_apart(a.vps, pages, 3, D), "the rows of the pages overlap");
+  SPRUCE_REQUIRE(Hq == 0 || rows_apart(a.qos, tokens, 2, D), "the rows of the output overlap");
   p.positions = a.positions;
   p.pos64 = a.pos64 != 0;
   p.tokens = (int)N;

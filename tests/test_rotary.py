@@ -266,3 +266,33 @@ def test_outputs_that_overlap_themselves_are_refused():
                          (attend, dict(os=(512, 64, 1)))):
         assert call(**kwargs) == -1, kwargs
         assert "overlap" in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
+
+
+def test_outputs_whose_dims_step_over_one_another_are_refused():
+    # Each stride holds a row, yet rows of two dims meet.
+    def rotate(qos=(0, 128, 512, 1), kos=(0, 128, 256, 1), B=1):
+        return _call("spruce_rotate_heads", rotary._ROTATE_ARGS, (
+            FAKE, 0, 128, 512, 1, FAKE, 0, 128, 256, 1, B, 4, 2, 8, 128, 0, FAKE, 0, 0, FAKE, 128, 0, 1.0, 0, 0, 2, 1e-6,
+            FAKE, *qos, FAKE, *kos))
+
+    def append(kps=(4096, 2048, 128, 1), vps=(4096, 2048, 128, 1), qos=(512, 128, 1), pages=9, page=16):
+        return _call("spruce_paged_append", paged._APPEND_ARGS, (
+            FAKE, 512, 128, 1, FAKE, *qos, FAKE, 256, 128, 1, FAKE, 256, 128, 1, 8, 4, 2, 128, 0, FAKE, *kps, FAKE, *vps,
+            pages, page, FAKE, 4, 4, FAKE, FAKE, 2, 0, 0, 0, 0, 0, 1.0, 0, 0, 2, 1e-6))
+
+    need = spruce_hip.lib().spruce_paged_attention_workspace_bytes(8, 2, 4, 2, 128, 64, 0)
+
+    def attend(os):
+        return _call("spruce_paged_attention", paged._ATTENTION_ARGS, (
+            FAKE, 512, 128, 1, FAKE, 4096, 2048, 128, 1, FAKE, 4096, 2048, 128, 1, 9, 16, FAKE, 4, 4, FAKE, FAKE, 2, 8, 4,
+            2, 128, 0, 0.1, 0, 1, 1, 1, 1, 1, 0, FAKE, *os, FAKE, need))
+    for call, kwargs in ((append, dict(kps=(128, 128, 128, 1))), (append, dict(kps=(4096, 128, 128, 1))),
+                         (append, dict(vps=(2048, 2048, 128, 1))), (append, dict(vps=(4096, 1920, 128, 1))),
+                         (append, dict(kps=(2048, 128, 2048, 1))), (append, dict(qos=(128, 128, 1))),
+                         (append, dict(qos=(384, 128, 1))), (append, dict(kps=(1 << 62, 128, 256, 1))),
+                         (attend, dict(os=(128, 128, 1))), (attend, dict(os=(128, 512, 1))),
+                         (attend, dict(os=(504, 128, 1))), (rotate, dict(qos=(0, 128, 128, 1))),
+                         (rotate, dict(qos=(0, 128, 384, 1))), (rotate, dict(kos=(0, 512, 128, 1))),
+                         (rotate, dict(B=2)), (rotate, dict(B=2, qos=(3968, 128, 512, 1), kos=(2048, 128, 256, 1)))):
+        assert call(**kwargs) == -1, kwargs
+        assert "overlap" in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
