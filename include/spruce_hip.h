@@ -691,7 +691,7 @@ int spruce_kernel_metadata(int variant, int64_t Hq, int64_t Hkv, int64_t D,
  * ascending) and kv_lens[s] positions in the cache (int32 [S]), its new tokens
  * included: new token i of n has position kv_lens[s] - n + i.  Position p is
  * slot p % page_size of page page_table[s][p / page_size] (int32
- * [S, table_width], rows table_stride apart); pages are
+ * [S, table_width], rows table_stride apart, 0: one row for all); pages are
  * [pages, Hkv, page_size, D] with any strides, contiguous along D.  All of
  * these are read on the device: a captured launch takes the values they hold
  * at replay.  Ids outside [0, pages) and positions past the table name no

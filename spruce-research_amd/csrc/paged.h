@@ -46,7 +46,8 @@ inline int prepare_batch(PagedBatch& b, const int32_t* table, int64_t table_stri
   SPRUCE_REQUIRE(N >= 0 && N < (int64_t)1 << 30, "invalid token count %lld", (long long)N);
   SPRUCE_REQUIRE(page >= 1 && page < (int64_t)1 << 30, "invalid page size %lld", (long long)page);
   SPRUCE_REQUIRE(pages >= 0 && pages < (int64_t)1 << 31, "invalid page count %lld", (long long)pages);
-  SPRUCE_REQUIRE(width >= 0 && table_stride >= width, "page_table rows (%lld) overlap (stride %lld)",
+  // (Stride 0: one row for all sequences.)
+  SPRUCE_REQUIRE(width >= 0 && (table_stride == 0 || table_stride >= width), "page_table rows (%lld) overlap (stride %lld)",
                  (long long)width, (long long)table_stride);
   // The kernels reach up to a tile past the last position in 32 bits.
   SPRUCE_REQUIRE(width <= (((int64_t)1 << 31) - 1024) / page, "page_table covers 2^31 - 1024 positions or more");

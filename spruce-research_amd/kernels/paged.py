@@ -9,7 +9,8 @@ that every call here takes, and reads on the device only:
 
 * ``page_table`` int32 ``[S, W]``: position p of sequence s lies in slot
   ``p % page_size`` of page ``page_table[s, p // page_size]``; ids outside
-  ``[0, pages)`` name no page;
+  ``[0, pages)`` name no page; one row expanded over sequences that share their
+  pages will do;
 * ``q_starts`` int32 ``[S + 1]``, ascending: the new tokens of sequence s are rows
   ``q_starts[s] .. q_starts[s + 1]`` of the packed ``[N, H, D]`` tensors; rows behind
   ``q_starts[S]`` belong to no sequence and are left alone;

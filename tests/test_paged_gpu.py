@@ -525,3 +525,27 @@ def test_long_lists(new, kv, page, Hq, Hkv, D, K, dtype):
     got = paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5, indices=idx.to(DEV))
     want, bar = attend64(q, kp, vp, table, new, kv, D ** -0.5, idx)
     check(got, want, bar)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_one_table_row_for_all_sequences(page):
+    # Sequences that share their pages: an expanded row, against a table that repeats it.
+    Hkv, D, dtype = 2, 128, torch.bfloat16
+    gen = torch.Generator(device=DEV).manual_seed(page)
+    new, kv = [1, 70, 3], [1300, 900, 1303]
+    row, _, _, total = make_batch(3, [1], [1400], page)
+    starts = torch.tensor([0, 1, 71, 74], dtype=torch.int32, device=DEV)
+    lens = torch.tensor(kv, dtype=torch.int32, device=DEV)
+    kp, vp = make_cache(gen, total, Hkv, page, D, dtype)
+    q, k, v = (torch.randn(sum(new), H, D, generator=gen, device=DEV).to(dtype) for H in (8, Hkv, Hkv))
+    shared, whole = row.expand(3, -1), row.repeat(3, 1)
+    assert shared.stride(0) == 0
+    caches = [(kp, vp), (kp.clone(), vp.clone())]
+    starts_own = torch.tensor([0, 0, 70, 70], dtype=torch.int32, device=DEV)    # one sequence writes
+    for table, (a, b) in zip((shared, whole), caches):
+        append_paged_kv(k, v, a, b, table, starts_own, lens)
+    assert torch.equal(caches[0][0], caches[1][0]) and torch.equal(caches[0][1], caches[1][1])
+    got = paged_chunk_attention(q, kp, vp, shared, starts, lens, D ** -0.5)
+    assert torch.equal(got, paged_chunk_attention(q, kp, vp, whole, starts, lens, D ** -0.5))
+    want, bar = attend64(q, kp, vp, whole, new, kv, D ** -0.5)
+    check(got, want, bar)

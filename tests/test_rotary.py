@@ -296,3 +296,14 @@ def test_outputs_whose_dims_step_over_one_another_are_refused():
                          (rotate, dict(B=2)), (rotate, dict(B=2, qos=(3968, 128, 512, 1), kos=(2048, 128, 256, 1)))):
         assert call(**kwargs) == -1, kwargs
         assert "overlap" in spruce_hip.last_error(), (kwargs, spruce_hip.last_error())
+
+
+def test_one_table_row_for_all_sequences_is_taken():
+    need = spruce_hip.lib().spruce_paged_attention_workspace_bytes(8, 2, 4, 2, 128, 64, 0)
+    for stride, want in ((0, 0), (4, 0), (3, -1), (-4, -1)):       # no new token: the checks alone
+        assert _call("spruce_paged_append", paged._APPEND_ARGS, (
+            0, 0, 0, 1, 0, 0, 0, 1, FAKE, 256, 128, 1, FAKE, 256, 128, 1, 0, 0, 2, 128, 0, FAKE, 4096, 2048, 128, 1, FAKE,
+            4096, 2048, 128, 1, 9, 16, FAKE, stride, 4, FAKE, FAKE, 2, 0, 0, 0, 0, 0, 1.0, 0, 0, 2, 1e-6)) == want
+        assert _call("spruce_paged_attention", paged._ATTENTION_ARGS, (
+            FAKE, 512, 128, 1, FAKE, 4096, 2048, 128, 1, FAKE, 4096, 2048, 128, 1, 9, 16, FAKE, stride, 4, FAKE, FAKE, 2, 0,
+            4, 2, 128, 0, 0.1, 0, 1, 1, 1, 1, 1, 0, FAKE, 512, 128, 1, FAKE, need)) == want
