@@ -17,12 +17,18 @@ struct Plan {
 
 template <typename SHAPE>
 int64_t tiles_bound(int64_t N, int64_t S, int64_t G, int64_t most, bool lists) {
-  // `most`: packed rows of one sequence at most; a sequence rounds up by one tile.
-  const int64_t seqs = S < N ? S : N;
-  if (!lists) return N * G / SHAPE::rows + seqs;
-  // Rows break at every 64 positions too.
-  const int64_t rows = most < kBlock * G ? most : kBlock * G;
-  return (N / kBlock + 2 * seqs) * ((rows + SHAPE::rows - 1) / SHAPE::rows);
+  // `most`: packed rows that a sequence of this kind has at most, and so its
+  // tokens; a sequence rounds up by one tile.  (By all tokens alone a large chunk
+  // passes for thousands of few-row tiles, which the rules below take whole:
+  // 16384 tokens of one sequence beside one token over 131072 keys, 32/8 heads
+  // of 128, 4031 us rather than 2564.)
+  const int64_t seqs = S < N ? S : N, tokens = most / G;
+  if (tokens == 0) return 0;
+  auto least = [](int64_t x, int64_t y) { return x < y ? x : y; };
+  auto tiles = [](int64_t rows) { return (rows + SHAPE::rows - 1) / SHAPE::rows; };
+  if (!lists) return least(N * G / SHAPE::rows + seqs, seqs * tiles(most));
+  // Rows break at every 64 positions too; n tokens touch (n - 2) / 64 + 2 such blocks at most, one token one.
+  return least(N / kBlock + 2 * seqs, seqs * ((tokens + kBlock - 2) / kBlock + 1)) * tiles(least(most, kBlock * G));
 }
 
 // The rules below go by sizes that the host knows; figures are of bf16 and f16,
@@ -45,6 +51,7 @@ Plan plan_of(int64_t N, int64_t S, int64_t G, int64_t Hkv, int64_t keys, bool li
   const int64_t longest = N > S ? N - S + 1 : 1;
   plan.few = S > 1 || N * G <= few_rows;
   plan.many = !plan.few || longest * G > 64;
+  if (plan.many && G > few_rows) plan.few = false;  // one token is past it
   plan.few_limit = !plan.many ? 0x7fffffff : (plan.few ? (int)few_rows : -1);
   if (plan.few) plan.few_tiles = tiles_bound<Few>(N, S, G, plan.many ? few_rows : N * G, lists) * Hkv;
   if (plan.many) plan.many_tiles = tiles_bound<Many>(N, S, G, N * G, lists) * Hkv;

@@ -549,3 +549,30 @@ def test_one_table_row_for_all_sequences(page):
     assert torch.equal(got, paged_chunk_attention(q, kp, vp, whole, starts, lens, D ** -0.5))
     want, bar = attend64(q, kp, vp, whole, new, kv, D ** -0.5)
     check(got, want, bar)
+
+
+@pytest.mark.parametrize("lists", [False, True])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new,kv,Hq,Hkv,D", [
+    ([150, 64, 64, 1], [900, 95, 640, 300], 2, 2, 64),      # two tiles of few rows, across a block border
+    ([150, 16, 17, 1, 0], [900, 71, 640, 300, 9], 8, 2, 128),
+    ([150, 21, 22, 2], [150, 700, 80, 900], 6, 2, 64),
+    ([90] + [8] * 20, [700] + [67 + 40 * s for s in range(20)], 8, 2, 64),       # one tile each
+    ([1, 2, 1, 3], [700, 66, 900, 64], 40, 1, 64),          # a token of 40 rows
+    ([9, 1], [500, 900], 64, 1, 128),
+    ([2, 1] * 20, [64 + 20 * s for s in range(40)], 33, 1, 64),                  # none has few rows
+])
+def test_mixed_batches_at_the_kinds_border(new, kv, Hq, Hkv, D, page, lists):
+    # Both with whole tiles (up to 1024 positions, 16 blocks) and shared out.
+    gen = torch.Generator(device=DEV).manual_seed(sum(kv))
+    for width, K in ((1024 // page, 5), (2048 // page, 33)):
+        print(f"case new={new[:5]} kv={kv[:5]} {Hq}/{Hkv} D={D} page={page} lists={lists} width={width}", flush=True)
+        table, starts, lens, total = make_batch(7, new, kv, page, width=width)
+        kp, vp = make_cache(gen, total, Hkv, page, D, torch.bfloat16)
+        q = torch.randn(sum(new), Hq, D, generator=gen, device=DEV).to(torch.bfloat16)
+        idx = _lists(K, new, kv, Hkv, K) if lists else None
+        out = torch.full((sum(new), Hq, D), 5.0, device=DEV, dtype=torch.bfloat16)
+        paged_chunk_attention(q, kp, vp, table, starts, lens, D ** -0.5, out=out,
+                              indices=None if idx is None else idx.to(DEV))
+        want, bar = attend64(q, kp, vp, table, new, kv, D ** -0.5, idx)
+        check(out, want, bar)

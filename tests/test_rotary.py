@@ -307,3 +307,12 @@ def test_one_table_row_for_all_sequences_is_taken():
         assert _call("spruce_paged_attention", paged._ATTENTION_ARGS, (
             FAKE, 512, 128, 1, FAKE, 4096, 2048, 128, 1, FAKE, 4096, 2048, 128, 1, 9, 16, FAKE, stride, 4, FAKE, FAKE, 2, 0,
             4, 2, 128, 0, 0.1, 0, 1, 1, 1, 1, 1, 0, FAKE, 512, 128, 1, FAKE, need)) == want
+
+
+@pytest.mark.parametrize("N,S,lists", [(40000, 2, 0), (40000, 9, 0), (60000, 3, 64)])
+def test_single_tokens_beside_a_large_chunk_are_shared_out(N, S, lists):
+    # The chunk's tiles go whole; those of the other sequences are few, of a token each, and their keys are
+    # shared out, for which the workspace holds two slots of 32 rows a workgroup.
+    Hq, Hkv, D = 32, 8, 128
+    got = spruce_hip.lib().spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D, 131072, lists)
+    assert got >= 2 * 256 * 32 * (D + 2) * 4
