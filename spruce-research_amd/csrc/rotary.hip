@@ -105,8 +105,11 @@ __device__ __forceinline__ void store8(char* p, const float* v) {
 }
 
 // PAST: rows go past the caches (see launch_rotary).
+// Four waves a SIMD for every type: at five the float32 append kept 22 registers
+// in scratch (16384 tokens of 32 + 8 + 8 heads of 128 176 us rather than 162, 8192 of
+// 16 + 8 + 8 heads of 64 47 rather than 38), and the float32 rotation was no faster.
 template <int EB, bool F16, int D, bool PAGED, bool PAST>
-__global__ __launch_bounds__(256, EB == 4 ? 5 : 4) void head_rotary_kernel(const RotaryParams p) {
+__global__ __launch_bounds__(256, 4) void head_rotary_kernel(const RotaryParams p) {
   constexpr int LPH = D / 16, HPW = 64 / LPH;  // lanes of a head row, head rows of a pass
   constexpr int kFlight = 8 / EB;              // passes in flight: 32 registers
   __shared__ float2 turns[4][D / 2];
