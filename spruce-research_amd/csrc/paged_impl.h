@@ -3,7 +3,8 @@
 // j over the cached positions up to the token's own, all of them or those of
 // the 64-key blocks listed for the token's 64-position block; m a running
 // maximum, sums in 32 bits, p rounded to the matrix cores' 16 bits (an error of
-// half a step a weight, of the size of the output's own rounding).
+// half a step a weight, of the size of the output's own rounding; in f16, which
+// has few exponents, of 2^-32 of the largest weight for those below 2^-21 of it).
 //
 // Rows of one (sequence, KV head) are packed token by token, head by head
 // (row r: token r / G, query head g G + r % G), so few tokens of a wide group
@@ -437,6 +438,12 @@ __device__ __forceinline__ int part_at(int row, int d) {
   return ((d >> 3) * 64 + row + 32 * ((d >> 2) & 1)) * 4 + (d & 3);
 }
 
+// Weights of f16 are 2^kLift times as large, their sum with them, so that what
+// lies far below a row's largest score keeps its bits: normal down to 2^-21 of
+// the running maximum, and at 2^(8 + 7), the most above it, still finite.
+template <bool F16>
+constexpr float kLift = F16 ? 7.f : 0.f;
+
 // x combined over the lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float quad_max(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x),
@@ -641,7 +648,7 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) acc[c][dt] *= alpha;
         }
-        const float nm = m[c] == -INFINITY ? 0.f : -m[c];
+        const float nm = m[c] == -INFINITY ? 0.f : kLift<F16> - m[c];
 #pragma unroll
         for (int h2 = 0; h2 < KH; ++h2) {
           float x[8];
@@ -945,7 +952,7 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[dt][r] *= alpha;
     }
-    const float nm = m == -INFINITY ? 0.f : -m;
+    const float nm = m == -INFINITY ? 0.f : kLift<F16> - m;
     float sum = 0.f;
 #pragma unroll
     for (int h2 = 0; h2 < 2; ++h2) {

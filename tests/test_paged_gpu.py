@@ -576,3 +576,34 @@ def test_mixed_batches_at_the_kinds_border(new, kv, Hq, Hkv, D, page, lists):
                               indices=None if idx is None else idx.to(DEV))
         want, bar = attend64(q, kp, vp, table, new, kv, D ** -0.5, idx)
         check(out, want, bar)
+
+
+@pytest.mark.parametrize("page,new,kv", [(16, 1, 1000), (16, 3, 20000), (64, 70, 1000), (16, 70, 1000), (64, 70, 20000)])
+@pytest.mark.parametrize("gap", [12.0, 16.0, 18.0])
+def test_float16_weights_far_below_the_largest(gap, page, new, kv):
+    # One key, with a value of zero, takes nearly all of the weight; the output is what the many others, `gap`
+    # below it, add up to.  Each of their weights w = exp(-gap) times the largest is rounded to 16 bits after a
+    # factor of 2^7: by 2^-11 of it where it stays normal (2^-14 and above), by 2^-25 / 2^7 below.
+    Hkv, D = 2, 64
+    gen = torch.Generator(device=DEV).manual_seed(new)
+    table, starts, lens, total = make_batch(2, [new], [kv], page)
+    kp, vp = make_cache(gen, total, Hkv, page, D, torch.float16)
+    kp.zero_()
+    vp.copy_((1 + 0.25 * torch.rand(vp.shape, generator=gen, device=DEV)).half())
+    at = 3
+    kp[int(table[0, at // page]), :, at % page, 0] = gap
+    vp[int(table[0, at // page]), :, at % page] = 0
+    q = torch.zeros(new, 8, D, device=DEV, dtype=torch.float16)
+    q[..., 0] = 1.0
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, 1.0).double()
+    keys = torch.arange(kv, device=DEV)
+    v = vp[table[0].long()[keys // page], :, keys % page].double()                  # [kv, Hkv, D]
+    w = torch.exp(torch.tensor(-gap, dtype=torch.float64)).item()
+    each = max(2.0 ** -11, 2.0 ** -32 / w) if w * 2 ** 7 < 2.0 ** -14 else 2.0 ** -11
+    sums = v.cumsum(0)
+    for i in range(new):
+        n = kv - new + i + 1
+        want = (w * sums[n - 1] / (1 + w * (n - 1))).repeat_interleave(4, 0)
+        # the weights; the output's rounding; 32-bit sums of positive terms (as in the file's bar, 4 e)
+        bar = want * (each + 2.0 ** -11 + 4 * (2.0 ** -24 * (D + 4) * gap + 2.0 ** -21)) + 2.0 ** -25
+        assert bool(((got[i] - want).abs() <= bar).all()), (i, float(((got[i] - want).abs() / bar).max()))
