@@ -101,7 +101,8 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
   SPRUCE_REQUIRE(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq < 1 << 16,
                  "query heads (%lld) must be divisible by KV heads (%lld)", (long long)Hq, (long long)Hkv);
   SPRUCE_REQUIRE(Hq / Hkv <= 64, "at most 64 query heads per KV head are supported");
-  SPRUCE_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
+  const float cs = scale * 1.4426950408889634f;  // of exp2
+  SPRUCE_REQUIRE(scale > 0.f && cs < INFINITY, "scale must be positive, and finite times log2(e)");
   SPRUCE_REQUIRE(a.qs[2] == 1 && a.kps[3] == 1 && a.vps[3] == 1 && a.os[2] == 1,
                  "q, the pages and out must have a contiguous final dimension");
   PagedAttn p{};
@@ -145,7 +146,7 @@ extern "C" int spruce_paged_attention(const spruce_paged_attention_args* args, v
   p.by_heads = divisor(Hkv);
   p.by_group = divisor(Hq / Hkv);
   p.G = (int)(Hq / Hkv);
-  p.cs = scale * 1.4426950408889634f;
+  p.cs = cs;
   if (K > 0) {
     p.idx = a.idx;
     for (int i = 0; i < 3; ++i) p.is[i] = a.is[i];

@@ -316,3 +316,13 @@ def test_single_tokens_beside_a_large_chunk_are_shared_out(N, S, lists):
     Hq, Hkv, D = 32, 8, 128
     got = spruce_hip.lib().spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D, 131072, lists)
     assert got >= 2 * 256 * 32 * (D + 2) * 4
+
+
+def test_scales_whose_product_leaves_32_bits_are_refused():
+    # exp(scale x) is formed as exp2(scale log2(e) x): an infinite factor would make NaN of a score of zero.
+    need = spruce_hip.lib().spruce_paged_attention_workspace_bytes(8, 2, 4, 2, 128, 64, 0)
+    for scale, N, want in ((2.5e38, 8, -1), (3.4e38, 8, -1), (1e39, 8, -1), (1e-50, 8, -1), (2.3e38, 0, 0), (1e-30, 0, 0)):
+        assert _call("spruce_paged_attention", paged._ATTENTION_ARGS, (
+            FAKE, 512, 128, 1, FAKE, 4096, 2048, 128, 1, FAKE, 4096, 2048, 128, 1, 9, 16, FAKE, 4, 4, FAKE, FAKE, 2, N,
+            4, 2, 128, 0, scale, 0, 1, 1, 1, 1, 1, 0, FAKE, 512, 128, 1, FAKE, need)) == want, scale
+        assert want == 0 or "scale must be positive" in spruce_hip.last_error()
