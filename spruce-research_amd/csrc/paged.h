@@ -90,13 +90,8 @@ inline bool rows_apart(const int64_t* strides, const int64_t* sizes, int n, int6
 
 __device__ __forceinline__ int page_of(const PagedBatch& b, int pos) { return b.by_page.of(pos); }
 
-// q_starts[s] and kv_lens[s] brought into range.
+// q_starts[s] brought into range.
 __device__ __forceinline__ int clamp_start(const PagedBatch& b, int v) { return v < 0 ? 0 : (v > b.N ? b.N : v); }
-__device__ __forceinline__ int start_at(const PagedBatch& b, int s) { return clamp_start(b, b.q_starts[s]); }
-__device__ __forceinline__ int keys_of(const PagedBatch& b, int s) {
-  const int v = b.kv_lens[s];
-  return v < 0 ? 0 : (v > b.cap ? b.cap : v);
-}
 
 // The table's entry for position pos (0 <= pos < cap) of sequence s, and
 // whether it names a page: apart, so that a caller can look entries up ahead
