@@ -26,15 +26,16 @@
 // shares the line out evenly, whatever the lengths are; tiles cut by a border
 // are joined by a second kernel, in the line's order, so results do not depend
 // on timing.  (Equal parts of each sequence instead: 64 sequences of 6 to 32
-// thousand keys 587 us rather than 511 at that stage.)
+// thousand keys 590 us rather than 512 at that stage.)
 //
 // Measured on one MI355X (bf16 but for the drafts, heads of 128 but for theirs):
 //   one token of each of 64 sequences of 6554 to 32768 keys, 28/4 heads, pages of 16: 440 us, 5.87 TB/s
 //   four drafted tokens of each of 16 sequences of 1800 to 9001 keys, 16/8 heads of 64: 44 us, 4.3 TB/s
 //   one token over 517 keys, 8/2 heads: 12 us
-//   512 tokens over 33000 keys, 28/4 heads: 252 us, 954 TFLOP/s
-//   4096 tokens over 32768 keys, 32/8 heads: 1903 us, 1080 TFLOP/s
-//   2048 tokens over 64 listed blocks each, 28/4 heads: 139 us, 858 TFLOP/s
+//   512 tokens over 33000 keys, 28/4 heads: 260 us, 925 TFLOP/s
+//   4096 tokens over 32768 keys, 32/8 heads: 1922 us, 1070 TFLOP/s (pages of 128; of 16 6% longer)
+//   2048 tokens over 64 listed blocks each, 28/4 heads: 141 us, 847 TFLOP/s
+//   one token of each of 64 sequences over 64 listed blocks, 28/4 heads: 116 us
 #pragma once
 
 #include "attention_impl.h"

@@ -19,8 +19,8 @@
 // every pair are in the lane.  The rows of four passes (two of float32) are in
 // flight before the look-ups (sequence, position, page) and the sines begin.
 //
-// Measured on one MI355X: 32768 tokens of 28 + 4 heads of 128, normed, bf16, 102 us
-// (5.26 TB/s); the append of 16384 tokens of 32 + 8 + 8 heads 78 us (5.14 TB/s); 8170
+// Measured on one MI355X: 32768 tokens of 28 + 4 heads of 128, normed, bf16, 103 us
+// (5.23 TB/s); the append of 16384 tokens of 32 + 8 + 8 heads 80 us (5.05 TB/s), 162 in float32; 8170
 // tokens of 16 + 8 heads of 64 in float32, interleaved, 25 us (4.0 TB/s); one token of each of
 // 64 sequences 4.9 us of kernel.  (Weights kept in LDS instead of registers: 119 us for 114.)
 #include "paged.h"

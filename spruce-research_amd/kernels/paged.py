@@ -76,7 +76,8 @@ def append_paged_kv(k, v, k_pages, v_pages, page_table, q_starts, kv_lens, *, qu
     are normed and rotated in the same launch and returned as a new tensor
     (rows of no sequence in it are unspecified); None otherwise.  A token without a
     page is not written.  Two tokens must not share a slot: which of them it then
-    holds is unspecified.
+    holds is unspecified.  bf16, f16 or f32; float32 pages are for a caller's own
+    use, ``paged_chunk_attention`` takes the 16-bit types.
     """
     device, dtype = k.device, k.dtype
     if k.dim() != 3 or k.shape != v.shape or v.dtype != dtype or v.device != device:
