@@ -445,6 +445,12 @@ __device__ __forceinline__ int part_at(int row, int d) {
 template <bool F16>
 constexpr float kLift = F16 ? 7.f : 0.f;
 
+// fmaf(s, cs, -m cs) is off by the rounding of m cs alone, for all of a row
+// alike: nothing, until half a step of it leaves the weights' range.  A unit whose
+// maximum reaches this size is done again like one with sums that are not
+// finite; there m is taken off first.
+constexpr float kLargeScore = 0x1p+22f;
+
 // x combined over the lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float quad_max(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x),
@@ -477,7 +483,7 @@ constexpr int kFewKeys = 32;  // keys of a wave's tile
 template <int D>
 constexpr int few_lds_bytes() {
   // Every wave's V rows, or later its O rows, 16 at a time; then the waves'
-  // maxima and sums, and which of the waves has a sum that is not finite.
+  // maxima and sums, and which of the waves has a unit to do again.
   static_assert(16 * (D + 4) * 4 <= kFewKeys * (D + 8) * 2, "a wave's O rows must fit its V rows");
   return kWaves * (kFewKeys * (D + 8) * 2 + 2 * 32 * 4 + 4);
 }
@@ -497,7 +503,8 @@ constexpr int many_lds_bytes() {
 // us where 32 took 55.2 (four drafted tokens of 16 sequences).
 //
 // A masked key has p = 0, but 0 times a NaN or infinity in its value row is
-// NaN.  Where sums come out non-finite nothing is written and the result is
+// NaN.  Where sums come out non-finite, or a maximum is of a size that the usual
+// exponent does not hold (kLargeScore), nothing is written and the result is
 // true: the unit is then done again, CAREFUL, with the partly masked tiles
 // taken one column at a time.
 template <int D, bool F16, bool CAREFUL>
@@ -565,7 +572,8 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
     wave_lds_fence();
   };
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m: of the scores as products, before cs
+  const float threshold = fminf(kRescaleThreshold / p.cs, 0x1.fffffep+127f);  // -inf's distance is past it
   f32x4v acc[2][DT];
   // Zeros that are no constant: constant ones are kept in registers, or worse,
   // for every later use of a zero.
@@ -640,16 +648,22 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
         float mx = s[c][0][0];
 #pragma unroll
         for (int i = 1; i < 4 * KT; ++i) mx = fmaxf(mx, s[c][i >> 2][i & 3]);
-        mx = quad_max(mx) * p.cs;
-        if (__ballot(mx > m[c] + kRescaleThreshold)) {
+        mx = quad_max(mx);
+        if (__ballot(mx - m[c] > threshold)) {
           const float mn = fmaxf(m[c], mx);
-          const float alpha = mn == -INFINITY ? 1.f : fast_exp2(m[c] - mn);
+          const float alpha = mn == -INFINITY ? 1.f : fast_exp2((m[c] - mn) * p.cs);
           m[c] = mn;
           l[c] *= alpha;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) acc[c][dt] *= alpha;
         }
-        const float nm = m[c] == -INFINITY ? 0.f : kLift<F16> - m[c];
+        float nm = m[c] == -INFINITY ? 0.f : fmaf(-m[c], p.cs, kLift<F16>);
+        if constexpr (CAREFUL) {
+          const float off = m[c] == -INFINITY ? 0.f : m[c];
+#pragma unroll
+          for (int i = 0; i < 4 * KT; ++i) s[c][i >> 2][i & 3] -= off;
+          nm = kLift<F16>;
+        }
 #pragma unroll
         for (int h2 = 0; h2 < KH; ++h2) {
           float x[8];
@@ -731,6 +745,8 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
   if constexpr (!CAREFUL) {
     bool odd = false;
 #pragma unroll
+    for (int c = 0; c < 2; ++c) odd |= m[c] != -INFINITY && !(fabsf(m[c] * p.cs) < kLargeScore);
+#pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -742,7 +758,7 @@ __device__ __forceinline__ bool few_rows(uintptr_t args, const Unit& u, const Pa
   for (int c = 0; c < 2; ++c) {
     l[c] = quad_sum(l[c]);
     if (g4 == 0) {
-      ml[wave * 64 + 16 * c + l16] = m[c];
+      ml[wave * 64 + 16 * c + l16] = m[c] * p.cs;
       ml[wave * 64 + 32 + 16 * c + l16] = l[c];
     }
   }
@@ -900,7 +916,8 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
     }
   };
 
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f;  // m: of the scores as products, before cs
+  const float threshold = fminf(kRescaleThreshold / p.cs, 0x1.fffffep+127f);  // -inf's distance is past it
   f32x16_t acc[DT];
   uint4 pk[2][2];
   auto scores = [&](const uint16_t* ks, f32x16_t& s0, f32x16_t& s1) {
@@ -942,10 +959,10 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
     for (int r = 2; r < 16; ++r) mx = fmaxf(mx, s0[r]);
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s1[r]);
-    mx = half_max(mx) * p.cs;
-    if (__ballot(mx > m + kRescaleThreshold) != 0) {
+    mx = half_max(mx);
+    if (__ballot(mx - m > threshold) != 0) {
       const float mn = fmaxf(m, mx);
-      const float alpha = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+      const float alpha = mn == -INFINITY ? 1.f : fast_exp2((m - mn) * p.cs);
       m = mn;
       l *= alpha;
 #pragma unroll
@@ -953,7 +970,16 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[dt][r] *= alpha;
     }
-    const float nm = m == -INFINITY ? 0.f : kLift<F16> - m;
+    float nm = m == -INFINITY ? 0.f : fmaf(-m, p.cs, kLift<F16>);
+    if constexpr (CAREFUL) {
+      const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s0[r] -= off;
+        s1[r] -= off;
+      }
+      nm = kLift<F16>;
+    }
     float sum = 0.f;
 #pragma unroll
     for (int h2 = 0; h2 < 2; ++h2) {
@@ -1090,7 +1116,7 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
     }
   }
   if constexpr (!CAREFUL) {
-    bool odd = false;
+    bool odd = m != -INFINITY && !(fabsf(m * p.cs) < kLargeScore);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -1114,7 +1140,7 @@ __device__ __forceinline__ bool many_rows(uintptr_t args, const Unit& u, const P
         *reinterpret_cast<float4*>(po + (dt * 4 + j) * 256) =
             float4{acc[dt][4 * j], acc[dt][4 * j + 1], acc[dt][4 * j + 2], acc[dt][4 * j + 3]};
     if (hl == 0) {
-      pe.part_ml[group * 64 + l32] = m;
+      pe.part_ml[group * 64 + l32] = m * pe.cs;
       pe.part_ml[group * 64 + 32 + l32] = l;
     }
     return false;

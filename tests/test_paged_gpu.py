@@ -607,3 +607,37 @@ def test_float16_weights_far_below_the_largest(gap, page, new, kv):
         # the weights; the output's rounding; 32-bit sums of positive terms (as in the file's bar, 4 e)
         bar = want * (each + 2.0 ** -11 + 4 * (2.0 ** -24 * (D + 4) * gap + 2.0 ** -21)) + 2.0 ** -25
         assert bool(((got[i] - want).abs() <= bar).all()), (i, float(((got[i] - want).abs() / bar).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,new,kv", [(16, 3, 300), (16, 3, 3000), (64, 70, 900), (16, 70, 900), (64, 70, 3000)])
+@pytest.mark.parametrize("size", [2.0 ** 8, 2.0 ** 9, 2.0 ** 10, 2.0 ** 14])
+def test_scores_whose_own_rounding_is_large(size, page, new, kv, dtype):
+    # Scores of some size^2 D, whose steps in 32 bits are up to 4096: a row is the value of its largest score where
+    # that stands alone by more than the products' own error, 2^-24 (D + 4) of it, and some mean of values in any case.
+    Hkv, D = 2, 128
+    gen = torch.Generator(device=DEV).manual_seed(kv)
+    table, starts, lens, total = make_batch(2, [new], [kv], page)
+    kp, vp = make_cache(gen, total, Hkv, page, D, dtype)
+    near = torch.rand(kp.shape, generator=gen, device=DEV) * 2.0 ** -9
+    kp.copy_((size * (1 + near)).to(dtype))
+    q = (size * (1 + torch.rand(new, 8, D, generator=gen, device=DEV))).to(dtype)
+    got = paged_chunk_attention(q, kp, vp, table, starts, lens, 1.0).double()
+    keys = torch.arange(kv, device=DEV)
+    ids, at = table[0].long()[keys // page], keys % page
+    k, v = (x[ids, :, at].double().repeat_interleave(4, 1) for x in (kp, vp))          # [kv, 8, D]
+    alone = 0
+    for i in range(new):
+        n = kv - new + i + 1
+        score = (q[i].double() * k[:n]).sum(-1)                                           # [n, 8]
+        top, where = score.max(0)
+        gap = top - score.scatter(0, where[None], -torch.inf).max(0).values
+        low, high = v[:n].amin(0), v[:n].amax(0)
+        half = torch.finfo(dtype).eps / 2
+        slack = 3 * half * v[:n].abs().amax(0) + 2.0 ** -25
+        assert bool(((got[i] >= low - slack) & (got[i] <= high + slack)).all()), i
+        one = gap > 4 * 2.0 ** -24 * (D + 4) * top + 40
+        alone += int(one.sum())
+        want = v[where, torch.arange(8, device=DEV)]
+        assert bool(((got[i] - want).abs() <= 3 * half * want.abs() + 2.0 ** -25)[one].all()), i
+    print(f"{alone} of {8 * new} rows of one key", flush=True)
