@@ -803,7 +803,8 @@ int spruce_paged_append(const spruce_paged_append_args* args, void* stream);
  * without a slot get no weight; what masked keys and values hold, NaN
  * included, reaches no row.  Rows of no sequence are left alone.
  *   q, out [N, Hq, D] (strides qs, os), bf16 / f16, D in {64, 128}, at most 64
- *   query heads per KV head, scale > 0; rows 16-byte aligned.
+ *   query heads per KV head, scale > 0 (and below 2^128 / log2(e)); rows
+ *   16-byte aligned.
  *   workspace: spruce_paged_attention_workspace_bytes(N, S, Hq, Hkv, D,
  *   table_width * page_size, K) bytes, 16-byte aligned, one call's own until it is done (long rows are
  *   split over workgroups and joined from there).
