@@ -835,6 +835,108 @@ typedef struct spruce_paged_attention_args {
 } spruce_paged_attention_args;
 int spruce_paged_attention(const spruce_paged_attention_args* args, void* stream);
 
+/*
+ * The attention weight that the cached keys get from the new tokens:
+ *   mass_j = sum over new tokens n at positions p >= j and query heads h of j's KV head of
+ *            softmax_j(scale * q_nh . k_j)
+ * written to mass_pages [pages, Hkv, page_size] float32 (strides mps, any in which no
+ * two values share memory), the slots of positions below kv_lens[s] of every sequence with new
+ * tokens.  With accumulate the weight is added to what the slot of a position before the new
+ * tokens holds; the new tokens' own slots are set.  Keys without a slot get no
+ * weight, what masked keys hold reaches no sum.  Sequences that share a page
+ * leave either's masses there.  Other arguments as for spruce_paged_attention;
+ * scale >= 2^-100.
+ *   workspace: spruce_paged_key_mass_workspace_bytes(N, S, Hq, Hkv,
+ *   table_width * page_size) bytes, 16-byte aligned, one call's own until it is done.
+ */
+int64_t spruce_paged_key_mass_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys);
+typedef struct spruce_paged_key_mass_args {
+  const void* q;
+  int64_t qs[3];
+  const void* k_pages;
+  int64_t kps[4];
+  float* mass_pages;
+  int64_t mps[3];
+  int64_t pages, page_size;
+  const int32_t* page_table;
+  int64_t table_stride, table_width;
+  const int32_t* q_starts;
+  const int32_t* kv_lens;
+  int64_t S, N, Hq, Hkv, D, dtype;
+  double scale;
+  int64_t accumulate;
+  void* workspace;
+  int64_t workspace_bytes;
+} spruce_paged_key_mass_args;
+int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, void* stream);
+
+/*
+ * Of every sequence's cached positions 0 .. kv_lens[s] - 1, per KV head, those
+ * with the largest masses: the first `first`, the last `recent`, and of those between as many
+ * of the largest (ties to the lowest position; NaN and positions without a
+ * slot count as -inf) as make `keep` together; all where there are no more than
+ * keep.  kept [S, Hkv, keep] int32 gets the kept positions in ascending order, -1
+ * behind them, new_lens [S] int32 their number, and the keys, values and masses of
+ * the r-th go to slot r % page_size of page out_table[s][r / page_size]
+ * (int32 [S, out_width], rows out_stride apart) of the same buffers.  The pages that
+ * out_table names must not be among those still to be read; a row may go to where it
+ * is.  A row whose page or whose place is none does not move.
+ *   k_pages, v_pages [pages, Hkv, page_size, D] (bf16 / f16 / f32, D in {64, 128},
+ *   rows 16-byte aligned), mass_pages [pages, Hkv, page_size] float32, of any
+ *   strides in which no two rows share memory.
+ */
+typedef struct spruce_paged_evict_args {
+  void* k_pages;
+  int64_t kps[4];
+  void* v_pages;
+  int64_t vps[4];
+  float* mass_pages;
+  int64_t mps[3];
+  int64_t pages, page_size;
+  const int32_t* page_table;
+  int64_t table_stride, table_width;
+  const int32_t* kv_lens;
+  int64_t S, Hkv, D, dtype;
+  const int32_t* out_table;
+  int64_t out_stride, out_width;
+  int64_t keep, first, recent;
+  int32_t* kept;
+  int32_t* new_lens;
+} spruce_paged_evict_args;
+int spruce_paged_evict(const spruce_paged_evict_args* args, void* stream);
+
+/*
+ * One token a row of logits x [B, V] (bf16 / f16 / f32, rows `stride` elements
+ * apart), given a random number u in [0, 1) a row (float32, or float64 with uniform64):
+ *   w_i = exp((x_i - max x) / temperature);
+ *   kept, in the order of x descending, ties by index ascending: the shortest of the
+ *   first top_k (0: all), the fewest of those whose weights reach top_p of all of
+ *   theirs (1: all), and those with w_i >= min_p;
+ *   tokens[b] = the first i, by index, with sum_{kept j <= i} w_j > u sum_{kept} w_j,
+ * and logprobs[b] (unless NULL) = log of w_i over the sum of the kept.  Temperature 0
+ * (or what is not above it): the first of the largest logits.  NaN logits count as -inf, which
+ * has no weight; among +inf logits all others have none.  A row of nothing but -inf
+ * gets token -1 and -inf.  Weights are formed in 64 bits and added as multiples of
+ * a unit of the largest, 2^-52 or the smallest power of two of which V stay within 2^63.  The four settings come one for all rows (temperature1, ..) or,
+ * where the pointers are given, one a row [B].  V <= 2088960.
+ */
+typedef struct spruce_sample_tokens_args {
+  const void* logits;
+  int64_t stride, B, V, dtype;
+  const void* uniform;
+  int64_t uniform64;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  double temperature1;
+  int64_t top_k1;
+  double top_p1, min_p1;
+  int64_t* tokens;
+  float* logprobs;
+} spruce_sample_tokens_args;
+int spruce_sample_tokens(const spruce_sample_tokens_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

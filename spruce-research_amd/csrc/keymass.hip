@@ -1,0 +1,502 @@
+// The attention weight that the cached keys of a paged K/V cache get from a
+// ragged batch's new tokens:
+//   mass_j (+)= sum over tokens i, heads h of a KV head, of exp(scale q_ih.k_j - lse_ih),
+//   lse_ih = log sum_{j <= pos_i} exp(scale q_ih.k_j).
+// A weight needs the sum over its row's keys and a mass the sum over its key's
+// rows, so there are two passes over the scores, each with one side held in
+// registers and the other streamed through LDS:
+//   rows  256 packed rows (as in the paged attention: token by token, head by
+//         head) against a range of keys: every lane has one row's maximum and
+//         sum over its part of the keys, which go to the workspace;
+//   keys  256 keys against the rows that see them: every lane has one key's sum.
+// Both are S = A B^T on the matrix cores with the streamed side as A, so what is
+// held lies in the columns, one a lane, and sums stay within the lane.
+#include "paged_impl.h"
+
+namespace spruce {
+
+struct KeyMass {
+  PagedAttn a;     // q, k, the batch; every sequence goes the many-row way
+  float* mass;
+  int64_t ms[3];   // page, head, slot strides
+  float2* stats;   // [N * Hq][parts]: maximum (of scores as products) and sum
+  int Hq, parts, accumulate;
+};
+
+namespace {
+
+constexpr int kRowsOf = Many::rows;   // rows, or keys, that a workgroup of 4 waves holds
+constexpr int kWave = 64;             // of which a wave
+constexpr int kStream = 64;           // rows, or keys, streamed between barriers
+
+// Scores enter the exponential as differences to the row's reference, which the
+// matrix cores take off as they accumulate: one product and one exponential an
+// element.  The difference is then as exact as a 32-bit score of the reference's
+// size; where that is large (times scale log2 e) it is formed from the finished
+// score instead, so that the largest weight of a row is one whatever the scores.
+constexpr float kLargeReference = 0x1p+10f;
+// A tile's sum past this moves the reference.
+constexpr float kRescaleSum = 0x1p+60f;
+
+// Rows (or keys) streamed: [kStream][D + 8] 16-bit elements.
+template <int D>
+struct Stream {
+  static constexpr int stride = D + 8, lanes = D / 8, rows = 256 / lanes, passes = kStream / rows;
+};
+
+// S^T's 32 x 64 block: streamed rows a (LDS), held columns b.
+template <int D, bool F16>
+__device__ __forceinline__ void products(const uint16_t* rows, const u32x4 (&b)[2][D / 16], int lane, f32x16_t& x0,
+                                         f32x16_t& x1) {
+  const uint16_t* at = rows + (lane & 31) * Stream<D>::stride + 8 * (lane >> 5);
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    const uint4 a = *reinterpret_cast<const uint4*>(at + 16 * kk);
+    x0 = mfma32x32x16<F16>(a, __builtin_bit_cast(uint4, b[0][kk]), x0);
+    x1 = mfma32x32x16<F16>(a, __builtin_bit_cast(uint4, b[1][kk]), x1);
+  }
+}
+
+// The streamed row of accumulator register r, within 32.
+__device__ __forceinline__ int row_of(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
+
+// One column's running sum of exp2(cs (s - m)); l is 0 until m is set.
+struct Sum {
+  float m = 0.f, l = 0.f;
+  // x: scores less m.
+  __device__ __forceinline__ void add(const f32x16_t& x, float cs) {
+    float t = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t += fast_exp2(x[r] * cs);
+    if (__ballot(l == 0.f || !(t < kRescaleSum))) {
+      float mx = x[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
+      if (mx > -INFINITY && (l == 0.f || !(t < kRescaleSum))) {
+        l *= l == 0.f ? 0.f : fast_exp2(-mx * cs);
+        m += mx;
+        t = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t += fast_exp2((x[r] - mx) * cs);
+      }
+    }
+    l += t;
+  }
+  // s: the scores.
+  __device__ __forceinline__ void add_large(const f32x16_t& s, float cs) {
+    float mx = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    if (mx == -INFINITY) return;
+    const float now = l == 0.f ? mx : fmaxf(m, mx);
+    float t = l == 0.f ? 0.f : l * fast_exp2((m - now) * cs);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t += fast_exp2((s[r] - now) * cs);
+    m = now;
+    l = t;
+  }
+  __device__ __forceinline__ void join(float m2, float l2, float cs) {
+    if (l2 == 0.f) return;
+    if (l == 0.f) {
+      m = m2;
+      l = l2;
+      return;
+    }
+    const float now = fmaxf(m, m2);
+    l = l * fast_exp2((m - now) * cs) + l2 * fast_exp2((m2 - now) * cs);
+    m = now;
+  }
+};
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256, 2) void key_mass_rows_kernel(const KeyMass a) {
+  typedef Stream<D> ST;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][kStream * ST::stride];
+  __shared__ int paged[2][kStream];
+  const PagedAttn& p = a.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int l32 = lane & 31, hl = lane >> 5;
+  const uint32_t block = flat_block();
+  const int g = (int)(block % (uint32_t)p.Hkv);
+  const uint32_t rest = block / (uint32_t)p.Hkv;
+  const int part = (int)(rest % (uint32_t)a.parts), at = (int)(rest / (uint32_t)a.parts);
+  Unit u;
+  if (!find_tile<Many>(p, at, g, lane, u)) return;
+  const TileRows tr = tile_rows(p, u);
+  if (tr.rows == 0) return;
+
+  // This lane's two columns.
+  const int mine = uniform(tr.rows - kWave * wave);  // rows of this wave, if positive
+  u32x4 held[2][D / 16];
+  int qpos[2];
+  int64_t out[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int i = kWave * wave + 32 * c + l32;
+    const int r = tr.row0 + (i < tr.rows ? i : tr.rows - 1);
+    const int t = p.by_group.of(r), h = g * p.G + r - t * p.G;
+    qpos[c] = clip(u.w.pos0 + t);
+    out[c] = (int64_t)(u.w.start + t) * a.Hq + h;
+    const uint16_t* src =
+        static_cast<const uint16_t*>(p.q) + (int64_t)(u.w.start + t) * p.qs[0] + (int64_t)h * p.qs[1] + 8 * hl;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) held[c][kk] = load16(src + 16 * kk);
+  }
+  const int first_pos = uniform(clip(u.w.pos0 + p.by_group.of(tr.row0 + (mine > 0 ? kWave * wave : 0))));
+
+  const int tiles = (tr.end + kStream - 1) / kStream, per = (tiles + a.parts - 1) / a.parts;
+  const int t0 = part * per < tiles ? part * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
+  const int lr = tid / ST::lanes, lc = tid % ST::lanes;
+  const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)g * p.ks[1] + 8 * lc;
+  int entry[ST::passes];
+  u32x4 row[ST::passes];
+  int there[ST::passes];
+  auto look_up = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < ST::passes; ++i)
+      entry[i] = page_entry(p.batch, u.s, nearest(tile * kStream + i * ST::rows + lr, tr.end));
+  };
+  auto load = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < ST::passes; ++i) {
+      const int key = tile * kStream + i * ST::rows + lr, in = nearest(key, tr.end);
+      const int slot = in - page_of(p.batch, in) * p.batch.page;
+      const bool ok = is_page(p.batch, entry[i]);
+      there[i] = ok && key < tr.end;
+      row[i] = load16(kbase + (int64_t)(ok ? entry[i] : 0) * p.ks[0] + (int64_t)slot * p.ks[2]);
+    }
+  };
+  Sum sum[2];
+  if (t0 < t1) {
+    look_up(t0);
+    load(t0);
+    if (t0 + 1 < t1) look_up(t0 + 1);
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int b = t & 1;
+#pragma unroll
+    for (int i = 0; i < ST::passes; ++i) {
+      *reinterpret_cast<u32x4*>(&lds[b][(i * ST::rows + lr) * ST::stride + 8 * lc]) = row[i];
+      if (lc == 0) paged[b][i * ST::rows + lr] = there[i];
+    }
+    __syncthreads();
+    if (t + 1 < t1) {
+      load(t + 1);
+      if (t + 2 < t1) look_up(t + 2);
+    }
+    if (mine <= 0) continue;
+    const uint64_t have = __ballot(paged[b][lane] != 0);
+    const int key0 = t * kStream;
+    const bool masked = have != ~0ull || key0 + kStream - 1 > first_pos;
+    const bool large =
+        __ballot(fabsf(sum[0].m * p.cs) >= kLargeReference || fabsf(sum[1].m * p.cs) >= kLargeReference) != 0;
+#pragma unroll 1
+    for (int sub = 0; sub < kStream / 32; ++sub) {
+      f32x16_t x[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float from = large ? 0.f : -sum[c].m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[c][r] = from;
+      }
+      products<D, F16>(&lds[b][32 * sub * ST::stride], held, lane, x[0], x[1]);
+      if (masked) {
+        const uint32_t in = (uint32_t)(have >> (32 * sub));
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int k = row_of(r, lane);
+            if (!(in >> k & 1) || key0 + 32 * sub + k > qpos[c]) x[c][r] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (large)
+          sum[c].add_large(x[c], p.cs);
+        else
+          sum[c].add(x[c], p.cs);
+      }
+      // (A reference that has just become large: the next 64 keys go by it.)
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    float m0, m1, s0, s1;
+    half_swap(sum[c].m, m0, m1);
+    half_swap(sum[c].l, s0, s1);
+    Sum all;
+    all.join(m0, s0, p.cs);
+    all.join(m1, s1, p.cs);
+    if (hl == 0 && 32 * c + l32 < mine) a.stats[out[c] * a.parts + part] = float2{all.m, all.l};
+  }
+}
+
+// The at-th of the key tiles of all sequences with new tokens.
+struct KeyTile {
+  int s, tile, len, start, n;
+  int64_t pos0;
+};
+__device__ __forceinline__ bool find_keys(const PagedAttn& p, int64_t at, int lane, KeyTile& k) {
+  int64_t count = 0;
+  for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
+    const Lengths len = lengths_of(p, s0 + lane);
+    const int a = clamp_start(p.batch, len.starts), e = clamp_start(p.batch, len.ends);
+    int keys = len.keys < 0 ? 0 : (len.keys < p.batch.cap ? len.keys : p.batch.cap);
+    if (e <= a || p.batch.pages == 0) keys = 0;
+    const int64_t pc = count + wave_prefix((int64_t)((keys + kRowsOf - 1) / kRowsOf));
+    const uint64_t past = __ballot(pc > at);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      k.s = s0 + l;
+      k.len = __builtin_amdgcn_readlane(keys, l);
+      k.tile = uniform((int)(at - lane_of(pc, l))) + (k.len + kRowsOf - 1) / kRowsOf;
+      k.start = __builtin_amdgcn_readlane(a, l);
+      k.n = __builtin_amdgcn_readlane(e, l) - k.start;
+      k.pos0 = lane_of((int64_t)len.keys - ((int64_t)len.ends - len.starts) + ((int64_t)a - len.starts), l);
+      return true;
+    }
+    count = lane_of(pc, 63);
+  }
+  return false;
+}
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) {
+  typedef Stream<D> ST;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][kStream * ST::stride];
+  // Of the streamed rows: what to take off the scores, its parts, and the position.
+  __shared__ __attribute__((aligned(16))) float less[2][kStream], top[2][kStream], log_sum[2][kStream];
+  __shared__ int pos[2][kStream], large[2];
+  const PagedAttn& p = a.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int l32 = lane & 31, hl = lane >> 5;
+  const int lr = tid / ST::lanes, lc = tid % ST::lanes;
+  const float per_cs = 1.f / p.cs;
+  for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
+    const int64_t at = unit / p.Hkv;
+    const int g = (int)(unit - at * p.Hkv);
+    KeyTile k;
+    if (!find_keys(p, at, lane, k)) return;
+    const int key0 = k.tile * kRowsOf + kWave * wave;
+    u32x4 held[2][D / 16];
+    int key[2], entry[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      key[c] = key0 + 32 * c + l32;
+      const int in = nearest(key[c], k.len);
+      entry[c] = page_entry(p.batch, k.s, in);
+      const bool ok = is_page(p.batch, entry[c]);
+      const int slot = in - page_of(p.batch, in) * p.batch.page;
+      const uint16_t* src = static_cast<const uint16_t*>(p.k) + (int64_t)(ok ? entry[c] : 0) * p.ks[0] +
+                            (int64_t)g * p.ks[1] + (int64_t)slot * p.ks[2] + 8 * hl;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) held[c][kk] = load16(src + 16 * kk);
+      if (key[c] >= k.len) entry[c] = -1;
+    }
+    // Rows from the first that sees the tile's first key on.
+    const int64_t skip = (int64_t)k.tile * kRowsOf - k.pos0;
+    const int rows = k.n * p.G;
+    const int row0 = skip <= 0 ? 0 : (skip < k.n ? (int)skip * p.G : rows);
+    u32x4 row[ST::passes];
+    Sum stat;
+    int row_pos = -1;
+    auto load = [&](int r0) {
+#pragma unroll
+      for (int i = 0; i < ST::passes; ++i) {
+        const int r = nearest(r0 + i * ST::rows + lr, rows);
+        const int t = p.by_group.of(r), h = g * p.G + r - t * p.G;
+        row[i] = load16(static_cast<const uint16_t*>(p.q) + (int64_t)(k.start + t) * p.qs[0] + (int64_t)h * p.qs[1] +
+                        8 * lc);
+      }
+      stat = Sum();
+      row_pos = -1;
+      if (tid < kStream && r0 + tid < rows) {
+        const int t = p.by_group.of(r0 + tid), h = g * p.G + r0 + tid - t * p.G;
+        row_pos = clip(k.pos0 + t);
+        const float2* st = a.stats + ((int64_t)(k.start + t) * a.Hq + h) * a.parts;
+        for (int i = 0; i < a.parts; ++i) stat.join(st[i].x, st[i].y, p.cs);
+      }
+    };
+    float sum[2] = {0.f, 0.f};
+    if (row0 < rows) load(row0);
+    int b = 0;
+    for (int r0 = row0; r0 < rows; r0 += kStream, b ^= 1) {
+#pragma unroll
+      for (int i = 0; i < ST::passes; ++i)
+        *reinterpret_cast<u32x4*>(&lds[b][(i * ST::rows + lr) * ST::stride + 8 * lc]) = row[i];
+      if (tid < kStream) {  // one wave
+        // No key: nothing of it reaches a sum.
+        const float lg = stat.l == 0.f ? INFINITY : __builtin_amdgcn_logf(stat.l);
+        const float ref = stat.m + lg * per_cs;
+        less[b][tid] = -ref;
+        top[b][tid] = stat.m;
+        log_sum[b][tid] = lg;
+        pos[b][tid] = row_pos;
+        const uint64_t odd = __ballot(stat.l != 0.f && !(fabsf(ref * p.cs) < kLargeReference));
+        if (tid == 0) large[b] = odd != 0;
+      }
+      __syncthreads();
+      if (r0 + kStream < rows) load(r0 + kStream);
+      if (key0 >= k.len) continue;
+      // (Rows go up with their positions.)
+      const bool masked = uniform(pos[b][0]) < key0 + kWave - 1;
+      const bool is_large = uniform(large[b]) != 0;
+#pragma unroll 1
+      for (int sub = 0; sub < kStream / 32; ++sub) {
+        f32x16_t x[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4_t v = *reinterpret_cast<const f32x4_t*>(&less[b][32 * sub + 8 * i + 4 * hl]);
+          if (is_large) v = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[0][4 * i + j] = x[1][4 * i + j] = v[j];
+        }
+        products<D, F16>(&lds[b][32 * sub * ST::stride], held, lane, x[0], x[1]);
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at_pos = pos[b][32 * sub + row_of(r, lane)];
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              if (key[c] > at_pos) x[c][r] = -INFINITY;
+          }
+        }
+        if (is_large) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float m = top[b][32 * sub + row_of(r, lane)], lg = log_sum[b][32 * sub + row_of(r, lane)];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              // No weight is above one, whatever a score's last bits are.
+              const float e = (x[c][r] - m) * p.cs - lg;
+              sum[c] += fast_exp2(e > 0.f ? 0.f : e);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) sum[c] += fast_exp2(x[c][r] * p.cs);
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float v = half_sum(sum[c]);
+      if (hl == c && is_page(p.batch, entry[c])) {
+        const int slot = key[c] - page_of(p.batch, key[c]) * p.batch.page;
+        float* to = a.mass + (int64_t)entry[c] * a.ms[0] + (int64_t)g * a.ms[1] + (int64_t)slot * a.ms[2];
+        *to = a.accumulate && key[c] < k.pos0 ? *to + v : v;
+      }
+    }
+    __syncthreads();  // LDS is free
+  }
+}
+
+struct MassPlan {
+  int64_t tiles, parts;
+};
+// Row tiles that a batch can have, and the parts of the keys of each: four
+// workgroups a CU, of at least 256 keys.
+MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) {
+  const int64_t G = Hq / Hkv;
+  MassPlan plan;
+  plan.tiles = N * G / kRowsOf + (S < N ? S : N);
+  int64_t parts = 4 * kCus / (plan.tiles * Hkv > 0 ? plan.tiles * Hkv : 1);
+  const int64_t most = (keys + 255) / 256;
+  if (parts > most) parts = most;
+  if (parts > 64) parts = 64;
+  plan.parts = parts < 1 ? 1 : parts;
+  return plan;
+}
+
+}  // namespace
+}  // namespace spruce
+
+using namespace spruce;
+
+extern "C" int64_t spruce_paged_key_mass_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) {
+  if (N < 1 || S < 1 || Hkv < 1 || Hq < Hkv || N >= (int64_t)1 << 30 || S >= (int64_t)1 << 20 || Hq >= 1 << 16) return 0;
+  return N * Hq * mass_plan(N, S, Hq, Hkv, keys).parts * (int64_t)sizeof(float2);
+}
+
+extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, void* stream) {
+  SPRUCE_REQUIRE(args != nullptr, "args must be non-null");
+  const spruce_paged_key_mass_args& a = *args;
+  const int64_t N = a.N, S = a.S, Hq = a.Hq, Hkv = a.Hkv, D = a.D;
+  const int dtype = (int)a.dtype;
+  const float scale = (float)a.scale;
+  SPRUCE_REQUIRE(D == 64 || D == 128, "kernel supports head_dim 64 or 128, got %lld", (long long)D);
+  SPRUCE_REQUIRE(dtype == SPRUCE_DTYPE_BF16 || dtype == SPRUCE_DTYPE_F16,
+                 "the key mass takes bf16 or f16, got dtype code %d", dtype);
+  SPRUCE_REQUIRE(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq < 1 << 16,
+                 "query heads (%lld) must be divisible by KV heads (%lld)", (long long)Hq, (long long)Hkv);
+  SPRUCE_REQUIRE(Hq / Hkv <= 64, "at most 64 query heads per KV head are supported");
+  const float cs = scale * 1.4426950408889634f;  // of exp2
+  // (The logarithm of a sum over scale log2 e must be finite.)
+  SPRUCE_REQUIRE(scale >= 0x1p-100f && cs < INFINITY, "scale must be at least 2^-100, and finite times log2(e)");
+  SPRUCE_REQUIRE(a.qs[2] == 1 && a.kps[3] == 1, "q and the pages must have a contiguous final dimension");
+  KeyMass m{};
+  const int rc = prepare_batch(m.a.batch, a.page_table, a.table_stride, a.table_width, a.q_starts, a.kv_lens, S, N,
+                               a.page_size, a.pages);
+  if (rc) return rc;
+  if (N == 0 || a.pages == 0) return SPRUCE_OK;
+  SPRUCE_REQUIRE(a.q && a.k_pages && a.mass_pages, "q and the pages must be non-null device pointers");
+  auto rows16 = [](const void* ptr, const int64_t* s, int n) {
+    if (reinterpret_cast<uintptr_t>(ptr) % 16) return false;
+    for (int i = 0; i < n; ++i)
+      if (s[i] % 8) return false;
+    return true;
+  };
+  SPRUCE_REQUIRE(rows16(a.q, a.qs, 2) && rows16(a.k_pages, a.kps, 3),
+                 "q and the pages must be 16-byte aligned with strides that keep rows 16-byte aligned");
+  SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(a.mass_pages) % 4 == 0, "mass_pages must be 4-byte aligned");
+  const int64_t sizes[3] = {a.pages, Hkv, a.page_size};
+  SPRUCE_REQUIRE(rows_apart(a.mps, sizes, 3, 1), "the values of mass_pages overlap");
+  const MassPlan plan = mass_plan(N, S, Hq, Hkv, m.a.batch.cap);
+  const int64_t need = N * Hq * plan.parts * (int64_t)sizeof(float2);
+  SPRUCE_REQUIRE(a.workspace && a.workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
+                 (long long)a.workspace_bytes, (long long)need);
+  SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0, "workspace must be 16-byte aligned");
+  SPRUCE_REQUIRE(N * (Hq / Hkv) < (int64_t)1 << 28 && plan.tiles < (int64_t)1 << 23, "too many tokens for one call");
+  m.a.q = a.q;
+  m.a.k = a.k_pages;
+  m.a.qs[0] = a.qs[0];
+  m.a.qs[1] = a.qs[1];
+  for (int i = 0; i < 3; ++i) {
+    m.a.ks[i] = a.kps[i];
+    m.ms[i] = a.mps[i];
+  }
+  m.a.Hkv = (int)Hkv;
+  m.a.G = (int)(Hq / Hkv);
+  m.a.by_heads = divisor(Hkv);
+  m.a.by_group = divisor(Hq / Hkv);
+  m.a.cs = cs;
+  m.a.few_limit = -1;
+  m.mass = a.mass_pages;
+  m.stats = static_cast<float2*>(a.workspace);
+  m.Hq = (int)Hq;
+  m.parts = (int)plan.parts;
+  m.accumulate = a.accumulate != 0;
+  const hipStream_t st = (hipStream_t)stream;
+  const int64_t units = plan.tiles * plan.parts * Hkv;
+  SPRUCE_REQUIRE(units < (int64_t)1 << 31, "too many tokens for one call");
+  int64_t key_units = (int64_t)S * ((m.a.batch.cap + kRowsOf - 1) / kRowsOf) * Hkv;
+  if (key_units > 8 * kCus) key_units = 8 * kCus;  // each takes more than one where there are more
+  if (key_units < 1) return SPRUCE_OK;             // a table of no page
+#define SPRUCE_KEY_MASS(D_, F16_)                                                                              \
+  do {                                                                                                         \
+    hipLaunchKernelGGL((key_mass_rows_kernel<D_, F16_>), flat_grid(units), dim3(256), 0, st, m);               \
+    hipLaunchKernelGGL((key_mass_keys_kernel<D_, F16_>), dim3((unsigned)key_units), dim3(256), 0, st, m);      \
+  } while (0)
+  if (D == 128) {
+    if (dtype == SPRUCE_DTYPE_F16) SPRUCE_KEY_MASS(128, true);
+    else SPRUCE_KEY_MASS(128, false);
+  } else {
+    if (dtype == SPRUCE_DTYPE_F16) SPRUCE_KEY_MASS(64, true);
+    else SPRUCE_KEY_MASS(64, false);
+  }
+#undef SPRUCE_KEY_MASS
+  return check_launch("paged key mass");
+}

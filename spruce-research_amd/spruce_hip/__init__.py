@@ -112,6 +112,9 @@ _SIGNATURES = {
     "spruce_rotate_heads": [ctypes.c_char_p, _p],
     "spruce_paged_append": [ctypes.c_char_p, _p],
     "spruce_paged_attention": [ctypes.c_char_p, _p],
+    "spruce_paged_key_mass": [ctypes.c_char_p, _p],
+    "spruce_paged_evict": [ctypes.c_char_p, _p],
+    "spruce_sample_tokens": [ctypes.c_char_p, _p],
     "spruce_sparse_prefill_mask": [
         _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _p, _STRIDES, _i64,
         _i64, _i64, _i64, _i64, _i64, ctypes.c_float, ctypes.c_int, ctypes.c_int,
@@ -153,6 +156,8 @@ def lib():
         handle.spruce_select_flat_workspace_bytes.argtypes = [_i64, _i64, _i64, _i64]
         handle.spruce_paged_attention_workspace_bytes.restype = _i64
         handle.spruce_paged_attention_workspace_bytes.argtypes = [_i64] * 7
+        handle.spruce_paged_key_mass_workspace_bytes.restype = _i64
+        handle.spruce_paged_key_mass_workspace_bytes.argtypes = [_i64] * 5
         _lib = handle
     return _lib
 
