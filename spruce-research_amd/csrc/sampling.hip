@@ -11,10 +11,14 @@
 // exact and no order of additions, of atomics among them, changes a result.  What
 // lies below half a unit weighs nothing.
 //
-// One workgroup has a row: its largest logit (pass A); with top_k or top_p a
-// histogram of counts and weights over 2048 equal ranges of logits (pass B),
-// the range within which a prefix ends, its members sorted (pass C); then sums
-// of the kept weights per 512 logits in index order (pass D), and the draw.
+// One workgroup has a row.  Its first pass finds the largest logit.  What can be
+// kept is then mostly few logits: a second pass lists those above a bound
+// (of top_k, from the threads' own largest; of min_p; of top_p, from a
+// histogram of the weights that needs a pass of its own), and the ends of the
+// prefixes and the draw are found among them: each is the first entry of some
+// order whose running sum passes a target, which select() narrows down digit by digit.
+// Rows that keep more than the list holds go the long way: the end of a prefix
+// within one range of the histogram, then sums of 512 logits each, in index order.
 #include "paged_impl.h"
 
 namespace spruce {
@@ -41,16 +45,16 @@ namespace {
 
 constexpr int kThreads = 1024, kRowWaves = kThreads / 64;
 constexpr int kBins = 2048;
-constexpr int kList = 4096;        // candidates that are sorted in LDS
-constexpr int kChunk = 8;          // logits of a lane
-constexpr int kPart = 64 * kChunk; // logits of a wave, and of one sum of pass D
-constexpr int kParts = 4096;       // such sums
+constexpr int kList = 4096, kEach = kList / kThreads;
+constexpr int kChunk = 8;           // logits that a lane reads at once
+constexpr int kPart = 64 * kChunk;  // logits of one sum of the long way
+constexpr int kParts = 4096;        // such sums
 constexpr int kTable = 64;
 
 // A unit is the smallest power of two of which V weights of one stay within 2^63,
 // and 2^-52 at the least.
 constexpr int kMostUnitBits = 52;
-constexpr float kNothing = 54.f;  // below 2^-54 a weight is zero units
+constexpr double kNothing = 54.0;  // below 2^-54 a weight is zero units
 
 // A logit's bits as a number that goes up with it.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -61,11 +65,12 @@ __device__ __forceinline__ float unordered(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// Eight logits from virtual place `at` on: NaN, and what lies outside of the
-// row, as -inf.  Places count from the last 16-byte border at or before the row,
-// so that all but the row's two ends are read 16 bytes at a time.
+// A row's logits by place.  Places count from the last 16-byte border at or
+// before the row, so that all but its two ends are read 16 bytes at a time; what lies
+// outside of it, and NaN, are -inf.
 template <typename T>
 struct Row {
+  typedef struct { u32x4 v[T::bytes / 2]; } Raw;  // eight logits
   const char* base;
   int first, end;  // places of the row's logits
   __device__ __forceinline__ void init(const void* logits, int64_t element, int V) {
@@ -75,124 +80,190 @@ struct Row {
     base = reinterpret_cast<const char*>(p - p % 16);
   }
   __device__ __forceinline__ static float widen(uint32_t bits) { return unpack1<T::code == SPRUCE_DTYPE_F16>(bits); }
-  __device__ __forceinline__ float one(int at) const {
-    if constexpr (T::bytes == 4)
-      return reinterpret_cast<const float*>(base)[at];
-    else
-      return widen(reinterpret_cast<const uint16_t*>(base)[at]);
-  }
-  __device__ __forceinline__ void load(int at, float (&x)[kChunk]) const {
+  __device__ __forceinline__ Raw load(int at) const {
+    constexpr uint32_t kInf = T::bytes == 4 ? 0xff800000u : (T::code == SPRUCE_DTYPE_F16 ? 0xfc00fc00u : 0xff80ff80u);
+    Raw r;
+#pragma unroll
+    for (int i = 0; i < T::bytes / 2; ++i) r.v[i] = u32x4{kInf, kInf, kInf, kInf};
     if (at >= first && at + kChunk <= end) {
-      if constexpr (T::bytes == 4) {
-        const f32x4v a = *reinterpret_cast<const f32x4v*>(base + (int64_t)at * 4),
-                     b = *reinterpret_cast<const f32x4v*>(base + (int64_t)at * 4 + 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = a[i];
-          x[4 + i] = b[i];
-        }
-      } else {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(base + (int64_t)at * 2);
+      for (int i = 0; i < T::bytes / 2; ++i)
+        r.v[i] = *reinterpret_cast<const u32x4*>(base + (int64_t)at * T::bytes + 16 * i);
+    } else if (at + kChunk > first && at < end) {  // the row's two ends, a 32-bit word at a time
+#pragma unroll 1
+      for (int i = 0; i < kChunk; ++i) {
+        if (at + i < first || at + i >= end) continue;
+        const int word = i * T::bytes / 4;
+        uint32_t x, old = kInf;
+        if constexpr (T::bytes == 4) {
+          x = reinterpret_cast<const uint32_t*>(base)[at + i];
+        } else {
+          x = reinterpret_cast<const uint16_t*>(base)[at + i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[2 * i] = widen(a[i] & 0xffffu);
-          x[2 * i + 1] = widen(a[i] >> 16);
+          for (int j = 0; j < 4; ++j)
+            if (j == word) old = r.v[0][j];
+          x = i & 1 ? (old & 0xffffu) | x << 16 : (old & 0xffff0000u) | x;
         }
+#pragma unroll
+        for (int j = 0; j < 2 * T::bytes; ++j)
+          if (j == word) r.v[j >> 2][j & 3] = x;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i) x[i] = at + i >= first && at + i < end ? one(at + i) : -INFINITY;
     }
+    return r;
+  }
+  static __device__ __forceinline__ void decode(const Raw& r, float (&x)[kChunk]) {
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) x[i] = x[i] == x[i] ? x[i] : -INFINITY;
+    for (int i = 0; i < kChunk; ++i) {
+      float y;
+      if constexpr (T::bytes == 4) {
+        const uint32_t bits = r.v[i >> 2][i & 3];  // (a bit cast of the element itself reads element 0)
+        y = __builtin_bit_cast(float, bits);
+      } else
+        y = widen(i & 1 ? r.v[0][i >> 1] >> 16 : r.v[0][i >> 1] & 0xffffu);
+      // (The maximum of a number and NaN is the number.)
+      x[i] = fmaxf(y, -INFINITY);
+    }
   }
 };
 
-// exp2(y) for y <= 0 in units, by 2^(n / 64) from a table and a polynomial in the rest: |z| <=
-// ln 2 / 128, so that z^5 / 120 is below 2^-44.
+// exp((x - max) / T) = 2^(n / 64) e^z: n by adding what leaves no bits for a
+// fraction, the power from a table and n's upper bits, and a polynomial in z,
+// |z| <= ln 2 / 128, so that the next term, z^5 / 120, is below 2^-44.
 struct Weights {
-  double max, c2;
-  const double* table;
-  double shift;  // 2^52 units
-  __device__ __forceinline__ double exact(float x) const {
-    // The difference first: of the largest logit it is zero whatever c2 is.
-    const double y = fmax(((double)x - max) * c2, -64.0);
-    const double n = __builtin_rint(y * kTable);
-    const double z = fma(n, -1.0 / kTable, y) * 0.69314718055994530942;
-    const int k = (int)n;
-    const double e = fma(z, fma(z, fma(z, fma(z, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0);
-    return __builtin_ldexp(e * table[k & (kTable - 1)], k >> 6);
-  }
+  double max, inv, steps, lowest;  // 1 / T, 64 log2(e) / T, and the difference past which weights are nothing
+  double shift;                    // 2^52 units
+  const uint64_t* table;
+  // (-inf comes out below half a unit.)
   __device__ __forceinline__ double of(float x) const {
-    if (max == INFINITY) return x == INFINITY ? 1.0 : 0.0;
-    return exact(x);
+    // The difference first: of the largest logit it is zero whatever T is.
+    const double d = fmax((double)x - max, lowest);
+    constexpr double kWhole = 0x1.8p+52;
+    const double t = fma(d, steps, kWhole);
+    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+    const double z = fma(t - kWhole, -0.69314718055994530942 / kTable, d * inv);
+    const double e = fma(z, fma(z, fma(z, fma(z, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0);
+    return e * __builtin_bit_cast(double, table[n & (kTable - 1)] + ((uint64_t)(uint32_t)(n >> 6) << 52));
   }
   __device__ __forceinline__ uint64_t units(double w) const {
     // Rounded to units as it is added to what has one as its last bit.
     return __builtin_bit_cast(uint64_t, w + shift) - __builtin_bit_cast(uint64_t, shift);
   }
+  // Those of eight, kept where they are for the compiler: moved under the conditions
+  // of their use they follow one another, each with its chain's latency (a pass over 150016
+  // logits 55 us).
+  __device__ __forceinline__ void of8(const float (&x)[kChunk], double (&w)[kChunk]) const {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) w[i] = of(x[i]);
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) asm volatile("" : "+v"(w[i]));
+  }
 };
 
+struct Small {
+  uint64_t key, weight;
+};
+
+// The same in every lane: kept in scalar registers.
+__device__ __forceinline__ double uniform(double x) {
+  return __builtin_bit_cast(double, lane_of(__builtin_bit_cast(int64_t, x), 0));
+}
+__device__ __forceinline__ float uniform(float x) {
+  return __builtin_bit_cast(float, spruce::uniform(__builtin_bit_cast(int, x)));
+}
+
 struct Shared {
-  double table[kTable];
+  uint64_t table[kTable];
   uint64_t weight[kBins];
   uint32_t count[kBins];
   uint64_t list[kList];     // order << 32 | ~place
   uint64_t part[kParts];
+  Small small[64];
   uint64_t waves[kRowWaves];
-  uint32_t wave_count[kRowWaves];
   uint64_t result[4];
   uint32_t size, lo, hi;
+  float top, least;
+  int infinite;
 };
 
-// Prefix sums over the workgroup's threads of a and b (up to and with this
-// one's), and their totals.
-__device__ __forceinline__ void block_prefix(Shared& sh, uint64_t& a, uint32_t& b, uint64_t& total_a, uint32_t& total_b) {
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+// Sums of a over the threads up to and with this one, and their total.  Ends with a barrier to come.
+__device__ __forceinline__ uint64_t block_prefix(Shared& sh, uint64_t a, uint64_t& total) {
+  const int lane = threadIdx.x & 63, wave = spruce::uniform(threadIdx.x >> 6);
   a = (uint64_t)wave_prefix((int64_t)a);
-  b = (uint32_t)wave_prefix((int)b);
   __syncthreads();
-  if (lane == 63) {
-    sh.waves[wave] = a;
-    sh.wave_count[wave] = b;
-  }
+  if (lane == 63) sh.waves[wave] = a;
   __syncthreads();
-  uint64_t before_a = 0;
-  uint32_t before_b = 0;
-  total_a = total_b = 0;
+  uint64_t before = 0;
+  total = 0;
 #pragma unroll
   for (int w = 0; w < kRowWaves; ++w) {
-    const uint64_t wa = sh.waves[w];
-    const uint32_t wb = sh.wave_count[w];
-    if (w < wave) {
-      before_a += wa;
-      before_b += wb;
-    }
-    total_a += wa;
-    total_b += wb;
+    const uint64_t x = sh.waves[w];
+    if (w < wave) before += x;
+    total += x;
   }
-  a += before_a;
-  b += before_b;
+  return a + before;
 }
 
-// The list's first n entries, in descending order (zeros behind them).
-__device__ __forceinline__ void sort_list(Shared& sh, int n) {
-  int size = 2;
-  while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += kThreads) sh.list[i] = 0;
+// Of up to kEach entries a thread, all keys different and those of a weight within [lo, hi],
+// the one that comes first, in descending order of the keys, with a sum of weights
+// (its own included) above `target`: its key.  target must be below the sum of all.
+__device__ __forceinline__ uint64_t select(Shared& sh, const uint64_t (&key)[kEach], const uint64_t (&weight)[kEach],
+                                           uint64_t lo, uint64_t hi, uint64_t target) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = spruce::uniform(tid >> 6);
+  uint64_t before = 0;
   __syncthreads();
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-        const int i = 2 * t - (t & (j - 1));
-        const uint64_t a = sh.list[i], b = sh.list[i + j];
-        if ((a < b) == ((i & k) == 0)) {
-          sh.list[i] = b;
-          sh.list[i + j] = a;
-        }
-      }
-      __syncthreads();
+  while (true) {
+    // A digit of what is left: as many bits as there are threads.
+    const int bits = 64 - __builtin_clzll((hi - lo) | 1);
+    const int shift = bits > 10 ? bits - 10 : 0;
+    sh.weight[tid] = 0;
+    if (tid < 64) sh.part[tid] = 0;
+    if (tid == 0) sh.size = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (weight[i] && key[i] >= lo && key[i] <= hi)
+        atomicAdd((unsigned long long*)&sh.weight[(hi - key[i]) >> shift], (unsigned long long)weight[i]);
+    __syncthreads();
+    const uint64_t mine = sh.weight[tid];
+    uint64_t total;
+    const uint64_t upto = before + block_prefix(sh, mine, total);
+    if (upto - mine <= target && target < upto) {
+      sh.result[0] = tid;
+      sh.result[1] = upto - mine;
     }
+    __syncthreads();
+    before = sh.result[1];
+    hi -= sh.result[0] << shift;
+    lo = hi - lo < (1ull << shift) ? lo : hi - ((1ull << shift) - 1);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (weight[i] && key[i] >= lo && key[i] <= hi) {
+        const uint32_t at = atomicAdd(&sh.size, 1u);
+        if (at < 64) sh.small[at] = Small{key[i], weight[i]};
+      }
+    __syncthreads();
+    if (sh.size <= 64) break;
+    __syncthreads();
+  }
+  // Few are left: each one's sum by comparison with all, every wave with some of them.
+  const int n = (int)sh.size;
+  if (lane < n) {
+    const uint64_t me = sh.small[lane].key;
+    uint64_t sum = 0;
+    for (int j = wave; j < n; j += kRowWaves) {
+      const Small o = sh.small[j];
+      if (o.key > me) sum += o.weight;
+    }
+    if (sum) atomicAdd((unsigned long long*)&sh.part[lane], (unsigned long long)sum);
+  }
+  __syncthreads();
+  if (tid < n) {
+    const Small me = sh.small[tid];
+    const uint64_t sum = before + sh.part[tid];
+    if (sum <= target && target < sum + me.weight) sh.result[2] = me.key;
+  }
+  __syncthreads();
+  return sh.result[2];
 }
 
 // Where a prefix of the order ends: with the place `last` of the value `key`.
@@ -201,189 +272,274 @@ struct Cut {
   uint32_t last;
 };
 __device__ __forceinline__ bool within(const Cut& c, uint32_t key, uint32_t place) {
-  return key > c.key || (key == c.key && place <= c.last);
+  return ((uint64_t)key << 32 | (uint32_t)~place) >= ((uint64_t)c.key << 32 | (uint32_t)~c.last);
 }
+
+// The target of the smallest prefix that reaches a mass.
+__device__ __forceinline__ uint64_t target_of(double mass) { return mass > 1.0 ? (uint64_t)ceil(mass) - 1 : 0; }
 
 template <typename T>
 struct Sampler {
   Shared& sh;
   Row<T> row;
   Weights w;
-  int steps;  // of kThreads * kChunk places
+  int steps;       // of kThreads * kChunk places
+  bool infinite;   // the largest logit is +inf: such are taken as 0, all others as -inf
   float top, per_bin;
 
+  __device__ __forceinline__ float bin_at(float x) const { return (x == top ? 0.f : top - x) * per_bin; }
   __device__ __forceinline__ int bin_of(float x) const {
-    const float d = x == top ? 0.f : top - x;
-    const float b = d * per_bin;
+    const float b = bin_at(x);
     return b < (float)(kBins - 1) ? (int)b : kBins - 1;
   }
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    for (int s = 0; s < steps; ++s) {
-      const int at = (s * kThreads + (int)threadIdx.x) * kChunk;
-      float x[kChunk];
-      row.load(at, x);
+  __device__ __forceinline__ void decode(const typename Row<T>::Raw& raw, float (&x)[kChunk]) const {
+    Row<T>::decode(raw, x);
+    if (infinite) {
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+    }
+  }
+  // f(eight logits, the place of the first); the loads of AHEAD and up to twice as many in flight.
+  template <int AHEAD, typename F>
+  __device__ __forceinline__ void chunks(F f) const {
+    chunks_while<AHEAD>(f, [] { return true; });
+  }
+  template <int AHEAD, typename F, typename G>
+  __device__ __forceinline__ void chunks_while(F f, G more) const {
+    typename Row<T>::Raw raw[AHEAD], next[AHEAD];
+    const int mine = (int)threadIdx.x * kChunk;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) raw[i] = row.load(mine + i * kThreads * kChunk);
+    for (int s = 0; s < steps && more(); s += AHEAD) {
+      const int at = s * kThreads * kChunk + mine;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) next[i] = row.load(at + (AHEAD + i) * kThreads * kChunk);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        float x[kChunk];
+        decode(raw[i], x);
+        f(x, at + i * kThreads * kChunk);
+        raw[i] = next[i];
+      }
+    }
+  }
+  static __device__ __forceinline__ float largest(const float (&x)[kChunk]) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < kChunk; ++i) m = fmaxf(m, x[i]);
+    return m;
+  }
+  // Appends a chunk's logits named by `bits` to the list: one addition to its length a wave.
+  __device__ __forceinline__ void append(const float (&x)[kChunk], int at, uint32_t bits) const {
+    if (__ballot(bits != 0) == 0) return;
+    const int mine = __builtin_popcount(bits), upto = wave_prefix(mine);
+    uint32_t to = 0;
+    if ((threadIdx.x & 63) == 63) to = atomicAdd(&sh.size, (uint32_t)upto);
+    to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - mine;
+    if (bits) {
 #pragma unroll
       for (int i = 0; i < kChunk; ++i)
-        if (x[i] > -INFINITY) f(x[i], at + i);
+        if (bits >> i & 1) {
+          if (to < kList) sh.list[to] = (uint64_t)ordered(x[i]) << 32 | (uint32_t)~(at + i);
+          ++to;
+        }
     }
   }
-
-  // Where the prefix ends that has the first `rank` (by_count), or as few as reach
-  // `mass` units: within bin `bin`, `above` and `above_mass` before it.  Its own
-  // weight in *total.  The bin holds what is asked for.
-  __device__ Cut resolve(int bin, bool by_count, uint32_t rank, double mass, uint32_t above, uint64_t above_mass,
-                         const Cut& limit, uint64_t* total) {
-    // Members of the bin as a range of orders.
-    if (threadIdx.x == 0) {
-      sh.lo = 0xffffffffu;
-      sh.hi = 0;
-      sh.size = 0;
-    }
+  // Lists what `is` names; false where there are more than fit.
+  template <typename F>
+  __device__ __forceinline__ bool collect(F is) const {
     __syncthreads();
-    each([&](float x, int at) {
-      if (bin_of(x) == bin) {
-        const uint32_t key = ordered(x);
-        if (!within(limit, key, (uint32_t)at)) return;
-        const uint32_t i = atomicAdd(&sh.size, 1u);
-        if (i < kList) sh.list[i] = (uint64_t)key << 32 | (uint32_t)~at;
-        atomicMin(&sh.lo, key);
-        atomicMax(&sh.hi, key);
-      }
-    });
+    if (threadIdx.x == 0) sh.size = 0;
     __syncthreads();
-    uint32_t lo = sh.lo, hi = sh.hi, n = sh.size;
-    // Too many to sort: narrowed to the range of orders that holds the end, or to one value.
-    while (n > kList && lo < hi) {
-      int shift = 0;
-      while ((hi - lo) >> shift >= kBins) ++shift;
-      __syncthreads();
-      for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        sh.count[i] = 0;
-        sh.weight[i] = 0;
-      }
-      __syncthreads();
-      each([&](float x, int at) {
-        const uint32_t key = ordered(x);
-        if (key < lo || key > hi || !within(limit, key, (uint32_t)at)) return;
-        const int b = (int)((hi - key) >> shift);
-        atomicAdd(&sh.count[b], 1u);
-        atomicAdd((unsigned long long*)&sh.weight[b], (unsigned long long)w.units(w.of(x)));
-      });
-      __syncthreads();
-      const int b = find_bin(by_count, rank, mass, above, above_mass);
-      const uint32_t top_key = hi - ((uint32_t)b << shift);
-      const uint32_t low_key = b == (int)((hi - lo) >> shift) ? lo : top_key - ((1u << shift) - 1);
-      hi = top_key;
-      lo = low_key;
-      n = sh.count[b];
-      __syncthreads();
-      if (n <= kList) {
-        if (threadIdx.x == 0) sh.size = 0;
-        __syncthreads();
-        each([&](float x, int at) {
-          const uint32_t key = ordered(x);
-          if (key < lo || key > hi || !within(limit, key, (uint32_t)at)) return;
-          sh.list[atomicAdd(&sh.size, 1u)] = (uint64_t)key << 32 | (uint32_t)~at;
-        });
-        __syncthreads();
-      }
-    }
-    if (n > kList) {
-      // One value: the first so many by place.
-      const uint64_t one = w.units(w.of(unordered(hi)));
-      uint64_t want;
-      if (by_count)
-        want = rank - above;
-      else
-        want = one == 0 ? 1 : (uint64_t)ceil((mass - (double)above_mass) / (double)one);
-      if (want < 1) want = 1;
-      if (want > n) want = n;
-      *total = above_mass + want * one;
-      return Cut{hi, nth_equal(hi, (uint32_t)want, limit)};
-    }
-    sort_list(sh, (int)n);
-    // The entry with which the prefix ends, four a thread.
-    uint64_t each_w[4], a = 0;
-    uint32_t b = 0;
+    chunks_while<T::bytes == 2 ? 4 : 2>([&](const float (&x)[kChunk], int at) {
+      uint32_t bits = 0;
+      if (is(largest(x), at)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = 4 * threadIdx.x + i;
-      each_w[i] = at < (int)n ? w.units(w.of(unordered((uint32_t)(sh.list[at] >> 32)))) : 0;
-      a += each_w[i];
-    }
-    const uint64_t mine = a;
-    uint64_t all_a;
-    uint32_t all_b;
-    block_prefix(sh, a, b, all_a, all_b);
-    if (threadIdx.x == 0) {
-      sh.result[0] = sh.list[n - 1];
-      sh.result[1] = above_mass + all_a;
-    }
-    __syncthreads();
-    uint64_t before = above_mass + a - mine;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = 4 * threadIdx.x + i;
-      // The last of the prefix: what is before it falls short, what is with it does not.
-      const bool last = by_count ? above + at + 1 == rank
-                                 : ((double)before < mass || (above == 0 && at == 0)) &&
-                                       !((double)(before + each_w[i]) < mass);
-      if (at < (int)n && last && (by_count || each_w[i] > 0)) {
-        sh.result[0] = sh.list[at];
-        sh.result[1] = before + each_w[i];
+        for (int i = 0; i < kChunk; ++i) bits |= (uint32_t)((x[i] > -INFINITY) & is(x[i], at + i)) << i;
       }
-      before += each_w[i];
+      append(x, at, bits);
+    }, [&] { return *(volatile uint32_t*)&sh.size <= kList; });
+    __syncthreads();
+    return sh.size <= kList;
+  }
+  __device__ __forceinline__ void clear_bins() const {
+    __syncthreads();
+#pragma unroll
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+      sh.count[i] = 0;
+      sh.weight[i] = 0;
     }
     __syncthreads();
-    const uint64_t end = sh.result[0];
-    *total = sh.result[1];
-    __syncthreads();
-    return Cut{(uint32_t)(end >> 32), ~(uint32_t)end};
+  }
+  // This thread's entries of the list.
+  __device__ __forceinline__ void entries(uint64_t (&key)[kEach]) const {
+    const uint32_t n = sh.size;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) key[i] = i * kThreads + threadIdx.x < n ? sh.list[i * kThreads + threadIdx.x] : 0;
   }
 
-  // The bin of the histogram in which the prefix ends; above and above_mass go on to
-  // what is before it.  (The last bin that holds anything, where none reaches.)
-  __device__ int find_bin(bool by_count, uint32_t rank, double mass, uint32_t& above, uint64_t& above_mass) {
+  // The first bin with which the histogram's counts (by_count), or weights, are above `target`, or the last that
+  // holds anything; above and above_mass go on to what is before it.
+  __device__ __forceinline__ int find_bin(bool by_count, uint64_t target, uint32_t& above, uint64_t& above_mass) {
     const int at = 2 * threadIdx.x;
     const uint32_t c0 = sh.count[at], c1 = sh.count[at + 1];
     const uint64_t w0 = sh.weight[at], w1 = sh.weight[at + 1];
-    uint64_t a = w0 + w1, all_a;
-    uint32_t b = c0 + c1, all_b;
-    block_prefix(sh, a, b, all_a, all_b);
-    const uint64_t a0 = above_mass + a - w0 - w1;
-    const uint32_t b0 = above + b - c0 - c1;
-    if (threadIdx.x == 0) sh.result[0] = 0xffffffffull;
-    if (threadIdx.x == 0) sh.result[3] = 0;
-    __syncthreads();
-    auto look = [&](int bin, uint32_t c, uint64_t wt, uint32_t before, uint64_t before_mass) {
-      if (c == 0) return;
-      atomicMax((unsigned long long*)&sh.result[3], (unsigned long long)bin);
-      const bool reaches = by_count ? before + c >= rank : !((double)(before_mass + wt) < mass);
-      if (reaches) atomicMin((unsigned long long*)&sh.result[0], (unsigned long long)bin);
-    };
-    look(at, c0, w0, b0, a0);
-    look(at + 1, c1, w1, b0 + c0, a0 + w0);
-    __syncthreads();
-    const int bin = (int)(sh.result[0] == 0xffffffffull ? sh.result[3] : sh.result[0]);
-    if (bin == at || bin == at + 1) {
-      sh.result[1] = bin == at ? a0 : a0 + w0;
-      sh.result[2] = bin == at ? b0 : b0 + c0;
+    uint64_t all_a, all_b;
+    const uint64_t a0 = above_mass + block_prefix(sh, w0 + w1, all_a) - w0 - w1;
+    const uint64_t b0 = above + block_prefix(sh, (uint64_t)c0 + c1, all_b) - c0 - c1;
+    const uint64_t all = by_count ? above + all_b : above_mass + all_a;
+    if (target >= all) target = all - 1;
+    const uint64_t before = by_count ? b0 : a0, v0 = by_count ? c0 : w0, v1 = by_count ? c1 : w1;
+    if (before <= target && target < before + v0 + v1) {
+      const bool second = target >= before + v0;
+      sh.result[0] = at + (second ? 1 : 0);
+      sh.result[1] = a0 + (second ? w0 : 0);
+      sh.result[2] = b0 + (second ? c0 : 0);
     }
     __syncthreads();
+    const int bin = (int)sh.result[0];
     above_mass = sh.result[1];
     above = (uint32_t)sh.result[2];
     __syncthreads();
     return bin;
   }
 
-  // The place of the want-th logit of one value.
-  __device__ uint32_t nth_equal(uint32_t key, uint32_t want, const Cut& limit) {
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  // Counts, and weights, of the logits within `limit`.
+  template <bool WEIGHTS>
+  __device__ __forceinline__ void histogram(const Cut& limit) {
+    clear_bins();
+    chunks<2>([&](const float (&x)[kChunk], int at) {
+      double weight[kChunk];
+      if (WEIGHTS) w.of8(x, weight);
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        if (!(x[i] > -INFINITY) || !within(limit, ordered(x[i]), (uint32_t)(at + i))) continue;
+        const int bin = bin_of(x[i]);
+        atomicAdd(&sh.count[bin], 1u);
+        if (WEIGHTS) atomicAdd((unsigned long long*)&sh.weight[bin], (unsigned long long)w.units(weight[i]));
+      }
+    });
+    __syncthreads();
+  }
+
+  // The long way to the end of a prefix: that of the logits within `limit` whose count (by_count), or
+  // weight, is the first above `target`.  It ends in bin `bin`, `above` and
+  // `above_mass` before it.  Its weight in *total.
+  __device__ __forceinline__ Cut resolve(int bin, bool by_count, uint64_t target, uint32_t above, uint64_t above_mass, const Cut& limit,
+                         uint64_t* total) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      sh.lo = 0xffffffffu;
+      sh.hi = 0;
+    }
+    uint32_t lo = 0, hi = 0xffffffffu;
+    auto members = [&](float x, uint32_t key, uint32_t at) {
+      return (x > -INFINITY) & (bin_of(x) == bin) & (key >= lo) & (key <= hi) & within(limit, key, at);
+    };
+    // f(logit, place) of the members; chunks that cannot hold one are passed over.
+    auto each_member = [&](auto f) {
+      chunks<T::bytes == 2 ? 4 : 2>([&](const float (&x)[kChunk], int at) {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) any |= (x[i] > -INFINITY) & (bin_of(x[i]) == bin);
+        if (any) {
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i)
+            if (members(x[i], ordered(x[i]), (uint32_t)(at + i))) f(x[i], at + i);
+        }
+      });
+    };
+    if (sh.count[bin] > kList) {
+      // As a range of orders.
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        sh.lo = 0xffffffffu;
+        sh.hi = 0;
+      }
+      __syncthreads();
+      uint32_t least = 0xffffffffu, most = 0;
+      each_member([&](float x, int) {
+        const uint32_t key = ordered(x);
+        least = key < least ? key : least;
+        most = key > most ? key : most;
+      });
+      atomicMin(&sh.lo, least);
+      atomicMax(&sh.hi, most);
+      __syncthreads();
+      lo = sh.lo;
+      hi = sh.hi;
+    }
+    // Narrowed until its members can be listed, or are of one value.
+    bool fits;
+    while (true) {
+      __syncthreads();
+      if (threadIdx.x == 0) sh.size = 0;
+      __syncthreads();
+      chunks<T::bytes == 2 ? 4 : 2>([&](const float (&x)[kChunk], int at) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) bits |= (uint32_t)members(x[i], ordered(x[i]), (uint32_t)(at + i)) << i;
+        append(x, at, bits);
+      });
+      __syncthreads();
+      fits = sh.size <= kList;
+      if (fits || lo == hi) break;
+      int shift = 0;
+      while ((hi - lo) >> shift >= kBins) ++shift;
+      clear_bins();
+      each_member([&](float x, int at) {
+        const int b = (int)((hi - ordered(x)) >> shift);
+        atomicAdd(&sh.count[b], 1u);
+        atomicAdd((unsigned long long*)&sh.weight[b], (unsigned long long)w.units(w.of(x)));
+      });
+      __syncthreads();
+      const uint32_t b = (uint32_t)find_bin(by_count, target, above, above_mass);
+      hi -= b << shift;
+      lo = hi - lo < (1u << shift) ? lo : hi - ((1u << shift) - 1);
+    }
+    if (!fits) {
+      // One value: the first so many by place.
+      const uint32_t n = sh.size;
+      const uint64_t one = w.units(w.of(unordered(hi)));
+      uint64_t more = by_count ? target - above : (one == 0 ? 0 : (target - above_mass) / one);
+      if (more >= n) more = n - 1;
+      *total = above_mass + (more + 1) * one;
+      __syncthreads();
+      return Cut{hi, nth_equal(hi, more, limit)};
+    }
+    uint64_t key[kEach], ones[kEach], units[kEach], all = 0;
+    entries(key);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      ones[i] = key[i] != 0;
+      units[i] = key[i] ? w.units(w.of(unordered((uint32_t)(key[i] >> 32)))) : 0;
+      if (!by_count) ones[i] = units[i];
+      all += ones[i];
+    }
+    const uint64_t from = by_count ? above : above_mass;
+    block_prefix(sh, all, all);
+    target = target - from < all ? target - from : all - 1;
+    // The bin's range of values, a little wider than it is.
+    const float slack = 0x1p-20f * (fabsf(top) + (bin + 1) / per_bin);
+    const uint64_t lowest = bin + 1 == kBins ? 0 : (uint64_t)ordered(top - (bin + 1) / per_bin - slack) << 32;
+    const uint64_t highest = (uint64_t)ordered(top - bin / per_bin + slack) << 32 | 0xffffffffu;
+    const uint64_t last = all ? select(sh, key, ones, lowest, highest, target) : 0;
+    uint64_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) mine += key[i] >= last ? units[i] : 0;
+    block_prefix(sh, mine, all);
+    *total = above_mass + all;
+    __syncthreads();
+    return Cut{(uint32_t)(last >> 32), ~(uint32_t)last};
+  }
+
+  // The place of the nth (from 0) logit of one value.
+  __device__ __forceinline__ uint32_t nth_equal(uint32_t key, uint64_t nth, const Cut& limit) {
+    const int lane = threadIdx.x & 63, wave = spruce::uniform(threadIdx.x >> 6);
     for (int s = 0; s < steps; ++s) {
       const int at = (s * kThreads + (int)threadIdx.x) * kChunk;
       float x[kChunk];
-      row.load(at, x);
+      decode(row.load(at), x);
       int c = 0;
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) c += x[i] > -INFINITY && ordered(x[i]) == key && within(limit, key, at + i);
@@ -391,24 +547,24 @@ struct Sampler {
       if (lane == 63) sh.part[s * kRowWaves + wave] = (uint64_t)all;
     }
     uint64_t before;
-    const int part = find_part(want - 1, before);
+    const int part = find_part(nth, before);
     if (wave == 0) {
       const int at = part * kPart + lane * kChunk;
       float x[kChunk];
-      row.load(at, x);
-      int c = 0, hit = -1;
+      decode(row.load(at), x);
+      int c = 0;
       bool is[kChunk];
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) {
         is[i] = x[i] > -INFINITY && ordered(x[i]) == key && within(limit, key, at + i);
         c += is[i];
       }
-      int upto = (int)before + wave_prefix(c) - c;
+      uint64_t upto = before + (uint64_t)(wave_prefix(c) - c);
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) {
-        if (is[i] && ++upto == (int)want) hit = at + i;
+        if (is[i] && upto == nth) sh.result[0] = (uint64_t)(at + i);
+        upto += is[i];
       }
-      if (hit >= 0) sh.result[0] = (uint64_t)hit;
     }
     __syncthreads();
     const uint32_t place = (uint32_t)sh.result[0];
@@ -416,26 +572,20 @@ struct Sampler {
     return place;
   }
 
-  // The first part whose sums, added up in order, are past `target`, and what is before it
-  // (the last part with anything where none is).
-  __device__ int find_part(uint64_t target, uint64_t& before) {
+  // The first of the sums with which they are above `target`, and what is before it.
+  __device__ __forceinline__ int find_part(uint64_t target, uint64_t& before) {
     const int n = steps * kRowWaves;
     constexpr int EACH = kParts / kThreads;
     __syncthreads();
-    uint64_t v[EACH], a = 0;
-    uint32_t b = 0;
+    uint64_t v[EACH], mine = 0, all;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int at = EACH * threadIdx.x + i;
       v[i] = at < n ? sh.part[at] : 0;
-      a += v[i];
+      mine += v[i];
     }
-    const uint64_t mine = a;
-    uint64_t all_a;
-    uint32_t all_b;
-    block_prefix(sh, a, b, all_a, all_b);
-    if (target >= all_a) target = all_a - 1;
-    uint64_t upto = a - mine;
+    uint64_t upto = block_prefix(sh, mine, all) - mine;
+    if (target >= all) target = all - 1;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       if (upto <= target && target < upto + v[i]) {
@@ -452,152 +602,125 @@ struct Sampler {
   }
 };
 
+// floor(u times a sum), below it.
+__device__ __forceinline__ uint64_t drawn(double u, uint64_t total) {
+  const double wanted = (u > 0.0 ? u : 0.0) * (double)total;
+  return wanted < (double)(total - 1) ? (uint64_t)wanted : total - 1;
+}
+
+// A row's settings.
+struct Settings {
+  double temperature, top_p, min_p, u;
+  int64_t top_k;
+  bool by_k, by_p;
+  __device__ __forceinline__ void init(const Sampling& p, int b) {
+    temperature = p.temperature ? (double)p.temperature[b] : p.temperature1;
+    top_k = p.top_k ? (int64_t)p.top_k[b] : p.top_k1;
+    top_p = p.top_p ? (double)p.top_p[b] : p.top_p1;
+    min_p = p.min_p ? (double)p.min_p[b] : p.min_p1;
+    min_p = min_p < 1.0 ? min_p : 1.0;
+    u = p.uniform64 ? static_cast<const double*>(p.uniform)[b] : (double)static_cast<const float*>(p.uniform)[b];
+    by_k = top_k > 0 && top_k < p.V;
+    by_p = top_p < 1.0;
+  }
+};
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
-  __shared__ Shared sh;
-  const int b = (int)flat_block(), tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  Sampler<T> s{sh};
+__device__ __forceinline__ void set_up(Sampler<T>& s, const Sampling& p, int b) {
   s.row.init(p.logits, (int64_t)b * p.stride, p.V);
   s.steps = (s.row.end + kThreads * kChunk - 1) / (kThreads * kChunk);
-  const double temperature = p.temperature ? (double)p.temperature[b] : p.temperature1;
-  const int64_t top_k = p.top_k ? (int64_t)p.top_k[b] : p.top_k1;
-  const double top_p = p.top_p ? (double)p.top_p[b] : p.top_p1;
-  double min_p = p.min_p ? (double)p.min_p[b] : p.min_p1;
-  min_p = min_p < 1.0 ? min_p : 1.0;
-  if (tid < kTable) sh.table[tid] = exp2((double)tid / kTable);
-
-  // Pass A: the largest logit with its first place, and the smallest.
-  uint64_t best = 0;
-  float least = INFINITY;
-  s.each([&](float x, int at) {
-    const uint64_t v = (uint64_t)ordered(x) << 32 | (uint32_t)~at;
-    best = v > best ? v : best;
-    least = fminf(least, x);
-  });
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) {
-    const uint64_t o = __shfl_xor(best, i);
-    best = o > best ? o : best;
-    least = fminf(least, __shfl_xor(least, i));
-  }
-  if (lane == 0) {
-    sh.waves[wave] = best;
-    sh.wave_count[wave] = __builtin_bit_cast(uint32_t, least);
-  }
-  __syncthreads();
-  for (int i = 0; i < kRowWaves; ++i) {
-    best = sh.waves[i] > best ? sh.waves[i] : best;
-    least = fminf(least, __builtin_bit_cast(float, sh.wave_count[i]));
-  }
-  __syncthreads();
-  const uint32_t first_place = ~(uint32_t)best;
-  if (best == 0 || !(temperature > 0)) {  // nothing to choose from, or the largest
-    if (tid == 0) {
-      p.tokens[b] = best == 0 ? -1 : (int64_t)(first_place - (uint32_t)s.row.first);
-      if (p.logprobs) p.logprobs[b] = best == 0 ? -INFINITY : 0.f;
-    }
-    return;
-  }
-  s.top = unordered((uint32_t)(best >> 32));
+}
+template <typename T>
+__device__ __forceinline__ void set_weights(Sampler<T>& s, const Sampling& p, double temperature, float top, float least) {
+  s.top = uniform(top);
   // (An infinite temperature: all weights one, but those of -inf.)
-  s.w = Weights{(double)s.top, fmax(1.44269504088896340736 / temperature, 1e-300), sh.table, p.shift};
+  const double inv = fmin(fmax(1.0 / temperature, 1e-300), 1e+300);
+  constexpr double kLog2e = 1.44269504088896340736;
+  s.w = Weights{uniform((double)top), uniform(inv), uniform(kTable * kLog2e * inv), uniform(-60.0 / (kLog2e * inv)),
+                p.shift, s.sh.table};
+  // Bins of equal width down to the smallest logit, or to where weights end.
+  float range = fminf(top - least, (float)(kNothing / (kLog2e * inv)));
+  range = range > 1e-30f ? (range < 1e30f ? range : 1e30f) : 1e-30f;
+  s.per_bin = uniform((float)(kBins - 1) / range);
+}
 
-  Cut cut{0, 0};  // all
-  const bool by_k = top_k > 0 && top_k < p.V, by_p = top_p < 1.0;
-  if (by_k || by_p) {
-    // Pass B.  Bins of equal width down to the smallest logit, or to where weights end.
-    float range = fminf(s.top - least, (float)(kNothing / s.w.c2));
-    range = range > 1e-30f ? (range < 1e30f ? range : 1e30f) : 1e-30f;
-    s.per_bin = (float)(kBins - 1) / range;
-    for (int i = tid; i < kBins; i += kThreads) {
-      sh.count[i] = 0;
-      sh.weight[i] = 0;
-    }
-    __syncthreads();
-    s.each([&](float x, int) {
-      const int bin = s.bin_of(x);
-      atomicAdd(&sh.count[bin], 1u);
-      atomicAdd((unsigned long long*)&sh.weight[bin], (unsigned long long)s.w.units(s.w.of(x)));
-    });
-    __syncthreads();
-    uint64_t a = sh.weight[2 * tid] + sh.weight[2 * tid + 1], total;
-    uint32_t c = sh.count[2 * tid] + sh.count[2 * tid + 1], all;
-    block_prefix(sh, a, c, total, all);
-    if (by_k && top_k < (int64_t)all) {
+// A row that keeps more than the list holds.  A function of its own, which sets
+// everything up again: what it would keep in registers pushed the usual way's out of them.
+template <typename T>
+__device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute__((address_space(3))) Shared* lds) {
+  const Sampling p = *(const Sampling*)(const __attribute__((address_space(4))) Sampling*)lane_of((int64_t)args, 0);
+  Shared& sh = *(Shared*)lds;
+  const int b = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = spruce::uniform(tid >> 6);
+  Settings set;
+  set.init(p, b);
+  Sampler<T> s{sh};
+  set_up(s, p, b);
+  __syncthreads();
+  s.infinite = spruce::uniform(sh.infinite) != 0;
+  set_weights(s, p, set.temperature, sh.top, sh.least);
+  Cut cut{0, 0xffffffffu};  // all
+  uint64_t total = 0;
+  if (set.by_k || set.by_p) {
+    if (set.by_k) s.template histogram<true>(cut);  // otherwise as it is
+    uint64_t all = sh.weight[2 * tid] + sh.weight[2 * tid + 1], count = sh.count[2 * tid] + sh.count[2 * tid + 1];
+    block_prefix(sh, all, total);
+    block_prefix(sh, count, count);
+    // First by count, then by weight, of what the first has left.
+    for (int turn = set.by_k && (uint64_t)set.top_k < count ? 0 : 1; turn < (set.by_p ? 2 : 1); ++turn) {
+      const bool by_count = turn == 0;
+      const uint64_t target = by_count ? (uint64_t)set.top_k - 1 : target_of(fmax(set.top_p, 0.0) * (double)total);
       uint32_t above = 0;
       uint64_t above_mass = 0;
-      const int bin = s.find_bin(true, (uint32_t)top_k, 0.0, above, above_mass);
+      const int bin = s.find_bin(by_count, target, above, above_mass);
       // (What is behind the last weight has none to choose by.)
-      if (above_mass < total) {
-        cut = s.resolve(bin, true, (uint32_t)top_k, 0.0, above, above_mass, cut, &total);
-        if (by_p) {  // the histogram again, of what is left
-          __syncthreads();
-          for (int i = tid; i < kBins; i += kThreads) {
-            sh.count[i] = 0;
-            sh.weight[i] = 0;
-          }
-          __syncthreads();
-          s.each([&](float x, int at) {
-            if (!within(cut, ordered(x), (uint32_t)at)) return;
-            const int bin2 = s.bin_of(x);
-            atomicAdd(&sh.count[bin2], 1u);
-            atomicAdd((unsigned long long*)&sh.weight[bin2], (unsigned long long)s.w.units(s.w.of(x)));
-          });
-          __syncthreads();
-        }
+      if (by_count && above_mass >= total) continue;
+      cut = s.resolve(bin, by_count, target, above, above_mass, cut, &all);
+      if (by_count && set.by_p) {
+        total = all;
+        s.template histogram<true>(cut);
       }
     }
-    if (by_p) {
-      const double mass = fmax(top_p, 0.0) * (double)total;
-      uint32_t above = 0;
-      uint64_t above_mass = 0;
-      const int bin = s.find_bin(false, 0, mass, above, above_mass);
-      uint64_t left;
-      cut = s.resolve(bin, false, 0, mass, above, above_mass, cut, &left);
-    }
   }
-
-  // Pass D.
-  const double least_weight = fmin(min_p, 1.0);
-  auto weight_at = [&](float x, int at) -> uint64_t {
-    if (!(x > -INFINITY) || !within(cut, ordered(x), (uint32_t)at)) return 0;
-    const double wt = s.w.of(x);
-    return wt >= least_weight ? s.w.units(wt) : 0;
-  };
-  for (int i = 0; i < s.steps; ++i) {
-    const int at = (i * kThreads + tid) * kChunk;
-    float x[kChunk];
-    s.row.load(at, x);
-    uint64_t sum = 0;
+  // The kept weights of eight logits.
+  auto weights_at = [&](const float (&x)[kChunk], int at, uint64_t (&units)[kChunk]) {
+    double weight[kChunk];
+    s.w.of8(x, weight);
+    if (cut.key) {
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) sum += weight_at(x[j], at + j);
+      for (int j = 0; j < kChunk; ++j)
+        if (!within(cut, ordered(x[j]), (uint32_t)(at + j))) weight[j] = -1.0;
+    }
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) units[j] = s.w.units(weight[j] >= set.min_p ? weight[j] : 0.0);
+  };
+  s.template chunks<2>([&](const float (&x)[kChunk], int at) {
+    uint64_t sum = 0;
+    if (__ballot(ordered(s.largest(x)) >= cut.key)) {
+      uint64_t units[kChunk];
+      weights_at(x, at, units);
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) sum += units[j];
+    }
     const int64_t upto = wave_prefix((int64_t)sum);
-    if (lane == 63) sh.part[i * kRowWaves + wave] = (uint64_t)upto;
-  }
+    if (lane == 63 && at / kPart < s.steps * kRowWaves) sh.part[at / kPart] = (uint64_t)upto;
+  });
   __syncthreads();
-  uint64_t total = 0;
   {
     uint64_t a = 0;
-    uint32_t c = 0, all;
     for (int i = tid; i < s.steps * kRowWaves; i += kThreads) a += sh.part[i];
-    block_prefix(sh, a, c, total, all);
+    block_prefix(sh, a, total);
   }
-  double u = p.uniform64 ? static_cast<const double*>(p.uniform)[b] : (double)static_cast<const float*>(p.uniform)[b];
-  u = u > 0.0 ? u : 0.0;
-  const double wanted = u * (double)total;
-  const uint64_t target = wanted < (double)(total - 1) ? (uint64_t)wanted : total - 1;
+  const uint64_t target = drawn(set.u, total);
   uint64_t before;
   const int part = s.find_part(target, before);
   if (wave == 0) {
     const int at = part * kPart + lane * kChunk;
     float x[kChunk];
-    s.row.load(at, x);
+    s.decode(s.row.load(at), x);
     uint64_t each_w[kChunk], sum = 0;
+    weights_at(x, at, each_w);
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) {
-      each_w[j] = weight_at(x[j], at + j);
-      sum += each_w[j];
-    }
+    for (int j = 0; j < kChunk; ++j) sum += each_w[j];
     uint64_t upto = before + (uint64_t)wave_prefix((int64_t)sum) - sum;
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
@@ -607,6 +730,197 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
       }
       upto += each_w[j];
     }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = spruce::uniform(tid >> 6);
+  Settings set;
+  set.init(p, b);
+  Sampler<T> s{sh};
+  set_up(s, p, b);
+  s.infinite = false;
+  if (tid < kTable) sh.table[tid] = __builtin_bit_cast(uint64_t, exp2((double)tid / kTable));
+
+  // The largest logit with its first place, and the smallest.
+  float most = -INFINITY, least = INFINITY;
+  int place = 0;
+  s.template chunks<T::bytes == 2 ? 4 : 2>([&](const float (&x)[kChunk], int at) {
+    const float m = s.largest(x);
+    if (m > most) {
+      most = m;
+      place = at;  // of the chunk
+    }
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) least = fminf(least, x[i] > -INFINITY ? x[i] : INFINITY);
+  });
+  uint64_t best = most > -INFINITY ? (uint64_t)ordered(most) << 32 | (uint32_t)~place : 0;
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) {
+    const uint64_t o = __shfl_xor(best, i);
+    best = o > best ? o : best;
+    least = fminf(least, __shfl_xor(least, i));
+  }
+  if (lane == 0) {
+    sh.waves[wave] = best;
+    sh.count[wave] = __builtin_bit_cast(uint32_t, least);
+  }
+  __syncthreads();
+  for (int i = 0; i < kRowWaves; ++i) {
+    best = sh.waves[i] > best ? sh.waves[i] : best;
+    least = fminf(least, __builtin_bit_cast(float, sh.count[i]));
+  }
+  __syncthreads();
+  const float top = unordered((uint32_t)(best >> 32));
+  if (best == 0 || !(set.temperature > 0)) {  // nothing to choose from, or the largest
+    if (tid == 0) {
+      int64_t token = -1;
+      if (best != 0) {
+        float x[kChunk];
+        const int at = (int)~(uint32_t)best;
+        s.decode(s.row.load(at), x);
+#pragma unroll
+        for (int i = kChunk - 1; i >= 0; --i)
+          if (x[i] == top) token = at + i - s.row.first;
+      }
+      p.tokens[b] = token;
+      if (p.logprobs) p.logprobs[b] = best == 0 ? -INFINITY : 0.f;
+    }
+    return;
+  }
+  s.infinite = top == INFINITY;
+  if (s.infinite) {
+    least = 0.f;
+    most = most == INFINITY ? 0.f : -INFINITY;
+  }
+  set_weights(s, p, set.temperature, s.infinite ? 0.f : top, least);
+  if (tid == 0) {
+    sh.top = s.top;
+    sh.least = least;
+    sh.infinite = s.infinite;
+  }
+
+  // The list: what is in bins below `end`, or at `low` or above.
+  uint64_t total = 0;
+  uint32_t above = 0;
+  uint64_t above_mass = 0;
+  float end = 0.f, low = -INFINITY;
+  bool far = false;
+  if (set.by_k && set.top_k <= kThreads / 2) {
+    // At least so many threads have a logit in the bin or above.
+    s.clear_bins();
+    if (most > -INFINITY) atomicAdd(&sh.count[s.bin_of(most)], 1u);
+    __syncthreads();
+    end = (float)(s.find_bin(true, (uint64_t)set.top_k - 1, above, above_mass) + 1);
+    // (Fewer threads than that with a logit: everything.)
+    if (above + sh.count[(int)end - 1] < (uint32_t)set.top_k) end = (float)kBins;
+  } else if (set.by_k || set.by_p) {
+    if (set.by_k)
+      s.template histogram<false>(Cut{0, 0xffffffffu});
+    else
+      s.template histogram<true>(Cut{0, 0xffffffffu});
+    uint64_t all = sh.weight[2 * tid] + sh.weight[2 * tid + 1];
+    block_prefix(sh, all, total);
+    const uint64_t target = set.by_k ? (uint64_t)set.top_k - 1 : target_of(fmax(set.top_p, 0.0) * (double)total);
+    end = (float)(s.find_bin(set.by_k, target, above, above_mass) + 1);
+    far = above + sh.count[(int)end - 1] > kList;
+  } else if (set.min_p > 0.0) {
+    // (A little lower than it is, for the roundings.)
+    const float bound = s.top + (float)(log(set.min_p) * 1.000001 / s.w.inv);
+    low = bound - fabsf(bound) * 0x1p-20f - fabsf(s.top) * 0x1p-20f;
+    end = INFINITY;
+  } else {
+    far = true;
+  }
+  if (end == (float)kBins) end = INFINITY;
+  if (!far) far = !s.collect([&](float x, int) { return !(x < low) & (s.bin_at(x) < end); });
+  if (far) {
+    sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh);
+    return;
+  }
+  const uint32_t n = sh.size;
+  auto done = [&](uint64_t entry, double weight, uint64_t sum) {
+    p.tokens[b] = (int64_t)(~(uint32_t)entry - (uint32_t)s.row.first);
+    if (p.logprobs) p.logprobs[b] = (float)log(weight / ((double)sum * (p.shift * 0x1p-52)));
+  };
+  if (n <= 64) {
+    // One wave: an entry a lane, its rank and the weight before it by comparison with all.
+    if (wave != 0) return;
+    const uint64_t mine = lane < (int)n ? sh.list[lane] : 0;
+    const double exact = lane < (int)n ? s.w.of(unordered((uint32_t)(mine >> 32))) : 0.0;
+    uint64_t units = s.w.units(exact);
+    sh.weight[lane] = units;
+    wave_lds_fence();
+    uint32_t rank = 0;
+    uint64_t before = 0;
+    if (set.by_k || set.by_p) {
+#pragma unroll 8
+      for (uint32_t j = 0; j < n; ++j) {
+        const bool first = sh.list[j] > mine;
+        rank += first;
+        before += first ? sh.weight[j] : 0;
+      }
+      if (set.by_k && rank >= set.top_k) units = 0;
+      if (set.by_p) {
+        const uint64_t all = (uint64_t)lane_of(wave_prefix((int64_t)units), 63);
+        if (before > target_of(fmax(set.top_p, 0.0) * (double)(set.by_k ? all : total))) units = 0;
+      }
+    }
+    if (!(exact >= set.min_p)) units = 0;
+    const uint64_t sum = (uint64_t)lane_of(wave_prefix((int64_t)units), 63), target = drawn(set.u, sum);
+    wave_lds_fence();
+    sh.weight[lane] = units;
+    wave_lds_fence();
+    before = 0;
+#pragma unroll 8
+    for (uint32_t j = 0; j < n; ++j) before += (uint32_t)sh.list[j] > (uint32_t)mine ? sh.weight[j] : 0;
+    if (before <= target && target < before + units) done(mine, exact, sum);
+    return;
+  }
+  uint64_t key[kEach], units[kEach], weight[kEach], sum = 0;
+  double exact[kEach];
+  s.entries(key);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    exact[i] = key[i] ? s.w.of(unordered((uint32_t)(key[i] >> 32))) : 0.0;
+    units[i] = s.w.units(exact[i]);
+    weight[i] = key[i] ? 1 : 0;
+  }
+  // The ends by count and by weight, then the draw: three selections.
+  // Its orders begin at the bound, a little lower than it is.
+  const float bound = end < INFINITY ? s.top - (end + 1.f) / s.per_bin : low;
+  const float from = fmaxf(bound - (fabsf(bound) + fabsf(s.top)) * 0x1p-20f, least);
+  const uint64_t lowest = (uint64_t)ordered(from) << 32, highest = (uint64_t)ordered(s.top) << 32 | 0xffffffffu;
+  for (int turn = set.by_k && (uint64_t)set.top_k < n ? 0 : (set.by_p ? 1 : 2);; turn = turn == 0 && set.by_p ? 1 : 2) {
+    uint64_t target = (uint64_t)set.top_k - 1;
+    if (turn > 0) {
+      sum = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (turn == 2) {
+          if (!(exact[i] >= set.min_p)) units[i] = 0;
+          key[i] = (uint32_t)key[i];  // goes down as the place goes up
+        }
+        weight[i] = units[i];
+        sum += units[i];
+      }
+      block_prefix(sh, sum, sum);
+      target = turn == 2 ? drawn(set.u, sum) : target_of(fmax(set.top_p, 0.0) * (double)(set.by_k ? sum : total));
+      if (target >= sum) target = sum - 1;
+    }
+    const uint64_t found = turn == 2 ? select(sh, key, weight, (uint32_t)~s.row.end, 0xffffffffu, target)
+                                     : select(sh, key, weight, lowest, highest, target);
+    if (turn == 2) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (units[i] && key[i] == found) done(found, exact[i], sum);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (key[i] < found) units[i] = 0;
   }
 }
 
