@@ -884,7 +884,11 @@ int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, void* stream);
  *   k_pages, v_pages [pages, Hkv, page_size, D] (bf16 / f16 / f32, D in {64, 128},
  *   rows 16-byte aligned), mass_pages [pages, Hkv, page_size] float32, of any
  *   strides in which no two rows share memory.
+ *   workspace: spruce_paged_evict_workspace_bytes(S, Hkv, table_width * page_size)
+ *   bytes (none for tables of up to 16384 positions), 16-byte aligned, one call's
+ *   own until it is done.
  */
+int64_t spruce_paged_evict_workspace_bytes(int64_t S, int64_t Hkv, int64_t keys);
 typedef struct spruce_paged_evict_args {
   void* k_pages;
   int64_t kps[4];
@@ -902,6 +906,8 @@ typedef struct spruce_paged_evict_args {
   int64_t keep, first, recent;
   int32_t* kept;
   int32_t* new_lens;
+  void* workspace;
+  int64_t workspace_bytes;
 } spruce_paged_evict_args;
 int spruce_paged_evict(const spruce_paged_evict_args* args, void* stream);
 

@@ -11,6 +11,11 @@
 //   keys  256 keys against the rows that see them: every lane has one key's sum.
 // Both are S = A B^T on the matrix cores with the streamed side as A, so what is
 // held lies in the columns, one a lane, and sums stay within the lane.
+//
+// Sequences of few packed rows (a decoding step, a few drafted tokens) are bound by
+// the read of their keys, which is done once: their scores, 4 bytes against a
+// key's 2 D, go to the workspace, with every row's maximum and sum by ranges of keys, and
+// a second kernel makes the weights of them.
 #include "paged_impl.h"
 
 namespace spruce {
@@ -21,6 +26,12 @@ struct KeyMass {
   int64_t ms[3];   // page, head, slot strides
   float2* stats;   // [N * Hq][parts]: maximum (of scores as products) and sum
   int Hq, parts, accumulate;
+  // Sequences of up to few_rows packed rows: stats by ranges of `range` keys, scores of a (KV head, sequence)
+  // as [32 keys][row][key] from its first packed row times key_room on.
+  int few_rows, range, ranges, key_room;
+  float* scores;
+  float2* few_stats;  // [N * Hq][ranges]
+  float cs_low;       // what scale log2 e has past p.cs
 };
 
 namespace {
@@ -35,6 +46,9 @@ constexpr int kStream = 64;           // rows, or keys, streamed between barrier
 // size; where that is large (times scale log2 e) it is formed from the finished
 // score instead, so that the largest weight of a row is one whatever the scores.
 constexpr float kLargeReference = 0x1p+10f;
+// Scores that the workspace may hold; more go by two passes over the keys.  (1 GiB: one token of 64 sequences
+// over 131072 keys, 28 heads, is 0.88.)
+constexpr int64_t kMostScores = (int64_t)1 << 28;
 // A tile's sum past this moves the reference.
 constexpr float kRescaleSum = 0x1p+60f;
 
@@ -87,8 +101,8 @@ struct Sum {
     float mx = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    if (mx == -INFINITY) return;
-    const float now = l == 0.f ? mx : fmaxf(m, mx);
+    float now = l == 0.f ? mx : fmaxf(m, mx);
+    if (now == -INFINITY) now = 0.f;  // nothing yet, but perhaps NaN
     float t = l == 0.f ? 0.f : l * fast_exp2((m - now) * cs);
 #pragma unroll
     for (int r = 0; r < 16; ++r) t += fast_exp2((s[r] - now) * cs);
@@ -232,6 +246,20 @@ __global__ __launch_bounds__(256, 2) void key_mass_rows_kernel(const KeyMass a) 
   }
 }
 
+// Joins the parts of every row's keys: its first part stands for all afterwards.
+__global__ __launch_bounds__(256) void key_mass_join_kernel(float2* stats, int64_t rows, int parts, float cs) {
+  const int64_t r = (int64_t)flat_block() * 256 + threadIdx.x;
+  if (r >= rows) return;
+  float2* st = stats + r * parts;
+  Sum all;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) {
+    const float2 x = st[i];
+    all.join(x.x, x.y, cs);
+  }
+  st[0] = float2{all.m, all.l};
+}
+
 // The at-th of the key tiles of all sequences with new tokens.
 struct KeyTile {
   int s, tile, len, start, n;
@@ -243,7 +271,7 @@ __device__ __forceinline__ bool find_keys(const PagedAttn& p, int64_t at, int la
     const Lengths len = lengths_of(p, s0 + lane);
     const int a = clamp_start(p.batch, len.starts), e = clamp_start(p.batch, len.ends);
     int keys = len.keys < 0 ? 0 : (len.keys < p.batch.cap ? len.keys : p.batch.cap);
-    if (e <= a || p.batch.pages == 0) keys = 0;
+    if (e <= a || (int64_t)(e - a) * p.G <= p.few_limit || p.batch.pages == 0) keys = 0;
     const int64_t pc = count + wave_prefix((int64_t)((keys + kRowsOf - 1) / kRowsOf));
     const uint64_t past = __ballot(pc > at);
     if (past) {
@@ -315,7 +343,8 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
         const int t = p.by_group.of(r0 + tid), h = g * p.G + r0 + tid - t * p.G;
         row_pos = clip(k.pos0 + t);
         const float2* st = a.stats + ((int64_t)(k.start + t) * a.Hq + h) * a.parts;
-        for (int i = 0; i < a.parts; ++i) stat.join(st[i].x, st[i].y, p.cs);
+        const float2 x = *st;
+        stat.join(x.x, x.y, p.cs);
       }
     };
     float sum[2] = {0.f, 0.f};
@@ -394,20 +423,243 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
   }
 }
 
+// ------------------------------------------------------------------ few rows
+
+constexpr int kFewTile = 32;  // rows, and keys, of a wave's tile
+constexpr int kMostRange = 1024;
+
+// exp2(cs d) with the product's rounding and cs's made good: the argument is some tens, so that half
+// a step of it is some 2^-20 of the result.
+__device__ __forceinline__ float weight_of(float d, float cs, float cs_low) {
+  const float y = d * cs;
+  const float off = fmaf(d, cs, -y) + d * cs_low;
+  return y < -150.f ? 0.f : fast_exp2(y) * fmaf(off, 0.69314718f, 1.f);  // (NaN stays NaN)
+}
+
+// The at-th range of `keys` keys of all sequences of few rows.
+__device__ __forceinline__ bool find_range(const KeyMass& a, int64_t at, int keys, int lane, KeyTile& k) {
+  const PagedAttn& p = a.a;
+  int64_t count = 0;
+  for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
+    const Lengths len = lengths_of(p, s0 + lane);
+    const int first = clamp_start(p.batch, len.starts), e = clamp_start(p.batch, len.ends);
+    int n = len.keys < 0 ? 0 : (len.keys < p.batch.cap ? len.keys : p.batch.cap);
+    if (e <= first || (int64_t)(e - first) * p.G > a.few_rows || p.batch.pages == 0) n = 0;
+    const int64_t pc = count + wave_prefix((int64_t)((n + keys - 1) / keys));
+    const uint64_t past = __ballot(pc > at);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      k.s = s0 + l;
+      k.len = __builtin_amdgcn_readlane(n, l);
+      k.tile = uniform((int)(at - lane_of(pc, l))) + (k.len + keys - 1) / keys;
+      k.start = __builtin_amdgcn_readlane(first, l);
+      k.n = __builtin_amdgcn_readlane(e, l) - k.start;
+      k.pos0 = lane_of((int64_t)len.keys - ((int64_t)len.ends - len.starts) + ((int64_t)first - len.starts), l);
+      return true;
+    }
+    count = lane_of(pc, 63);
+  }
+  return false;
+}
+
+__device__ __forceinline__ float* scores_of(const KeyMass& a, const KeyTile& k, int g) {
+  return a.scores + ((int64_t)g * a.a.batch.N + k.start) * a.a.G * (int64_t)a.key_room;
+}
+
+// The scores of a range of keys: every wave takes 32 keys at a time of its own, as in
+// the paged attention: whole rows from memory, past the caches, through the wave's own LDS.
+template <int D, bool F16>
+__global__ __launch_bounds__(256, 3) void key_scores_kernel(const KeyMass a) {
+  constexpr int STR = D + 8, LROWS = 512 / D, LI = kFewTile / LROWS;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[4][kFewTile * STR];
+  __shared__ float2 sums[4][2][kFewTile];
+  const PagedAttn& p = a.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int l32 = lane & 31, hl = lane >> 5, lr = lane / (D / 8), lc = lane % (D / 8);
+  uint16_t* mine = lds[wave];
+  for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
+    const int64_t at = unit / p.Hkv;
+    const int g = (int)(unit - at * p.Hkv);
+    KeyTile k;
+    if (!find_range(a, at, a.range, lane, k)) return;
+    const int rows = k.n * p.G;
+    const int r = l32 < rows ? l32 : rows - 1, t = p.by_group.of(r), h = g * p.G + r - t * p.G;
+    const int qpos = clip(k.pos0 + t);
+    const uint16_t* src =
+        static_cast<const uint16_t*>(p.q) + (int64_t)(k.start + t) * p.qs[0] + (int64_t)h * p.qs[1] + 8 * hl;
+    u32x4 held[D / 16];
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) held[kk] = load16(src + 16 * kk);
+    const int k0 = k.tile * a.range + kFewTile * wave;
+    const int k1 = (k.tile + 1) * a.range < k.len ? (k.tile + 1) * a.range : k.len;
+    const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)g * p.ks[1] + 8 * lc;
+    float* out = scores_of(a, k, g) + l32 * kFewTile + 4 * hl;
+    const int first_pos = uniform(clip(k.pos0));
+    // The next tile of keys in flight, its table entries looked up a tile before.  (Two tiles in
+    // flight: 333 us where one took 327.)
+    constexpr int STEP = 4 * kFewTile;
+    u32x4 x[LI];
+    int entry, ahead;
+    auto look_up = [&](int key0) { return page_entry(p.batch, k.s, nearest(key0 + l32, k.len)); };
+    auto load = [&](int key0, int e) {
+#pragma unroll
+      for (int i = 0; i < LI; ++i) {
+        const int from = __shfl(e, i * LROWS + lr);
+        const int key = nearest(key0 + i * LROWS + lr, k.len);
+        const int slot = key - page_of(p.batch, key) * p.batch.page;
+        x[i] = load16_once(kbase + (int64_t)(is_page(p.batch, from) ? from : 0) * p.ks[0] + (int64_t)slot * p.ks[2]);
+      }
+    };
+    Sum sum;
+    if (k0 < k1) {
+      entry = look_up(k0);
+      load(k0, entry);
+      ahead = look_up(k0 + STEP);
+    }
+    for (int key0 = k0; key0 < k1; key0 += STEP) {
+      uint32_t have = (uint32_t)__ballot(is_page(p.batch, entry));
+      if (k.len - key0 < kFewTile) have &= (1u << (k.len - key0)) - 1;
+#pragma unroll
+      for (int i = 0; i < LI; ++i) *reinterpret_cast<u32x4*>(mine + (i * LROWS + lr) * STR + 8 * lc) = x[i];
+      wave_lds_fence();
+      entry = ahead;
+      if (key0 + STEP < k1) {
+        load(key0 + STEP, entry);
+        ahead = look_up(key0 + 2 * STEP);
+      }
+      f32x16_t s = {};
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint4 row = *reinterpret_cast<const uint4*>(mine + l32 * STR + 8 * hl + 16 * kk);
+        s = mfma32x32x16<F16>(row, __builtin_bit_cast(uint4, held[kk]), s);
+      }
+      wave_lds_fence();
+      if (have != 0xffffffffu || key0 + kFewTile - 1 > first_pos) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!(have >> row_of(i, lane) & 1) || key0 + row_of(i, lane) > qpos) s[i] = -INFINITY;
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      float now = sum.l == 0.f ? mx : fmaxf(sum.m, mx);
+      if (now == -INFINITY) now = 0.f;  // nothing yet, but perhaps NaN
+      float l = sum.l == 0.f ? 0.f : sum.l * weight_of(sum.m - now, p.cs, a.cs_low);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) l += weight_of(s[i] - now, p.cs, a.cs_low);
+      sum.m = now;
+      sum.l = l;
+      if (l32 < rows) {
+        float* to = out + (int64_t)(key0 / kFewTile) * rows * kFewTile;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f32x4_t*>(to + 8 * i) = f32x4_t{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+      }
+    }
+    sums[wave][hl][l32] = float2{sum.m, sum.l};
+    __syncthreads();
+    if (wave == 0 && hl == 0 && l32 < rows) {
+      Sum all;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) all.join(sums[i >> 1][i & 1][l32].x, sums[i >> 1][i & 1][l32].y, p.cs);
+      a.few_stats[((int64_t)(k.start + t) * a.Hq + h) * a.ranges + k.tile] = float2{all.m, all.l};
+    }
+    __syncthreads();
+  }
+}
+
+// The weights of 1024 keys, four a thread, from their scores.
+constexpr int kWeightKeys = 1024;
+__global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
+  __shared__ float2 parts[8][kFewTile], row[kFewTile];
+  const PagedAttn& p = a.a;
+  const int tid = threadIdx.x, lane = tid & 63;
+  for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
+    const int64_t at = unit / p.Hkv;
+    const int g = (int)(unit - at * p.Hkv);
+    KeyTile k;
+    if (!find_range(a, at, kWeightKeys, lane, k)) return;
+    const int rows = k.n * p.G, ranges = (k.len + a.range - 1) / a.range;
+    {
+      const int r = tid % kFewTile, t = p.by_group.of(r), h = g * p.G + r - t * p.G;
+      Sum sum;
+      if (r < rows) {
+        const float2* st = a.few_stats + ((int64_t)(k.start + t) * a.Hq + h) * a.ranges;
+        for (int i = tid / kFewTile; i < ranges; i += 8) sum.join(st[i].x, st[i].y, p.cs);
+      }
+      parts[tid / kFewTile][r] = float2{sum.m, sum.l};
+      __syncthreads();
+      if (tid < kFewTile) {
+        Sum all;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) all.join(parts[i][tid].x, parts[i][tid].y, p.cs);
+        row[tid] = float2{all.m, all.l == 0.f ? 0.f : 1.f / all.l};
+      }
+      __syncthreads();
+    }
+    const float* scores = scores_of(a, k, g);
+    int key[4], entry[4];
+    const float* from[4];
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      key[i] = k.tile * kWeightKeys + i * 256 + tid;
+      const int in = nearest(key[i], k.len);
+      entry[i] = page_entry(p.batch, k.s, in);
+      from[i] = scores + (int64_t)(in / kFewTile) * rows * kFewTile + in % kFewTile;
+    }
+#pragma unroll 2
+    for (int r = 0; r < rows; ++r) {
+      const float2 ml = row[r];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sum[i] += weight_of(from[i][r * kFewTile] - ml.x, p.cs, a.cs_low) * ml.y;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (key[i] >= k.len || !is_page(p.batch, entry[i])) continue;
+      const int slot = key[i] - page_of(p.batch, key[i]) * p.batch.page;
+      float* to = a.mass + (int64_t)entry[i] * a.ms[0] + (int64_t)g * a.ms[1] + (int64_t)slot * a.ms[2];
+      *to = a.accumulate && key[i] < k.pos0 ? *to + sum[i] : sum[i];
+    }
+    __syncthreads();
+  }
+}
+
 struct MassPlan {
-  int64_t tiles, parts;
+  bool few, many;
+  int64_t tiles, parts;  // row tiles that a batch can have, and the parts of the keys of each
+  int64_t range, ranges, key_room;
+  int64_t many_bytes, few_stats_bytes, score_bytes;
+  int64_t bytes() const { return many_bytes + few_stats_bytes + score_bytes; }
 };
-// Row tiles that a batch can have, and the parts of the keys of each: four
-// workgroups a CU, of at least 256 keys.
 MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) {
   const int64_t G = Hq / Hkv;
-  MassPlan plan;
-  plan.tiles = N * G / kRowsOf + (S < N ? S : N);
-  int64_t parts = 4 * kCus / (plan.tiles * Hkv > 0 ? plan.tiles * Hkv : 1);
-  const int64_t most = (keys + 255) / 256;
-  if (parts > most) parts = most;
-  if (parts > 64) parts = 64;
-  plan.parts = parts < 1 ? 1 : parts;
+  MassPlan plan{};
+  // As in the attention's plan: the lengths are not known here, but every sequence has a new token
+  // in all but odd batches.
+  const int64_t longest = N > S ? N - S + 1 : 1;
+  plan.key_room = (keys + kFewTile - 1) / kFewTile * kFewTile;
+  plan.few = (N * G <= S * kFewTile || S > 8) && G <= kFewTile && N * Hq * plan.key_room <= kMostScores;
+  plan.many = !plan.few || longest * G > kFewTile;
+  if (plan.few) {
+    // Ranges of 1024 keys, fewer where that leaves CUs without one.
+    plan.range = kMostRange;
+    while (plan.range > 4 * kFewTile && S * Hkv * ((keys + plan.range - 1) / plan.range) < 4 * kCus) plan.range /= 2;
+    plan.ranges = (keys + plan.range - 1) / plan.range;
+    plan.score_bytes = N * Hq * plan.key_room * 4;
+    plan.few_stats_bytes = (N * Hq * plan.ranges * 8 + 15) / 16 * 16;
+  }
+  if (plan.many) {
+    // Four workgroups a CU, of at least 256 keys.
+    plan.tiles = N * G / kRowsOf + (S < N ? S : N);
+    int64_t parts = 4 * kCus / (plan.tiles * Hkv > 0 ? plan.tiles * Hkv : 1);
+    const int64_t most = (keys + 255) / 256;
+    if (parts > most) parts = most;
+    if (parts > 64) parts = 64;
+    plan.parts = parts < 1 ? 1 : parts;
+    plan.many_bytes = (N * Hq * plan.parts * 8 + 15) / 16 * 16;
+  }
   return plan;
 }
 
@@ -418,7 +670,7 @@ using namespace spruce;
 
 extern "C" int64_t spruce_paged_key_mass_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) {
   if (N < 1 || S < 1 || Hkv < 1 || Hq < Hkv || N >= (int64_t)1 << 30 || S >= (int64_t)1 << 20 || Hq >= 1 << 16) return 0;
-  return N * Hq * mass_plan(N, S, Hq, Hkv, keys).parts * (int64_t)sizeof(float2);
+  return mass_plan(N, S, Hq, Hkv, keys).bytes();
 }
 
 extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, void* stream) {
@@ -441,7 +693,7 @@ extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, voi
   const int rc = prepare_batch(m.a.batch, a.page_table, a.table_stride, a.table_width, a.q_starts, a.kv_lens, S, N,
                                a.page_size, a.pages);
   if (rc) return rc;
-  if (N == 0 || a.pages == 0) return SPRUCE_OK;
+  if (N == 0 || a.pages == 0 || m.a.batch.cap == 0) return SPRUCE_OK;
   SPRUCE_REQUIRE(a.q && a.k_pages && a.mass_pages, "q and the pages must be non-null device pointers");
   auto rows16 = [](const void* ptr, const int64_t* s, int n) {
     if (reinterpret_cast<uintptr_t>(ptr) % 16) return false;
@@ -455,7 +707,7 @@ extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, voi
   const int64_t sizes[3] = {a.pages, Hkv, a.page_size};
   SPRUCE_REQUIRE(rows_apart(a.mps, sizes, 3, 1), "the values of mass_pages overlap");
   const MassPlan plan = mass_plan(N, S, Hq, Hkv, m.a.batch.cap);
-  const int64_t need = N * Hq * plan.parts * (int64_t)sizeof(float2);
+  const int64_t need = plan.bytes();
   SPRUCE_REQUIRE(a.workspace && a.workspace_bytes >= need, "workspace too small: %lld bytes, need %lld",
                  (long long)a.workspace_bytes, (long long)need);
   SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0, "workspace must be 16-byte aligned");
@@ -473,22 +725,39 @@ extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, voi
   m.a.by_heads = divisor(Hkv);
   m.a.by_group = divisor(Hq / Hkv);
   m.a.cs = cs;
-  m.a.few_limit = -1;
+  m.a.few_limit = plan.few ? kFewTile : -1;
   m.mass = a.mass_pages;
-  m.stats = static_cast<float2*>(a.workspace);
   m.Hq = (int)Hq;
-  m.parts = (int)plan.parts;
   m.accumulate = a.accumulate != 0;
+  char* work = static_cast<char*>(a.workspace);
+  m.stats = reinterpret_cast<float2*>(work);
+  m.parts = (int)plan.parts;
+  m.few_stats = reinterpret_cast<float2*>(work + plan.many_bytes);
+  m.scores = reinterpret_cast<float*>(work + plan.many_bytes + plan.few_stats_bytes);
+  m.few_rows = kFewTile;
+  m.range = (int)plan.range;
+  m.ranges = (int)plan.ranges;
+  m.key_room = (int)plan.key_room;
+  m.cs_low = (float)(a.scale * 1.44269504088896340736 - (double)cs);
   const hipStream_t st = (hipStream_t)stream;
   const int64_t units = plan.tiles * plan.parts * Hkv;
   SPRUCE_REQUIRE(units < (int64_t)1 << 31, "too many tokens for one call");
-  int64_t key_units = (int64_t)S * ((m.a.batch.cap + kRowsOf - 1) / kRowsOf) * Hkv;
-  if (key_units > 8 * kCus) key_units = 8 * kCus;  // each takes more than one where there are more
-  if (key_units < 1) return SPRUCE_OK;             // a table of no page
+  // Workgroups take more than one unit where there are more.
+  auto grid = [&](int64_t keys, int64_t most) {
+    const int64_t all = S * ((m.a.batch.cap + keys - 1) / keys) * Hkv;
+    return dim3((unsigned)(all < most ? all : most));
+  };
 #define SPRUCE_KEY_MASS(D_, F16_)                                                                              \
   do {                                                                                                         \
-    hipLaunchKernelGGL((key_mass_rows_kernel<D_, F16_>), flat_grid(units), dim3(256), 0, st, m);               \
-    hipLaunchKernelGGL((key_mass_keys_kernel<D_, F16_>), dim3((unsigned)key_units), dim3(256), 0, st, m);      \
+    if (plan.many) {                                                                                           \
+      hipLaunchKernelGGL((key_mass_rows_kernel<D_, F16_>), flat_grid(units), dim3(256), 0, st, m);             \
+      if (plan.parts > 1)                                                                                      \
+        hipLaunchKernelGGL(key_mass_join_kernel, flat_grid((N * Hq + 255) / 256), dim3(256), 0, st, m.stats,   \
+                           N * Hq, m.parts, cs);                                                               \
+      hipLaunchKernelGGL((key_mass_keys_kernel<D_, F16_>), grid(kRowsOf, 8 * kCus), dim3(256), 0, st, m);      \
+    }                                                                                                          \
+    if (plan.few)                                                                                              \
+      hipLaunchKernelGGL((key_scores_kernel<D_, F16_>), grid(plan.range, 16 * kCus), dim3(256), 0, st, m);     \
   } while (0)
   if (D == 128) {
     if (dtype == SPRUCE_DTYPE_F16) SPRUCE_KEY_MASS(128, true);
@@ -498,5 +767,6 @@ extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, voi
     else SPRUCE_KEY_MASS(64, false);
   }
 #undef SPRUCE_KEY_MASS
+  if (plan.few) hipLaunchKernelGGL(key_weights_kernel, grid(kWeightKeys, 16 * kCus), dim3(256), 0, st, m);
   return check_launch("paged key mass");
 }

@@ -29,7 +29,7 @@ __all__ = ["evict_paged_kv", "paged_key_mass"]
 
 # struct spruce_paged_key_mass_args and spruce_paged_evict_args, field by field.
 _MASS_ARGS = struct.Struct("=q3qq4qq3qqqqqqqqqqqqqqdqqq")
-_EVICT_ARGS = struct.Struct("=q4qq4qq3qqqqqqqqqqqqqqqqqqq")
+_EVICT_ARGS = struct.Struct("=q4qq4qq3qqqqqqqqqqqqqqqqqqqqq")
 
 
 def _check_pages(k_pages, mass_pages, page_table, kv_lens, device):
@@ -58,6 +58,11 @@ def _check_pages(k_pages, mass_pages, page_table, kv_lens, device):
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(*shape):
     return spruce_hip.lib().spruce_paged_key_mass_workspace_bytes(*shape)
+
+
+@functools.lru_cache(maxsize=1024)
+def _evict_workspace_bytes(*shape):
+    return spruce_hip.lib().spruce_paged_evict_workspace_bytes(*shape)
 
 
 def paged_key_mass(q, k_pages, mass_pages, page_table, q_starts, kv_lens, scale, *, accumulate=True):
@@ -160,12 +165,14 @@ def evict_paged_kv(k_pages, v_pages, mass_pages, page_table, kv_lens, out_table,
         raise RuntimeError("the paged HIP backend requires GPU tensors")
     kept = kv_lens.new_empty_strided((S, Hkv, keep), (Hkv * keep, keep, 1))
     lens = kv_lens.new_empty_strided((S,), (1,))
+    need = _evict_workspace_bytes(S, Hkv, W * page_size)
+    work = kv_lens.new_empty_strided((need,), (1,), dtype=torch.uint8) if need else None
     with spruce_hip.on_device(device):
         rc = spruce_hip.lib().spruce_paged_evict(_EVICT_ARGS.pack(
             k_pages.data_ptr(), *k_pages.stride(), v_pages.data_ptr(), *v_pages.stride(), mass_pages.data_ptr(),
             *mass_pages.stride(), pages, page_size, page_table.data_ptr(), page_table.stride()[0] if S > 1 else W, W,
             kv_lens.data_ptr(), S, Hkv, D, code, out_table.data_ptr(), out_table.stride()[0] if S > 1 else W2, W2,
-            keep, first, recent, kept.data_ptr(), lens.data_ptr()), spruce_hip.raw_stream(device.index))
+            keep, first, recent, kept.data_ptr(), lens.data_ptr(), work.data_ptr() if need else 0, need), spruce_hip.raw_stream(device.index))
     if rc:
         spruce_hip.check(rc, "spruce_paged_evict")
     return kept, lens

@@ -131,7 +131,7 @@ def test_entry_points_refuse_before_the_launch():
               width=2, out=FAKE, at=FAKE, k=FAKE, kept=FAKE, S=2, page=16):
         return _call("spruce_paged_evict", eviction._EVICT_ARGS, (
             k, *kps, FAKE, 4096, 2048, 128, 1, at, *mps, 9, page, FAKE, 4, 4, FAKE, S, Hkv, D, dtype, out, stride, width,
-            keep, first, recent, kept, FAKE))
+            keep, first, recent, kept, FAKE, 0, 0))
     for kwargs, message in ((dict(D=96), "head_dim 64 or 128"), (dict(dtype=3), "dtype"), (dict(Hkv=0), "KV head"),
                             (dict(keep=0), "keep"), (dict(keep=1 << 30), "keep"), (dict(first=-1), "first"),
                             (dict(first=18), "first"), (dict(kps=(4096, 2048, 128, 2)), "contiguous final"),
