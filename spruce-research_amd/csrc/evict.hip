@@ -303,18 +303,23 @@ __global__ __launch_bounds__(kSelectThreads) void evict_end_kernel(const Evict e
     const int shift = level == 1 ? kShift[1] : kShift[2];
     const uint32_t bits = level == 2 ? 1023u : 2047u;
     clear_hist(sh);
-    for (int p = 0; p < parts; ++p)
-      for (int i = tid; i < part_of[p].listed; i += kSelectThreads) {
+    for (int p = wave; p < parts; p += kSelectWaves) {
+      const int n = part_of[p].listed;
+#pragma unroll 4
+      for (int i = lane; i < n; i += 64) {
         const uint32_t key = listed[(int64_t)p * kPartKeys + i];
         if ((key & mask) == prefix) atomicAdd(&sh.hist[key >> shift & bits], 1u);
       }
+    }
     __syncthreads();
     prefix |= find_digit(sh, need) << shift;
     mask |= bits << shift;
   }
   for (int p = wave; p < parts; p += kSelectWaves) {
     int larger = 0, equal = 0;
-    for (int i = lane; i < part_of[p].listed; i += 64) {
+    const int n = part_of[p].listed;
+#pragma unroll 4
+    for (int i = lane; i < n; i += 64) {
       const uint32_t key = listed[(int64_t)p * kPartKeys + i];
       larger += key > prefix;
       equal += key == prefix;

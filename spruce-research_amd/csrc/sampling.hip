@@ -126,31 +126,34 @@ struct Row {
   }
 };
 
-// exp((x - max) / T) = 2^(n / 64) e^z: n by adding what leaves no bits for a
-// fraction, the power from a table and n's upper bits, and a polynomial in z,
-// |z| <= ln 2 / 128, so that the next term, z^5 / 120, is below 2^-44.
+// exp((x - max) / T) = 2^(n / 64) 2^(r / 64): n by adding what leaves no bits for a fraction, its power
+// from a table, with n's upper bits added to the exponent (and its lower six taken off in the table), and a
+// polynomial in r, |r| <= 1 / 2, of ln 2 / 64 so small that the next term is below 2^-44.
 struct Weights {
-  double max, inv, steps, lowest;  // 1 / T, 64 log2(e) / T, and the difference past which weights are nothing
-  double shift;                    // 2^52 units
-  const uint64_t* table;
-  // (-inf comes out below half a unit.)
+  double max, steps, lowest;  // 64 log2(e) / T, and the difference past which weights are nothing
+  double shift;               // 2^52 units
+  const uint2* table;
+  // (-inf comes out below half a unit.  No product is fused with the sum of units(): a weight's units are the same
+  // wherever they are formed, so that sums of some hold against sums of all.)
   __device__ __forceinline__ double of(float x) const {
+#pragma clang fp contract(off)
     // The difference first: of the largest logit it is zero whatever T is.
     const double d = fmax((double)x - max, lowest);
-    constexpr double kWhole = 0x1.8p+52;
+    constexpr double kWhole = 0x1.8p+52, kStep = 0.69314718055994530942 / kTable;
     const double t = fma(d, steps, kWhole);
-    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
-    const double z = fma(t - kWhole, -0.69314718055994530942 / kTable, d * inv);
-    const double e = fma(z, fma(z, fma(z, fma(z, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0);
-    return e * __builtin_bit_cast(double, table[n & (kTable - 1)] + ((uint64_t)(uint32_t)(n >> 6) << 52));
+    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
+    const double r = fma(d, steps, kWhole - t);
+    const double e = fma(r, fma(r, fma(r, fma(r, kStep * kStep * kStep * kStep / 24, kStep * kStep * kStep / 6), kStep * kStep / 2), kStep), 1.0);
+    const uint2 p = table[n & (kTable - 1)];
+    return e * __builtin_bit_cast(double, (uint64_t)(p.y + (n << 14)) << 32 | p.x);
   }
   __device__ __forceinline__ uint64_t units(double w) const {
+#pragma clang fp contract(off)
     // Rounded to units as it is added to what has one as its last bit.
     return __builtin_bit_cast(uint64_t, w + shift) - __builtin_bit_cast(uint64_t, shift);
   }
   // Those of eight, kept where they are for the compiler: moved under the conditions
-  // of their use they follow one another, each with its chain's latency (a pass over 150016
-  // logits 55 us).
+  // of their use they follow one another, each with its chain's latency.
   __device__ __forceinline__ void of8(const float (&x)[kChunk], double (&w)[kChunk]) const {
 #pragma unroll
     for (int i = 0; i < kChunk; ++i) w[i] = of(x[i]);
@@ -172,17 +175,18 @@ __device__ __forceinline__ float uniform(float x) {
 }
 
 struct Shared {
-  uint64_t table[kTable];
+  uint2 table[kTable];
   uint64_t weight[kBins];
-  uint32_t count[kBins];
   uint64_t list[kList];     // order << 32 | ~place
   uint64_t part[kParts];
   Small small[64];
   uint64_t waves[kRowWaves];
-  uint64_t result[4];
-  uint32_t size, lo, hi;
-  float top, least;
-  int infinite;
+  uint64_t result[3];
+  uint32_t size;
+  // What the long way goes on with.
+  float top;
+  int infinite, bin;        // of the first end by weight or count; -1: none yet
+  uint64_t before, total;   // of the bin, and of all weights
 };
 
 // Sums of a over the threads up to and with this one, and their total.  Ends with a barrier to come.
@@ -287,10 +291,24 @@ struct Sampler {
   bool infinite;   // the largest logit is +inf: such are taken as 0, all others as -inf
   float top, per_bin;
 
-  __device__ __forceinline__ float bin_at(float x) const { return (x == top ? 0.f : top - x) * per_bin; }
+  // Ranges of logits that the histogram tells apart, from the top down.
   __device__ __forceinline__ int bin_of(float x) const {
-    const float b = bin_at(x);
-    return b < (float)(kBins - 1) ? (int)b : kBins - 1;
+    return (int)fminf((top - x) * per_bin, (float)(kBins - 1));
+  }
+  // The smallest logit in a bin, or above it: 64 orders tried at once.
+  __device__ __forceinline__ float bin_end(int bin) const {
+    if (bin >= kBins - 1) return -3.402823466e+38f;
+    uint32_t lo = ordered(-INFINITY), hi = ordered(top);  // lo is past the bin, hi is not
+    while (hi - lo > 1) {
+      const uint32_t step = (hi - lo) / 65 + 1, rest = hi - lo, mine = step * ((threadIdx.x & 63) + 1);
+      const uint64_t in = __ballot(mine >= rest || bin_of(unordered(lo + mine)) <= bin);
+      // (step * 64 may fall short of hi, which is within.)
+      const uint32_t first = in ? (uint32_t)__builtin_ctzll(in) : 64;
+      const uint32_t to = step * (first + 1);
+      hi = to < rest ? lo + to : hi;
+      lo += step * first;
+    }
+    return uniform(unordered(hi));
   }
   __device__ __forceinline__ void decode(const typename Row<T>::Raw& raw, float (&x)[kChunk]) const {
     Row<T>::decode(raw, x);
@@ -345,17 +363,20 @@ struct Sampler {
         }
     }
   }
-  // Lists what `is` names; false where there are more than fit.
-  template <typename F>
-  __device__ __forceinline__ bool collect(F is) const {
+  // Lists the logits from `low` to `high`, within `limit`; false where there are more than fit.
+  __device__ __forceinline__ bool collect(float low, float high, const Cut& limit) const {
     __syncthreads();
     if (threadIdx.x == 0) sh.size = 0;
     __syncthreads();
+    const bool limited = limit.key != 0;
     chunks_while<T::bytes == 2 ? 4 : 2>([&](const float (&x)[kChunk], int at) {
       uint32_t bits = 0;
-      if (is(largest(x), at)) {
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) bits |= (uint32_t)((x[i] > -INFINITY) & is(x[i], at + i)) << i;
+      for (int i = 0; i < kChunk; ++i) bits |= (uint32_t)((x[i] >= low) & (x[i] <= high)) << i;
+      if (limited && bits) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i)
+          if (!within(limit, ordered(x[i]), (uint32_t)(at + i))) bits &= ~(1u << i);
       }
       append(x, at, bits);
     }, [&] { return *(volatile uint32_t*)&sh.size <= kList; });
@@ -364,11 +385,8 @@ struct Sampler {
   }
   __device__ __forceinline__ void clear_bins() const {
     __syncthreads();
-#pragma unroll
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-      sh.count[i] = 0;
-      sh.weight[i] = 0;
-    }
+    sh.weight[threadIdx.x] = 0;
+    sh.weight[threadIdx.x + kThreads] = 0;
     __syncthreads();
   }
   // This thread's entries of the list.
@@ -378,158 +396,99 @@ struct Sampler {
     for (int i = 0; i < kEach; ++i) key[i] = i * kThreads + threadIdx.x < n ? sh.list[i * kThreads + threadIdx.x] : 0;
   }
 
-  // The first bin with which the histogram's counts (by_count), or weights, are above `target`, or the last that
-  // holds anything; above and above_mass go on to what is before it.
-  __device__ __forceinline__ int find_bin(bool by_count, uint64_t target, uint32_t& above, uint64_t& above_mass) {
+  // The first bin with which the histogram's sum, `before` it, is above `target`, or the last that holds
+  // anything; `before` goes on to what is before the bin, `all` gets the whole.
+  __device__ __forceinline__ int find_bin(uint64_t target, uint64_t& before, uint64_t& all) {
     const int at = 2 * threadIdx.x;
-    const uint32_t c0 = sh.count[at], c1 = sh.count[at + 1];
     const uint64_t w0 = sh.weight[at], w1 = sh.weight[at + 1];
-    uint64_t all_a, all_b;
-    const uint64_t a0 = above_mass + block_prefix(sh, w0 + w1, all_a) - w0 - w1;
-    const uint64_t b0 = above + block_prefix(sh, (uint64_t)c0 + c1, all_b) - c0 - c1;
-    const uint64_t all = by_count ? above + all_b : above_mass + all_a;
+    const uint64_t from = before + block_prefix(sh, w0 + w1, all) - w0 - w1;
+    all += before;
     if (target >= all) target = all - 1;
-    const uint64_t before = by_count ? b0 : a0, v0 = by_count ? c0 : w0, v1 = by_count ? c1 : w1;
-    if (before <= target && target < before + v0 + v1) {
-      const bool second = target >= before + v0;
+    if (from <= target && target < from + w0 + w1) {
+      const bool second = target >= from + w0;
       sh.result[0] = at + (second ? 1 : 0);
-      sh.result[1] = a0 + (second ? w0 : 0);
-      sh.result[2] = b0 + (second ? c0 : 0);
+      sh.result[1] = from + (second ? w0 : 0);
     }
     __syncthreads();
     const int bin = (int)sh.result[0];
-    above_mass = sh.result[1];
-    above = (uint32_t)sh.result[2];
+    before = sh.result[1];
     __syncthreads();
     return bin;
   }
 
-  // Counts, and weights, of the logits within `limit`.
-  template <bool WEIGHTS>
-  __device__ __forceinline__ void histogram(const Cut& limit) {
+  // Weights of the logits within `limit`, or their number.
+  __device__ __forceinline__ void weigh(const Cut& limit) {
     clear_bins();
+    const bool limited = limit.key != 0;
     chunks<2>([&](const float (&x)[kChunk], int at) {
       double weight[kChunk];
-      if (WEIGHTS) w.of8(x, weight);
+      w.of8(x, weight);
+      if (limited) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i)
+          if (!within(limit, ordered(x[i]), (uint32_t)(at + i))) weight[i] = 0.0;
+      }
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) {
-        if (!(x[i] > -INFINITY) || !within(limit, ordered(x[i]), (uint32_t)(at + i))) continue;
-        const int bin = bin_of(x[i]);
-        atomicAdd(&sh.count[bin], 1u);
-        if (WEIGHTS) atomicAdd((unsigned long long*)&sh.weight[bin], (unsigned long long)w.units(weight[i]));
+        const uint64_t units = w.units(weight[i]);
+        if (units) atomicAdd((unsigned long long*)&sh.weight[bin_of(x[i])], (unsigned long long)units);
       }
     });
     __syncthreads();
   }
-
-  // The long way to the end of a prefix: that of the logits within `limit` whose count (by_count), or
-  // weight, is the first above `target`.  It ends in bin `bin`, `above` and
-  // `above_mass` before it.  Its weight in *total.
-  __device__ __forceinline__ Cut resolve(int bin, bool by_count, uint64_t target, uint32_t above, uint64_t above_mass, const Cut& limit,
-                         uint64_t* total) {
+  __device__ __forceinline__ void count() {
+    clear_bins();
+    chunks<T::bytes == 2 ? 4 : 2>([&](const float (&x)[kChunk], int) {
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i)
+        if (x[i] > -INFINITY) atomicAdd((unsigned long long*)&sh.weight[bin_of(x[i])], 1ull);
+    });
     __syncthreads();
-    if (threadIdx.x == 0) {
-      sh.lo = 0xffffffffu;
-      sh.hi = 0;
-    }
-    uint32_t lo = 0, hi = 0xffffffffu;
-    auto members = [&](float x, uint32_t key, uint32_t at) {
-      return (x > -INFINITY) & (bin_of(x) == bin) & (key >= lo) & (key <= hi) & within(limit, key, at);
-    };
-    // f(logit, place) of the members; chunks that cannot hold one are passed over.
-    auto each_member = [&](auto f) {
-      chunks<T::bytes == 2 ? 4 : 2>([&](const float (&x)[kChunk], int at) {
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) any |= (x[i] > -INFINITY) & (bin_of(x[i]) == bin);
-        if (any) {
-#pragma unroll
-          for (int i = 0; i < kChunk; ++i)
-            if (members(x[i], ordered(x[i]), (uint32_t)(at + i))) f(x[i], at + i);
-        }
-      });
-    };
-    if (sh.count[bin] > kList) {
-      // As a range of orders.
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        sh.lo = 0xffffffffu;
-        sh.hi = 0;
-      }
-      __syncthreads();
-      uint32_t least = 0xffffffffu, most = 0;
-      each_member([&](float x, int) {
-        const uint32_t key = ordered(x);
-        least = key < least ? key : least;
-        most = key > most ? key : most;
-      });
-      atomicMin(&sh.lo, least);
-      atomicMax(&sh.hi, most);
-      __syncthreads();
-      lo = sh.lo;
-      hi = sh.hi;
-    }
+  }
+
+  // The long way to the end of a prefix: that of the logits within `limit` whose number (by_count), or
+  // weight, is the first above `target`.  It ends in bin `bin`, `before` before it.
+  __device__ __forceinline__ Cut resolve(int bin, bool by_count, uint64_t target, uint64_t before, const Cut& limit) {
+    uint32_t lo = ordered(bin_end(bin)), hi = bin == 0 ? ordered(top) : ordered(bin_end(bin - 1)) - 1;
     // Narrowed until its members can be listed, or are of one value.
     bool fits;
-    while (true) {
-      __syncthreads();
-      if (threadIdx.x == 0) sh.size = 0;
-      __syncthreads();
-      chunks<T::bytes == 2 ? 4 : 2>([&](const float (&x)[kChunk], int at) {
-        uint32_t bits = 0;
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) bits |= (uint32_t)members(x[i], ordered(x[i]), (uint32_t)(at + i)) << i;
-        append(x, at, bits);
-      });
-      __syncthreads();
-      fits = sh.size <= kList;
-      if (fits || lo == hi) break;
+    while (!(fits = collect(unordered(lo), unordered(hi), limit)) && lo < hi) {
       int shift = 0;
       while ((hi - lo) >> shift >= kBins) ++shift;
       clear_bins();
-      each_member([&](float x, int at) {
-        const int b = (int)((hi - ordered(x)) >> shift);
-        atomicAdd(&sh.count[b], 1u);
-        atomicAdd((unsigned long long*)&sh.weight[b], (unsigned long long)w.units(w.of(x)));
+      const float low = unordered(lo), high = unordered(hi);
+      chunks<2>([&](const float (&x)[kChunk], int at) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+          const uint32_t key = ordered(x[i]);
+          if (!((x[i] >= low) & (x[i] <= high)) || !within(limit, key, (uint32_t)(at + i))) continue;
+          const uint64_t units = by_count ? 1 : w.units(w.of(x[i]));
+          atomicAdd((unsigned long long*)&sh.weight[(hi - key) >> shift], (unsigned long long)units);
+        }
       });
       __syncthreads();
-      const uint32_t b = (uint32_t)find_bin(by_count, target, above, above_mass);
+      uint64_t all;
+      const uint32_t b = (uint32_t)find_bin(target, before, all);
       hi -= b << shift;
       lo = hi - lo < (1u << shift) ? lo : hi - ((1u << shift) - 1);
     }
     if (!fits) {
       // One value: the first so many by place.
-      const uint32_t n = sh.size;
-      const uint64_t one = w.units(w.of(unordered(hi)));
-      uint64_t more = by_count ? target - above : (one == 0 ? 0 : (target - above_mass) / one);
-      if (more >= n) more = n - 1;
-      *total = above_mass + (more + 1) * one;
-      __syncthreads();
+      const uint64_t one = by_count ? 1 : w.units(w.of(unordered(hi)));
+      const uint64_t more = one == 0 ? 0 : (target - before) / one;
       return Cut{hi, nth_equal(hi, more, limit)};
     }
-    uint64_t key[kEach], ones[kEach], units[kEach], all = 0;
+    uint64_t key[kEach], ones[kEach], all = 0;
     entries(key);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      ones[i] = key[i] != 0;
-      units[i] = key[i] ? w.units(w.of(unordered((uint32_t)(key[i] >> 32)))) : 0;
-      if (!by_count) ones[i] = units[i];
+      ones[i] = key[i] == 0 ? 0 : (by_count ? 1 : w.units(w.of(unordered((uint32_t)(key[i] >> 32)))));
       all += ones[i];
     }
-    const uint64_t from = by_count ? above : above_mass;
     block_prefix(sh, all, all);
-    target = target - from < all ? target - from : all - 1;
-    // The bin's range of values, a little wider than it is.
-    const float slack = 0x1p-20f * (fabsf(top) + (bin + 1) / per_bin);
-    const uint64_t lowest = bin + 1 == kBins ? 0 : (uint64_t)ordered(top - (bin + 1) / per_bin - slack) << 32;
-    const uint64_t highest = (uint64_t)ordered(top - bin / per_bin + slack) << 32 | 0xffffffffu;
-    const uint64_t last = all ? select(sh, key, ones, lowest, highest, target) : 0;
-    uint64_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) mine += key[i] >= last ? units[i] : 0;
-    block_prefix(sh, mine, all);
-    *total = above_mass + all;
-    __syncthreads();
+    if (all == 0) return Cut{lo, 0xffffffffu};  // no weight to choose by
+    target = target - before < all ? target - before : all - 1;
+    const uint64_t last = select(sh, key, ones, (uint64_t)lo << 32, (uint64_t)hi << 32 | 0xffffffffu, target);
     return Cut{(uint32_t)(last >> 32), ~(uint32_t)last};
   }
 
@@ -631,17 +590,16 @@ __device__ __forceinline__ void set_up(Sampler<T>& s, const Sampling& p, int b) 
   s.steps = (s.row.end + kThreads * kChunk - 1) / (kThreads * kChunk);
 }
 template <typename T>
-__device__ __forceinline__ void set_weights(Sampler<T>& s, const Sampling& p, double temperature, float top, float least) {
+__device__ __forceinline__ void set_weights(Sampler<T>& s, const Sampling& p, double temperature, float top) {
   s.top = uniform(top);
   // (An infinite temperature: all weights one, but those of -inf.)
   const double inv = fmin(fmax(1.0 / temperature, 1e-300), 1e+300);
   constexpr double kLog2e = 1.44269504088896340736;
-  s.w = Weights{uniform((double)top), uniform(inv), uniform(kTable * kLog2e * inv), uniform(-60.0 / (kLog2e * inv)),
-                p.shift, s.sh.table};
-  // Bins of equal width down to the smallest logit, or to where weights end.
-  float range = fminf(top - least, (float)(kNothing / (kLog2e * inv)));
-  range = range > 1e-30f ? (range < 1e30f ? range : 1e30f) : 1e-30f;
-  s.per_bin = uniform((float)(kBins - 1) / range);
+  s.w = Weights{uniform((double)top), uniform(kTable * kLog2e * inv), uniform(-60.0 / (kLog2e * inv)), p.shift,
+                s.sh.table};
+  // Bins of equal width down to where weights end.
+  const float range = (float)(kNothing / (kLog2e * inv));
+  s.per_bin = uniform((float)(kBins - 1) / (range > 1e-30f ? (range < 1e30f ? range : 1e30f) : 1e-30f));
 }
 
 // A row that keeps more than the list holds.  A function of its own, which sets
@@ -657,49 +615,52 @@ __device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute_
   set_up(s, p, b);
   __syncthreads();
   s.infinite = spruce::uniform(sh.infinite) != 0;
-  set_weights(s, p, set.temperature, sh.top, sh.least);
+  set_weights(s, p, set.temperature, sh.top);
   Cut cut{0, 0xffffffffu};  // all
-  uint64_t total = 0;
-  if (set.by_k || set.by_p) {
-    if (set.by_k) s.template histogram<true>(cut);  // otherwise as it is
-    uint64_t all = sh.weight[2 * tid] + sh.weight[2 * tid + 1], count = sh.count[2 * tid] + sh.count[2 * tid + 1];
-    block_prefix(sh, all, total);
-    block_prefix(sh, count, count);
-    // First by count, then by weight, of what the first has left.
-    for (int turn = set.by_k && (uint64_t)set.top_k < count ? 0 : 1; turn < (set.by_p ? 2 : 1); ++turn) {
-      const bool by_count = turn == 0;
-      const uint64_t target = by_count ? (uint64_t)set.top_k - 1 : target_of(fmax(set.top_p, 0.0) * (double)total);
-      uint32_t above = 0;
-      uint64_t above_mass = 0;
-      const int bin = s.find_bin(by_count, target, above, above_mass);
-      // (What is behind the last weight has none to choose by.)
-      if (by_count && above_mass >= total) continue;
-      cut = s.resolve(bin, by_count, target, above, above_mass, cut, &all);
-      if (by_count && set.by_p) {
-        total = all;
-        s.template histogram<true>(cut);
-      }
+  int bin = spruce::uniform(sh.bin);
+  uint64_t total = sh.total, before = sh.before;
+  if (set.by_k) {
+    const uint64_t target = (uint64_t)set.top_k - 1;
+    uint64_t all = target + 1;
+    if (bin < 0) {
+      s.count();
+      before = 0;
+      bin = s.find_bin(target, before, all);
+    }
+    if (target < all) cut = s.resolve(bin, true, target, before, cut);  // else all there are
+    if (set.by_p) {
+      s.weigh(cut);
+      before = 0;
+      uint64_t mine = sh.weight[tid] + sh.weight[tid + kThreads];
+      block_prefix(sh, mine, total);
+      bin = s.find_bin(target_of(fmax(set.top_p, 0.0) * (double)total), before, all);
     }
   }
-  // The kept weights of eight logits.
-  auto weights_at = [&](const float (&x)[kChunk], int at, uint64_t (&units)[kChunk]) {
-    double weight[kChunk];
+  if (set.by_p) cut = s.resolve(bin, false, target_of(fmax(set.top_p, 0.0) * (double)total), before, cut);
+  // The weights of eight logits, zero where they are not kept.
+  const float end = unordered(cut.key);
+  auto weights_at = [&](const float (&x)[kChunk], int at, double (&weight)[kChunk]) {
     s.w.of8(x, weight);
     if (cut.key) {
 #pragma unroll
       for (int j = 0; j < kChunk; ++j)
-        if (!within(cut, ordered(x[j]), (uint32_t)(at + j))) weight[j] = -1.0;
+        if (!((x[j] > end) | ((x[j] == end) & ((uint32_t)(at + j) <= cut.last)))) weight[j] = 0.0;
     }
+    if (set.min_p > 0.0) {
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) units[j] = s.w.units(weight[j] >= set.min_p ? weight[j] : 0.0);
+      for (int j = 0; j < kChunk; ++j)
+        if (weight[j] < set.min_p) weight[j] = 0.0;
+    }
   };
   s.template chunks<2>([&](const float (&x)[kChunk], int at) {
     uint64_t sum = 0;
-    if (__ballot(ordered(s.largest(x)) >= cut.key)) {
-      uint64_t units[kChunk];
-      weights_at(x, at, units);
+    if (cut.key == 0 || __ballot(s.largest(x) >= end)) {
+      double weight[kChunk];
+      weights_at(x, at, weight);
+      // (What the units are rounded against is taken off once.)
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) sum += units[j];
+      for (int j = 0; j < kChunk; ++j) sum += __builtin_bit_cast(uint64_t, weight[j] + s.w.shift);
+      sum -= kChunk * __builtin_bit_cast(uint64_t, s.w.shift);
     }
     const int64_t upto = wave_prefix((int64_t)sum);
     if (lane == 63 && at / kPart < s.steps * kRowWaves) sh.part[at / kPart] = (uint64_t)upto;
@@ -711,16 +672,16 @@ __device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute_
     block_prefix(sh, a, total);
   }
   const uint64_t target = drawn(set.u, total);
-  uint64_t before;
   const int part = s.find_part(target, before);
   if (wave == 0) {
     const int at = part * kPart + lane * kChunk;
     float x[kChunk];
     s.decode(s.row.load(at), x);
+    double weight[kChunk];
     uint64_t each_w[kChunk], sum = 0;
-    weights_at(x, at, each_w);
+    weights_at(x, at, weight);
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) sum += each_w[j];
+    for (int j = 0; j < kChunk; ++j) sum += each_w[j] = s.w.units(weight[j]);
     uint64_t upto = before + (uint64_t)wave_prefix((int64_t)sum) - sum;
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
@@ -742,36 +703,29 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
   Sampler<T> s{sh};
   set_up(s, p, b);
   s.infinite = false;
-  if (tid < kTable) sh.table[tid] = __builtin_bit_cast(uint64_t, exp2((double)tid / kTable));
+  if (tid < kTable) {
+    const uint64_t power = __builtin_bit_cast(uint64_t, exp2((double)tid / kTable));
+    sh.table[tid] = uint2{(uint32_t)power, (uint32_t)(power >> 32) - ((uint32_t)tid << 14)};
+  }
 
-  // The largest logit with its first place, and the smallest.
-  float most = -INFINITY, least = INFINITY;
+  // The largest logit with its first place.
+  float most = -INFINITY;
   int place = 0;
-  s.template chunks<T::bytes == 2 ? 4 : 2>([&](const float (&x)[kChunk], int at) {
+  s.template chunks<4>([&](const float (&x)[kChunk], int at) {
     const float m = s.largest(x);
-    if (m > most) {
-      most = m;
-      place = at;  // of the chunk
-    }
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) least = fminf(least, x[i] > -INFINITY ? x[i] : INFINITY);
+    place = m > most ? at : place;  // of the chunk
+    most = fmaxf(most, m);
   });
   uint64_t best = most > -INFINITY ? (uint64_t)ordered(most) << 32 | (uint32_t)~place : 0;
 #pragma unroll
   for (int i = 1; i < 64; i <<= 1) {
     const uint64_t o = __shfl_xor(best, i);
     best = o > best ? o : best;
-    least = fminf(least, __shfl_xor(least, i));
   }
-  if (lane == 0) {
-    sh.waves[wave] = best;
-    sh.count[wave] = __builtin_bit_cast(uint32_t, least);
-  }
+  if (lane == 0) sh.waves[wave] = best;
   __syncthreads();
-  for (int i = 0; i < kRowWaves; ++i) {
-    best = sh.waves[i] > best ? sh.waves[i] : best;
-    least = fminf(least, __builtin_bit_cast(float, sh.count[i]));
-  }
+#pragma unroll
+  for (int i = 0; i < kRowWaves; ++i) best = sh.waves[i] > best ? sh.waves[i] : best;
   __syncthreads();
   const float top = unordered((uint32_t)(best >> 32));
   if (best == 0 || !(set.temperature > 0)) {  // nothing to choose from, or the largest
@@ -791,52 +745,49 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
     return;
   }
   s.infinite = top == INFINITY;
-  if (s.infinite) {
-    least = 0.f;
-    most = most == INFINITY ? 0.f : -INFINITY;
-  }
-  set_weights(s, p, set.temperature, s.infinite ? 0.f : top, least);
-  if (tid == 0) {
-    sh.top = s.top;
-    sh.least = least;
-    sh.infinite = s.infinite;
-  }
+  if (s.infinite) most = most == INFINITY ? 0.f : -INFINITY;
+  set_weights(s, p, set.temperature, s.infinite ? 0.f : top);
 
-  // The list: what is in bins below `end`, or at `low` or above.
-  uint64_t total = 0;
-  uint32_t above = 0;
-  uint64_t above_mass = 0;
-  float end = 0.f, low = -INFINITY;
+  // The list: everything from `low` on.
+  uint64_t total = 0, before = 0;
+  int bin = -1;
+  float low = -3.402823466e+38f;
   bool far = false;
   if (set.by_k && set.top_k <= kThreads / 2) {
-    // At least so many threads have a logit in the bin or above.
+    // At least so many threads have a logit in the bin or above; where fewer have any, everything.
     s.clear_bins();
-    if (most > -INFINITY) atomicAdd(&sh.count[s.bin_of(most)], 1u);
+    if (most > -INFINITY) atomicAdd((unsigned long long*)&sh.weight[s.bin_of(most)], 1ull);
     __syncthreads();
-    end = (float)(s.find_bin(true, (uint64_t)set.top_k - 1, above, above_mass) + 1);
-    // (Fewer threads than that with a logit: everything.)
-    if (above + sh.count[(int)end - 1] < (uint32_t)set.top_k) end = (float)kBins;
-  } else if (set.by_k || set.by_p) {
-    if (set.by_k)
-      s.template histogram<false>(Cut{0, 0xffffffffu});
-    else
-      s.template histogram<true>(Cut{0, 0xffffffffu});
-    uint64_t all = sh.weight[2 * tid] + sh.weight[2 * tid + 1];
-    block_prefix(sh, all, total);
-    const uint64_t target = set.by_k ? (uint64_t)set.top_k - 1 : target_of(fmax(set.top_p, 0.0) * (double)total);
-    end = (float)(s.find_bin(set.by_k, target, above, above_mass) + 1);
-    far = above + sh.count[(int)end - 1] > kList;
+    uint64_t all;
+    const int last = s.find_bin((uint64_t)set.top_k - 1, before, all);
+    if ((uint64_t)set.top_k <= all) low = s.bin_end(last);
+  } else if (set.by_k) {
+    s.count();
+    uint64_t all;
+    bin = s.find_bin((uint64_t)set.top_k - 1, before, all);
+    low = s.bin_end(bin);
+  } else if (set.by_p) {
+    s.weigh(Cut{0, 0xffffffffu});
+    uint64_t mine = sh.weight[tid] + sh.weight[tid + kThreads];
+    block_prefix(sh, mine, total);
+    bin = s.find_bin(target_of(fmax(set.top_p, 0.0) * (double)total), before, mine);
+    low = s.bin_end(bin);
   } else if (set.min_p > 0.0) {
     // (A little lower than it is, for the roundings.)
-    const float bound = s.top + (float)(log(set.min_p) * 1.000001 / s.w.inv);
-    low = bound - fabsf(bound) * 0x1p-20f - fabsf(s.top) * 0x1p-20f;
-    end = INFINITY;
+    const float bound = s.top + (float)(log(set.min_p) * 1.000001 * kTable * 1.44269504088896340736 / s.w.steps);
+    low = fmaxf(low, bound - (fabsf(bound) + fabsf(s.top)) * 0x1p-20f);
   } else {
     far = true;
   }
-  if (end == (float)kBins) end = INFINITY;
-  if (!far) far = !s.collect([&](float x, int) { return !(x < low) & (s.bin_at(x) < end); });
+  if (!far) far = !s.collect(low, INFINITY, Cut{0, 0xffffffffu});
   if (far) {
+    if (tid == 0) {
+      sh.top = s.top;
+      sh.infinite = s.infinite;
+      sh.bin = bin;
+      sh.before = before;
+      sh.total = total;
+    }
     sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh);
     return;
   }
@@ -889,10 +840,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
     weight[i] = key[i] ? 1 : 0;
   }
   // The ends by count and by weight, then the draw: three selections.
-  // Its orders begin at the bound, a little lower than it is.
-  const float bound = end < INFINITY ? s.top - (end + 1.f) / s.per_bin : low;
-  const float from = fmaxf(bound - (fabsf(bound) + fabsf(s.top)) * 0x1p-20f, least);
-  const uint64_t lowest = (uint64_t)ordered(from) << 32, highest = (uint64_t)ordered(s.top) << 32 | 0xffffffffu;
+  const uint64_t lowest = (uint64_t)ordered(low) << 32, highest = (uint64_t)ordered(s.top) << 32 | 0xffffffffu;
   for (int turn = set.by_k && (uint64_t)set.top_k < n ? 0 : (set.by_p ? 1 : 2);; turn = turn == 0 && set.by_p ? 1 : 2) {
     uint64_t target = (uint64_t)set.top_k - 1;
     if (turn > 0) {
