@@ -16,6 +16,13 @@
 // the read of their keys, which is done once: their scores, 4 bytes against a
 // key's 2 D, go to the workspace, with every row's maximum and sum by ranges of keys, and
 // a second kernel makes the weights of them.
+//
+// Measured on one MI355X:
+//   one token of each of 64 sequences of 6554 to 32768 keys, 28/4 heads of 128, bf16: 327 us, 3.9 TB/s of keys
+//   (by two passes over the keys 952)
+//   one token over 517 keys, 8/2 heads: 14 us
+//   windows of 8 to 40 tokens over four prompts of up to 33000 keys, 16/8 heads of 64: 69 us
+//   4096 tokens over 32768 keys, 28/4 heads: 2210 us, 820 TFLOP/s of its two products
 #include "paged_impl.h"
 
 namespace spruce {
@@ -26,6 +33,8 @@ struct KeyMass {
   int64_t ms[3];   // page, head, slot strides
   float2* stats;   // [N * Hq][parts]: maximum (of scores as products) and sum
   int Hq, parts, accumulate;
+  int row_parts;   // of the rows that a key tile sees, where there are few tiles: each a workgroup's
+  float* partial;  // their sums, [key tile][KV head][row_parts][256]
   // Sequences of up to few_rows packed rows: stats by ranges of `range` keys, scores of a (KV head, sequence)
   // as [32 keys][row][key] from its first packed row times key_room on.
   int few_rows, range, ranges, key_room;
@@ -58,17 +67,25 @@ struct Stream {
   static constexpr int stride = D + 8, lanes = D / 8, rows = 256 / lanes, passes = kStream / rows;
 };
 
-// S^T's 32 x 64 block: streamed rows a (LDS), held columns b.
+// S^T's 32 x 64 block: streamed rows a (LDS), held columns b, what to begin with c.
 template <int D, bool F16>
-__device__ __forceinline__ void products(const uint16_t* rows, const u32x4 (&b)[2][D / 16], int lane, f32x16_t& x0,
-                                         f32x16_t& x1) {
+__device__ __forceinline__ void products(const uint16_t* rows, const u32x4 (&b)[2][D / 16], int lane, const f32x16_t& c0,
+                                         const f32x16_t& c1, f32x16_t& x0, f32x16_t& x1) {
   const uint16_t* at = rows + (lane & 31) * Stream<D>::stride + 8 * (lane >> 5);
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
     const uint4 a = *reinterpret_cast<const uint4*>(at + 16 * kk);
-    x0 = mfma32x32x16<F16>(a, __builtin_bit_cast(uint4, b[0][kk]), x0);
-    x1 = mfma32x32x16<F16>(a, __builtin_bit_cast(uint4, b[1][kk]), x1);
+    x0 = mfma32x32x16<F16>(a, __builtin_bit_cast(uint4, b[0][kk]), kk == 0 ? c0 : x0);
+    x1 = mfma32x32x16<F16>(a, __builtin_bit_cast(uint4, b[1][kk]), kk == 0 ? c1 : x1);
   }
+}
+
+// What is held is there from here on, for the compiler too: in the loop it would wait for all loads in flight,
+// the next tile's among them, before the first use.
+template <int N>
+__device__ __forceinline__ void settle(u32x4 (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
 // The streamed row of accumulator register r, within 32.
@@ -122,8 +139,12 @@ struct Sum {
   }
 };
 
-template <int D, bool F16>
-__global__ __launch_bounds__(256, 2) void key_mass_rows_kernel(const KeyMass a) {
+// EVEN: pages hold whole passes of the stream's loads, so a pass has one page, and its address but
+// for the lane's part is found on the scalar unit (looked up by every lane, as with other pages, a chunk of
+// 4096 tokens over 32768 keys takes 1342 us here rather than 1282).  Three waves a SIMD, without the registers
+// that would have a wave's own products and exponentials overlap (two waves: 1395).
+template <int D, bool F16, bool EVEN>
+__global__ __launch_bounds__(256, 3) void key_mass_rows_kernel(const KeyMass a) {
   typedef Stream<D> ST;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2][kStream * ST::stride];
   __shared__ int paged[2][kStream];
@@ -165,19 +186,44 @@ __global__ __launch_bounds__(256, 2) void key_mass_rows_kernel(const KeyMass a) 
   int entry[ST::passes];
   u32x4 row[ST::passes];
   int there[ST::passes];
+  uint64_t have_next = 0;
+  const int64_t lane_part = lr * p.ks[2];
   auto look_up = [&](int tile) {
 #pragma unroll
-    for (int i = 0; i < ST::passes; ++i)
-      entry[i] = page_entry(p.batch, u.s, nearest(tile * kStream + i * ST::rows + lr, tr.end));
+    for (int i = 0; i < ST::passes; ++i) {
+      if constexpr (EVEN) {
+        const int at_page = uniform(page_of(p.batch, nearest(tile * kStream + i * ST::rows, tr.end)));
+        const int32_t* table = p.batch.table + (int64_t)u.s * p.batch.table_stride;
+        entry[i] = ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)table)[at_page];
+      } else {
+        entry[i] = page_entry(p.batch, u.s, nearest(tile * kStream + i * ST::rows + lr, tr.end));
+      }
+    }
   };
   auto load = [&](int tile) {
+    if constexpr (EVEN) {
+      have_next = 0;
 #pragma unroll
-    for (int i = 0; i < ST::passes; ++i) {
-      const int key = tile * kStream + i * ST::rows + lr, in = nearest(key, tr.end);
-      const int slot = in - page_of(p.batch, in) * p.batch.page;
-      const bool ok = is_page(p.batch, entry[i]);
-      there[i] = ok && key < tr.end;
-      row[i] = load16(kbase + (int64_t)(ok ? entry[i] : 0) * p.ks[0] + (int64_t)slot * p.ks[2]);
+      for (int i = 0; i < ST::passes; ++i) {
+        const int key = uniform(nearest(tile * kStream + i * ST::rows, tr.end));
+        const int first = key - uniform(page_of(p.batch, key)) * p.batch.page;
+        const bool ok = is_page(p.batch, entry[i]);
+        // (Past the end the pass begins at the last key: its page's rows are read from that row's pass on.)
+        const int slot = first - first % ST::rows;
+        row[i] = load16(kbase + ((int64_t)(ok ? entry[i] : 0) * p.ks[0] + (int64_t)slot * p.ks[2]) + lane_part);
+        if (ok) have_next |= (ST::rows == 64 ? ~0ull : (1ull << (ST::rows & 63)) - 1) << (i * ST::rows);
+      }
+      const int left = tr.end - tile * kStream;
+      if (left < kStream) have_next &= (1ull << left) - 1;
+    } else {
+#pragma unroll
+      for (int i = 0; i < ST::passes; ++i) {
+        const int key = tile * kStream + i * ST::rows + lr, in = nearest(key, tr.end);
+        const int slot = in - page_of(p.batch, in) * p.batch.page;
+        const bool ok = is_page(p.batch, entry[i]);
+        there[i] = ok && key < tr.end;
+        row[i] = load16(kbase + (int64_t)(ok ? entry[i] : 0) * p.ks[0] + (int64_t)slot * p.ks[2]);
+      }
     }
   };
   Sum sum[2];
@@ -186,20 +232,23 @@ __global__ __launch_bounds__(256, 2) void key_mass_rows_kernel(const KeyMass a) 
     load(t0);
     if (t0 + 1 < t1) look_up(t0 + 1);
   }
+  settle(held[0]);
+  settle(held[1]);
   for (int t = t0; t < t1; ++t) {
     const int b = t & 1;
 #pragma unroll
     for (int i = 0; i < ST::passes; ++i) {
       *reinterpret_cast<u32x4*>(&lds[b][(i * ST::rows + lr) * ST::stride + 8 * lc]) = row[i];
-      if (lc == 0) paged[b][i * ST::rows + lr] = there[i];
+      if (!EVEN && lc == 0) paged[b][i * ST::rows + lr] = there[i];
     }
+    const uint64_t have_now = have_next;
     __syncthreads();
     if (t + 1 < t1) {
       load(t + 1);
       if (t + 2 < t1) look_up(t + 2);
     }
     if (mine <= 0) continue;
-    const uint64_t have = __ballot(paged[b][lane] != 0);
+    const uint64_t have = EVEN ? have_now : __ballot(paged[b][lane] != 0);
     const int key0 = t * kStream;
     const bool masked = have != ~0ull || key0 + kStream - 1 > first_pos;
     const bool large =
@@ -207,20 +256,25 @@ __global__ __launch_bounds__(256, 2) void key_mass_rows_kernel(const KeyMass a) 
 #pragma unroll 1
     for (int sub = 0; sub < kStream / 32; ++sub) {
       f32x16_t x[2];
+      if (large) {
+        const f32x16_t zero = {};
+        products<D, F16>(&lds[b][32 * sub * ST::stride], held, lane, zero, zero, x[0], x[1]);
+      } else {
+        f32x16_t less[2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float from = large ? 0.f : -sum[c].m;
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[c][r] = from;
+          for (int r = 0; r < 16; ++r) less[c][r] = -sum[c].m;
+        products<D, F16>(&lds[b][32 * sub * ST::stride], held, lane, less[0], less[1], x[0], x[1]);
       }
-      products<D, F16>(&lds[b][32 * sub * ST::stride], held, lane, x[0], x[1]);
       if (masked) {
         const uint32_t in = (uint32_t)(have >> (32 * sub));
+        const int lane_now = lane + opaque_zero();  // the keys' bits are found here, not kept in 32 registers
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int k = row_of(r, lane);
+            const int k = row_of(r, lane_now);
             if (!(in >> k & 1) || key0 + 32 * sub + k > qpos[c]) x[c][r] = -INFINITY;
           }
       }
@@ -289,6 +343,31 @@ __device__ __forceinline__ bool find_keys(const PagedAttn& p, int64_t at, int la
   return false;
 }
 
+// Key `key` of a sequence, in the table's entry `entry`, has got v.
+__device__ __forceinline__ void set_mass(const KeyMass& a, const KeyTile& k, int g, int key, int entry, float v) {
+  const int slot = key - page_of(a.a.batch, key) * a.a.batch.page;
+  float* to = a.mass + (int64_t)entry * a.ms[0] + (int64_t)g * a.ms[1] + (int64_t)slot * a.ms[2];
+  *to = a.accumulate && key < k.pos0 ? *to + v : v;
+}
+
+// Joins the sums of key tiles whose rows were shared out, in their order.
+__global__ __launch_bounds__(256) void key_mass_add_kernel(const KeyMass a) {
+  const PagedAttn& p = a.a;
+  const int tid = threadIdx.x, lane = tid & 63;
+  for (int64_t tile = blockIdx.x;; tile += gridDim.x) {
+    const int64_t at = tile / p.Hkv;
+    const int g = (int)(tile - at * p.Hkv);
+    KeyTile k;
+    if (!find_keys(p, at, lane, k)) return;
+    float v = 0.f;
+    for (int i = 0; i < a.row_parts; ++i) v += a.partial[(tile * a.row_parts + i) * kRowsOf + tid];
+    const int key = k.tile * kRowsOf + tid;
+    if (key >= k.len) continue;
+    const int entry = page_entry(p.batch, k.s, key);
+    if (is_page(p.batch, entry)) set_mass(a, k, g, key, entry, v);
+  }
+}
+
 template <int D, bool F16>
 __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) {
   typedef Stream<D> ST;
@@ -302,8 +381,8 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
   const int lr = tid / ST::lanes, lc = tid % ST::lanes;
   const float per_cs = 1.f / p.cs;
   for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
-    const int64_t at = unit / p.Hkv;
-    const int g = (int)(unit - at * p.Hkv);
+    const int64_t tile = unit / a.row_parts, at = tile / p.Hkv;
+    const int row_part = (int)(unit - tile * a.row_parts), g = (int)(tile - at * p.Hkv);
     KeyTile k;
     if (!find_keys(p, at, lane, k)) return;
     const int key0 = k.tile * kRowsOf + kWave * wave;
@@ -324,31 +403,52 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
     }
     // Rows from the first that sees the tile's first key on.
     const int64_t skip = (int64_t)k.tile * kRowsOf - k.pos0;
-    const int rows = k.n * p.G;
-    const int row0 = skip <= 0 ? 0 : (skip < k.n ? (int)skip * p.G : rows);
+    int rows = k.n * p.G, row0 = skip <= 0 ? 0 : (skip < k.n ? (int)skip * p.G : rows);
+    if (a.row_parts > 1) {
+      const int steps = (rows - row0 + kStream - 1) / kStream, per = (steps + a.row_parts - 1) / a.row_parts * kStream;
+      const int begin = row0 + row_part * per;
+      row0 = begin < rows ? begin : rows;
+      rows = row0 + per < rows ? row0 + per : rows;
+    }
+    // The stream's rows follow by kStream packed rows: a row's head goes on by what that leaves of
+    // the group, its token by the rest.
     u32x4 row[ST::passes];
-    Sum stat;
+    const uint16_t* from[ST::passes];
+    int head[ST::passes];
+    const int tokens = kStream / p.G, heads = kStream - tokens * p.G;
+    const int64_t plain = tokens * p.qs[0] + heads * p.qs[1], wrapped = plain + p.qs[0] - p.G * p.qs[1];
+#pragma unroll
+    for (int i = 0; i < ST::passes; ++i) {
+      const int r = nearest(row0 + i * ST::rows + lr, rows), t = p.by_group.of(r);
+      head[i] = r - t * p.G;
+      from[i] = static_cast<const uint16_t*>(p.q) + (int64_t)(k.start + t) * p.qs[0] +
+                (int64_t)(g * p.G + head[i]) * p.qs[1] + 8 * lc;
+    }
+    float2 stat{0.f, 0.f};
     int row_pos = -1;
     auto load = [&](int r0) {
 #pragma unroll
       for (int i = 0; i < ST::passes; ++i) {
-        const int r = nearest(r0 + i * ST::rows + lr, rows);
-        const int t = p.by_group.of(r), h = g * p.G + r - t * p.G;
-        row[i] = load16(static_cast<const uint16_t*>(p.q) + (int64_t)(k.start + t) * p.qs[0] + (int64_t)h * p.qs[1] +
-                        8 * lc);
+        if (r0 > row0 && r0 + i * ST::rows + lr < rows) {
+          const int next = head[i] + heads;
+          const bool wrap = next >= p.G;
+          head[i] = wrap ? next - p.G : next;
+          from[i] += wrap ? wrapped : plain;
+        }
+        row[i] = load16(from[i]);
       }
-      stat = Sum();
+      stat = float2{0.f, 0.f};
       row_pos = -1;
       if (tid < kStream && r0 + tid < rows) {
         const int t = p.by_group.of(r0 + tid), h = g * p.G + r0 + tid - t * p.G;
         row_pos = clip(k.pos0 + t);
-        const float2* st = a.stats + ((int64_t)(k.start + t) * a.Hq + h) * a.parts;
-        const float2 x = *st;
-        stat.join(x.x, x.y, p.cs);
+        stat = a.stats[((int64_t)(k.start + t) * a.Hq + h) * a.parts];
       }
     };
     float sum[2] = {0.f, 0.f};
     if (row0 < rows) load(row0);
+    settle(held[0]);
+    settle(held[1]);
     int b = 0;
     for (int r0 = row0; r0 < rows; r0 += kStream, b ^= 1) {
 #pragma unroll
@@ -356,13 +456,13 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
         *reinterpret_cast<u32x4*>(&lds[b][(i * ST::rows + lr) * ST::stride + 8 * lc]) = row[i];
       if (tid < kStream) {  // one wave
         // No key: nothing of it reaches a sum.
-        const float lg = stat.l == 0.f ? INFINITY : __builtin_amdgcn_logf(stat.l);
-        const float ref = stat.m + lg * per_cs;
+        const float lg = stat.y == 0.f ? INFINITY : __builtin_amdgcn_logf(stat.y);
+        const float ref = stat.x + lg * per_cs;
         less[b][tid] = -ref;
-        top[b][tid] = stat.m;
+        top[b][tid] = stat.x;
         log_sum[b][tid] = lg;
         pos[b][tid] = row_pos;
-        const uint64_t odd = __ballot(stat.l != 0.f && !(fabsf(ref * p.cs) < kLargeReference));
+        const uint64_t odd = __ballot(stat.y != 0.f && !(fabsf(ref * p.cs) < kLargeReference));
         if (tid == 0) large[b] = odd != 0;
       }
       __syncthreads();
@@ -373,15 +473,15 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
       const bool is_large = uniform(large[b]) != 0;
 #pragma unroll 1
       for (int sub = 0; sub < kStream / 32; ++sub) {
-        f32x16_t x[2];
+        f32x16_t x[2], c;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          f32x4_t v = *reinterpret_cast<const f32x4_t*>(&less[b][32 * sub + 8 * i + 4 * hl]);
-          if (is_large) v = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          const f32x4_t v = *reinterpret_cast<const f32x4_t*>(&less[b][32 * sub + 8 * i + 4 * hl]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[0][4 * i + j] = x[1][4 * i + j] = v[j];
+          for (int j = 0; j < 4; ++j) c[4 * i + j] = v[j];
         }
-        products<D, F16>(&lds[b][32 * sub * ST::stride], held, lane, x[0], x[1]);
+        if (is_large) c = f32x16_t{};
+        products<D, F16>(&lds[b][32 * sub * ST::stride], held, lane, c, c, x[0], x[1]);
         if (masked) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
@@ -413,11 +513,11 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const float v = half_sum(sum[c]);
-      if (hl == c && is_page(p.batch, entry[c])) {
-        const int slot = key[c] - page_of(p.batch, key[c]) * p.batch.page;
-        float* to = a.mass + (int64_t)entry[c] * a.ms[0] + (int64_t)g * a.ms[1] + (int64_t)slot * a.ms[2];
-        *to = a.accumulate && key[c] < k.pos0 ? *to + v : v;
-      }
+      if (hl != c) continue;
+      if (a.row_parts > 1)
+        a.partial[unit * kRowsOf + kWave * wave + 32 * c + l32] = v;
+      else if (is_page(p.batch, entry[c]))
+        set_mass(a, k, g, key[c], entry[c], v);
     }
     __syncthreads();  // LDS is free
   }
@@ -426,7 +526,7 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
 // ------------------------------------------------------------------ few rows
 
 constexpr int kFewTile = 32;  // rows, and keys, of a wave's tile
-constexpr int kMostRange = 1024;
+constexpr int kMostRange = 1024;  // keys of a workgroup (64 sequences: 327 us; 2048: 334, 512: 334)
 
 // exp2(cs d) with the product's rounding and cs's made good: the argument is some tens, so that half
 // a step of it is some 2^-20 of the result.
@@ -516,6 +616,7 @@ __global__ __launch_bounds__(256, 3) void key_scores_kernel(const KeyMass a) {
       load(k0, entry);
       ahead = look_up(k0 + STEP);
     }
+    settle(held);
     for (int key0 = k0; key0 < k1; key0 += STEP) {
       uint32_t have = (uint32_t)__ballot(is_page(p.batch, entry));
       if (k.len - key0 < kFewTile) have &= (1u << (k.len - key0)) - 1;
@@ -618,9 +719,7 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (key[i] >= k.len || !is_page(p.batch, entry[i])) continue;
-      const int slot = key[i] - page_of(p.batch, key[i]) * p.batch.page;
-      float* to = a.mass + (int64_t)entry[i] * a.ms[0] + (int64_t)g * a.ms[1] + (int64_t)slot * a.ms[2];
-      *to = a.accumulate && key[i] < k.pos0 ? *to + sum[i] : sum[i];
+      set_mass(a, k, g, key[i], entry[i], sum[i]);
     }
     __syncthreads();
   }
@@ -630,8 +729,9 @@ struct MassPlan {
   bool few, many;
   int64_t tiles, parts;  // row tiles that a batch can have, and the parts of the keys of each
   int64_t range, ranges, key_room;
-  int64_t many_bytes, few_stats_bytes, score_bytes;
-  int64_t bytes() const { return many_bytes + few_stats_bytes + score_bytes; }
+  int64_t row_parts;     // of the rows of a key tile
+  int64_t many_bytes, partial_bytes, few_stats_bytes, score_bytes;
+  int64_t bytes() const { return many_bytes + partial_bytes + few_stats_bytes + score_bytes; }
 };
 MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) {
   const int64_t G = Hq / Hkv;
@@ -640,6 +740,8 @@ MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) 
   // in all but odd batches.
   const int64_t longest = N > S ? N - S + 1 : 1;
   plan.key_room = (keys + kFewTile - 1) / kFewTile * kFewTile;
+  // Where the average is past it too, few sequences are taken to be alike: the launches of the other kind cost more
+  // than they save (four windows of 8 to 40 tokens: 69 us, 120 with both).
   plan.few = (N * G <= S * kFewTile || S > 8) && G <= kFewTile && N * Hq * plan.key_room <= kMostScores;
   plan.many = !plan.few || longest * G > kFewTile;
   if (plan.few) {
@@ -659,6 +761,14 @@ MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) 
     if (parts > 64) parts = 64;
     plan.parts = parts < 1 ? 1 : parts;
     plan.many_bytes = (N * Hq * plan.parts * 8 + 15) / 16 * 16;
+    // Two workgroups a CU, of at least 256 rows.  (2048 tokens over themselves, 28/4 heads: 84 us, with
+    // whole tiles 497; 1000 over 3000 keys, 8/2 heads: 48 and 154.)
+    const int64_t key_tiles = S * ((keys + kRowsOf - 1) / kRowsOf) * Hkv;
+    plan.row_parts = key_tiles > 0 ? 2 * kCus / key_tiles : 1;
+    if (plan.row_parts > longest * G / 256) plan.row_parts = longest * G / 256;
+    if (plan.row_parts > 16) plan.row_parts = 16;
+    if (plan.row_parts < 1) plan.row_parts = 1;
+    if (plan.row_parts > 1) plan.partial_bytes = key_tiles * plan.row_parts * kRowsOf * 4;
   }
   return plan;
 }
@@ -732,8 +842,10 @@ extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, voi
   char* work = static_cast<char*>(a.workspace);
   m.stats = reinterpret_cast<float2*>(work);
   m.parts = (int)plan.parts;
-  m.few_stats = reinterpret_cast<float2*>(work + plan.many_bytes);
-  m.scores = reinterpret_cast<float*>(work + plan.many_bytes + plan.few_stats_bytes);
+  m.row_parts = (int)plan.row_parts;
+  m.partial = reinterpret_cast<float*>(work += plan.many_bytes);
+  m.few_stats = reinterpret_cast<float2*>(work += plan.partial_bytes);
+  m.scores = reinterpret_cast<float*>(work += plan.few_stats_bytes);
   m.few_rows = kFewTile;
   m.range = (int)plan.range;
   m.ranges = (int)plan.ranges;
@@ -743,18 +855,24 @@ extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, voi
   const int64_t units = plan.tiles * plan.parts * Hkv;
   SPRUCE_REQUIRE(units < (int64_t)1 << 31, "too many tokens for one call");
   // Workgroups take more than one unit where there are more.
-  auto grid = [&](int64_t keys, int64_t most) {
-    const int64_t all = S * ((m.a.batch.cap + keys - 1) / keys) * Hkv;
+  auto grid = [&](int64_t keys, int64_t most, int64_t times = 1) {
+    const int64_t all = S * ((m.a.batch.cap + keys - 1) / keys) * Hkv * times;
     return dim3((unsigned)(all < most ? all : most));
   };
 #define SPRUCE_KEY_MASS(D_, F16_)                                                                              \
   do {                                                                                                         \
     if (plan.many) {                                                                                           \
-      hipLaunchKernelGGL((key_mass_rows_kernel<D_, F16_>), flat_grid(units), dim3(256), 0, st, m);             \
+      if (a.page_size % Stream<D_>::rows == 0)                                                                 \
+        hipLaunchKernelGGL((key_mass_rows_kernel<D_, F16_, true>), flat_grid(units), dim3(256), 0, st, m);     \
+      else                                                                                                     \
+        hipLaunchKernelGGL((key_mass_rows_kernel<D_, F16_, false>), flat_grid(units), dim3(256), 0, st, m);    \
       if (plan.parts > 1)                                                                                      \
         hipLaunchKernelGGL(key_mass_join_kernel, flat_grid((N * Hq + 255) / 256), dim3(256), 0, st, m.stats,   \
                            N * Hq, m.parts, cs);                                                               \
-      hipLaunchKernelGGL((key_mass_keys_kernel<D_, F16_>), grid(kRowsOf, 8 * kCus), dim3(256), 0, st, m);      \
+      hipLaunchKernelGGL((key_mass_keys_kernel<D_, F16_>), grid(kRowsOf, 8 * kCus, plan.row_parts), dim3(256), \
+                         0, st, m);                                                                            \
+      if (plan.row_parts > 1)                                                                                  \
+        hipLaunchKernelGGL(key_mass_add_kernel, grid(kRowsOf, 8 * kCus), dim3(256), 0, st, m);                 \
     }                                                                                                          \
     if (plan.few)                                                                                              \
       hipLaunchKernelGGL((key_scores_kernel<D_, F16_>), grid(plan.range, 16 * kCus), dim3(256), 0, st, m);     \
