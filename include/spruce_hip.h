@@ -925,7 +925,11 @@ int spruce_paged_evict(const spruce_paged_evict_args* args, void* stream);
  * gets token -1 and -inf.  Weights are formed in 64 bits and added as multiples of
  * a unit of the largest, 2^-52 or the smallest power of two of which V stay within 2^63.  The four settings come one for all rows (temperature1, ..) or,
  * where the pointers are given, one a row [B].  V <= 2088960.
+ *   workspace: 16-byte aligned, one call's own until it is done; needed without top_k, min_p and
+ *   a temperature of 0 for all rows, of spruce_sample_tokens_workspace_bytes(B, V, by_p) bytes (by_p: a
+ *   top_p other than 1 is given), which may be none.
  */
+int64_t spruce_sample_tokens_workspace_bytes(int64_t B, int64_t V, int64_t by_p);
 typedef struct spruce_sample_tokens_args {
   const void* logits;
   int64_t stride, B, V, dtype;
@@ -940,6 +944,8 @@ typedef struct spruce_sample_tokens_args {
   double top_p1, min_p1;
   int64_t* tokens;
   float* logprobs;
+  void* workspace;
+  int64_t workspace_bytes;
 } spruce_sample_tokens_args;
 int spruce_sample_tokens(const spruce_sample_tokens_args* args, void* stream);
 

@@ -19,6 +19,13 @@
 // order whose running sum passes a target, which select() narrows down digit by digit.
 // Rows that keep more than the list holds go the long way: the end of a prefix
 // within one range of the histogram, then sums of 512 logits each, in index order.
+//
+// What bounds it: a row's logits pass one CU, where every instruction on each of 150016 logits takes about
+// a microsecond, and the steps after the lists are chains of a few dozen barriers; the bytes are nothing to it (19 MB
+// take 4 us).  So a weight is two additions, a fused one and a polynomial of four terms, only rows of a histogram
+// need all of them, and few long rows without top_k and min_p are shared by workgroups.
+// Measured: top_k 50, top_p 0.95, min_p 0.02 of [1, 32003] f16 16 us; top_k 1000, top_p 0.9 of [24, 50021]
+// bf16 75; top_p 0.95 of [64, 150016] bf16 103; min_p 0.001 of [256, 131072] f32 77.
 #include "paged_impl.h"
 
 namespace spruce {
@@ -39,6 +46,28 @@ struct Sampling {
   double shift;  // of weights
   int64_t* tokens;
   float* logprobs;  // or null
+  // Rows that more than one workgroup shares: parts of part_places places, and what they leave each other.
+  int parts, part_places;
+  uint64_t* best;             // [B][parts] the largest logit's order << 32 | ~place of its chunk
+  uint64_t* hists;            // [B][parts][2048]
+  uint64_t* lists;            // [B][parts][4096]
+  struct PartList* part_list; // [B][parts]
+  uint64_t* sums;             // [B][4096]
+  struct RowState* states;    // [B]
+};
+// kind: everything from the bound on; the members of the bin that holds an end (kMembers: the rest did not
+// fit); or not even those (kTooMany).
+struct PartList {
+  uint32_t size;
+  int kind;
+};
+struct RowState {
+  uint32_t done[3];          // parts that are done with each of the steps
+  int stage;
+  int bin, whole;            // of the first end; all that comes before it is listed too
+  uint64_t before, total;    // of the bin, and of all weights
+  float low, high;           // logits that lists begin and the bin's end with
+  uint32_t cut_key, cut_last;
 };
 
 namespace {
@@ -50,6 +79,16 @@ constexpr int kChunk = 8;           // logits that a lane reads at once
 constexpr int kPart = 64 * kChunk;  // logits of one sum of the long way
 constexpr int kParts = 4096;        // such sums
 constexpr int kTable = 64;
+constexpr int kMostParts = 16;      // of a row
+// Rows that are shared out, to as many workgroups: of so many logits at the least, with top_p and without.
+// Shared and not, in us: top_p 0.95 of bf16 [1, 100000] 49 and 68, [8, 150016] 72 and 147, [64, 150016]
+// 103 and 152, [128, 256000] 166 and 241, but [128, 100000] 91 and 83, and at 50021 logits the launches' own
+// latency takes all that is gained; without top_p [1, 50021] 16 and 29, [128, 150016] 42 and 60, [64, 32003] 24 and 24.
+// (With top_k or min_p the lists are short, and it lost at every size: top_k 50 of [1, 150016] 40 and 34.)
+constexpr int kSharers = kCus;
+constexpr int64_t kLeastByP = 65536, kLeastPlain = 32768;
+constexpr int kWhole = 0, kMembers = 1, kTooMany = 2;              // of a PartList
+constexpr int kWeighed = 0, kSummed = 1;                           // of a RowState: what it waits for next
 
 // A unit is the smallest power of two of which V weights of one stay within 2^63,
 // and 2^-52 at the least.
@@ -139,10 +178,10 @@ struct Weights {
 #pragma clang fp contract(off)
     // The difference first: of the largest logit it is zero whatever T is.
     const double d = fmax((double)x - max, lowest);
-    constexpr double kWhole = 0x1.8p+52, kStep = 0.69314718055994530942 / kTable;
-    const double t = fma(d, steps, kWhole);
+    constexpr double kRound = 0x1.8p+52, kStep = 0.69314718055994530942 / kTable;
+    const double t = fma(d, steps, kRound);
     const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
-    const double r = fma(d, steps, kWhole - t);
+    const double r = fma(d, steps, kRound - t);
     const double e = fma(r, fma(r, fma(r, fma(r, kStep * kStep * kStep * kStep / 24, kStep * kStep * kStep / 6), kStep * kStep / 2), kStep), 1.0);
     const uint2 p = table[n & (kTable - 1)];
     return e * __builtin_bit_cast(double, (uint64_t)(p.y + (n << 14)) << 32 | p.x);
@@ -183,6 +222,7 @@ struct Shared {
   uint64_t waves[kRowWaves];
   uint64_t result[3];
   uint32_t size;
+  uint32_t starts[kMostParts];
   // What the long way goes on with.
   float top;
   int infinite, bin;        // of the first end by weight or count; -1: none yet
@@ -287,7 +327,7 @@ struct Sampler {
   Shared& sh;
   Row<T> row;
   Weights w;
-  int steps;       // of kThreads * kChunk places
+  int begin, steps;  // the first place, and steps of kThreads * kChunk from there on
   bool infinite;   // the largest logit is +inf: such are taken as 0, all others as -inf
   float top, per_bin;
 
@@ -325,7 +365,7 @@ struct Sampler {
   template <int AHEAD, typename F, typename G>
   __device__ __forceinline__ void chunks_while(F f, G more) const {
     typename Row<T>::Raw raw[AHEAD], next[AHEAD];
-    const int mine = (int)threadIdx.x * kChunk;
+    const int mine = begin + (int)threadIdx.x * kChunk;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) raw[i] = row.load(mine + i * kThreads * kChunk);
     for (int s = 0; s < steps && more(); s += AHEAD) {
@@ -478,6 +518,10 @@ struct Sampler {
       const uint64_t more = one == 0 ? 0 : (target - before) / one;
       return Cut{hi, nth_equal(hi, more, limit)};
     }
+    return end_among(by_count, target, before, lo, hi);
+  }
+  // The same among the list, of orders from lo to hi.
+  __device__ __forceinline__ Cut end_among(bool by_count, uint64_t target, uint64_t before, uint32_t lo, uint32_t hi) const {
     uint64_t key[kEach], ones[kEach], all = 0;
     entries(key);
 #pragma unroll
@@ -582,13 +626,37 @@ struct Settings {
     by_k = top_k > 0 && top_k < p.V;
     by_p = top_p < 1.0;
   }
+  // Of rows that parts share.
+  __device__ __forceinline__ void init_shared(const Sampling& p, int b) {
+    init(p, b);
+    by_k = false;
+    min_p = 0.0;
+  }
 };
 
 template <typename T>
 __device__ __forceinline__ void set_up(Sampler<T>& s, const Sampling& p, int b) {
   s.row.init(p.logits, (int64_t)b * p.stride, p.V);
+  s.begin = 0;
   s.steps = (s.row.end + kThreads * kChunk - 1) / (kThreads * kChunk);
+  s.infinite = false;
 }
+// Of a part of the row alone: what is behind it counts as behind the row.
+template <typename T>
+__device__ __forceinline__ void set_up(Sampler<T>& s, const Sampling& p, int b, int part) {
+  set_up(s, p, b);
+  s.begin = part * p.part_places;
+  const int end = s.begin + p.part_places;
+  s.row.end = end < s.row.end ? end : s.row.end;
+  s.steps = s.row.end > s.begin ? (s.row.end - s.begin + kThreads * kChunk - 1) / (kThreads * kChunk) : 0;
+}
+__device__ __forceinline__ void fill_table(Shared& sh) {
+  if (threadIdx.x < kTable) {
+    const uint64_t power = __builtin_bit_cast(uint64_t, exp2((double)threadIdx.x / kTable));
+    sh.table[threadIdx.x] = uint2{(uint32_t)power, (uint32_t)(power >> 32) - (threadIdx.x << 14)};
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void set_weights(Sampler<T>& s, const Sampling& p, double temperature, float top) {
   s.top = uniform(top);
@@ -602,13 +670,82 @@ __device__ __forceinline__ void set_weights(Sampler<T>& s, const Sampling& p, do
   s.per_bin = uniform((float)(kBins - 1) / (range > 1e-30f ? (range < 1e30f ? range : 1e30f) : 1e-30f));
 }
 
-// A row that keeps more than the list holds.  A function of its own, which sets
+// The weights of eight logits, zero where they are not kept.
+template <typename T>
+__device__ __forceinline__ void weights_at(const Sampler<T>& s, const Settings& set, const Cut& cut,
+                                           const float (&x)[kChunk], int at, double (&weight)[kChunk]) {
+  s.w.of8(x, weight);
+  if (cut.key) {
+    const float end = unordered(cut.key);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j)
+      if (!((x[j] > end) | ((x[j] == end) & ((uint32_t)(at + j) <= cut.last)))) weight[j] = 0.0;
+  }
+  if (set.min_p > 0.0) {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j)
+      if (weight[j] < set.min_p) weight[j] = 0.0;
+  }
+}
+
+// The kept weights' sums of 512 logits each.
+template <typename T>
+__device__ __forceinline__ void sum_up(const Sampler<T>& s, const Settings& set, const Cut& cut, uint64_t* sums) {
+  const int lane = threadIdx.x & 63, most = (s.begin + s.steps * kThreads * kChunk) / kPart;
+  const float end = unordered(cut.key);
+  s.template chunks<2>([&](const float (&x)[kChunk], int at) {
+    uint64_t sum = 0;
+    if (cut.key == 0 || __ballot(s.largest(x) >= end)) {
+      double weight[kChunk];
+      weights_at(s, set, cut, x, at, weight);
+      // (What the units are rounded against is taken off once.)
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) sum += __builtin_bit_cast(uint64_t, weight[j] + s.w.shift);
+      sum -= kChunk * __builtin_bit_cast(uint64_t, s.w.shift);
+    }
+    const int64_t upto = wave_prefix((int64_t)sum);
+    if (lane == 63 && at / kPart < most) sums[at / kPart] = (uint64_t)upto;
+  });
+}
+
+// The draw from the row's sums in LDS.
+template <typename T>
+__device__ __forceinline__ void draw_summed(Shared& sh, Sampler<T>& s, const Sampling& p, const Settings& set,
+                                            const Cut& cut, int b) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = spruce::uniform(tid >> 6);
+  __syncthreads();
+  uint64_t a = 0, total, before;
+  for (int i = tid; i < s.steps * kRowWaves; i += kThreads) a += sh.part[i];
+  block_prefix(sh, a, total);
+  const uint64_t target = drawn(set.u, total);
+  const int part = s.find_part(target, before);
+  if (wave != 0) return;
+  const int at = part * kPart + lane * kChunk;
+  float x[kChunk];
+  s.decode(s.row.load(at), x);
+  double weight[kChunk];
+  uint64_t units[kChunk], sum = 0;
+  weights_at(s, set, cut, x, at, weight);
+#pragma unroll
+  for (int j = 0; j < kChunk; ++j) sum += units[j] = s.w.units(weight[j]);
+  uint64_t upto = before + (uint64_t)wave_prefix((int64_t)sum) - sum;
+#pragma unroll
+  for (int j = 0; j < kChunk; ++j) {
+    if (upto <= target && target < upto + units[j]) {
+      p.tokens[b] = at + j - s.row.first;
+      if (p.logprobs) p.logprobs[b] = (float)log(weight[j] / ((double)total * (p.shift * 0x1p-52)));
+    }
+    upto += units[j];
+  }
+}
+
+// A row that keeps more than the list holds, by one workgroup.  A function of its own, which sets
 // everything up again: what it would keep in registers pushed the usual way's out of them.
 template <typename T>
-__device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute__((address_space(3))) Shared* lds) {
+__device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute__((address_space(3))) Shared* lds, int row) {
   const Sampling p = *(const Sampling*)(const __attribute__((address_space(4))) Sampling*)lane_of((int64_t)args, 0);
   Shared& sh = *(Shared*)lds;
-  const int b = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = spruce::uniform(tid >> 6);
+  const int b = spruce::uniform(row), tid = threadIdx.x;
   Settings set;
   set.init(p, b);
   Sampler<T> s{sh};
@@ -637,83 +774,20 @@ __device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute_
     }
   }
   if (set.by_p) cut = s.resolve(bin, false, target_of(fmax(set.top_p, 0.0) * (double)total), before, cut);
-  // The weights of eight logits, zero where they are not kept.
-  const float end = unordered(cut.key);
-  auto weights_at = [&](const float (&x)[kChunk], int at, double (&weight)[kChunk]) {
-    s.w.of8(x, weight);
-    if (cut.key) {
-#pragma unroll
-      for (int j = 0; j < kChunk; ++j)
-        if (!((x[j] > end) | ((x[j] == end) & ((uint32_t)(at + j) <= cut.last)))) weight[j] = 0.0;
-    }
-    if (set.min_p > 0.0) {
-#pragma unroll
-      for (int j = 0; j < kChunk; ++j)
-        if (weight[j] < set.min_p) weight[j] = 0.0;
-    }
-  };
-  s.template chunks<2>([&](const float (&x)[kChunk], int at) {
-    uint64_t sum = 0;
-    if (cut.key == 0 || __ballot(s.largest(x) >= end)) {
-      double weight[kChunk];
-      weights_at(x, at, weight);
-      // (What the units are rounded against is taken off once.)
-#pragma unroll
-      for (int j = 0; j < kChunk; ++j) sum += __builtin_bit_cast(uint64_t, weight[j] + s.w.shift);
-      sum -= kChunk * __builtin_bit_cast(uint64_t, s.w.shift);
-    }
-    const int64_t upto = wave_prefix((int64_t)sum);
-    if (lane == 63 && at / kPart < s.steps * kRowWaves) sh.part[at / kPart] = (uint64_t)upto;
-  });
-  __syncthreads();
-  {
-    uint64_t a = 0;
-    for (int i = tid; i < s.steps * kRowWaves; i += kThreads) a += sh.part[i];
-    block_prefix(sh, a, total);
-  }
-  const uint64_t target = drawn(set.u, total);
-  const int part = s.find_part(target, before);
-  if (wave == 0) {
-    const int at = part * kPart + lane * kChunk;
-    float x[kChunk];
-    s.decode(s.row.load(at), x);
-    double weight[kChunk];
-    uint64_t each_w[kChunk], sum = 0;
-    weights_at(x, at, weight);
-#pragma unroll
-    for (int j = 0; j < kChunk; ++j) sum += each_w[j] = s.w.units(weight[j]);
-    uint64_t upto = before + (uint64_t)wave_prefix((int64_t)sum) - sum;
-#pragma unroll
-    for (int j = 0; j < kChunk; ++j) {
-      if (upto <= target && target < upto + each_w[j]) {
-        p.tokens[b] = at + j - s.row.first;
-        if (p.logprobs) p.logprobs[b] = (float)log(s.w.of(x[j]) / ((double)total * (p.shift * 0x1p-52)));
-      }
-      upto += each_w[j];
-    }
-  }
+  sum_up(s, set, cut, sh.part);
+  draw_summed(sh, s, p, set, cut, b);
 }
 
+// The largest logit of the sampler's places: its order << 32 | ~place of its chunk, 0 for none; and this thread's
+// own.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
-  __shared__ Shared sh;
-  const int b = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = spruce::uniform(tid >> 6);
-  Settings set;
-  set.init(p, b);
-  Sampler<T> s{sh};
-  set_up(s, p, b);
-  s.infinite = false;
-  if (tid < kTable) {
-    const uint64_t power = __builtin_bit_cast(uint64_t, exp2((double)tid / kTable));
-    sh.table[tid] = uint2{(uint32_t)power, (uint32_t)(power >> 32) - ((uint32_t)tid << 14)};
-  }
-
-  // The largest logit with its first place.
-  float most = -INFINITY;
+__device__ __forceinline__ uint64_t largest_logit(Shared& sh, const Sampler<T>& s, float& most) {
+  const int lane = threadIdx.x & 63, wave = spruce::uniform(threadIdx.x >> 6);
+  most = -INFINITY;
   int place = 0;
   s.template chunks<4>([&](const float (&x)[kChunk], int at) {
     const float m = s.largest(x);
-    place = m > most ? at : place;  // of the chunk
+    place = m > most ? at : place;
     most = fmaxf(most, m);
   });
   uint64_t best = most > -INFINITY ? (uint64_t)ordered(most) << 32 | (uint32_t)~place : 0;
@@ -727,70 +801,39 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
 #pragma unroll
   for (int i = 0; i < kRowWaves; ++i) best = sh.waves[i] > best ? sh.waves[i] : best;
   __syncthreads();
-  const float top = unordered((uint32_t)(best >> 32));
-  if (best == 0 || !(set.temperature > 0)) {  // nothing to choose from, or the largest
-    if (tid == 0) {
-      int64_t token = -1;
-      if (best != 0) {
-        float x[kChunk];
-        const int at = (int)~(uint32_t)best;
-        s.decode(s.row.load(at), x);
-#pragma unroll
-        for (int i = kChunk - 1; i >= 0; --i)
-          if (x[i] == top) token = at + i - s.row.first;
-      }
-      p.tokens[b] = token;
-      if (p.logprobs) p.logprobs[b] = best == 0 ? -INFINITY : 0.f;
-    }
-    return;
-  }
-  s.infinite = top == INFINITY;
-  if (s.infinite) most = most == INFINITY ? 0.f : -INFINITY;
-  set_weights(s, p, set.temperature, s.infinite ? 0.f : top);
+  return best;
+}
 
-  // The list: everything from `low` on.
-  uint64_t total = 0, before = 0;
-  int bin = -1;
-  float low = -3.402823466e+38f;
-  bool far = false;
-  if (set.by_k && set.top_k <= kThreads / 2) {
-    // At least so many threads have a logit in the bin or above; where fewer have any, everything.
-    s.clear_bins();
-    if (most > -INFINITY) atomicAdd((unsigned long long*)&sh.weight[s.bin_of(most)], 1ull);
-    __syncthreads();
-    uint64_t all;
-    const int last = s.find_bin((uint64_t)set.top_k - 1, before, all);
-    if ((uint64_t)set.top_k <= all) low = s.bin_end(last);
-  } else if (set.by_k) {
-    s.count();
-    uint64_t all;
-    bin = s.find_bin((uint64_t)set.top_k - 1, before, all);
-    low = s.bin_end(bin);
-  } else if (set.by_p) {
-    s.weigh(Cut{0, 0xffffffffu});
-    uint64_t mine = sh.weight[tid] + sh.weight[tid + kThreads];
-    block_prefix(sh, mine, total);
-    bin = s.find_bin(target_of(fmax(set.top_p, 0.0) * (double)total), before, mine);
-    low = s.bin_end(bin);
-  } else if (set.min_p > 0.0) {
-    // (A little lower than it is, for the roundings.)
-    const float bound = s.top + (float)(log(set.min_p) * 1.000001 * kTable * 1.44269504088896340736 / s.w.steps);
-    low = fmaxf(low, bound - (fabsf(bound) + fabsf(s.top)) * 0x1p-20f);
-  } else {
-    far = true;
+// The token of a row with nothing to choose: the first of its largest logits, or -1.
+template <typename T>
+__device__ __forceinline__ void take_largest(const Sampler<T>& s, const Sampling& p, uint64_t best, int b) {
+  if (threadIdx.x != 0) return;
+  int64_t token = -1;
+  if (best != 0) {
+    float x[kChunk];
+    const int at = (int)~(uint32_t)best;
+    Row<T>::decode(s.row.load(at), x);
+#pragma unroll
+    for (int i = kChunk - 1; i >= 0; --i)
+      if (x[i] == unordered((uint32_t)(best >> 32))) token = at + i - s.row.first;
   }
-  if (!far) far = !s.collect(low, INFINITY, Cut{0, 0xffffffffu});
-  if (far) {
-    if (tid == 0) {
-      sh.top = s.top;
-      sh.infinite = s.infinite;
-      sh.bin = bin;
-      sh.before = before;
-      sh.total = total;
-    }
-    sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh);
-    return;
-  }
+  p.tokens[b] = token;
+  if (p.logprobs) p.logprobs[b] = best == 0 ? -INFINITY : 0.f;
+}
+
+// What a row's list begins with by min_p, a little lower than it is, for the roundings.
+template <typename T>
+__device__ __forceinline__ float least_by_share(const Sampler<T>& s, double min_p) {
+  const float bound = s.top + (float)(log(min_p) * 1.000001 * kTable * 1.44269504088896340736 / s.w.steps);
+  return fmaxf(-3.402823466e+38f, bound - (fabsf(bound) + fabsf(s.top)) * 0x1p-20f);
+}
+
+// The ends and the draw of a row whose kept logits are all in LDS: those from `low` on.
+// total: all weights, where the ends go by them alone.
+template <typename T>
+__device__ __forceinline__ void draw_listed(Shared& sh, const Sampler<T>& s, const Sampling& p, const Settings& set,
+                                            float low, uint64_t total, int b) {
+  const int lane = threadIdx.x & 63, wave = spruce::uniform(threadIdx.x >> 6);
   const uint32_t n = sh.size;
   auto done = [&](uint64_t entry, double weight, uint64_t sum) {
     p.tokens[b] = (int64_t)(~(uint32_t)entry - (uint32_t)s.row.first);
@@ -872,10 +915,347 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
   }
 }
 
+// The bound of a row's (or a part's) list by top_k, from the threads' own largest: at least so many threads have
+// a logit in that bin or above; everything where fewer have any.
+template <typename T>
+__device__ __forceinline__ float least_by_rank(Shared& sh, Sampler<T>& s, int64_t top_k, float most) {
+  s.clear_bins();
+  if (most > -INFINITY) atomicAdd((unsigned long long*)&sh.weight[s.bin_of(most)], 1ull);
+  __syncthreads();
+  uint64_t before = 0, all;
+  uint64_t mine = sh.weight[threadIdx.x] + sh.weight[threadIdx.x + kThreads];
+  block_prefix(sh, mine, all);
+  if ((uint64_t)top_k > all) return -3.402823466e+38f;
+  return s.bin_end(s.find_bin((uint64_t)top_k - 1, before, all));
+}
+
+// A row by one workgroup.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.x, tid = threadIdx.x;
+  Settings set;
+  set.init(p, b);
+  Sampler<T> s{sh};
+  set_up(s, p, b);
+  fill_table(sh);
+  float most;
+  const uint64_t best = largest_logit(sh, s, most);
+  if (best == 0 || !(set.temperature > 0)) {
+    take_largest(s, p, best, b);
+    return;
+  }
+  s.infinite = unordered((uint32_t)(best >> 32)) == INFINITY;
+  if (s.infinite) most = most == INFINITY ? 0.f : -INFINITY;
+  set_weights(s, p, set.temperature, s.infinite ? 0.f : unordered((uint32_t)(best >> 32)));
+
+  // The list: everything from `low` on.
+  uint64_t total = 0, before = 0;
+  int bin = -1;
+  float low = -3.402823466e+38f;
+  bool far = false;
+  if (set.by_k && set.top_k <= kThreads / 2) {
+    low = least_by_rank(sh, s, set.top_k, most);
+  } else if (set.by_k) {
+    s.count();
+    uint64_t all;
+    bin = s.find_bin((uint64_t)set.top_k - 1, before, all);
+    low = s.bin_end(bin);
+  } else if (set.by_p) {
+    s.weigh(Cut{0, 0xffffffffu});
+    uint64_t mine = sh.weight[tid] + sh.weight[tid + kThreads];
+    block_prefix(sh, mine, total);
+    bin = s.find_bin(target_of(fmax(set.top_p, 0.0) * (double)total), before, mine);
+    low = s.bin_end(bin);
+  } else if (set.min_p > 0.0) {
+    low = least_by_share(s, set.min_p);
+  } else {
+    far = true;
+  }
+  if (!far) far = !s.collect(low, INFINITY, Cut{0, 0xffffffffu});
+  if (!far) {
+    draw_listed(sh, s, p, set, low, total, b);
+    return;
+  }
+  if (tid == 0) {
+    sh.top = s.top;
+    sh.infinite = s.infinite;
+    sh.bin = bin;
+    sh.before = before;
+    sh.total = total;
+  }
+  sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh, b);
+}
+
+// ------------------------------------------------------------------ rows by more than one workgroup
+// Rows without top_k and min_p, whose lists are long or none: the same steps, the passes over a row part by part.
+// (An instruction on each of 150016 logits is a microsecond of one workgroup.)  What all parts have to know before
+// the next step is found by the workgroup that is the row's last to be done with one.
+
+// True in the workgroup that comes here last of its row's: it sees what the others wrote before.
+__device__ __forceinline__ bool last_of_row(Shared& sh, const Sampling& p, int b, int step) {
+  __syncthreads();
+  if (threadIdx.x == 0)
+    sh.result[2] = __hip_atomic_fetch_add(&p.states[b].done[step], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return (int)sh.result[2] == p.parts - 1;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void part_largest_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.y, part = (int)blockIdx.x;
+  Sampler<T> s{sh};
+  set_up(s, p, b, part);
+  float most;
+  const uint64_t best = largest_logit(sh, s, most);
+  if (threadIdx.x == 0) p.best[(int64_t)b * p.parts + part] = best;
+  if (part == 0 && threadIdx.x == 0) {
+    RowState state{};
+    state.stage = kSummed;
+    state.cut_last = 0xffffffffu;
+    p.states[b] = state;
+  }
+}
+
+// Sets a part up behind its row's largest logit; the largest, 0 where there is none.
+template <typename T>
+__device__ __forceinline__ uint64_t set_up_behind(Sampler<T>& s, const Sampling& p, const Settings& set, int b, int part) {
+  set_up(s, p, b, part);
+  uint64_t best = 0;
+  for (int i = 0; i < p.parts; ++i) {
+    const uint64_t x = p.best[(int64_t)b * p.parts + i];
+    best = x > best ? x : best;
+  }
+  if (best == 0 || !(set.temperature > 0)) return best;
+  s.infinite = unordered((uint32_t)(best >> 32)) == INFINITY;
+  set_weights(s, p, set.temperature, s.infinite ? 0.f : unordered((uint32_t)(best >> 32)));
+  fill_table(s.sh);
+  __syncthreads();
+  return best;
+}
+// The whole row in its place.
+template <typename T>
+__device__ __forceinline__ void widen(Sampler<T>& s, const Sampling& p, int b) {
+  const bool infinite = s.infinite;
+  set_up(s, p, b);
+  s.infinite = infinite;
+}
+
+// The list of a part to where the row's end finds it.
+__device__ __forceinline__ void leave_list(Shared& sh, const Sampling& p, int b, int part, int kind) {
+  const int64_t at = (int64_t)b * p.parts + part;
+  const uint32_t n = kind == kTooMany ? 0 : sh.size;
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) p.lists[at * kList + i] = sh.list[i];
+  if (threadIdx.x == 0) p.part_list[at] = PartList{n, kind};
+}
+
+// The end of a row whose parts have left their lists: the draw, where they hold all that is kept; the end by count
+// or weight, where they hold its bin; by this workgroup alone everything where they do not.
+template <typename T>
+__device__ __forceinline__ void end_row(Shared& sh, Sampler<T>& s, const Sampling& p, const Settings& set,
+                                        const RowState& state, int b) {
+  const int tid = threadIdx.x;
+  widen(s, p, b);
+  const PartList* lists = p.part_list + (int64_t)b * p.parts;
+  int worst = kWhole;
+  uint32_t all = 0;
+  for (int i = 0; i < p.parts; ++i) {
+    const PartList x = lists[i];
+    worst = x.kind > worst ? x.kind : worst;
+    if (tid == 0) sh.starts[i] = all;
+    all += x.size;
+  }
+  const bool listed = worst == kWhole && all <= kList;
+  bool members = !listed && worst != kTooMany;
+  const uint32_t most = ordered(members ? state.high : INFINITY);
+  if (tid == 0) sh.size = 0;
+  __syncthreads();
+  if (listed || members) {
+    for (uint32_t i = 0; i < all; i += kThreads * 4) {
+      uint64_t x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t at = i + j * kThreads + tid;
+        int part = 0;
+        for (int k = 1; k < p.parts; ++k) part = sh.starts[k] <= at ? k : part;
+        x[j] = at < all ? p.lists[((int64_t)b * p.parts + part) * kList + (at - sh.starts[part])] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = x[j] && (uint32_t)(x[j] >> 32) <= most;
+        const uint64_t mask = __ballot(in);
+        if (mask == 0) continue;
+        uint32_t to = 0;
+        if ((threadIdx.x & 63) == 0) to = atomicAdd(&sh.size, (uint32_t)__builtin_popcountll(mask));
+        to = (uint32_t)lane_of((int)to, 0) + (uint32_t)__builtin_popcountll(mask & ((1ull << (threadIdx.x & 63)) - 1));
+        if (in && to < kList) sh.list[to] = x[j];
+      }
+    }
+    __syncthreads();
+    members = members && sh.size <= kList;
+  }
+  if (listed) {
+    draw_listed(sh, s, p, set, state.low, state.total, b);
+    return;
+  }
+  if (members) {
+    const uint64_t target = target_of(fmax(set.top_p, 0.0) * (double)state.total);
+    const Cut cut = s.end_among(false, target, state.before, ordered(state.low), most);
+    if (tid == 0) {
+      p.states[b].cut_key = cut.key;
+      p.states[b].cut_last = cut.last;
+      p.states[b].stage = kSummed;
+    }
+    return;
+  }
+  if (tid == 0) {
+    sh.top = s.top;
+    sh.infinite = s.infinite;
+    sh.bin = state.bin;
+    sh.before = state.before;
+    sh.total = state.total;
+  }
+  sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh, b);
+}
+
+// The weights' histogram, and the bin of the end by top_p.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void part_weights_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.y, part = (int)blockIdx.x, tid = threadIdx.x;
+  Settings set;
+  set.init_shared(p, b);
+  if (!set.by_p) return;
+  Sampler<T> s{sh};
+  const uint64_t best = set_up_behind(s, p, set, b, part);
+  if (best == 0 || !(set.temperature > 0)) return;
+  s.weigh(Cut{0, 0xffffffffu});
+  uint64_t* hists = p.hists + (int64_t)b * p.parts * kBins;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) hists[(int64_t)part * kBins + tid + i * kThreads] = sh.weight[tid + i * kThreads];
+  if (!last_of_row(sh, p, b, 0)) return;
+  uint64_t h0 = 0, h1 = 0;
+#pragma unroll 4
+  for (int i = 0; i < p.parts; ++i) {
+    h0 += hists[(int64_t)i * kBins + tid];
+    h1 += hists[(int64_t)i * kBins + tid + kThreads];
+  }
+  sh.weight[tid] = h0;
+  sh.weight[tid + kThreads] = h1;
+  uint64_t total, before = 0, all;
+  block_prefix(sh, h0 + h1, total);
+  const int bin = s.find_bin(target_of(fmax(set.top_p, 0.0) * (double)total), before, all);
+  // About as many logits are before the bin or in it: a list of them all is not tried if they are too many.
+  uint64_t many = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = tid + i * kThreads;
+    if (at <= bin) many += (uint64_t)((double)(i ? h1 : h0) / (double)(s.w.units(s.w.of(s.top - (float)at / s.per_bin)) + 1));
+  }
+  block_prefix(sh, many, many);
+  const float low = s.bin_end(bin), high = bin == 0 ? INFINITY : unordered(ordered(s.bin_end(bin - 1)) - 1);
+  if (tid == 0) {
+    RowState& out = p.states[b];
+    out.stage = kWeighed;
+    out.bin = bin;
+    out.whole = many <= kList;
+    out.before = before;
+    out.total = total;
+    out.low = low;
+    out.high = high;
+  }
+}
+
+// The lists of what is before the first end and in its bin, or of the bin alone, and the row's end.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void part_list_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.y, part = (int)blockIdx.x;
+  const RowState state = p.states[b];
+  if (state.stage != kWeighed) return;
+  Settings set;
+  set.init_shared(p, b);
+  Sampler<T> s{sh};
+  set_up_behind(s, p, set, b, part);
+  int kind = kWhole;
+  if (!state.whole || !s.collect(state.low, INFINITY, Cut{0, 0xffffffffu}))
+    kind = s.collect(state.low, state.high, Cut{0, 0xffffffffu}) ? kMembers : kTooMany;
+  leave_list(sh, p, b, part, kind);
+  if (last_of_row(sh, p, b, 1)) end_row(sh, s, p, set, state, b);
+}
+
+// The sums of rows whose ends are known, and the draw.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void part_sums_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.y, part = (int)blockIdx.x;
+  if (p.states[b].stage != kSummed) return;
+  const Cut cut{p.states[b].cut_key, p.states[b].cut_last};
+  Settings set;
+  set.init_shared(p, b);
+  Sampler<T> s{sh};
+  const uint64_t best = set_up_behind(s, p, set, b, part);
+  if (best == 0 || !(set.temperature > 0)) {
+    widen(s, p, b);
+    if (part == 0) take_largest(s, p, best, b);
+    return;
+  }
+  uint64_t* sums = p.sums + (int64_t)b * kParts;
+  sum_up(s, set, cut, sums);
+  if (!last_of_row(sh, p, b, 2)) return;
+  widen(s, p, b);
+  for (int i = threadIdx.x; i < s.steps * kRowWaves; i += kThreads) sh.part[i] = i * kPart < s.row.end ? sums[i] : 0;
+  draw_summed(sh, s, p, set, cut, b);
+}
+
+struct SamplePlan {
+  int64_t parts, places;  // 1: a workgroup a row
+  int64_t best, hists, lists, part_list, sums, states;
+  int64_t bytes() const { return best + hists + lists + part_list + sums + states; }
+};
+// Parts of whole steps of a workgroup, a workgroup a CU at the most.
+SamplePlan sample_plan(int64_t B, int64_t V, bool by_p) {
+  constexpr int64_t kStep = kThreads * kChunk;
+  SamplePlan plan{};
+  const int64_t steps = (V + 7 + kStep - 1) / kStep;
+  int64_t parts = V >= (by_p ? kLeastByP : kLeastPlain) ? kSharers / B : 1;
+  if (parts > kMostParts) parts = kMostParts;
+  if (parts > steps) parts = steps;
+  if (parts < 2) {
+    plan.parts = 1;
+    return plan;
+  }
+  const int64_t each = (steps + parts - 1) / parts;
+  plan.parts = (steps + each - 1) / each;
+  plan.places = each * kStep;
+  const int64_t all = B * plan.parts;
+  plan.best = (all * 8 + 15) / 16 * 16;
+  plan.hists = all * kBins * 8;
+  plan.lists = all * kList * 8;
+  plan.part_list = (all * (int64_t)sizeof(PartList) + 15) / 16 * 16;
+  plan.sums = B * kParts * 8;
+  plan.states = B * (int64_t)sizeof(RowState);
+  return plan;
+}
+
+template <typename T>
+void launch_parts(const Sampling& p, int64_t B, bool ends, hipStream_t st) {
+  const dim3 parts((unsigned)p.parts, (unsigned)B), threads(kThreads);
+  hipLaunchKernelGGL(part_largest_kernel<T>, parts, threads, 0, st, p);
+  if (ends) hipLaunchKernelGGL(part_weights_kernel<T>, parts, threads, 0, st, p);
+  if (ends) hipLaunchKernelGGL(part_list_kernel<T>, parts, threads, 0, st, p);
+  hipLaunchKernelGGL(part_sums_kernel<T>, parts, threads, 0, st, p);
+}
+
 }  // namespace
 }  // namespace spruce
 
 using namespace spruce;
+
+extern "C" int64_t spruce_sample_tokens_workspace_bytes(int64_t B, int64_t V, int64_t by_p) {
+  return B < 1 || V < 1 || B >= (int64_t)1 << 30 || V >= (int64_t)1 << 31 ? 0 : sample_plan(B, V, by_p != 0).bytes();
+}
 
 extern "C" int spruce_sample_tokens(const spruce_sample_tokens_args* args, void* stream) {
   SPRUCE_REQUIRE(args != nullptr, "args must be non-null");
@@ -912,8 +1292,32 @@ extern "C" int spruce_sample_tokens(const spruce_sample_tokens_args* args, void*
   p.shift = __builtin_ldexp(1.0, kMostUnitBits - (bits < kMostUnitBits ? bits : kMostUnitBits));
   p.tokens = a.tokens;
   p.logprobs = a.logprobs;
-  const hipStream_t st = (hipStream_t)stream;
   SPRUCE_REQUIRE(a.B <= kGridX, "too many rows for one call");
+  const bool by_k = a.top_k || (a.top_k1 > 0 && a.top_k1 < a.V), by_p = a.top_p || a.top_p1 < 1;
+  const bool by_share = a.min_p || a.min_p1 > 0, greedy = !a.temperature && a.temperature1 == 0;
+  SamplePlan plan{};
+  if (!by_k && !by_share && !greedy) plan = sample_plan(a.B, a.V, by_p);
+  SPRUCE_REQUIRE(plan.bytes() == 0 || (a.workspace && a.workspace_bytes >= plan.bytes()),
+                 "workspace too small: %lld bytes, need %lld", (long long)a.workspace_bytes, (long long)plan.bytes());
+  SPRUCE_REQUIRE(reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0, "workspace must be 16-byte aligned");
+  const hipStream_t st = (hipStream_t)stream;
+  if (plan.parts > 1) {
+    char* work = static_cast<char*>(a.workspace);
+    p.parts = (int)plan.parts;
+    p.part_places = (int)plan.places;
+    p.best = reinterpret_cast<uint64_t*>(work);
+    p.hists = reinterpret_cast<uint64_t*>(work += plan.best);
+    p.lists = reinterpret_cast<uint64_t*>(work += plan.hists);
+    p.part_list = reinterpret_cast<PartList*>(work += plan.lists);
+    p.sums = reinterpret_cast<uint64_t*>(work += plan.part_list);
+    p.states = reinterpret_cast<RowState*>(work += plan.sums);
+    switch (a.dtype) {
+      case SPRUCE_DTYPE_BF16: launch_parts<InBF16>(p, a.B, by_p, st); break;
+      case SPRUCE_DTYPE_F16: launch_parts<InF16>(p, a.B, by_p, st); break;
+      default: launch_parts<InF32>(p, a.B, by_p, st); break;
+    }
+    return check_launch("token sampling");
+  }
   const dim3 grid((unsigned)a.B);
   switch (a.dtype) {
     case SPRUCE_DTYPE_BF16: hipLaunchKernelGGL(sample_kernel<InBF16>, grid, dim3(kThreads), 0, st, p); break;

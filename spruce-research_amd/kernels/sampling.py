@@ -4,6 +4,7 @@ serving step whose beginning and middle are ``kernels.rotary`` and ``kernels.pag
 Random numbers are an input, so a draw can be repeated.  Calls run on the
 current stream of the tensors' device, wait for nothing and can be captured.
 """
+import functools
 import struct
 
 import torch
@@ -13,7 +14,12 @@ import spruce_hip
 __all__ = ["sample_tokens"]
 
 # struct spruce_sample_tokens_args, field by field.
-_SAMPLE_ARGS = struct.Struct("=qqqqqqqqqqqdqddqq")
+_SAMPLE_ARGS = struct.Struct("=qqqqqqqqqqqdqddqqqq")
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*shape):
+    return spruce_hip.lib().spruce_sample_tokens_workspace_bytes(*shape)
 
 
 def _setting(x, name, dtype, B, device):
@@ -77,11 +83,16 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
         raise RuntimeError("the sampling HIP backend requires GPU tensors")
     tokens = logits.new_empty_strided((B,), (1,), dtype=torch.int64)
     logprobs = logits.new_empty_strided((B,), (1,), dtype=torch.float32) if return_logprobs else None
+    # Rows that nothing bounds, or top_p alone, may be shared by several workgroups.
+    alone = most or 0 < most1 < V or least or least1 > 0 or (not heat and heat1 == 0)
+    need = 0 if alone else _workspace_bytes(B, V, 1 if mass or mass1 < 1 else 0)
+    work = logits.new_empty_strided((need,), (1,), dtype=torch.uint8) if need else None
     with spruce_hip.on_device(device):
         rc = spruce_hip.lib().spruce_sample_tokens(_SAMPLE_ARGS.pack(
             logits.data_ptr(), stride[0] if B > 1 else V, B, V, code, uniform.data_ptr(),
             uniform.dtype == torch.float64, heat, most, mass, least, heat1, min(most1, V), mass1, least1,
-            tokens.data_ptr(), logprobs.data_ptr() if return_logprobs else 0), spruce_hip.raw_stream(device.index))
+            tokens.data_ptr(), logprobs.data_ptr() if return_logprobs else 0, work.data_ptr() if need else 0, need),
+            spruce_hip.raw_stream(device.index))
     if rc:
         spruce_hip.check(rc, "spruce_sample_tokens")
     return (tokens, logprobs) if return_logprobs else tokens

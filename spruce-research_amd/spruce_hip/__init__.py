@@ -160,6 +160,8 @@ def lib():
         handle.spruce_paged_key_mass_workspace_bytes.argtypes = [_i64] * 5
         handle.spruce_paged_evict_workspace_bytes.restype = _i64
         handle.spruce_paged_evict_workspace_bytes.argtypes = [_i64] * 3
+        handle.spruce_sample_tokens_workspace_bytes.restype = _i64
+        handle.spruce_sample_tokens_workspace_bytes.argtypes = [_i64] * 3
         _lib = handle
     return _lib
 

@@ -146,7 +146,7 @@ def test_entry_points_refuse_before_the_launch():
 
     def sample(B=2, V=9, dtype=2, logits=FAKE, u=FAKE, out=FAKE, heat=1.0, k=0, p=1.0, m=0.0):
         return _call("spruce_sample_tokens", sampling._SAMPLE_ARGS, (
-            logits, V, B, V, dtype, u, 0, 0, 0, 0, 0, heat, k, p, m, out, 0))
+            logits, V, B, V, dtype, u, 0, 0, 0, 0, 0, heat, k, p, m, out, 0, 0, 0))
     for kwargs, message in ((dict(dtype=3), "dtype"), (dict(V=0), "vocabulary"), (dict(V=2088961), "vocabulary"),
                             (dict(B=-1), "row count"), (dict(logits=0), "non-null"), (dict(u=0), "non-null"),
                             (dict(out=0), "non-null"), (dict(logits=FAKE + 2), "aligned"), (dict(heat=-1.0), "temperature"),

@@ -225,3 +225,59 @@ def test_the_largest_vocabulary_and_many_rows():
     tokens = sample_tokens(x, u, temperature=0.5)
     assert int(tokens[-1]) == 123 and torch.equal(tokens[:-1], (u[:-1].double() * V).floor().long())
     assert sample_tokens(x[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [65536, 70001, 131071])
+def test_shared_rows_draw_as_lone_ones(V, dtype):
+    # A few long rows are shared by workgroups, many are not.  Weights are whole units, so tokens and sums are
+    # the same to the last bit.
+    inf, lowest = float("inf"), torch.finfo(dtype).min
+    gen = torch.Generator(device=DEV).manual_seed(V)
+    wide = logits(gen, 16, V + 5, dtype)
+    x = wide[:, 3:3 + V]                        # rows that begin anywhere
+    x[0] = -inf
+    x[1], x[1, V - 1] = float("nan"), 0.5       # one, in the last part
+    x[2, 100], x[2, V - 2] = inf, inf
+    x[3] = 1.0                                  # all alike: the bin of an end holds more than a list
+    x[4] = lowest
+    x[5, :-1] = lowest
+    x[6] = (torch.rand(V, generator=gen, device=DEV) * 3).floor().to(dtype)
+    x[7, 5] = 60.0                              # peaked: a short list
+    x[8, 1000:] = -inf                          # parts with nothing
+    x[9] = (x[9].float() * 0.01).to(dtype)      # flat
+    B = x.shape[0]
+    heat = torch.full((B,), 0.8, device=DEV)
+    heat[10], heat[11], heat[12], heat[13] = 0.0, 3.0, inf, 1e-30
+    mass = torch.rand(B, generator=gen, device=DEV)
+    mass[14], mass[15], mass[11] = 1.0, 0.0, 0.999
+    many = x.repeat(9, 1)
+    for v in (0.0, 0.4, 1.0 - 2.0 ** -24):
+        u = torch.full((9 * B,), v, device=DEV)
+        for setting in (dict(), dict(top_p=0.9), dict(top_p=0.3, temperature=2.0), dict(temperature=heat),
+                        dict(temperature=heat, top_p=mass)):
+            long = {n: s.repeat(9) if torch.is_tensor(s) else s for n, s in setting.items()}
+            tokens, logprobs = sample_tokens(x, u[:B], return_logprobs=True, **setting)
+            lone, alone = sample_tokens(many, u, return_logprobs=True, **long)
+            for i in range(9):
+                assert torch.equal(lone[i * B:i * B + B], tokens), setting
+                assert torch.equal(alone[i * B:i * B + B], logprobs), setting
+
+
+def test_shared_rows_in_a_graph():
+    B, V = 3, 100003
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    x, u = logits(gen, B, V, torch.bfloat16), torch.rand(B, generator=gen, device=DEV)
+    sample_tokens(x, u, top_p=0.9)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        free = sample_tokens(x, u)
+        some = sample_tokens(x, u, top_p=0.9)
+    for i in range(5):
+        x.copy_(logits(gen, B, V, torch.bfloat16, spread=0.1 + i))
+        u.copy_(torch.rand(B, generator=gen, device=DEV))
+        graph.replay()
+        got = free.clone(), some.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], sample_tokens(x, u)) and torch.equal(got[1], sample_tokens(x, u, top_p=0.9))
