@@ -491,6 +491,10 @@ extern "C" int spruce_paged_evict(const spruce_paged_evict_args* args, void* str
     e.ms[i] = a.mps[i];
   }
   e.mass = a.mass_pages;
+  if (a.pages == 0) {  // what is read in place of masses without a page, and not used, has to be memory
+    e.mass = reinterpret_cast<float*>(a.kept);
+    e.ms[0] = e.ms[1] = e.ms[2] = 0;
+  }
   e.Hkv = (int)Hkv;
   e.keep = (int)a.keep;
   e.first = (int)a.first;

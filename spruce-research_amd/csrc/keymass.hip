@@ -35,7 +35,7 @@ struct KeyMass {
   int Hq, parts, accumulate;
   int row_parts;   // of the rows that a key tile sees, where there are few tiles: each a workgroup's
   float* partial;  // their sums, [key tile][KV head][row_parts][256]
-  // Sequences of up to few_rows packed rows: stats by ranges of `range` keys, scores of a (KV head, sequence)
+  // Sequences of up to few_rows packed rows (all, where no other kernels run): stats by ranges of `range` keys, scores of a (KV head, sequence)
   // as [32 keys][row][key] from its first packed row times key_room on.
   int few_rows, range, ranges, key_room;
   float* scores;
@@ -317,6 +317,7 @@ __global__ __launch_bounds__(256) void key_mass_join_kernel(float2* stats, int64
 // The at-th of the key tiles of all sequences with new tokens.
 struct KeyTile {
   int s, tile, len, start, n;
+  int row;  // the first of the rows, of a unit that has only 32
   int64_t pos0;
 };
 __device__ __forceinline__ bool find_keys(const PagedAttn& p, int64_t at, int lane, KeyTile& k) {
@@ -537,6 +538,8 @@ __device__ __forceinline__ float weight_of(float d, float cs, float cs_low) {
 }
 
 // The at-th range of `keys` keys of all sequences of few rows.
+// BY_ROWS: of its rows, 32 at a time.
+template <bool BY_ROWS>
 __device__ __forceinline__ bool find_range(const KeyMass& a, int64_t at, int keys, int lane, KeyTile& k) {
   const PagedAttn& p = a.a;
   int64_t count = 0;
@@ -545,13 +548,20 @@ __device__ __forceinline__ bool find_range(const KeyMass& a, int64_t at, int key
     const int first = clamp_start(p.batch, len.starts), e = clamp_start(p.batch, len.ends);
     int n = len.keys < 0 ? 0 : (len.keys < p.batch.cap ? len.keys : p.batch.cap);
     if (e <= first || (int64_t)(e - first) * p.G > a.few_rows || p.batch.pages == 0) n = 0;
-    const int64_t pc = count + wave_prefix((int64_t)((n + keys - 1) / keys));
+    const int64_t row_tiles = BY_ROWS && e > first ? ((int64_t)(e - first) * p.G + kFewTile - 1) / kFewTile : 1;
+    const int64_t pc = count + wave_prefix((n + keys - 1) / keys * row_tiles);
     const uint64_t past = __ballot(pc > at);
     if (past) {
       const int l = __builtin_ctzll(past);
       k.s = s0 + l;
       k.len = __builtin_amdgcn_readlane(n, l);
-      k.tile = uniform((int)(at - lane_of(pc, l))) + (k.len + keys - 1) / keys;
+      const int ranges = (k.len + keys - 1) / keys, tiles = BY_ROWS ? (int)lane_of(row_tiles, l) : 1;
+      k.tile = uniform((int)(at - lane_of(pc, l) + (int64_t)ranges * tiles));
+      k.row = 0;
+      if (tiles > 1) {
+        k.row = k.tile % tiles * kFewTile;
+        k.tile /= tiles;
+      }
       k.start = __builtin_amdgcn_readlane(first, l);
       k.n = __builtin_amdgcn_readlane(e, l) - k.start;
       k.pos0 = lane_of((int64_t)len.keys - ((int64_t)len.ends - len.starts) + ((int64_t)first - len.starts), l);
@@ -581,9 +591,9 @@ __global__ __launch_bounds__(256, 3) void key_scores_kernel(const KeyMass a) {
     const int64_t at = unit / p.Hkv;
     const int g = (int)(unit - at * p.Hkv);
     KeyTile k;
-    if (!find_range(a, at, a.range, lane, k)) return;
+    if (!find_range<true>(a, at, a.range, lane, k)) return;
     const int rows = k.n * p.G;
-    const int r = l32 < rows ? l32 : rows - 1, t = p.by_group.of(r), h = g * p.G + r - t * p.G;
+    const int r = k.row + l32 < rows ? k.row + l32 : rows - 1, t = p.by_group.of(r), h = g * p.G + r - t * p.G;
     const int qpos = clip(k.pos0 + t);
     const uint16_t* src =
         static_cast<const uint16_t*>(p.q) + (int64_t)(k.start + t) * p.qs[0] + (int64_t)h * p.qs[1] + 8 * hl;
@@ -593,7 +603,7 @@ __global__ __launch_bounds__(256, 3) void key_scores_kernel(const KeyMass a) {
     const int k0 = k.tile * a.range + kFewTile * wave;
     const int k1 = (k.tile + 1) * a.range < k.len ? (k.tile + 1) * a.range : k.len;
     const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)g * p.ks[1] + 8 * lc;
-    float* out = scores_of(a, k, g) + l32 * kFewTile + 4 * hl;
+    float* out = scores_of(a, k, g) + (k.row + l32) * kFewTile + 4 * hl;
     const int first_pos = uniform(clip(k.pos0));
     // The next tile of keys in flight, its table entries looked up a tile before.  (Two tiles in
     // flight: 333 us where one took 327.)
@@ -650,7 +660,7 @@ __global__ __launch_bounds__(256, 3) void key_scores_kernel(const KeyMass a) {
       for (int i = 0; i < 16; ++i) l += weight_of(s[i] - now, p.cs, a.cs_low);
       sum.m = now;
       sum.l = l;
-      if (l32 < rows) {
+      if (k.row + l32 < rows) {
         float* to = out + (int64_t)(key0 / kFewTile) * rows * kFewTile;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -659,7 +669,7 @@ __global__ __launch_bounds__(256, 3) void key_scores_kernel(const KeyMass a) {
     }
     sums[wave][hl][l32] = float2{sum.m, sum.l};
     __syncthreads();
-    if (wave == 0 && hl == 0 && l32 < rows) {
+    if (wave == 0 && hl == 0 && k.row + l32 < rows) {
       Sum all;
 #pragma unroll
       for (int i = 0; i < 8; ++i) all.join(sums[i >> 1][i & 1][l32].x, sums[i >> 1][i & 1][l32].y, p.cs);
@@ -679,25 +689,8 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
     const int64_t at = unit / p.Hkv;
     const int g = (int)(unit - at * p.Hkv);
     KeyTile k;
-    if (!find_range(a, at, kWeightKeys, lane, k)) return;
+    if (!find_range<false>(a, at, kWeightKeys, lane, k)) return;
     const int rows = k.n * p.G, ranges = (k.len + a.range - 1) / a.range;
-    {
-      const int r = tid % kFewTile, t = p.by_group.of(r), h = g * p.G + r - t * p.G;
-      Sum sum;
-      if (r < rows) {
-        const float2* st = a.few_stats + ((int64_t)(k.start + t) * a.Hq + h) * a.ranges;
-        for (int i = tid / kFewTile; i < ranges; i += 8) sum.join(st[i].x, st[i].y, p.cs);
-      }
-      parts[tid / kFewTile][r] = float2{sum.m, sum.l};
-      __syncthreads();
-      if (tid < kFewTile) {
-        Sum all;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) all.join(parts[i][tid].x, parts[i][tid].y, p.cs);
-        row[tid] = float2{all.m, all.l == 0.f ? 0.f : 1.f / all.l};
-      }
-      __syncthreads();
-    }
     const float* scores = scores_of(a, k, g);
     int key[4], entry[4];
     const float* from[4];
@@ -709,19 +702,37 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
       entry[i] = page_entry(p.batch, k.s, in);
       from[i] = scores + (int64_t)(in / kFewTile) * rows * kFewTile + in % kFewTile;
     }
-#pragma unroll 2
-    for (int r = 0; r < rows; ++r) {
-      const float2 ml = row[r];
+    for (int r0 = 0; r0 < rows; r0 += kFewTile) {
+      const int n = rows - r0 < kFewTile ? rows - r0 : kFewTile;
+      const int of = tid % kFewTile, r = r0 + of, t = p.by_group.of(r), h = g * p.G + r - t * p.G;
+      Sum one;
+      if (of < n) {
+        const float2* st = a.few_stats + ((int64_t)(k.start + t) * a.Hq + h) * a.ranges;
+        for (int i = tid / kFewTile; i < ranges; i += 8) one.join(st[i].x, st[i].y, p.cs);
+      }
+      parts[tid / kFewTile][of] = float2{one.m, one.l};
+      __syncthreads();
+      if (tid < kFewTile) {
+        Sum all;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sum[i] += weight_of(from[i][r * kFewTile] - ml.x, p.cs, a.cs_low) * ml.y;
+        for (int i = 0; i < 8; ++i) all.join(parts[i][tid].x, parts[i][tid].y, p.cs);
+        row[tid] = float2{all.m, all.l == 0.f ? 0.f : 1.f / all.l};
+      }
+      __syncthreads();
+#pragma unroll 2
+      for (int i = 0; i < n; ++i) {
+        const float2 ml = row[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sum[j] += weight_of(from[j][(int64_t)(r0 + i) * kFewTile] - ml.x, p.cs, a.cs_low) * ml.y;
+      }
+      __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (key[i] >= k.len || !is_page(p.batch, entry[i])) continue;
       set_mass(a, k, g, key[i], entry[i], sum[i]);
     }
-    __syncthreads();
   }
 }
 
@@ -737,7 +748,7 @@ MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) 
   const int64_t G = Hq / Hkv;
   MassPlan plan{};
   // As in the attention's plan: the lengths are not known here, but every sequence has a new token
-  // in all but odd batches.
+  // in all but odd batches (whose longer ones then go the few-row way, 32 rows at a time).
   const int64_t longest = N > S ? N - S + 1 : 1;
   plan.key_room = (keys + kFewTile - 1) / kFewTile * kFewTile;
   // Where the average is past it too, few sequences are taken to be alike: the launches of the other kind cost more
@@ -846,7 +857,7 @@ extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, voi
   m.partial = reinterpret_cast<float*>(work += plan.many_bytes);
   m.few_stats = reinterpret_cast<float2*>(work += plan.partial_bytes);
   m.scores = reinterpret_cast<float*>(work += plan.few_stats_bytes);
-  m.few_rows = kFewTile;
+  m.few_rows = plan.many ? kFewTile : 0x7fffffff;
   m.range = (int)plan.range;
   m.ranges = (int)plan.ranges;
   m.key_room = (int)plan.key_room;

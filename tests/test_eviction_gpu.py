@@ -106,6 +106,10 @@ CASES = [
     ([40, 33], [9000, 5003], 32, 16, 8, 64, True),
     ([600], [600], 16, 64, 1, 64, False),
     ([1500, 2], [1500, 40], 48, 14, 2, 128, True),
+    # Sequences without new tokens beside long ones.
+    ([9, 0, 0, 0, 0, 0, 0, 0, 0, 0], [700] * 10, 32, 8, 2, 128, True),
+    ([0] * 30 + [60] + [0] * 40, [33] * 30 + [1500] + [7] * 40, 16, 16, 4, 64, False),
+    ([0, 1, 33, 0, 1, 0, 40, 0, 0, 1], [500] * 10, 16, 4, 4, 64, True),
 ]
 
 
@@ -349,6 +353,37 @@ def test_evict_without_pages_and_in_place():
     assert bool((kept == -1).all()) and new_lens.tolist() == [0, 0, 0]
     kept, new_lens = evict_paged_kv(kp, vp, mp, table[:, :0], lens, out[:, :0], keep)
     assert bool((kept == -1).all()) and new_lens.tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize("cols", [6, 1200])
+def test_evict_where_no_pages_are(cols):
+    # A cache of no page, tables on either side of what one workgroup holds: the lowest positions stay.
+    page, Hkv, D = 16, 2, 64
+    none = torch.empty(0, Hkv, page, D, dtype=torch.bfloat16, device=DEV)
+    mass = torch.empty(0, Hkv, page, device=DEV)
+    table = torch.zeros(2, cols, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([cols * page, 20], dtype=torch.int32, device=DEV)
+    kept, new_lens = evict_paged_kv(none, none.clone(), mass, table, lens, table, 40, first=1, recent=9)
+    want = list(range(31)) + list(range(cols * page - 9, cols * page))
+    assert kept[0].tolist() == [want] * Hkv and new_lens.tolist() == [40, 20]
+    assert kept[1].tolist() == [list(range(20)) + [-1] * 20] * Hkv
+
+
+@pytest.mark.parametrize("kv", [[4096, 4095, 4097], [16384, 9000, 301], [16385, 16384, 8193], [24576, 24577, 8192, 300]])
+def test_evict_at_the_borders_of_its_parts(kv):
+    # Positions that one workgroup holds, and that a part of a longer table has.
+    page, Hkv, D, keep = 1, 2, 64, 300
+    gen = torch.Generator(device=DEV).manual_seed(kv[0])
+    both, _, _, total = make_batch(4, [1] * (2 * len(kv)), kv + [keep] * len(kv), page)
+    table, out = both[:len(kv)], both[len(kv):, :keep]
+    kp, vp = make_cache(gen, total, Hkv, page, D, torch.bfloat16)
+    mp = (torch.rand(total, Hkv, page, generator=gen, device=DEV) * 100).round()
+    want = evict_plain(kp, vp, mp, table, kv, out, keep, 3, 5)
+    lens = torch.tensor(kv, dtype=torch.int32, device=DEV)
+    kept, new_lens = evict_paged_kv(kp, vp, mp, table, lens, out, keep, first=3, recent=5)
+    assert torch.equal(kept.cpu(), want[0]) and new_lens.tolist() == want[1]
+    for got, exact in zip((kp, vp, mp), want[2:]):
+        assert torch.equal(bits(got), bits(exact))
 
 
 def test_evict_long_and_far():
