@@ -25,7 +25,7 @@
 // take 4 us).  So a weight is two additions, a fused one and a polynomial of four terms, only rows of a histogram
 // need all of them, and few long rows without top_k and min_p are shared by workgroups.
 // Measured: top_k 50, top_p 0.95, min_p 0.02 of [1, 32003] f16 16 us; top_k 1000, top_p 0.9 of [24, 50021]
-// bf16 75; top_p 0.95 of [64, 150016] bf16 103; min_p 0.001 of [256, 131072] f32 77.
+// bf16 75; top_p 0.95 of [64, 150016] bf16 95; min_p 0.001 of [256, 131072] f32 77.
 #include "paged_impl.h"
 
 namespace spruce {
@@ -62,9 +62,7 @@ struct PartList {
   int kind;
 };
 struct RowState {
-  uint32_t done[3];          // parts that are done with each of the steps
-  int stage;
-  int bin, whole;            // of the first end; all that comes before it is listed too
+  int stage, bin;            // that the end is in
   uint64_t before, total;    // of the bin, and of all weights
   float low, high;           // logits that lists begin and the bin's end with
   uint32_t cut_key, cut_last;
@@ -81,9 +79,9 @@ constexpr int kParts = 4096;        // such sums
 constexpr int kTable = 64;
 constexpr int kMostParts = 16;      // of a row
 // Rows that are shared out, to as many workgroups: of so many logits at the least, with top_p and without.
-// Shared and not, in us: top_p 0.95 of bf16 [1, 100000] 49 and 68, [8, 150016] 72 and 147, [64, 150016]
-// 103 and 152, [128, 256000] 166 and 241, but [128, 100000] 91 and 83, and at 50021 logits the launches' own
-// latency takes all that is gained; without top_p [1, 50021] 16 and 29, [128, 150016] 42 and 60, [64, 32003] 24 and 24.
+// Shared and not, in us: top_p 0.95 of bf16 [1, 100000] 50 and 68, [8, 150016] 73 and 147, [64, 150016]
+// 95 and 152, [128, 256000] 156 and 241, [128, 100000] 79 and 83; at 50021 logits the launches' own latency
+// takes all that is gained; without top_p [1, 50021] 17 and 29, [128, 150016] 40 and 60.
 // (With top_k or min_p the lists are short, and it lost at every size: top_k 50 of [1, 150016] 40 and 34.)
 constexpr int kSharers = kCus;
 constexpr int64_t kLeastByP = 65536, kLeastPlain = 32768;
@@ -742,10 +740,10 @@ __device__ __forceinline__ void draw_summed(Shared& sh, Sampler<T>& s, const Sam
 // A row that keeps more than the list holds, by one workgroup.  A function of its own, which sets
 // everything up again: what it would keep in registers pushed the usual way's out of them.
 template <typename T>
-__device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute__((address_space(3))) Shared* lds, int row) {
+__device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute__((address_space(3))) Shared* lds) {
   const Sampling p = *(const Sampling*)(const __attribute__((address_space(4))) Sampling*)lane_of((int64_t)args, 0);
   Shared& sh = *(Shared*)lds;
-  const int b = spruce::uniform(row), tid = threadIdx.x;
+  const int b = (int)blockIdx.x, tid = threadIdx.x;
   Settings set;
   set.init(p, b);
   Sampler<T> s{sh};
@@ -984,22 +982,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
     sh.before = before;
     sh.total = total;
   }
-  sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh, b);
+  sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh);
 }
 
 // ------------------------------------------------------------------ rows by more than one workgroup
-// Rows without top_k and min_p, whose lists are long or none: the same steps, the passes over a row part by part.
-// (An instruction on each of 150016 logits is a microsecond of one workgroup.)  What all parts have to know before
-// the next step is found by the workgroup that is the row's last to be done with one.
-
-// True in the workgroup that comes here last of its row's: it sees what the others wrote before.
-__device__ __forceinline__ bool last_of_row(Shared& sh, const Sampling& p, int b, int step) {
-  __syncthreads();
-  if (threadIdx.x == 0)
-    sh.result[2] = __hip_atomic_fetch_add(&p.states[b].done[step], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  return (int)sh.result[2] == p.parts - 1;
-}
+// Rows without top_k and min_p, whose lists are long or none: the same steps, the passes over a row part by part, a
+// launch each.  (An instruction on each of 150016 logits is a microsecond of one workgroup.  Steps between them in
+// whichever workgroup of a row is done last need every wave's stores written back from its L2 before: top_p 0.95 of
+// bf16 [64, 150016] took 258 us so, 95 in launches of their own.)
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void part_largest_kernel(const Sampling p) {
@@ -1010,12 +1000,7 @@ __global__ __launch_bounds__(kThreads) void part_largest_kernel(const Sampling p
   float most;
   const uint64_t best = largest_logit(sh, s, most);
   if (threadIdx.x == 0) p.best[(int64_t)b * p.parts + part] = best;
-  if (part == 0 && threadIdx.x == 0) {
-    RowState state{};
-    state.stage = kSummed;
-    state.cut_last = 0xffffffffu;
-    p.states[b] = state;
-  }
+  if (part == 0 && threadIdx.x == 0) p.states[b] = RowState{kSummed, 0, 0, 0, 0.f, 0.f, 0, 0xffffffffu};
 }
 
 // Sets a part up behind its row's largest logit; the largest, 0 where there is none.
@@ -1042,20 +1027,77 @@ __device__ __forceinline__ void widen(Sampler<T>& s, const Sampling& p, int b) {
   s.infinite = infinite;
 }
 
-// The list of a part to where the row's end finds it.
-__device__ __forceinline__ void leave_list(Shared& sh, const Sampling& p, int b, int part, int kind) {
-  const int64_t at = (int64_t)b * p.parts + part;
-  const uint32_t n = kind == kTooMany ? 0 : sh.size;
-  for (uint32_t i = threadIdx.x; i < n; i += kThreads) p.lists[at * kList + i] = sh.list[i];
-  if (threadIdx.x == 0) p.part_list[at] = PartList{n, kind};
+// The weights' histogram.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void part_weights_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.y, part = (int)blockIdx.x, tid = threadIdx.x;
+  Settings set;
+  set.init_shared(p, b);
+  if (!set.by_p) return;
+  Sampler<T> s{sh};
+  const uint64_t best = set_up_behind(s, p, set, b, part);
+  if (best == 0 || !(set.temperature > 0)) return;
+  s.weigh(Cut{0, 0xffffffffu});
+  uint64_t* hists = p.hists + (int64_t)b * p.parts * kBins;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) hists[(int64_t)part * kBins + tid + i * kThreads] = sh.weight[tid + i * kThreads];
 }
 
-// The end of a row whose parts have left their lists: the draw, where they hold all that is kept; the end by count
-// or weight, where they hold its bin; by this workgroup alone everything where they do not.
+// The bin of the end by top_p, and the lists of what is before it and in it, or of the bin alone.
 template <typename T>
-__device__ __forceinline__ void end_row(Shared& sh, Sampler<T>& s, const Sampling& p, const Settings& set,
-                                        const RowState& state, int b) {
-  const int tid = threadIdx.x;
+__global__ __launch_bounds__(kThreads) void part_list_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.y, part = (int)blockIdx.x, tid = threadIdx.x;
+  Settings set;
+  set.init_shared(p, b);
+  if (!set.by_p) return;
+  Sampler<T> s{sh};
+  const uint64_t best = set_up_behind(s, p, set, b, part);
+  if (best == 0 || !(set.temperature > 0)) return;
+  const uint64_t* hists = p.hists + (int64_t)b * p.parts * kBins;
+  uint64_t h0 = 0, h1 = 0;
+#pragma unroll 4
+  for (int i = 0; i < p.parts; ++i) {
+    h0 += hists[(int64_t)i * kBins + tid];
+    h1 += hists[(int64_t)i * kBins + tid + kThreads];
+  }
+  sh.weight[tid] = h0;
+  sh.weight[tid + kThreads] = h1;
+  uint64_t total, before = 0, all;
+  block_prefix(sh, h0 + h1, total);
+  const int bin = s.find_bin(target_of(fmax(set.top_p, 0.0) * (double)total), before, all);
+  // About as many logits are before the bin or in it: a list of them all is not tried if they are too many.
+  uint64_t many = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = tid + i * kThreads;
+    if (at <= bin) many += (uint64_t)((double)(i ? h1 : h0) / (double)(s.w.units(s.w.of(s.top - (float)at / s.per_bin)) + 1));
+  }
+  block_prefix(sh, many, many);
+  const float low = s.bin_end(bin), high = bin == 0 ? INFINITY : unordered(ordered(s.bin_end(bin - 1)) - 1);
+  if (part == 0 && tid == 0) p.states[b] = RowState{kWeighed, bin, before, total, low, high, 0, 0xffffffffu};
+  int kind = kWhole;
+  if (many > kList || !s.collect(low, INFINITY, Cut{0, 0xffffffffu}))
+    kind = s.collect(low, high, Cut{0, 0xffffffffu}) ? kMembers : kTooMany;
+  const int64_t at = (int64_t)b * p.parts + part;
+  const uint32_t n = kind == kTooMany ? 0 : sh.size;
+  for (uint32_t i = tid; i < n; i += kThreads) p.lists[at * kList + i] = sh.list[i];
+  if (tid == 0) p.part_list[at] = PartList{n, kind};
+}
+
+// The end of a row whose parts have left their lists: the draw, where they hold all that is kept; the end by
+// weight, where they hold its bin; by this workgroup alone everything where they do not.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void row_end_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.x, tid = threadIdx.x;
+  const RowState state = p.states[b];
+  if (state.stage != kWeighed) return;
+  Settings set;
+  set.init_shared(p, b);
+  Sampler<T> s{sh};
+  set_up_behind(s, p, set, b, 0);
   widen(s, p, b);
   const PartList* lists = p.part_list + (int64_t)b * p.parts;
   int worst = kWhole;
@@ -1087,8 +1129,8 @@ __device__ __forceinline__ void end_row(Shared& sh, Sampler<T>& s, const Samplin
         const uint64_t mask = __ballot(in);
         if (mask == 0) continue;
         uint32_t to = 0;
-        if ((threadIdx.x & 63) == 0) to = atomicAdd(&sh.size, (uint32_t)__builtin_popcountll(mask));
-        to = (uint32_t)lane_of((int)to, 0) + (uint32_t)__builtin_popcountll(mask & ((1ull << (threadIdx.x & 63)) - 1));
+        if ((tid & 63) == 0) to = atomicAdd(&sh.size, (uint32_t)__builtin_popcountll(mask));
+        to = (uint32_t)lane_of((int)to, 0) + (uint32_t)__builtin_popcountll(mask & ((1ull << (tid & 63)) - 1));
         if (in && to < kList) sh.list[to] = x[j];
       }
     }
@@ -1116,97 +1158,43 @@ __device__ __forceinline__ void end_row(Shared& sh, Sampler<T>& s, const Samplin
     sh.before = state.before;
     sh.total = state.total;
   }
-  sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh, b);
+  sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh);
 }
 
-// The weights' histogram, and the bin of the end by top_p.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void part_weights_kernel(const Sampling p) {
-  __shared__ Shared sh;
-  const int b = (int)blockIdx.y, part = (int)blockIdx.x, tid = threadIdx.x;
-  Settings set;
-  set.init_shared(p, b);
-  if (!set.by_p) return;
-  Sampler<T> s{sh};
-  const uint64_t best = set_up_behind(s, p, set, b, part);
-  if (best == 0 || !(set.temperature > 0)) return;
-  s.weigh(Cut{0, 0xffffffffu});
-  uint64_t* hists = p.hists + (int64_t)b * p.parts * kBins;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) hists[(int64_t)part * kBins + tid + i * kThreads] = sh.weight[tid + i * kThreads];
-  if (!last_of_row(sh, p, b, 0)) return;
-  uint64_t h0 = 0, h1 = 0;
-#pragma unroll 4
-  for (int i = 0; i < p.parts; ++i) {
-    h0 += hists[(int64_t)i * kBins + tid];
-    h1 += hists[(int64_t)i * kBins + tid + kThreads];
-  }
-  sh.weight[tid] = h0;
-  sh.weight[tid + kThreads] = h1;
-  uint64_t total, before = 0, all;
-  block_prefix(sh, h0 + h1, total);
-  const int bin = s.find_bin(target_of(fmax(set.top_p, 0.0) * (double)total), before, all);
-  // About as many logits are before the bin or in it: a list of them all is not tried if they are too many.
-  uint64_t many = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int at = tid + i * kThreads;
-    if (at <= bin) many += (uint64_t)((double)(i ? h1 : h0) / (double)(s.w.units(s.w.of(s.top - (float)at / s.per_bin)) + 1));
-  }
-  block_prefix(sh, many, many);
-  const float low = s.bin_end(bin), high = bin == 0 ? INFINITY : unordered(ordered(s.bin_end(bin - 1)) - 1);
-  if (tid == 0) {
-    RowState& out = p.states[b];
-    out.stage = kWeighed;
-    out.bin = bin;
-    out.whole = many <= kList;
-    out.before = before;
-    out.total = total;
-    out.low = low;
-    out.high = high;
-  }
-}
-
-// The lists of what is before the first end and in its bin, or of the bin alone, and the row's end.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void part_list_kernel(const Sampling p) {
-  __shared__ Shared sh;
-  const int b = (int)blockIdx.y, part = (int)blockIdx.x;
-  const RowState state = p.states[b];
-  if (state.stage != kWeighed) return;
-  Settings set;
-  set.init_shared(p, b);
-  Sampler<T> s{sh};
-  set_up_behind(s, p, set, b, part);
-  int kind = kWhole;
-  if (!state.whole || !s.collect(state.low, INFINITY, Cut{0, 0xffffffffu}))
-    kind = s.collect(state.low, state.high, Cut{0, 0xffffffffu}) ? kMembers : kTooMany;
-  leave_list(sh, p, b, part, kind);
-  if (last_of_row(sh, p, b, 1)) end_row(sh, s, p, set, state, b);
-}
-
-// The sums of rows whose ends are known, and the draw.
+// The sums of rows whose ends are known.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void part_sums_kernel(const Sampling p) {
   __shared__ Shared sh;
   const int b = (int)blockIdx.y, part = (int)blockIdx.x;
-  if (p.states[b].stage != kSummed) return;
-  const Cut cut{p.states[b].cut_key, p.states[b].cut_last};
+  const RowState state = p.states[b];
+  if (state.stage != kSummed) return;
   Settings set;
   set.init_shared(p, b);
   Sampler<T> s{sh};
   const uint64_t best = set_up_behind(s, p, set, b, part);
+  if (best == 0 || !(set.temperature > 0)) return;
+  sum_up(s, set, Cut{state.cut_key, state.cut_last}, p.sums + (int64_t)b * kParts);
+}
+
+// The draw by them.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void row_draw_kernel(const Sampling p) {
+  __shared__ Shared sh;
+  const int b = (int)blockIdx.x;
+  const RowState state = p.states[b];
+  if (state.stage != kSummed) return;
+  Settings set;
+  set.init_shared(p, b);
+  Sampler<T> s{sh};
+  const uint64_t best = set_up_behind(s, p, set, b, 0);
+  widen(s, p, b);
   if (best == 0 || !(set.temperature > 0)) {
-    widen(s, p, b);
-    if (part == 0) take_largest(s, p, best, b);
+    take_largest(s, p, best, b);
     return;
   }
-  uint64_t* sums = p.sums + (int64_t)b * kParts;
-  sum_up(s, set, cut, sums);
-  if (!last_of_row(sh, p, b, 2)) return;
-  widen(s, p, b);
-  for (int i = threadIdx.x; i < s.steps * kRowWaves; i += kThreads) sh.part[i] = i * kPart < s.row.end ? sums[i] : 0;
-  draw_summed(sh, s, p, set, cut, b);
+  for (int i = threadIdx.x; i < s.steps * kRowWaves; i += kThreads)
+    sh.part[i] = i * kPart < s.row.end ? p.sums[(int64_t)b * kParts + i] : 0;
+  draw_summed(sh, s, p, set, Cut{state.cut_key, state.cut_last}, b);
 }
 
 struct SamplePlan {
@@ -1241,11 +1229,15 @@ SamplePlan sample_plan(int64_t B, int64_t V, bool by_p) {
 
 template <typename T>
 void launch_parts(const Sampling& p, int64_t B, bool ends, hipStream_t st) {
-  const dim3 parts((unsigned)p.parts, (unsigned)B), threads(kThreads);
+  const dim3 parts((unsigned)p.parts, (unsigned)B), rows((unsigned)B), threads(kThreads);
   hipLaunchKernelGGL(part_largest_kernel<T>, parts, threads, 0, st, p);
-  if (ends) hipLaunchKernelGGL(part_weights_kernel<T>, parts, threads, 0, st, p);
-  if (ends) hipLaunchKernelGGL(part_list_kernel<T>, parts, threads, 0, st, p);
+  if (ends) {
+    hipLaunchKernelGGL(part_weights_kernel<T>, parts, threads, 0, st, p);
+    hipLaunchKernelGGL(part_list_kernel<T>, parts, threads, 0, st, p);
+    hipLaunchKernelGGL(row_end_kernel<T>, rows, threads, 0, st, p);
+  }
   hipLaunchKernelGGL(part_sums_kernel<T>, parts, threads, 0, st, p);
+  hipLaunchKernelGGL(row_draw_kernel<T>, rows, threads, 0, st, p);
 }
 
 }  // namespace

@@ -281,3 +281,20 @@ def test_shared_rows_in_a_graph():
         got = free.clone(), some.clone()
         torch.cuda.synchronize()
         assert torch.equal(got[0], sample_tokens(x, u)) and torch.equal(got[1], sample_tokens(x, u, top_p=0.9))
+
+
+@pytest.mark.parametrize("B,V", [(3, 150001), (40, 70000)])
+def test_shared_rows_time_after_time(B, V):
+    # Calls that follow one another in one workspace, each with other settings: nothing of the last one's is left.
+    gen = torch.Generator(device=DEV).manual_seed(B)
+    x, u = logits(gen, B, V, torch.float16), torch.rand(B, generator=gen, device=DEV)
+    many, all_u = x.repeat(129 // B + 1, 1), u.repeat(129 // B + 1)
+    settings = [dict(top_p=p, temperature=t) for t in (0.7, 1.0, 2.0) for p in (0.5, 0.95, 0.999, 1.0)]
+    want = [[y[:B] for y in sample_tokens(many, all_u, return_logprobs=True, **s)] for s in settings]
+    got = []
+    for _ in range(20):
+        for s in settings:
+            got.append(sample_tokens(x, u, return_logprobs=True, **s))
+    for i, (tokens, logprobs) in enumerate(got):
+        exact = want[i % len(settings)]
+        assert torch.equal(tokens, exact[0]) and torch.equal(logprobs, exact[1]), (i, settings[i % len(settings)])
