@@ -687,8 +687,8 @@ __device__ __forceinline__ void weights_at(const Sampler<T>& s, const Settings& 
 }
 
 // The kept weights' sums of 512 logits each.
-template <typename T>
-__device__ __forceinline__ void sum_up(const Sampler<T>& s, const Settings& set, const Cut& cut, uint64_t* sums) {
+template <typename T, typename F>
+__device__ __forceinline__ void sum_up(const Sampler<T>& s, const Settings& set, const Cut& cut, F store) {
   const int lane = threadIdx.x & 63, most = (s.begin + s.steps * kThreads * kChunk) / kPart;
   const float end = unordered(cut.key);
   s.template chunks<2>([&](const float (&x)[kChunk], int at) {
@@ -702,7 +702,7 @@ __device__ __forceinline__ void sum_up(const Sampler<T>& s, const Settings& set,
       sum -= kChunk * __builtin_bit_cast(uint64_t, s.w.shift);
     }
     const int64_t upto = wave_prefix((int64_t)sum);
-    if (lane == 63 && at / kPart < most) sums[at / kPart] = (uint64_t)upto;
+    if (lane == 63 && at / kPart < most) store(at / kPart, (uint64_t)upto);
   });
 }
 
@@ -731,15 +731,16 @@ __device__ __forceinline__ void draw_summed(Shared& sh, Sampler<T>& s, const Sam
   for (int j = 0; j < kChunk; ++j) {
     if (upto <= target && target < upto + units[j]) {
       p.tokens[b] = at + j - s.row.first;
-      if (p.logprobs) p.logprobs[b] = (float)log(weight[j] / ((double)total * (p.shift * 0x1p-52)));
+      if (p.logprobs) p.logprobs[b] = (float)log(s.w.of(x[j]) / ((double)total * (p.shift * 0x1p-52)));
     }
     upto += units[j];
   }
 }
 
 // A row that keeps more than the list holds, by one workgroup.  A function of its own, which sets
-// everything up again: what it would keep in registers pushed the usual way's out of them.
-template <typename T>
+// everything up again: what it would keep in registers pushed the usual way's out of them.  (And one for each
+// of its two callers: with both, 74 us of sample_kernel were 79.)
+template <typename T, bool SHARED>
 __device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute__((address_space(3))) Shared* lds) {
   const Sampling p = *(const Sampling*)(const __attribute__((address_space(4))) Sampling*)lane_of((int64_t)args, 0);
   Shared& sh = *(Shared*)lds;
@@ -772,7 +773,7 @@ __device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute_
     }
   }
   if (set.by_p) cut = s.resolve(bin, false, target_of(fmax(set.top_p, 0.0) * (double)total), before, cut);
-  sum_up(s, set, cut, sh.part);
+  sum_up(s, set, cut, [&](int i, uint64_t sum) { sh.part[i] = sum; });
   draw_summed(sh, s, p, set, cut, b);
 }
 
@@ -982,7 +983,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
     sh.before = before;
     sh.total = total;
   }
-  sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh);
+  sample_far<T, false>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh);
 }
 
 // ------------------------------------------------------------------ rows by more than one workgroup
@@ -1158,7 +1159,7 @@ __global__ __launch_bounds__(kThreads) void row_end_kernel(const Sampling p) {
     sh.before = state.before;
     sh.total = state.total;
   }
-  sample_far<T>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh);
+  sample_far<T, true>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (__attribute__((address_space(3))) Shared*)&sh);
 }
 
 // The sums of rows whose ends are known.
@@ -1173,7 +1174,8 @@ __global__ __launch_bounds__(kThreads) void part_sums_kernel(const Sampling p) {
   Sampler<T> s{sh};
   const uint64_t best = set_up_behind(s, p, set, b, part);
   if (best == 0 || !(set.temperature > 0)) return;
-  sum_up(s, set, Cut{state.cut_key, state.cut_last}, p.sums + (int64_t)b * kParts);
+  uint64_t* sums = p.sums + (int64_t)b * kParts;
+  sum_up(s, set, Cut{state.cut_key, state.cut_last}, [&](int i, uint64_t sum) { sums[i] = sum; });
 }
 
 // The draw by them.
