@@ -24,8 +24,8 @@
 // a microsecond, and the steps after the lists are chains of a few dozen barriers; the bytes are nothing to it (19 MB
 // take 4 us).  So a weight is two additions, a fused one and a polynomial of four terms, only rows of a histogram
 // need all of them, and few long rows without top_k and min_p are shared by workgroups.
-// Measured: top_k 50, top_p 0.95, min_p 0.02 of [1, 32003] f16 16 us; top_k 1000, top_p 0.9 of [24, 50021]
-// bf16 75; top_p 0.95 of [64, 150016] bf16 95; min_p 0.001 of [256, 131072] f32 77.
+// Measured: top_k 50, top_p 0.95 of [1, 32003] f16 19 us; rows of all kinds up to top_k 1000, top_p 0.9 of [24, 50021]
+// bf16 68; top_p 0.95 of [64, 150016] bf16 90; min_p 0.001 of [256, 131072] f32 76.
 #include "paged_impl.h"
 
 namespace spruce {
@@ -428,6 +428,22 @@ struct Sampler {
     __syncthreads();
   }
   // This thread's entries of the list.
+  // An entry without the bits that all entries have alike, the lower ones of 16-bit logits and the upper ones of
+  // places: select() would go through them a digit at a time, with all additions in one place.  ([24, 50021] bf16 of
+  // up to top_k 1000: 75 us, 68 without; the end within a bin of [64, 150016] bf16: 31 and 26.)
+  static constexpr int kSame = T::bytes == 4 ? 0 : (T::code == SPRUCE_DTYPE_F16 ? 13 : 16), kPlaceBits = 22;
+  static constexpr uint64_t kPlace = ((uint64_t)1 << kPlaceBits) - 1;
+  static __device__ __forceinline__ uint64_t tight(uint64_t entry) {
+    return entry >> (32 + kSame) << kPlaceBits | (entry & kPlace);
+  }
+  static __device__ __forceinline__ uint64_t tight(uint32_t order, bool last) {
+    return tight((uint64_t)order << 32 | (last ? 0xffffffffu : 0));
+  }
+  static __device__ __forceinline__ uint32_t place_of(uint64_t tightened) { return (uint32_t)(kPlace - (tightened & kPlace)); }
+  static __device__ __forceinline__ uint32_t order_of(uint64_t tightened) {
+    const uint32_t order = (uint32_t)(tightened >> kPlaceBits) << kSame;
+    return order & 0x80000000u ? order : order | ((1u << kSame) - 1);
+  }
   __device__ __forceinline__ void entries(uint64_t (&key)[kEach]) const {
     const uint32_t n = sh.size;
 #pragma unroll
@@ -525,13 +541,14 @@ struct Sampler {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       ones[i] = key[i] == 0 ? 0 : (by_count ? 1 : w.units(w.of(unordered((uint32_t)(key[i] >> 32)))));
+      key[i] = tight(key[i]);
       all += ones[i];
     }
     block_prefix(sh, all, all);
     if (all == 0) return Cut{lo, 0xffffffffu};  // no weight to choose by
     target = target - before < all ? target - before : all - 1;
-    const uint64_t last = select(sh, key, ones, (uint64_t)lo << 32, (uint64_t)hi << 32 | 0xffffffffu, target);
-    return Cut{(uint32_t)(last >> 32), ~(uint32_t)last};
+    const uint64_t last = select(sh, key, ones, tight(lo, false), tight(hi, true), target);
+    return Cut{order_of(last), place_of(last)};
   }
 
   // The place of the nth (from 0) logit of one value.
@@ -834,8 +851,8 @@ __device__ __forceinline__ void draw_listed(Shared& sh, const Sampler<T>& s, con
                                             float low, uint64_t total, int b) {
   const int lane = threadIdx.x & 63, wave = spruce::uniform(threadIdx.x >> 6);
   const uint32_t n = sh.size;
-  auto done = [&](uint64_t entry, double weight, uint64_t sum) {
-    p.tokens[b] = (int64_t)(~(uint32_t)entry - (uint32_t)s.row.first);
+  auto done = [&](uint32_t place, double weight, uint64_t sum) {
+    p.tokens[b] = (int64_t)(place - (uint32_t)s.row.first);
     if (p.logprobs) p.logprobs[b] = (float)log(weight / ((double)sum * (p.shift * 0x1p-52)));
   };
   if (n <= 64) {
@@ -869,7 +886,7 @@ __device__ __forceinline__ void draw_listed(Shared& sh, const Sampler<T>& s, con
     before = 0;
 #pragma unroll 8
     for (uint32_t j = 0; j < n; ++j) before += (uint32_t)sh.list[j] > (uint32_t)mine ? sh.weight[j] : 0;
-    if (before <= target && target < before + units) done(mine, exact, sum);
+    if (before <= target && target < before + units) done(~(uint32_t)mine, exact, sum);
     return;
   }
   uint64_t key[kEach], units[kEach], weight[kEach], sum = 0;
@@ -880,9 +897,10 @@ __device__ __forceinline__ void draw_listed(Shared& sh, const Sampler<T>& s, con
     exact[i] = key[i] ? s.w.of(unordered((uint32_t)(key[i] >> 32))) : 0.0;
     units[i] = s.w.units(exact[i]);
     weight[i] = key[i] ? 1 : 0;
+    key[i] = s.tight(key[i]);
   }
   // The ends by count and by weight, then the draw: three selections.
-  const uint64_t lowest = (uint64_t)ordered(low) << 32, highest = (uint64_t)ordered(s.top) << 32 | 0xffffffffu;
+  const uint64_t lowest = s.tight(ordered(low), false), highest = s.tight(ordered(s.top), true);
   for (int turn = set.by_k && (uint64_t)set.top_k < n ? 0 : (set.by_p ? 1 : 2);; turn = turn == 0 && set.by_p ? 1 : 2) {
     uint64_t target = (uint64_t)set.top_k - 1;
     if (turn > 0) {
@@ -891,7 +909,7 @@ __device__ __forceinline__ void draw_listed(Shared& sh, const Sampler<T>& s, con
       for (int i = 0; i < kEach; ++i) {
         if (turn == 2) {
           if (!(exact[i] >= set.min_p)) units[i] = 0;
-          key[i] = (uint32_t)key[i];  // goes down as the place goes up
+          key[i] &= s.kPlace;  // goes down as the place goes up
         }
         weight[i] = units[i];
         sum += units[i];
@@ -900,12 +918,12 @@ __device__ __forceinline__ void draw_listed(Shared& sh, const Sampler<T>& s, con
       target = turn == 2 ? drawn(set.u, sum) : target_of(fmax(set.top_p, 0.0) * (double)(set.by_k ? sum : total));
       if (target >= sum) target = sum - 1;
     }
-    const uint64_t found = turn == 2 ? select(sh, key, weight, (uint32_t)~s.row.end, 0xffffffffu, target)
+    const uint64_t found = turn == 2 ? select(sh, key, weight, s.kPlace - s.row.end, s.kPlace, target)
                                      : select(sh, key, weight, lowest, highest, target);
     if (turn == 2) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i)
-        if (units[i] && key[i] == found) done(found, exact[i], sum);
+        if (units[i] && key[i] == found) done(s.place_of(found), exact[i], sum);
       return;
     }
 #pragma unroll
