@@ -5,7 +5,7 @@
 //
 // The smallest mass that is kept is found digit by digit from the top: histograms of 11, 11
 // and 10 bits of the masses' bits, ordered as numbers.  Where a table has no more
-// than 16384 positions, one workgroup holds the masses in registers, does all of it, and
+// than 32768 positions, one workgroup holds the masses in registers, does all of it, and
 // writes the kept positions in order (read again for every digit, 64 sequences of up to 16384 took 48 us of
 // selection, 21 held).  Longer ones are shared out: the first
 // histogram part by part, the members of the bin that holds the end listed, and the end found
@@ -64,9 +64,11 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-constexpr int kWholeKeys = 16 * kSelectThreads;  // that one workgroup holds
+// That one workgroup holds.  (In parts, and held: a head of 20000 positions 28 us and 25, 64 sequences of them, 8 heads,
+// 90 and 61, 64 of 32768, 4 heads, 69 and 45, but 8 heads of 32768 31 and 33.)
+constexpr int kWholeKeys = 32 * kSelectThreads;
 // Of a longer table, in parts.  (One sequence of 131072 positions, 4 heads: 65 us in all, with twice as many a part
-// 70, half as many 72; five of up to 20011, 8 heads: 40, 48 and 37.)
+// 70, half as many 72.)
 constexpr int kPartKeys = 8 * kSelectThreads;
 
 // What a (sequence, KV head) has to choose from.
@@ -121,7 +123,7 @@ struct SelectLds {
   uint32_t hist[2048];
   uint32_t waves[kSelectWaves];
   uint32_t found[2];
-  uint32_t counts[16 * kSelectWaves];
+  uint32_t counts[kWholeKeys / 64];
 };
 
 // From the top: the bin of the histogram within which the need-th lies; need goes on to its place there.
@@ -169,7 +171,7 @@ __device__ __forceinline__ void write_kept(SelectLds& sh, const Evict& e, const 
   }
   __syncthreads();
   if (wave == 0) {
-    // Sums before each 64 of them: E / 4 a lane.  (Up to 16384 of either, so the halves hold.)
+    // Sums before each 64 of them: E / 4 a lane.  (Up to 32768 of either, so the halves hold.)
     constexpr int EACH = E * kSelectWaves / 64;
     uint32_t v[EACH], mine = 0;
 #pragma unroll
@@ -514,8 +516,12 @@ extern "C" int spruce_paged_evict(const spruce_paged_evict_args* args, void* str
   if (plan.parts == 0) {
     if (e.batch.cap <= 4 * kSelectThreads)
       hipLaunchKernelGGL(evict_select_kernel<4>, pairs, dim3(kSelectThreads), 0, st, e);
-    else
+    else if (e.batch.cap <= 16 * kSelectThreads)
       hipLaunchKernelGGL(evict_select_kernel<16>, pairs, dim3(kSelectThreads), 0, st, e);
+    else if (e.batch.cap <= 24 * kSelectThreads)
+      hipLaunchKernelGGL(evict_select_kernel<24>, pairs, dim3(kSelectThreads), 0, st, e);
+    else
+      hipLaunchKernelGGL(evict_select_kernel<32>, pairs, dim3(kSelectThreads), 0, st, e);
   } else {
     char* work = static_cast<char*>(a.workspace);
     e.parts = (int)plan.parts;

@@ -355,7 +355,7 @@ def test_evict_without_pages_and_in_place():
     assert bool((kept == -1).all()) and new_lens.tolist() == [0, 0, 0]
 
 
-@pytest.mark.parametrize("cols", [6, 1200])
+@pytest.mark.parametrize("cols", [6, 1200, 2100])
 def test_evict_where_no_pages_are(cols):
     # A cache of no page, tables on either side of what one workgroup holds: the lowest positions stay.
     page, Hkv, D = 16, 2, 64
@@ -369,7 +369,8 @@ def test_evict_where_no_pages_are(cols):
     assert kept[1].tolist() == [list(range(20)) + [-1] * 20] * Hkv
 
 
-@pytest.mark.parametrize("kv", [[4096, 4095, 4097], [16384, 9000, 301], [16385, 16384, 8193], [24576, 24577, 8192, 300]])
+@pytest.mark.parametrize("kv", [[4096, 4095, 4097], [16384, 9000, 301], [16385, 16384, 8193], [32768, 301],
+                                [32769, 32768, 8192, 300], [40960, 40961, 24577]])
 def test_evict_at_the_borders_of_its_parts(kv):
     # Positions that one workgroup holds, and that a part of a longer table has.
     page, Hkv, D, keep = 1, 2, 64, 300
