@@ -158,6 +158,34 @@ def test_entry_points_refuse_before_the_launch():
     assert spruce_hip.lib().spruce_sample_tokens(None, None) == -1
 
 
+def test_workspaces_are_checked_before_the_launch():
+    lib = spruce_hip.lib()
+    # A few long rows are shared, many, short or bounded ones are not.
+    assert lib.spruce_sample_tokens_workspace_bytes(2, 70000, 1) > lib.spruce_sample_tokens_workspace_bytes(1, 70000, 1) > 0
+    assert lib.spruce_sample_tokens_workspace_bytes(2, 40000, 0) > 0 == lib.spruce_sample_tokens_workspace_bytes(2, 40000, 1)
+    for B, V in ((129, 70000), (2, 1000), (0, 70000), (-1, 70000), (2, 0), (1 << 40, 70000), (2, 1 << 40)):
+        assert lib.spruce_sample_tokens_workspace_bytes(B, V, 0) == 0
+
+    def sample(work, size, V=70000, p=0.9):
+        return _call("spruce_sample_tokens", sampling._SAMPLE_ARGS, (
+            FAKE, V, 2, V, 0, FAKE, 0, 0, 0, 0, 0, 1.0, 0, p, 0.0, FAKE, 0, work, size))
+    need = lib.spruce_sample_tokens_workspace_bytes(2, 70000, 1)
+    for args, message in (((0, need), "too small"), ((FAKE, need - 1), "too small"), ((FAKE, 0), "too small"),
+                          ((FAKE + 8, need), "16-byte"), ((FAKE, 64, 40000, 1.0), "too small")):
+        assert sample(*args) == -1, args
+        assert message in spruce_hip.last_error(), (args, spruce_hip.last_error())
+    assert lib.spruce_paged_evict_workspace_bytes(2, 2, 32768) == 0
+    need = lib.spruce_paged_evict_workspace_bytes(2, 2, 32784)
+
+    def evict(work, size):
+        return _call("spruce_paged_evict", eviction._EVICT_ARGS, (
+            FAKE, 4096, 2048, 128, 1, FAKE, 4096, 2048, 128, 1, FAKE, 32, 16, 1, 9, 16, FAKE, 2049, 2049, FAKE, 2, 2, 128, 0,
+            FAKE, 2, 2, 20, 2, 3, FAKE, FAKE, work, size))
+    for args, message in (((0, need), "too small"), ((FAKE, need - 1), "too small"), ((FAKE + 8, need), "16-byte")):
+        assert evict(*args) == -1, args
+        assert message in spruce_hip.last_error(), (args, spruce_hip.last_error())
+
+
 def test_argument_blocks_match_the_header():
     # The packed fields, in order: pointers, integers and arrays are 8 bytes each, doubles "d".
     text = open(os.path.join(os.path.dirname(spruce_hip.LIB_PATH), "..", "..", "include", "spruce_hip.h")).read()

@@ -110,6 +110,8 @@ CASES = [
     ([9, 0, 0, 0, 0, 0, 0, 0, 0, 0], [700] * 10, 32, 8, 2, 128, True),
     ([0] * 30 + [60] + [0] * 40, [33] * 30 + [1500] + [7] * 40, 16, 16, 4, 64, False),
     ([0, 1, 33, 0, 1, 0, 40, 0, 0, 1], [500] * 10, 16, 4, 4, 64, True),
+    # Both ways in one call, past the sequences that a wave looks at together.
+    ([1] * 41 + [50] + [2] * 40, [300 + s for s in range(41)] + [1200] + [90] * 40, 16, 8, 2, 64, True),
 ]
 
 
@@ -196,6 +198,20 @@ def test_lengths_that_do_not_fit_and_missing_pages():
     empty = torch.empty(0, Hkv, page, D, device=DEV, dtype=dtype)
     paged_key_mass(q[:2], empty, torch.empty(0, Hkv, page, device=DEV), table[:1], two, none + 9, 0.125)
     assert torch.equal(mp, before)
+
+
+def test_single_tokens_of_wide_tables():
+    # As many scores as the tables have room for would not fit into a workspace: two passes over the keys.
+    new, kv, page, dtype = [1] * 64, [1 + 5 * s for s in range(64)], 64, torch.bfloat16
+    table, starts, lens, total = make_batch(1, new, kv, page, width=2500)
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    kp = make_cache(gen, total, 4, page, 64, dtype)[0]
+    q = torch.randn(64, 28, 64, generator=gen, device=DEV).to(dtype)
+    before = torch.rand(total, 4, page, generator=gen, device=DEV)
+    for accumulate in (False, True):
+        mp = before.clone()
+        paged_key_mass(q, kp, mp, table, starts, lens, 0.125, accumulate=accumulate)
+        check_mass(mp, before, q, kp, table, new, kv, 0.125, accumulate)
 
 
 def test_hostile_starts_stay_in_bounds():
@@ -470,6 +486,28 @@ def test_streams_graphs_and_two_calls_at_once():
             assert torch.equal(mine, mps[i])
             for a, b in zip(outs[i], eager):
                 assert torch.equal(a, b), (turn, i)
+
+
+def test_one_row_of_tables_for_all_and_empty_batches():
+    # A table's row expanded over sequences of different lengths (a shared prompt), whose masses are set by one
+    # of them at a time; sequences of which none has a token.
+    page, Hq, Hkv, D, dtype = 16, 8, 2, 64, torch.float16
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    table, _, _, total = make_batch(9, [1], [600], page)
+    kp = make_cache(gen, total, Hkv, page, D, dtype)[0]
+    q = torch.randn(7, Hq, D, generator=gen, device=DEV).to(dtype)
+    before = torch.rand(total, Hkv, page, generator=gen, device=DEV)
+    lens = torch.tensor([600, 433, 20], dtype=torch.int32, device=DEV)
+    for who in range(3):
+        new = [7 if s == who else 0 for s in range(3)]
+        starts = torch.tensor([0, *new]).cumsum(0).to(torch.int32).to(DEV)
+        mp = before.clone()
+        paged_key_mass(q, kp, mp, table.expand(3, -1), starts, lens, 0.125)
+        check_mass(mp, before, q, kp, table.expand(3, -1), new, [600, 433, 20], 0.125, True)
+    mp = before.clone()
+    paged_key_mass(q, kp, mp, table.expand(3, -1), starts * 0, lens, 0.125)
+    paged_key_mass(q[:0], kp, mp, table.expand(3, -1), starts * 0, lens, 0.125)
+    assert torch.equal(mp, before)
 
 
 def test_a_cut_cache_serves_on():

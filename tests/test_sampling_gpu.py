@@ -298,3 +298,17 @@ def test_shared_rows_time_after_time(B, V):
     for i, (tokens, logprobs) in enumerate(got):
         exact = want[i % len(settings)]
         assert torch.equal(tokens, exact[0]) and torch.equal(logprobs, exact[1]), (i, settings[i % len(settings)])
+
+
+def test_other_layouts():
+    # Rows one by one, one row for all, a batch of another batch's rows, a vocabulary of one.
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    x, u = logits(gen, 6, 70007, torch.bfloat16), torch.rand(6, generator=gen, device=DEV)
+    for setting in (dict(), dict(top_p=0.8), dict(top_k=40, top_p=0.8)):
+        tokens = sample_tokens(x, u, **setting)
+        for b in range(6):
+            assert int(sample_tokens(x[b:b + 1], u[b:b + 1], **setting)) == int(tokens[b])
+        assert torch.equal(sample_tokens(x[::2], u[::2].contiguous(), **setting), tokens[::2])
+        assert torch.equal(sample_tokens(x[2:3].expand(6, -1), u, **setting),
+                           sample_tokens(x[2:3].repeat(6, 1), u, **setting))
+    assert sample_tokens(x[:, 5:6], u, top_p=0.5).tolist() == [0] * 6
