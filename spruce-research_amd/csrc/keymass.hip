@@ -21,8 +21,8 @@
 //   one token of each of 64 sequences of 6554 to 32768 keys, 28/4 heads of 128, bf16: 327 us, 3.9 TB/s of keys
 //   (by two passes over the keys 952)
 //   one token over 517 keys, 8/2 heads: 14 us
-//   windows of 8 to 40 tokens over four prompts of up to 33000 keys, 16/8 heads of 64: 69 us
-//   4096 tokens over 32768 keys, 28/4 heads: 2210 us, 820 TFLOP/s of its two products
+//   windows of 8 to 40 tokens over four prompts of up to 33000 keys, 16/8 heads of 64: 60 us
+//   4096 tokens over 32768 keys, 28/4 heads: 2030 us, 890 TFLOP/s of its two products
 #include "paged_impl.h"
 
 namespace spruce {
@@ -161,13 +161,17 @@ __global__ __launch_bounds__(256, 3) void key_mass_rows_kernel(const KeyMass a) 
   if (tr.rows == 0) return;
 
   // This lane's two columns.
-  const int mine = uniform(tr.rows - kWave * wave);  // rows of this wave, if positive
+  // Up to two waves' rows: the other two take the second half of every tile's keys.  (Windows of 8 to 40 tokens
+  // over four prompts, 16/8 heads of 64: 33 us, 26 so.)
+  const bool halves = tr.rows <= 2 * kWave;
+  const int group = halves ? wave & 1 : wave, sub0 = halves ? wave >> 1 : 0, sub1 = halves ? sub0 + 1 : kStream / 32;
+  const int mine = uniform(tr.rows - kWave * group);  // rows of this wave, if positive
   u32x4 held[2][D / 16];
   int qpos[2];
   int64_t out[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const int i = kWave * wave + 32 * c + l32;
+    const int i = kWave * group + 32 * c + l32;
     const int r = tr.row0 + (i < tr.rows ? i : tr.rows - 1);
     const int t = p.by_group.of(r), h = g * p.G + r - t * p.G;
     qpos[c] = clip(u.w.pos0 + t);
@@ -177,7 +181,7 @@ __global__ __launch_bounds__(256, 3) void key_mass_rows_kernel(const KeyMass a) 
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) held[c][kk] = load16(src + 16 * kk);
   }
-  const int first_pos = uniform(clip(u.w.pos0 + p.by_group.of(tr.row0 + (mine > 0 ? kWave * wave : 0))));
+  const int first_pos = uniform(clip(u.w.pos0 + p.by_group.of(tr.row0 + (mine > 0 ? kWave * group : 0))));
 
   const int tiles = (tr.end + kStream - 1) / kStream, per = (tiles + a.parts - 1) / a.parts;
   const int t0 = part * per < tiles ? part * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
@@ -254,7 +258,7 @@ __global__ __launch_bounds__(256, 3) void key_mass_rows_kernel(const KeyMass a) 
     const bool large =
         __ballot(fabsf(sum[0].m * p.cs) >= kLargeReference || fabsf(sum[1].m * p.cs) >= kLargeReference) != 0;
 #pragma unroll 1
-    for (int sub = 0; sub < kStream / 32; ++sub) {
+    for (int sub = sub0; sub < sub1; ++sub) {
       f32x16_t x[2];
       if (large) {
         const f32x16_t zero = {};
@@ -288,6 +292,8 @@ __global__ __launch_bounds__(256, 3) void key_mass_rows_kernel(const KeyMass a) 
       // (A reference that has just become large: the next 64 keys go by it.)
     }
   }
+  __syncthreads();
+  float2* other = reinterpret_cast<float2*>(lds);  // of the second half's waves
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     float m0, m1, s0, s1;
@@ -296,6 +302,18 @@ __global__ __launch_bounds__(256, 3) void key_mass_rows_kernel(const KeyMass a) 
     Sum all;
     all.join(m0, s0, p.cs);
     all.join(m1, s1, p.cs);
+    sum[c] = all;
+    if (halves && wave >= 2 && hl == 0) other[(wave - 2) * kWave + 32 * c + l32] = float2{all.m, all.l};
+  }
+  __syncthreads();
+  if (halves && wave >= 2) return;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    Sum all = sum[c];
+    if (halves) {
+      const float2 x = other[wave * kWave + 32 * c + l32];
+      all.join(x.x, x.y, p.cs);
+    }
     if (hl == 0 && 32 * c + l32 < mine) a.stats[out[c] * a.parts + part] = float2{all.m, all.l};
   }
 }
@@ -752,7 +770,7 @@ MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) 
   const int64_t longest = N > S ? N - S + 1 : 1;
   plan.key_room = (keys + kFewTile - 1) / kFewTile * kFewTile;
   // Where the average is past it too, few sequences are taken to be alike: the launches of the other kind cost more
-  // than they save (four windows of 8 to 40 tokens: 69 us, 120 with both).
+  // than they save (four windows of 8 to 40 tokens, by these kernels alone then: 69 us, 120 with both).
   plan.few = (N * G <= S * kFewTile || S > 8) && G <= kFewTile && N * Hq * plan.key_room <= kMostScores;
   plan.many = !plan.few || longest * G > kFewTile;
   if (plan.few) {
@@ -764,19 +782,27 @@ MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) 
     plan.few_stats_bytes = (N * Hq * plan.ranges * 8 + 15) / 16 * 16;
   }
   if (plan.many) {
-    // Four workgroups a CU, of at least 256 keys.
     plan.tiles = N * G / kRowsOf + (S < N ? S : N);
-    int64_t parts = 4 * kCus / (plan.tiles * Hkv > 0 ? plan.tiles * Hkv : 1);
-    const int64_t most = (keys + 255) / 256;
-    if (parts > most) parts = most;
+    // Four workgroups a CU, of at least 256 keys; or up to 24 of at least 1024, which even out what a chunk's tiles
+    // see.  (4096 tokens over 32768 keys, 28/4 heads: 2307 us with four alone, 2132; with more parts of rows below
+    // too, 16384 over themselves, 32/8 heads, 3327 and 2451, 4096 292 and 227.)
+    const int64_t tiles = plan.tiles * Hkv > 0 ? plan.tiles * Hkv : 1;
+    int64_t parts = 4 * kCus / tiles, more = 24 * kCus / tiles;
+    if (parts > (keys + 255) / 256) parts = (keys + 255) / 256;
+    if (more > keys / 1024) more = keys / 1024;
+    if (parts < more) parts = more;
     if (parts > 64) parts = 64;
     plan.parts = parts < 1 ? 1 : parts;
     plan.many_bytes = (N * Hq * plan.parts * 8 + 15) / 16 * 16;
-    // Two workgroups a CU, of at least 256 rows.  (2048 tokens over themselves, 28/4 heads: 84 us, with
-    // whole tiles 497; 1000 over 3000 keys, 8/2 heads: 48 and 154.)
+    // Two workgroups a CU, of at least 256 rows, or up to twelve of at least 2048 on average.  (2048 tokens over
+    // themselves, 28/4 heads: 84 us, with whole tiles 497; 1000 over 3000 keys, 8/2 heads: 48 and 154.)
     const int64_t key_tiles = S * ((keys + kRowsOf - 1) / kRowsOf) * Hkv;
-    plan.row_parts = key_tiles > 0 ? 2 * kCus / key_tiles : 1;
+    const int64_t each = key_tiles > 0 ? key_tiles : 1;
+    plan.row_parts = 2 * kCus / each;
     if (plan.row_parts > longest * G / 256) plan.row_parts = longest * G / 256;
+    int64_t more_rows = 12 * kCus / each;
+    if (more_rows > N * G / S / 2048) more_rows = N * G / S / 2048;
+    if (plan.row_parts < more_rows) plan.row_parts = more_rows;
     if (plan.row_parts > 16) plan.row_parts = 16;
     if (plan.row_parts < 1) plan.row_parts = 1;
     if (plan.row_parts > 1) plan.partial_bytes = key_tiles * plan.row_parts * kRowsOf * 4;
