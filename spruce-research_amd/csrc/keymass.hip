@@ -18,7 +18,7 @@
 // a second kernel makes the weights of them.
 //
 // Measured on one MI355X:
-//   one token of each of 64 sequences of 6554 to 32768 keys, 28/4 heads of 128, bf16: 327 us, 3.9 TB/s of keys
+//   one token of each of 64 sequences of 6554 to 32768 keys, 28/4 heads of 128, bf16: 318 us, 4.1 TB/s of keys
 //   (by two passes over the keys 952)
 //   one token over 517 keys, 8/2 heads: 14 us
 //   windows of 8 to 40 tokens over four prompts of up to 33000 keys, 16/8 heads of 64: 60 us
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(256) void key_mass_join_kernel(float2* stats, int64
 // The at-th of the key tiles of all sequences with new tokens.
 struct KeyTile {
   int s, tile, len, start, n;
-  int row;  // the first of the rows, of a unit that has only 32
+  int row;  // the first of the rows, of a unit that has not all
   int64_t pos0;
 };
 __device__ __forceinline__ bool find_keys(const PagedAttn& p, int64_t at, int lane, KeyTile& k) {
@@ -556,8 +556,8 @@ __device__ __forceinline__ float weight_of(float d, float cs, float cs_low) {
 }
 
 // The at-th range of `keys` keys of all sequences of few rows.
-// BY_ROWS: of its rows, 32 at a time.
-template <bool BY_ROWS>
+// ROWS: of its rows, so many at a time (0: all).
+template <int ROWS>
 __device__ __forceinline__ bool find_range(const KeyMass& a, int64_t at, int keys, int lane, KeyTile& k) {
   const PagedAttn& p = a.a;
   int64_t count = 0;
@@ -566,18 +566,18 @@ __device__ __forceinline__ bool find_range(const KeyMass& a, int64_t at, int key
     const int first = clamp_start(p.batch, len.starts), e = clamp_start(p.batch, len.ends);
     int n = len.keys < 0 ? 0 : (len.keys < p.batch.cap ? len.keys : p.batch.cap);
     if (e <= first || (int64_t)(e - first) * p.G > a.few_rows || p.batch.pages == 0) n = 0;
-    const int64_t row_tiles = BY_ROWS && e > first ? ((int64_t)(e - first) * p.G + kFewTile - 1) / kFewTile : 1;
+    const int64_t row_tiles = ROWS && e > first ? ((int64_t)(e - first) * p.G + ROWS - 1) / (ROWS ? ROWS : 1) : 1;
     const int64_t pc = count + wave_prefix((n + keys - 1) / keys * row_tiles);
     const uint64_t past = __ballot(pc > at);
     if (past) {
       const int l = __builtin_ctzll(past);
       k.s = s0 + l;
       k.len = __builtin_amdgcn_readlane(n, l);
-      const int ranges = (k.len + keys - 1) / keys, tiles = BY_ROWS ? (int)lane_of(row_tiles, l) : 1;
+      const int ranges = (k.len + keys - 1) / keys, tiles = ROWS ? (int)lane_of(row_tiles, l) : 1;
       k.tile = uniform((int)(at - lane_of(pc, l) + (int64_t)ranges * tiles));
       k.row = 0;
       if (tiles > 1) {
-        k.row = k.tile % tiles * kFewTile;
+        k.row = k.tile % tiles * ROWS;
         k.tile /= tiles;
       }
       k.start = __builtin_amdgcn_readlane(first, l);
@@ -596,32 +596,44 @@ __device__ __forceinline__ float* scores_of(const KeyMass& a, const KeyTile& k, 
 
 // The scores of a range of keys: every wave takes 32 keys at a time of its own, as in
 // the paged attention: whole rows from memory, past the caches, through the wave's own LDS.
-template <int D, bool F16>
-__global__ __launch_bounds__(256, 3) void key_scores_kernel(const KeyMass a) {
+// The rows are columns of the products, one a lane: 32, or 16 where sequences have no more, which halves what
+// is done for columns without a row.  (One token of each of 64 sequences of 16384 keys, 28/4 heads, by 32 columns and by
+// 16: 249 us and 241, of one of 32768 29 and 27, two tokens of 16 of 16384 97 and 89; of four of 131072, 16/8 heads, 234
+// and 238.)
+template <int D, bool F16, int COLS>
+__global__ __launch_bounds__(256, COLS == 16 ? 4 : 3) void key_scores_kernel(const KeyMass a) {
   constexpr int STR = D + 8, LROWS = 512 / D, LI = kFewTile / LROWS;
+  constexpr int GROUPS = 64 / COLS, DEPTH = 8 * GROUPS, SCORES = kFewTile / GROUPS;  // scores of a lane
   __shared__ __attribute__((aligned(16))) uint16_t lds[4][kFewTile * STR];
-  __shared__ float2 sums[4][2][kFewTile];
+  __shared__ float2 sums[4 * GROUPS][COLS];
   const PagedAttn& p = a.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int l32 = lane & 31, hl = lane >> 5, lr = lane / (D / 8), lc = lane % (D / 8);
+  const int l32 = lane & 31, col = lane % COLS, group = lane / COLS, lr = lane / (D / 8), lc = lane % (D / 8);
   uint16_t* mine = lds[wave];
+  // Of a lane's i-th score: its key.
+  auto key_of = [](int i, int lane) {
+    if constexpr (COLS == 32)
+      return row_of(i, lane);
+    else
+      return 16 * (i >> 2) + 4 * (lane >> 4) + (i & 3);
+  };
   for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
     const int64_t at = unit / p.Hkv;
     const int g = (int)(unit - at * p.Hkv);
     KeyTile k;
-    if (!find_range<true>(a, at, a.range, lane, k)) return;
+    if (!find_range<COLS>(a, at, a.range, lane, k)) return;
     const int rows = k.n * p.G;
-    const int r = k.row + l32 < rows ? k.row + l32 : rows - 1, t = p.by_group.of(r), h = g * p.G + r - t * p.G;
+    const int r = k.row + col < rows ? k.row + col : rows - 1, t = p.by_group.of(r), h = g * p.G + r - t * p.G;
     const int qpos = clip(k.pos0 + t);
     const uint16_t* src =
-        static_cast<const uint16_t*>(p.q) + (int64_t)(k.start + t) * p.qs[0] + (int64_t)h * p.qs[1] + 8 * hl;
-    u32x4 held[D / 16];
+        static_cast<const uint16_t*>(p.q) + (int64_t)(k.start + t) * p.qs[0] + (int64_t)h * p.qs[1] + 8 * group;
+    u32x4 held[D / DEPTH];
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) held[kk] = load16(src + 16 * kk);
+    for (int kk = 0; kk < D / DEPTH; ++kk) held[kk] = load16(src + DEPTH * kk);
     const int k0 = k.tile * a.range + kFewTile * wave;
     const int k1 = (k.tile + 1) * a.range < k.len ? (k.tile + 1) * a.range : k.len;
     const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + (int64_t)g * p.ks[1] + 8 * lc;
-    float* out = scores_of(a, k, g) + (k.row + l32) * kFewTile + 4 * hl;
+    float* out = scores_of(a, k, g) + (k.row + col) * kFewTile + 4 * group;
     const int first_pos = uniform(clip(k.pos0));
     // The next tile of keys in flight, its table entries looked up a tile before.  (Two tiles in
     // flight: 333 us where one took 327.)
@@ -656,41 +668,57 @@ __global__ __launch_bounds__(256, 3) void key_scores_kernel(const KeyMass a) {
         load(key0 + STEP, entry);
         ahead = look_up(key0 + 2 * STEP);
       }
-      f32x16_t s = {};
+      float s[SCORES];
+      if constexpr (COLS == 32) {
+        f32x16_t x = {};
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint4 row = *reinterpret_cast<const uint4*>(mine + l32 * STR + 8 * hl + 16 * kk);
-        s = mfma32x32x16<F16>(row, __builtin_bit_cast(uint4, held[kk]), s);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint4 row = *reinterpret_cast<const uint4*>(mine + l32 * STR + 8 * group + 16 * kk);
+          x = mfma32x32x16<F16>(row, __builtin_bit_cast(uint4, held[kk]), x);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = x[i];
+      } else {
+        f32x4v x[2] = {};
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const u32x4 row = *reinterpret_cast<const u32x4*>(mine + (16 * i + col) * STR + 8 * group + 32 * kk);
+            x[i] = mfma16x16x32<F16>(row, held[kk], x[i]);
+          }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = x[i >> 2][i & 3];
       }
       wave_lds_fence();
       if (have != 0xffffffffu || key0 + kFewTile - 1 > first_pos) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (!(have >> row_of(i, lane) & 1) || key0 + row_of(i, lane) > qpos) s[i] = -INFINITY;
+        for (int i = 0; i < SCORES; ++i)
+          if (!(have >> key_of(i, lane) & 1) || key0 + key_of(i, lane) > qpos) s[i] = -INFINITY;
       }
       float mx = s[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      for (int i = 1; i < SCORES; ++i) mx = fmaxf(mx, s[i]);
       float now = sum.l == 0.f ? mx : fmaxf(sum.m, mx);
       if (now == -INFINITY) now = 0.f;  // nothing yet, but perhaps NaN
       float l = sum.l == 0.f ? 0.f : sum.l * weight_of(sum.m - now, p.cs, a.cs_low);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) l += weight_of(s[i] - now, p.cs, a.cs_low);
+      for (int i = 0; i < SCORES; ++i) l += weight_of(s[i] - now, p.cs, a.cs_low);
       sum.m = now;
       sum.l = l;
-      if (k.row + l32 < rows) {
+      if (k.row + col < rows) {
         float* to = out + (int64_t)(key0 / kFewTile) * rows * kFewTile;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<f32x4_t*>(to + 8 * i) = f32x4_t{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+        for (int i = 0; i < SCORES / 4; ++i)
+          *reinterpret_cast<f32x4_t*>(to + 4 * GROUPS * i) = f32x4_t{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
       }
     }
-    sums[wave][hl][l32] = float2{sum.m, sum.l};
+    sums[GROUPS * wave + group][col] = float2{sum.m, sum.l};
     __syncthreads();
-    if (wave == 0 && hl == 0 && k.row + l32 < rows) {
+    if (tid < COLS && k.row + col < rows) {
       Sum all;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) all.join(sums[i >> 1][i & 1][l32].x, sums[i >> 1][i & 1][l32].y, p.cs);
+      for (int i = 0; i < 4 * GROUPS; ++i) all.join(sums[i][col].x, sums[i][col].y, p.cs);
       a.few_stats[((int64_t)(k.start + t) * a.Hq + h) * a.ranges + k.tile] = float2{all.m, all.l};
     }
     __syncthreads();
@@ -707,7 +735,7 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
     const int64_t at = unit / p.Hkv;
     const int g = (int)(unit - at * p.Hkv);
     KeyTile k;
-    if (!find_range<false>(a, at, kWeightKeys, lane, k)) return;
+    if (!find_range<0>(a, at, kWeightKeys, lane, k)) return;
     const int rows = k.n * p.G, ranges = (k.len + a.range - 1) / a.range;
     const float* scores = scores_of(a, k, g);
     int key[4], entry[4];
@@ -756,6 +784,7 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
 
 struct MassPlan {
   bool few, many;
+  bool narrow;  // few rows as 16 columns
   int64_t tiles, parts;  // row tiles that a batch can have, and the parts of the keys of each
   int64_t range, ranges, key_room;
   int64_t row_parts;     // of the rows of a key tile
@@ -773,6 +802,7 @@ MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) 
   // than they save (four windows of 8 to 40 tokens, by these kernels alone then: 69 us, 120 with both).
   plan.few = (N * G <= S * kFewTile || S > 8) && G <= kFewTile && N * Hq * plan.key_room <= kMostScores;
   plan.many = !plan.few || longest * G > kFewTile;
+  plan.narrow = N * G <= S * 16;
   if (plan.few) {
     // Ranges of 1024 keys, fewer where that leaves CUs without one.
     plan.range = kMostRange;
@@ -911,8 +941,10 @@ extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, voi
       if (plan.row_parts > 1)                                                                                  \
         hipLaunchKernelGGL(key_mass_add_kernel, grid(kRowsOf, 8 * kCus), dim3(256), 0, st, m);                 \
     }                                                                                                          \
-    if (plan.few)                                                                                              \
-      hipLaunchKernelGGL((key_scores_kernel<D_, F16_>), grid(plan.range, 16 * kCus), dim3(256), 0, st, m);     \
+    if (plan.few && plan.narrow)                                                                               \
+      hipLaunchKernelGGL((key_scores_kernel<D_, F16_, 16>), grid(plan.range, 16 * kCus), dim3(256), 0, st, m); \
+    else if (plan.few)                                                                                         \
+      hipLaunchKernelGGL((key_scores_kernel<D_, F16_, 32>), grid(plan.range, 16 * kCus), dim3(256), 0, st, m); \
   } while (0)
   if (D == 128) {
     if (dtype == SPRUCE_DTYPE_F16) SPRUCE_KEY_MASS(128, true);

@@ -110,6 +110,9 @@ CASES = [
     ([9, 0, 0, 0, 0, 0, 0, 0, 0, 0], [700] * 10, 32, 8, 2, 128, True),
     ([0] * 30 + [60] + [0] * 40, [33] * 30 + [1500] + [7] * 40, 16, 16, 4, 64, False),
     ([0, 1, 33, 0, 1, 0, 40, 0, 0, 1], [500] * 10, 16, 4, 4, 64, True),
+    # Few rows as 32 columns.
+    ([4, 3], [900, 2000], 32, 28, 4, 128, False),
+    ([1, 1, 1], [333, 64, 3000], 16, 32, 1, 64, True),
     # Both ways in one call, past the sequences that a wave looks at together.
     ([1] * 41 + [50] + [2] * 40, [300 + s for s in range(41)] + [1200] + [90] * 40, 16, 8, 2, 64, True),
 ]
