@@ -224,7 +224,7 @@ struct Shared {
   // What the long way goes on with.
   float top;
   int infinite, bin;        // of the first end by weight or count; -1: none yet
-  uint64_t before, total;   // of the bin, and of all weights
+  uint64_t before, total;   // of the bin, and of all weights (of an end by count: the number of logits)
 };
 
 // Sums of a over the threads up to and with this one, and their total.  Ends with a barrier to come.
@@ -565,7 +565,7 @@ struct Sampler {
       if (lane == 63) sh.part[s * kRowWaves + wave] = (uint64_t)all;
     }
     uint64_t before;
-    const int part = find_part(nth, before);
+    const int part = find_part(nth, before);  // (the last of them where there are no more than nth)
     if (wave == 0) {
       const int at = part * kPart + lane * kChunk;
       float x[kChunk];
@@ -590,8 +590,9 @@ struct Sampler {
     return place;
   }
 
-  // The first of the sums with which they are above `target`, and what is before it.
-  __device__ __forceinline__ int find_part(uint64_t target, uint64_t& before) {
+  // The first of the sums with which they are above `target`, and what is before it.  A target past them all
+  // becomes the last within them.
+  __device__ __forceinline__ int find_part(uint64_t& target, uint64_t& before) {
     const int n = steps * kRowWaves;
     constexpr int EACH = kParts / kThreads;
     __syncthreads();
@@ -732,7 +733,7 @@ __device__ __forceinline__ void draw_summed(Shared& sh, Sampler<T>& s, const Sam
   uint64_t a = 0, total, before;
   for (int i = tid; i < s.steps * kRowWaves; i += kThreads) a += sh.part[i];
   block_prefix(sh, a, total);
-  const uint64_t target = drawn(set.u, total);
+  uint64_t target = drawn(set.u, total);
   const int part = s.find_part(target, before);
   if (wave != 0) return;
   const int at = part * kPart + lane * kChunk;
@@ -774,7 +775,7 @@ __device__ __attribute__((noinline)) void sample_far(uint64_t args, __attribute_
   uint64_t total = sh.total, before = sh.before;
   if (set.by_k) {
     const uint64_t target = (uint64_t)set.top_k - 1;
-    uint64_t all = target + 1;
+    uint64_t all = total;
     if (bin < 0) {
       s.count();
       before = 0;
@@ -975,8 +976,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
     low = least_by_rank(sh, s, set.top_k, most);
   } else if (set.by_k) {
     s.count();
-    uint64_t all;
-    bin = s.find_bin((uint64_t)set.top_k - 1, before, all);
+    bin = s.find_bin((uint64_t)set.top_k - 1, before, total);
     low = s.bin_end(bin);
   } else if (set.by_p) {
     s.weigh(Cut{0, 0xffffffffu});

@@ -312,3 +312,42 @@ def test_other_layouts():
         assert torch.equal(sample_tokens(x[2:3].expand(6, -1), u, **setting),
                            sample_tokens(x[2:3].repeat(6, 1), u, **setting))
     assert sample_tokens(x[:, 5:6], u, top_p=0.5).tolist() == [0] * 6
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", ["ends", "behind", "between", "least"])
+def test_top_k_past_the_logits_that_are_there(rows, dtype):
+    # More of the lowest logit than a list holds, the rest of the row masked: top_k from below their number to the
+    # whole row.
+    V, inf = 20000, float("inf")
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.full((3, V), -inf, device=DEV)
+    if rows == "ends":
+        x[0, :10000], x[1, :5000], x[2, :17000] = 0.0, -2.0, 1.0
+    elif rows == "behind":
+        x[0, 10000:], x[1, 15000:], x[2, 3001:] = 0.0, -2.0, 1.0
+    elif rows == "between":
+        x[0, ::2], x[1, 1::3], x[2, 5::2] = 0.0, -2.0, 1.0
+    else:       # 2000 different logits above the many of the lowest
+        for r, n in enumerate((4500, 9000, 16000)):
+            at = torch.randperm(V, generator=gen, device=DEV)[:2000 + n]
+            x[r, at] = -1.0
+            x[r, at[:2000]] = 4 * torch.rand(2000, generator=gen, device=DEV)
+    x = x.to(dtype)
+    there = (x > -inf).sum(dim=1).tolist()
+    last = [int((x[r] > -inf).nonzero()[-1]) for r in range(3)]
+    counts = sorted({k for n in there for k in (n - 1, n, n + 1)} | {4000, 18500, V - 1})
+    names = dict(top_p="p", min_p="floor")
+    for k in counts:
+        each = torch.tensor([k, there[1] + 100, V - 1], dtype=torch.int32, device=DEV)
+        for setting in (dict(), dict(top_p=0.5), dict(top_p=0.83127), dict(min_p=0.02)):
+            print(f"case {rows} {dtype} top_k={k} {setting}", flush=True)
+            for v in (0.0, 0.37, 1.0 - 2.0 ** -24):
+                u = torch.full((3,), v, device=DEV)
+                for top_k in (k, each):
+                    tokens, logprobs = sample_tokens(x, u, top_k=top_k, return_logprobs=True, **setting)
+                    check(x, u, tokens, logprobs, k=top_k, **{names[n]: s for n, s in setting.items()})
+                    if not setting and v > 0.9 and rows != "least":
+                        want = [last[r] for r in range(3) if (k if top_k is k else int(each[r])) >= there[r]]
+                        assert [t for r, t in enumerate(tokens.tolist())
+                                if (k if top_k is k else int(each[r])) >= there[r]] == want
