@@ -838,10 +838,12 @@ __device__ __forceinline__ void take_largest(const Sampler<T>& s, const Sampling
   if (p.logprobs) p.logprobs[b] = best == 0 ? -INFINITY : 0.f;
 }
 
-// What a row's list begins with by min_p, a little lower than it is, for the roundings.
+// What a row's list begins with by min_p, a little lower than it is, for the roundings: a weight's own, of
+// less than 2^-43, is all that counts where the temperature is so high, or min_p so near to one, that weights do not
+// tell logits apart.
 template <typename T>
 __device__ __forceinline__ float least_by_share(const Sampler<T>& s, double min_p) {
-  const float bound = s.top + (float)(log(min_p) * 1.000001 * kTable * 1.44269504088896340736 / s.w.steps);
+  const float bound = s.top + (float)((log(min_p) * 1.000001 - 0x1p-40) * (kTable * 1.44269504088896340736) / s.w.steps);
   return fmaxf(-3.402823466e+38f, bound - (fabsf(bound) + fabsf(s.top)) * 0x1p-20f);
 }
 

@@ -351,3 +351,25 @@ def test_top_k_past_the_logits_that_are_there(rows, dtype):
                         want = [last[r] for r in range(3) if (k if top_k is k else int(each[r])) >= there[r]]
                         assert [t for r, t in enumerate(tokens.tolist())
                                 if (k if top_k is k else int(each[r])) >= there[r]] == want
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [50, 700, 9001])
+def test_min_p_where_the_temperature_leaves_all_alike(V, dtype):
+    # The logarithm of min_p times a temperature says nothing of weights that are one, or one to the last bits.
+    inf = float("inf")
+    gen = torch.Generator(device=DEV).manual_seed(V)
+    x = logits(gen, 4, V, dtype)
+    x[1, ::3] = -inf
+    x[2] = x[2] * 0.0 + 5.0
+    x[3, 7] = torch.finfo(dtype).max
+    heats = [inf, 1e30, 2.0 ** 70]
+    for heat in heats + [torch.tensor([inf, 1e25, 1e35, inf], device=DEV)]:
+        for floor in (1.0, 1.0 - 2.0 ** -24, 0.5, torch.tensor([1.0, 1.0, 0.75, 1.0], device=DEV)):
+            for v in (0.0, 0.6, 1.0 - 2.0 ** -24):
+                u = torch.full((4,), v, device=DEV)
+                tokens, logprobs = sample_tokens(x, u, temperature=heat, min_p=floor, return_logprobs=True)
+                check(x, u, tokens, logprobs, T=heat, floor=floor)
+    # All but the masked have the same share.
+    tokens = sample_tokens(x, torch.full((4,), 1.0 - 2.0 ** -24, device=DEV), temperature=inf, min_p=1.0)
+    assert tokens.tolist() == [V - 1, V - 1 if (V - 1) % 3 else V - 2, V - 1, V - 1]
