@@ -514,11 +514,12 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const float m = top[b][32 * sub + row_of(r, lane)], lg = log_sum[b][32 * sub + row_of(r, lane)];
+            const int at_pos = pos[b][32 * sub + row_of(r, lane)];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               // No weight is above one, whatever a score's last bits are.
-              const float e = (x[c][r] - m) * p.cs - lg;
-              sum[c] += fast_exp2(e > 0.f ? 0.f : e);
+              const float e = (x[c][r] - m) * p.cs - lg, w = fast_exp2(e > 0.f ? 0.f : e);
+              sum[c] += key[c] <= at_pos ? w : 0.f;  // (of a row whose sum is NaN too)
             }
           }
         } else {
@@ -730,6 +731,7 @@ __global__ __launch_bounds__(256, COLS == 16 ? 4 : 3) void key_scores_kernel(con
 constexpr int kWeightKeys = 1024;
 __global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
   __shared__ float2 parts[8][kFewTile], row[kFewTile];
+  __shared__ int reach;  // the last position of a row whose sum is NaN
   const PagedAttn& p = a.a;
   const int tid = threadIdx.x, lane = tid & 63;
   for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
@@ -763,7 +765,12 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
         Sum all;
 #pragma unroll
         for (int i = 0; i < 8; ++i) all.join(parts[i][tid].x, parts[i][tid].y, p.cs);
-        row[tid] = float2{all.m, all.l == 0.f ? 0.f : 1.f / all.l};
+        // Of a row whose sum is NaN the keys that it sees get NaN, by `reach`, and masked ones nothing (their weight
+        // of zero times NaN would be NaN).
+        const bool none = !(all.l == all.l);
+        row[tid] = float2{none ? INFINITY : all.m, none || all.l == 0.f ? 0.f : 1.f / all.l};
+        const uint64_t bad = __ballot(none);
+        if (tid == 0) reach = bad ? clip(k.pos0 + p.by_group.of(r0 + 63 - __builtin_clzll(bad))) : -1;
       }
       __syncthreads();
 #pragma unroll 2
@@ -773,6 +780,9 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
         for (int j = 0; j < 4; ++j)
           sum[j] += weight_of(from[j][(int64_t)(r0 + i) * kFewTile] - ml.x, p.cs, a.cs_low) * ml.y;
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (key[j] <= reach) sum[j] = NAN;
       __syncthreads();
     }
 #pragma unroll

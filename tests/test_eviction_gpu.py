@@ -564,3 +564,28 @@ def test_a_cut_cache_serves_on():
         assert float((added - want).abs().max()) <= 2.0 ** -14 * Hq * 4 + 2.0 ** -23 * float(mp[t, :, slot].max())
         token = sample_tokens(o.view(1, -1).float() @ W, torch.rand(1, generator=gen, device=DEV), top_k=50, top_p=0.9)
         assert 0 <= int(token) < 999
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,Hkv,new,kv,at", [(8, 2, 3, 40, 1), (8, 2, 5, 700, 0), (28, 4, 4, 1500, 2), (8, 2, 70, 300, 30),
+                                              (16, 8, 300, 1000, 100), (4, 4, 600, 600, 599), (8, 2, 64, 64, 0)])
+def test_a_token_of_nan_reaches_only_keys_it_sees(Hq, Hkv, new, kv, at, dtype):
+    # Its weights are NaN: those of the keys up to its position, and of no later token's.
+    page, D = 16, 64
+    gen = torch.Generator(device=DEV).manual_seed(new)
+    table, starts, lens, total = make_batch(kv, [new], [kv], page)
+    kp = make_cache(gen, total, Hkv, page, D, dtype)[0]
+    q = (2 * torch.randn(new, Hq, D, generator=gen, device=DEV)).to(dtype)
+    G = Hq // Hkv
+    for bad in (float("nan"), float("inf")):
+        q[at, G - 1] = bad          # (an infinite query's products are of both signs, their sum NaN)
+        mp = torch.zeros(total, Hkv, page, device=DEV)
+        paged_key_mass(q, kp, mp, table, starts, lens, D ** -0.5)
+        plain = q.clone()
+        plain[at, G - 1] = 0.0
+        want, bar = mass64(plain, kp, table, [new], [kv], D ** -0.5)
+        _, p, t, slot = places(table, [kv], page, total)
+        later, got = p > kv - new + at, mp[t, :, slot].double()
+        assert bool(torch.isnan(got[~later, 0]).all())
+        off = (got - want[0, :, p].T).abs() <= bar[0, :, p].T
+        assert bool(off[later].all()) and bool(off[:, 1:].all())
