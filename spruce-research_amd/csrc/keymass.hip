@@ -811,7 +811,7 @@ MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) 
   plan.key_room = (keys + kFewTile - 1) / kFewTile * kFewTile;
   // Where the average is past it too, few sequences are taken to be alike: the launches of the other kind cost more
   // than they save (four windows of 8 to 40 tokens, by these kernels alone then: 69 us, 120 with both).
-  plan.few = (N * G <= S * kFewTile || S > 8) && G <= kFewTile && N * Hq * plan.key_room <= kMostScores;
+  plan.few = (N * G <= S * kFewTile || S > 8) && G <= kFewTile && plan.key_room <= kMostScores / (N * Hq);
   plan.many = !plan.few || longest * G > kFewTile;
   plan.narrow = N * G <= S * 16;
   if (plan.few) {
@@ -857,7 +857,9 @@ MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) 
 using namespace spruce;
 
 extern "C" int64_t spruce_paged_key_mass_workspace_bytes(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) {
-  if (N < 1 || S < 1 || Hkv < 1 || Hq < Hkv || N >= (int64_t)1 << 30 || S >= (int64_t)1 << 20 || Hq >= 1 << 16) return 0;
+  if (N < 1 || S < 1 || Hkv < 1 || Hq < Hkv || N >= (int64_t)1 << 30 || S >= (int64_t)1 << 20 || Hq >= 1 << 16 || keys < 0 ||
+      keys >= (int64_t)1 << 31)
+    return 0;
   return mass_plan(N, S, Hq, Hkv, keys).bytes();
 }
 

@@ -199,3 +199,12 @@ def test_argument_blocks_match_the_header():
                 kinds += ("d" if line.strip().startswith("double") else "q") * (int(size.group(1)) if size else 1)
         code = re.sub(r"(\d)q", lambda m: "q" * int(m.group(1)), layout.format.lstrip("="))
         assert code == kinds, name
+
+
+def test_mass_workspaces_of_the_largest_calls():
+    # More scores than 63 bits count (queries of one row for all tokens take no memory): the sums of the two passes.
+    size = spruce_hip.lib().spruce_paged_key_mass_workspace_bytes
+    for N, Hq in ((1 << 24, 512), (1 << 25, 256), ((1 << 25) + 77, 511)):
+        assert size(N, 16, Hq, Hq, (1 << 31) - 1024) >= 8 * N * Hq
+    for keys in (-1, 1 << 31, 1 << 40):
+        assert size(8, 2, 4, 2, keys) == 0
