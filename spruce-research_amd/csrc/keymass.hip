@@ -464,7 +464,9 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
         stat = a.stats[((int64_t)(k.start + t) * a.Hq + h) * a.parts];
       }
     };
-    float sum[2] = {0.f, 0.f};
+    // A key's weights are added up 64 rows at a time, and these sums with what each addition rounds off kept for the
+    // next: tens of thousands of rows of about one weight, in one line, were off by 3e-4 of their sum.
+    float sum[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};
     if (row0 < rows) load(row0);
     settle(held[0]);
     settle(held[1]);
@@ -490,6 +492,7 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
       // (Rows go up with their positions.)
       const bool masked = uniform(pos[b][0]) < key0 + kWave - 1;
       const bool is_large = uniform(large[b]) != 0;
+      float now[2] = {0.f, 0.f};
 #pragma unroll 1
       for (int sub = 0; sub < kStream / 32; ++sub) {
         f32x16_t x[2], c;
@@ -519,15 +522,21 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
             for (int c = 0; c < 2; ++c) {
               // No weight is above one, whatever a score's last bits are.
               const float e = (x[c][r] - m) * p.cs - lg, w = fast_exp2(e > 0.f ? 0.f : e);
-              sum[c] += key[c] <= at_pos ? w : 0.f;  // (of a row whose sum is NaN too)
+              now[c] += key[c] <= at_pos ? w : 0.f;  // (of a row whose sum is NaN too)
             }
           }
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) sum[c] += fast_exp2(x[c][r] * p.cs);
+            for (int c = 0; c < 2; ++c) now[c] += fast_exp2(x[c][r] * p.cs);
         }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float more = now[c] - lost[c], all = sum[c] + more;
+        lost[c] = (all - sum[c]) - more;
+        sum[c] = all;
       }
     }
 #pragma unroll

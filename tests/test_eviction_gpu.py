@@ -589,3 +589,22 @@ def test_a_token_of_nan_reaches_only_keys_it_sees(Hq, Hkv, new, kv, at, dtype):
         assert bool(torch.isnan(got[~later, 0]).all())
         off = (got - want[0, :, p].T).abs() <= bar[0, :, p].T
         assert bool(off[later].all()) and bool(off[:, 1:].all())
+
+
+def test_masses_of_many_equal_weights():
+    # 57344 rows that attend the same 1999 keys alike, at weights of 1 / 1999: summed up in one line they are off by
+    # up to half a step each, all the same way (3e-4 of the mass here).  Counted in 2^-24 of a mass: the
+    # logarithm of the row's sum, 11 bits, times ln 2 at four roundings (31), the two exponentials (4), sums of 32
+    # at a time (32), these added up with what is rounded off carried on, and the halves (4).
+    page, Hq, Hkv, D, new, dtype = 1999, 56, 8, 64, 8192, torch.bfloat16
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    table = torch.full((1, 66), -1, dtype=torch.int32, device=DEV)     # one page, room for many
+    table[0, 0] = 0
+    kp = torch.randn(1, Hkv, page, D, generator=gen, device=DEV).to(dtype)
+    q = torch.zeros(new, Hq, D, device=DEV, dtype=dtype)
+    starts = torch.tensor([0, new], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([2000 + new], dtype=torch.int32, device=DEV)
+    mp = torch.zeros(1, Hkv, page, device=DEV)
+    paged_key_mass(q, kp, mp, table, starts, lens, 0.125)
+    want = new * (Hq // Hkv) / page
+    assert float((mp.double() / want - 1).abs().max()) <= 71 * 2.0 ** -24
