@@ -31,7 +31,7 @@ struct KeyMass {
   PagedAttn a;     // q, k, the batch; every sequence goes the many-row way
   float* mass;
   int64_t ms[3];   // page, head, slot strides
-  float2* stats;   // [N * Hq][parts]: maximum (of scores as products) and sum
+  float2* stats;   // [N * Hq][parts]: maximum (of scores as products) and sum, of a whole row its logarithm
   int Hq, parts, accumulate;
   int row_parts;   // of the rows that a key tile sees, where there are few tiles: each a workgroup's
   float* partial;  // their sums, [key tile][KV head][row_parts][256]
@@ -138,6 +138,13 @@ struct Sum {
     m = now;
   }
 };
+
+// What a row's weights are formed with: its maximum, and the logarithm of its sum, infinite where it has no key.
+// (With what the instruction's result lacks: the same way in all rows, it was 3e-7 of every mass.)
+__device__ __forceinline__ float2 whole_row(const Sum& s) {
+  const float lg = __builtin_amdgcn_logf(s.l);
+  return float2{s.m, s.l == 0.f ? INFINITY : fmaf(s.l, fast_exp2(-lg), -1.f) * 1.44269504f + lg};
+}
 
 // EVEN: pages hold whole passes of the stream's loads, so a pass has one page, and its address but
 // for the lane's part is found on the scalar unit (looked up by every lane, as with other pages, a chunk of
@@ -314,11 +321,12 @@ __global__ __launch_bounds__(256, 3) void key_mass_rows_kernel(const KeyMass a) 
       const float2 x = other[wave * kWave + 32 * c + l32];
       all.join(x.x, x.y, p.cs);
     }
-    if (hl == 0 && 32 * c + l32 < mine) a.stats[out[c] * a.parts + part] = float2{all.m, all.l};
+    if (hl == 0 && 32 * c + l32 < mine)
+      a.stats[out[c] * a.parts + part] = a.parts == 1 ? whole_row(all) : float2{all.m, all.l};
   }
 }
 
-// Joins the parts of every row's keys: its first part stands for all afterwards.
+// Joins the parts of every row's keys: the first part's place has the whole row's afterwards.
 __global__ __launch_bounds__(256) void key_mass_join_kernel(float2* stats, int64_t rows, int parts, float cs) {
   const int64_t r = (int64_t)flat_block() * 256 + threadIdx.x;
   if (r >= rows) return;
@@ -329,7 +337,7 @@ __global__ __launch_bounds__(256) void key_mass_join_kernel(float2* stats, int64
     const float2 x = st[i];
     all.join(x.x, x.y, cs);
   }
-  st[0] = float2{all.m, all.l};
+  st[0] = whole_row(all);
 }
 
 // The at-th of the key tiles of all sequences with new tokens.
@@ -443,7 +451,7 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
       from[i] = static_cast<const uint16_t*>(p.q) + (int64_t)(k.start + t) * p.qs[0] +
                 (int64_t)(g * p.G + head[i]) * p.qs[1] + 8 * lc;
     }
-    float2 stat{0.f, 0.f};
+    float2 stat{0.f, INFINITY};
     int row_pos = -1;
     auto load = [&](int r0) {
 #pragma unroll
@@ -456,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
         }
         row[i] = load16(from[i]);
       }
-      stat = float2{0.f, 0.f};
+      stat = float2{0.f, INFINITY};
       row_pos = -1;
       if (tid < kStream && r0 + tid < rows) {
         const int t = p.by_group.of(r0 + tid), h = g * p.G + r0 + tid - t * p.G;
@@ -476,14 +484,14 @@ __global__ __launch_bounds__(256, 2) void key_mass_keys_kernel(const KeyMass a) 
       for (int i = 0; i < ST::passes; ++i)
         *reinterpret_cast<u32x4*>(&lds[b][(i * ST::rows + lr) * ST::stride + 8 * lc]) = row[i];
       if (tid < kStream) {  // one wave
-        // No key: nothing of it reaches a sum.
-        const float lg = stat.y == 0.f ? INFINITY : __builtin_amdgcn_logf(stat.y);
-        const float ref = stat.x + lg * per_cs;
+        // No key: nothing of it reaches a sum.  (The quotient is mended: its error is the same in all rows.)
+        const float lg = stat.y, by = lg * per_cs;
+        const float ref = lg == INFINITY ? lg : stat.x + fmaf(fmaf(-by, p.cs, lg), per_cs, by);
         less[b][tid] = -ref;
         top[b][tid] = stat.x;
         log_sum[b][tid] = lg;
         pos[b][tid] = row_pos;
-        const uint64_t odd = __ballot(stat.y != 0.f && !(fabsf(ref * p.cs) < kLargeReference));
+        const uint64_t odd = __ballot(lg != INFINITY && !(fabsf(ref * p.cs) < kLargeReference));
         if (tid == 0) large[b] = odd != 0;
       }
       __syncthreads();

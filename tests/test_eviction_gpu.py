@@ -608,3 +608,20 @@ def test_masses_of_many_equal_weights():
     paged_key_mass(q, kp, mp, table, starts, lens, 0.125)
     want = new * (Hq // Hkv) / page
     assert float((mp.double() / want - 1).abs().max()) <= 71 * 2.0 ** -24
+
+
+def test_the_masses_of_a_chunk_come_to_its_rows():
+    # Every row gives a weight of one.  What its roundings make of that goes either way and averages out over the rows:
+    # six of scores and references of up to 128, half a step each, at scale 0.0884, come to a deviation of under 2^-19
+    # a row, six of which are allowed.  What all rows have alike, the exponential's and the logarithm's own errors,
+    # is in their sums as in their weights: 2^-23 is left for it.
+    new, kv, page, Hq, Hkv, D = 512, 4000, 64, 32, 4, 128
+    for dtype in (torch.bfloat16, torch.float16):
+        gen = torch.Generator(device=DEV).manual_seed(1)
+        table, starts, lens, total = make_batch(8, [new], [kv], page)
+        kp = make_cache(gen, total, Hkv, page, D, dtype)[0]
+        q = (0.5 * torch.randn(new, Hq, D, generator=gen, device=DEV)).to(dtype)
+        mp = torch.zeros(total, Hkv, page, device=DEV)
+        paged_key_mass(q, kp, mp, table, starts, lens, D ** -0.5)
+        rows = new * Hq
+        assert abs(float(mp.double().sum()) / rows - 1) <= 2.0 ** -23 + 6 * 2.0 ** -19 / math.sqrt(rows)
