@@ -28,7 +28,7 @@
 namespace spruce {
 
 struct KeyMass {
-  PagedAttn a;     // q, k, the batch; every sequence goes the many-row way
+  PagedAttn a;     // q, k, the batch; sequences past few_limit packed rows go the many-row way
   float* mass;
   int64_t ms[3];   // page, head, slot strides
   float2* stats;   // [N * Hq][parts]: maximum (of scores as products) and sum, of a whole row its logarithm
@@ -36,10 +36,11 @@ struct KeyMass {
   int row_parts;   // of the rows that a key tile sees, where there are few tiles: each a workgroup's
   float* partial;  // their sums, [key tile][KV head][row_parts][256]
   // Sequences of up to few_rows packed rows (all, where no other kernels run): stats by ranges of `range` keys, scores of a (KV head, sequence)
-  // as [32 keys][row][key] from its first packed row times key_room on.
-  int few_rows, range, ranges, key_room;
+  // as [32 keys][row][key] from its first packed row (of few_tokens, those of such sequences alone where that
+  // is fewer than N) times key_room on.
+  int few_rows, range, ranges, key_room, few_tokens;
   float* scores;
-  float2* few_stats;  // [N * Hq][ranges]
+  float2* few_stats;  // [few_tokens * Hq][ranges]
   float cs_low;       // what scale log2 e has past p.cs
 };
 
@@ -55,8 +56,8 @@ constexpr int kStream = 64;           // rows, or keys, streamed between barrier
 // size; where that is large (times scale log2 e) it is formed from the finished
 // score instead, so that the largest weight of a row is one whatever the scores.
 constexpr float kLargeReference = 0x1p+10f;
-// Scores that the workspace may hold; more go by two passes over the keys.  (1 GiB: one token of 64 sequences
-// over 131072 keys, 28 heads, is 0.88.)
+// Scores that the tokens of a call may have for them to go to the workspace; with more all sequences go by two
+// passes over the keys.  (1 GiB: one token of 64 sequences over 131072 keys, 28 heads, is 0.88.)
 constexpr int64_t kMostScores = (int64_t)1 << 28;
 // A tile's sum past this moves the reference.
 constexpr float kRescaleSum = 0x1p+60f;
@@ -344,6 +345,7 @@ __global__ __launch_bounds__(256) void key_mass_join_kernel(float2* stats, int64
 struct KeyTile {
   int s, tile, len, start, n;
   int row;  // the first of the rows, of a unit that has not all
+  int place;  // of the first token among few_tokens
   int64_t pos0;
 };
 __device__ __forceinline__ bool find_keys(const PagedAttn& p, int64_t at, int lane, KeyTile& k) {
@@ -579,12 +581,16 @@ __device__ __forceinline__ float weight_of(float d, float cs, float cs_low) {
 template <int ROWS>
 __device__ __forceinline__ bool find_range(const KeyMass& a, int64_t at, int keys, int lane, KeyTile& k) {
   const PagedAttn& p = a.a;
+  const bool own_places = a.few_tokens < p.batch.N;
   int64_t count = 0;
+  int tokens = 0;
   for (int s0 = 0; s0 < p.batch.S; s0 += 64) {
     const Lengths len = lengths_of(p, s0 + lane);
     const int first = clamp_start(p.batch, len.starts), e = clamp_start(p.batch, len.ends);
     int n = len.keys < 0 ? 0 : (len.keys < p.batch.cap ? len.keys : p.batch.cap);
-    if (e <= first || (int64_t)(e - first) * p.G > a.few_rows || p.batch.pages == 0) n = 0;
+    const bool few = e > first && (int64_t)(e - first) * p.G <= a.few_rows;
+    if (!few || p.batch.pages == 0) n = 0;
+    const int mine = few ? e - first : 0, upto = own_places ? tokens + wave_prefix(mine) : 0;
     const int64_t row_tiles = ROWS && e > first ? ((int64_t)(e - first) * p.G + ROWS - 1) / (ROWS ? ROWS : 1) : 1;
     const int64_t pc = count + wave_prefix((n + keys - 1) / keys * row_tiles);
     const uint64_t past = __ballot(pc > at);
@@ -601,16 +607,18 @@ __device__ __forceinline__ bool find_range(const KeyMass& a, int64_t at, int key
       }
       k.start = __builtin_amdgcn_readlane(first, l);
       k.n = __builtin_amdgcn_readlane(e, l) - k.start;
+      k.place = own_places ? __builtin_amdgcn_readlane(upto, l) - k.n : k.start;
       k.pos0 = lane_of((int64_t)len.keys - ((int64_t)len.ends - len.starts) + ((int64_t)first - len.starts), l);
       return true;
     }
     count = lane_of(pc, 63);
+    tokens = __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
 
 __device__ __forceinline__ float* scores_of(const KeyMass& a, const KeyTile& k, int g) {
-  return a.scores + ((int64_t)g * a.a.batch.N + k.start) * a.a.G * (int64_t)a.key_room;
+  return a.scores + ((int64_t)g * a.few_tokens + k.place) * a.a.G * (int64_t)a.key_room;
 }
 
 // The scores of a range of keys: every wave takes 32 keys at a time of its own, as in
@@ -738,7 +746,7 @@ __global__ __launch_bounds__(256, COLS == 16 ? 4 : 3) void key_scores_kernel(con
       Sum all;
 #pragma unroll
       for (int i = 0; i < 4 * GROUPS; ++i) all.join(sums[i][col].x, sums[i][col].y, p.cs);
-      a.few_stats[((int64_t)(k.start + t) * a.Hq + h) * a.ranges + k.tile] = float2{all.m, all.l};
+      a.few_stats[((int64_t)(k.place + t) * a.Hq + h) * a.ranges + k.tile] = float2{all.m, all.l};
     }
     __syncthreads();
   }
@@ -773,7 +781,7 @@ __global__ __launch_bounds__(256) void key_weights_kernel(const KeyMass a) {
       const int of = tid % kFewTile, r = r0 + of, t = p.by_group.of(r), h = g * p.G + r - t * p.G;
       Sum one;
       if (of < n) {
-        const float2* st = a.few_stats + ((int64_t)(k.start + t) * a.Hq + h) * a.ranges;
+        const float2* st = a.few_stats + ((int64_t)(k.place + t) * a.Hq + h) * a.ranges;
         for (int i = tid / kFewTile; i < ranges; i += 8) one.join(st[i].x, st[i].y, p.cs);
       }
       parts[tid / kFewTile][of] = float2{one.m, one.l};
@@ -814,7 +822,7 @@ struct MassPlan {
   bool few, many;
   bool narrow;  // few rows as 16 columns
   int64_t tiles, parts;  // row tiles that a batch can have, and the parts of the keys of each
-  int64_t range, ranges, key_room;
+  int64_t range, ranges, key_room, few_tokens;
   int64_t row_parts;     // of the rows of a key tile
   int64_t many_bytes, partial_bytes, few_stats_bytes, score_bytes;
   int64_t bytes() const { return many_bytes + partial_bytes + few_stats_bytes + score_bytes; }
@@ -836,8 +844,11 @@ MassPlan mass_plan(int64_t N, int64_t S, int64_t Hq, int64_t Hkv, int64_t keys) 
     plan.range = kMostRange;
     while (plan.range > 4 * kFewTile && S * Hkv * ((keys + plan.range - 1) / plan.range) < 4 * kCus) plan.range /= 2;
     plan.ranges = (keys + plan.range - 1) / plan.range;
-    plan.score_bytes = N * Hq * plan.key_room * 4;
-    plan.few_stats_bytes = (N * Hq * plan.ranges * 8 + 15) / 16 * 16;
+    // Beside longer sequences, room for the tokens that these can have, however many the longer ones do.
+    const int64_t most = S * (kFewTile / G);
+    plan.few_tokens = plan.many && most < N ? most : N;
+    plan.score_bytes = plan.few_tokens * Hq * plan.key_room * 4;
+    plan.few_stats_bytes = (plan.few_tokens * Hq * plan.ranges * 8 + 15) / 16 * 16;
   }
   if (plan.many) {
     plan.tiles = N * G / kRowsOf + (S < N ? S : N);
@@ -947,6 +958,7 @@ extern "C" int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, voi
   m.range = (int)plan.range;
   m.ranges = (int)plan.ranges;
   m.key_room = (int)plan.key_room;
+  m.few_tokens = (int)plan.few_tokens;
   m.cs_low = (float)(a.scale * 1.44269504088896340736 - (double)cs);
   const hipStream_t st = (hipStream_t)stream;
   const int64_t units = plan.tiles * plan.parts * Hkv;

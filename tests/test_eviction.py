@@ -208,3 +208,11 @@ def test_mass_workspaces_of_the_largest_calls():
         assert size(N, 16, Hq, Hq, (1 << 31) - 1024) >= 8 * N * Hq
     for keys in (-1, 1 << 31, 1 << 40):
         assert size(8, 2, 4, 2, keys) == 0
+
+
+def test_mass_workspaces_have_room_for_what_few_rows_need():
+    # Scores are kept of sequences of up to 32 packed rows: beside longer ones 8 tokens each of four heads a KV head.
+    size = spruce_hip.lib().spruce_paged_key_mass_workspace_bytes
+    scores = 16 * 8 * 32 * 12000 * 4
+    assert scores <= size(640, 16, 32, 8, 12000) <= 1.2 * scores
+    assert size(640, 16, 32, 8, 12000) < size(640, 80, 32, 8, 12000)     # 640 tokens of which each may count

@@ -625,3 +625,38 @@ def test_the_masses_of_a_chunk_come_to_its_rows():
         paged_key_mass(q, kp, mp, table, starts, lens, D ** -0.5)
         rows = new * Hq
         assert abs(float(mp.double().sum()) / rows - 1) <= 2.0 ** -23 + 6 * 2.0 ** -19 / math.sqrt(rows)
+
+
+@pytest.mark.parametrize("new,kv,page,Hq,Hkv,D", [
+    ([1, 60, 3, 0, 200, 4, 2, 5, 1, 1], [900, 60, 3, 50, 1000, 700, 333, 90, 1, 2000], 32, 16, 2, 64),
+    ([0] * 9 + [500] + [2] * 3, [40] * 9 + [500] + [77, 2, 1500], 16, 28, 4, 128),
+    ([(7 * s) % 4 for s in range(66)] + [300, 0, 1, 3, 130, 2], [200 + 5 * s for s in range(72)], 16, 32, 4, 64),
+    ([300] + [1] * 130, [777] + [90 + s for s in range(130)], 48, 32, 1, 64),
+])
+def test_few_rows_beside_more_tokens_than_they_have_room_for(new, kv, page, Hq, Hkv, D):
+    assert sum(new) > len(new) * (32 // (Hq // Hkv)) and len(new) > 8
+    gen = torch.Generator(device=DEV).manual_seed(sum(new))
+    for dtype in (torch.bfloat16, torch.float16):
+        table, starts, lens, total = make_batch(page, new, kv, page)
+        kp = make_cache(gen, total, Hkv, page, D, dtype)[0]
+        q = (2 * torch.randn(sum(new), Hq, D, generator=gen, device=DEV)).to(dtype)
+        before = torch.rand(total, Hkv, page, generator=gen, device=DEV)
+        for accumulate in (False, True):
+            mp = before.clone()
+            paged_key_mass(q, kp, mp, table, starts, lens, D ** -0.5, accumulate=accumulate)
+            check_mass(mp, before, q, kp, table, new, kv, D ** -0.5, accumulate)
+
+
+def test_hostile_starts_of_many_sequences_stay_in_bounds():
+    # As above, with places of their own for the few rows: sequences that overlap, go back and leave the batch.
+    page, dtype, S = 16, torch.bfloat16, 12
+    table, _, _, total = make_batch(1, [1] * S, [80] * S, page)
+    kp = make_cache(torch.Generator(device=DEV).manual_seed(0), total, 2, page, 64, dtype)[0]
+    q = torch.randn(400, 4, 64, device=DEV, dtype=dtype)
+    lens = torch.tensor([80, 80, -3, 2 ** 31 - 1] * 3, dtype=torch.int32, device=DEV)
+    for starts in ([0, 16, 0, 16] * 3 + [0], [0, 1, 17, 33] * 3 + [400], [396, 400, 2 ** 31 - 1, -7] * 3 + [16],
+                   [400 - 33 * s for s in range(13)]):
+        mp = torch.full((total + 2, 2, page), 5.0, device=DEV)
+        at = torch.tensor(starts, dtype=torch.int32, device=DEV)
+        paged_key_mass(q, kp, mp[1:-1], table, at, lens, 0.125)
+        assert bool((mp[0] == 5.0).all()) and bool((mp[-1] == 5.0).all())
