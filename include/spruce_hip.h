@@ -885,7 +885,7 @@ int spruce_paged_key_mass(const spruce_paged_key_mass_args* args, void* stream);
  *   rows 16-byte aligned), mass_pages [pages, Hkv, page_size] float32, of any
  *   strides in which no two rows share memory.
  *   workspace: spruce_paged_evict_workspace_bytes(S, Hkv, table_width * page_size)
- *   bytes (none for tables of up to 16384 positions), 16-byte aligned, one call's
+ *   bytes (none for tables of up to 32768 positions), 16-byte aligned, one call's
  *   own until it is done.
  */
 int64_t spruce_paged_evict_workspace_bytes(int64_t S, int64_t Hkv, int64_t keys);

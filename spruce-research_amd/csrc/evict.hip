@@ -7,7 +7,7 @@
 // and 10 bits of the masses' bits, ordered as numbers.  Where a table has no more
 // than 32768 positions, one workgroup holds the masses in registers, does all of it, and
 // writes the kept positions in order (read again for every digit, 64 sequences of up to 16384 took 48 us of
-// selection, 21 held).  Longer ones are shared out: the first
+// selection, 19 held).  Longer ones are shared out: the first
 // histogram part by part, the members of the bin that holds the end listed, and the end found
 // among these by one workgroup.  Then the rows move, 16 bytes a lane.
 #include "paged_impl.h"
@@ -67,8 +67,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 // That one workgroup holds.  (In parts, and held: a head of 20000 positions 28 us and 25, 64 sequences of them, 8 heads,
 // 90 and 61, 64 of 32768, 4 heads, 69 and 45, but 8 heads of 32768 31 and 33.)
 constexpr int kWholeKeys = 32 * kSelectThreads;
-// Of a longer table, in parts.  (One sequence of 131072 positions, 4 heads: 65 us in all, with twice as many a part
-// 70, half as many 72.)
+// Of a longer table, in parts.  (One sequence of 131072 positions, 4 heads, with the kernels of that stage: 65 us in
+// all, with twice as many a part 70, half as many 72; 54 to 57 now.)
 constexpr int kPartKeys = 8 * kSelectThreads;
 
 // What a (sequence, KV head) has to choose from.
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_write_kernel(const Evict
 
 // Rows of ROW bytes: a workgroup moves kMoveRows of one (sequence, KV head).  HBM bounds it, and rows are
 // used once: past the caches 243 us in all for 64 sequences that keep 4096, 256 through them (32 rows a
-// workgroup: 246).
+// workgroup: 246; on a faster card 206).
 constexpr int kMoveRows = 16;
 template <int ROW>
 __global__ __launch_bounds__(256) void evict_move_kernel(const Evict e, int tiles) {

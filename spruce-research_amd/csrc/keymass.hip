@@ -18,11 +18,11 @@
 // a second kernel makes the weights of them.
 //
 // Measured on one MI355X:
-//   one token of each of 64 sequences of 6554 to 32768 keys, 28/4 heads of 128, bf16: 318 us, 4.1 TB/s of keys
-//   (by two passes over the keys 952)
-//   one token over 517 keys, 8/2 heads: 14 us
+//   one token of each of 64 sequences of 6554 to 32768 keys, 28/4 heads of 128, bf16: 289 to 318 us, 4.1 to
+//   4.5 TB/s of keys (by two passes over the keys 952)
+//   one token over 517 keys, 8/2 heads: 12 to 14 us
 //   windows of 8 to 40 tokens over four prompts of up to 33000 keys, 16/8 heads of 64: 60 us
-//   4096 tokens over 32768 keys, 28/4 heads: 2030 us, 890 TFLOP/s of its two products
+//   4096 tokens over 32768 keys, 28/4 heads: 2060 to 2090 us, 870 TFLOP/s of its two products
 #include "paged_impl.h"
 
 namespace spruce {
@@ -149,7 +149,7 @@ __device__ __forceinline__ float2 whole_row(const Sum& s) {
 
 // EVEN: pages hold whole passes of the stream's loads, so a pass has one page, and its address but
 // for the lane's part is found on the scalar unit (looked up by every lane, as with other pages, a chunk of
-// 4096 tokens over 32768 keys takes 1342 us here rather than 1282).  Three waves a SIMD, without the registers
+// 4096 tokens over 32768 keys took 1342 us here rather than 1282 at that stage, 1000 now).  Three waves a SIMD, without the registers
 // that would have a wave's own products and exponentials overlap (two waves: 1395).
 template <int D, bool F16, bool EVEN>
 __global__ __launch_bounds__(256, 3) void key_mass_rows_kernel(const KeyMass a) {

@@ -24,8 +24,8 @@
 // a microsecond, and the steps after the lists are chains of a few dozen barriers; the bytes are nothing to it (19 MB
 // take 4 us).  So a weight is two additions, a fused one and a polynomial of four terms, only rows of a histogram
 // need all of them, and few long rows without top_k and min_p are shared by workgroups.
-// Measured: top_k 50, top_p 0.95 of [1, 32003] f16 19 us; rows of all kinds up to top_k 1000, top_p 0.9 of [24, 50021]
-// bf16 68; top_p 0.95 of [64, 150016] bf16 90; min_p 0.001 of [256, 131072] f32 76.
+// Measured: top_k 50, top_p 0.95 of [1, 32003] f16 20 us; rows of all kinds up to top_k 1000, top_p 0.9 of [24, 50021]
+// bf16 46 to 68, by the inputs; top_p 0.95 of [64, 150016] bf16 89; min_p 0.001 of [256, 131072] f32 77 to 82.
 #include "paged_impl.h"
 
 namespace spruce {
@@ -79,9 +79,9 @@ constexpr int kParts = 4096;        // such sums
 constexpr int kTable = 64;
 constexpr int kMostParts = 16;      // of a row
 // Rows that are shared out, to as many workgroups: of so many logits at the least, with top_p and without.
-// Shared and not, in us: top_p 0.95 of bf16 [1, 100000] 50 and 68, [8, 150016] 73 and 147, [64, 150016]
-// 95 and 152, [128, 256000] 156 and 241, [128, 100000] 79 and 83; at 50021 logits the launches' own latency
-// takes all that is gained; without top_p [1, 50021] 17 and 29, [128, 150016] 40 and 60.
+// Shared and not, in us: top_p 0.95 of bf16 [1, 100000] 55 and 95, [8, 150016] 64 and 130, [64, 150016]
+// 89 and 130, [128, 256000] 149 and 216, [128, 100000] 93 and 109; at 50021 logits the launches' own latency
+// takes all that is gained; without top_p [1, 50021] 18 and 26, [128, 150016] 38 and 56.
 // (With top_k or min_p the lists are short, and it lost at every size: top_k 50 of [1, 150016] 40 and 34.)
 constexpr int kSharers = kCus;
 constexpr int64_t kLeastByP = 65536, kLeastPlain = 32768;
@@ -1010,7 +1010,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Sampling p) {
 // Rows without top_k and min_p, whose lists are long or none: the same steps, the passes over a row part by part, a
 // launch each.  (An instruction on each of 150016 logits is a microsecond of one workgroup.  Steps between them in
 // whichever workgroup of a row is done last need every wave's stores written back from its L2 before: top_p 0.95 of
-// bf16 [64, 150016] took 258 us so, 95 in launches of their own.)
+// bf16 [64, 150016] took 258 us so, 89 in launches of their own.)
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void part_largest_kernel(const Sampling p) {
